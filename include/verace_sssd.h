@@ -419,6 +419,77 @@ int vmi_halting_update(const void* out, const void* h, void* h_next, const void*
                        void* acc, void* depth, const uint8_t* active, uint8_t* still, void* final_h,
                        float threshold, int mode, int dtype, int64_t rows, int64_t d, void* stream);
 
+/* The norms either side of a block with its gate and residual scale, one pass over [rows, d]:
+ *   r = w1 ? y w1 / sqrt(mean(y^2) + eps1) : y
+ *   s = residual + (scale ? scale : 1) (gate ? act(gate) : 1) r        act: 0 sigmoid, 1 x sigmoid(x)
+ *   n = s w2 / sqrt(mean(s^2) + eps2)                                  (w2 and n together, or both NULL)
+ * y, residual, gate have rows of their own stride (elements), the other tensors are contiguous; w1, scale,
+ * w2 [d] are w_dtype (dtype or F32).  fp32 inside, each result rounded once, n from the unrounded s.
+ * stats (NULL or [2][rows] floats) receives the two reciprocal roots for the backward.  d <= 8192 (F32: 4096).
+ *
+ * Backward: ds, dn (either may be NULL: zero) give dy, dresidual, dgate [rows, d] and dw1, dscale, dw2 [d]
+ * (any may be NULL: not wanted; a workspace of the queried size is needed for the last three). */
+int vmi_gated_norm(const void* y, int64_t y_stride, const void* residual, int64_t r_stride,
+                   const void* gate, int64_t g_stride, const void* w1, const void* scale, const void* w2,
+                   int dtype, int w_dtype, int gate_act, float eps1, float eps2, void* s, void* n,
+                   float* stats, int64_t rows, int64_t d, void* stream);
+int vmi_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t d, int dtype, size_t* bytes);
+int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* residual, int64_t r_stride,
+                       const void* gate, int64_t g_stride, const void* w1, const void* scale, const void* w2,
+                       int dtype, int w_dtype, int gate_act, const float* stats, const void* ds,
+                       const void* dn, void* dy, void* dresidual, void* dgate, void* dw1, void* dscale,
+                       void* dw2, int64_t rows, int64_t d, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Short causal depthwise convolution:
+ *   y[b,t,c] = act(bias[c] + sum_{j<K} w[c,j] row[b, t - (K-1) + j, c]),  K = 2 .. 4,
+ * rows before the first from state_in [B, K-1, C] (NULL: zeros).  x rows have strides x_stride (tokens) and
+ * x_batch (items), in elements; w [C, K] and bias [C] (or NULL) are w_dtype; act 0: none, 1: x sigmoid(x).
+ * lengths (NULL, or [B] int32, int64 if lengths64): item b's first lengths[b] tokens (clamped to 0 .. T)
+ * count; y behind them is 0 and x there is not read.  state_out (or NULL) [B, K-1, C] receives the last K-1
+ * counted rows.  The step takes one token per item and moves `state` up a row in place (items with
+ * mask[b] = 0 keep theirs and give zeros). */
+int vmi_short_conv(const void* x, int64_t x_stride, int64_t x_batch, const void* w, const void* bias,
+                   int dtype, int w_dtype, int act, const void* state_in, const void* lengths,
+                   int lengths64, void* y, void* state_out, int64_t B, int64_t T, int64_t C, int64_t K,
+                   void* stream);
+int vmi_short_conv_step(const void* x, int64_t x_batch, const void* w, const void* bias, int dtype,
+                        int w_dtype, int act, const uint8_t* mask, void* state, void* y, int64_t B,
+                        int64_t C, int64_t K, void* stream);
+/* Gradients: dy (NULL: zero; own strides) and dstate_out (NULL: zero) give dx [B, T, C] (zero behind the
+ * lengths), dw, dbias (w_dtype) and dstate_in; any may be NULL.  The workspace is needed for dw and dbias. */
+int vmi_short_conv_bwd_workspace_bytes(int64_t B, int64_t T, int64_t C, int64_t K, size_t* bytes);
+int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_batch, const void* w, const void* bias,
+                       int dtype, int w_dtype, int act, const void* state_in, const void* lengths,
+                       int lengths64, const void* dy, int64_t dy_stride, int64_t dy_batch,
+                       const void* dstate_out, void* dx, void* dw, void* dbias, void* dstate_in, int64_t B,
+                       int64_t T, int64_t C, int64_t K, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Selective state space scan, per item b and head h (S [P, N] fp32):
+ *   d_t = softplus ? log(1 + exp(delta_t + delta_bias)) : delta_t + delta_bias
+ *   S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T,   y_t = S_t C_t + D x_t
+ * x rows [H, P], delta rows [H] (delta_dtype), bm and cm rows [G, N] have token strides *_t and item strides
+ * *_b (elements); head h uses group h / (H / G); A, D, delta_bias [H] fp32 (D, delta_bias may be NULL).
+ * state_in [B, H, P, N] (NULL: zeros) is not written and must not be state_out.  lengths as for the
+ * convolution; y [B, T, H, P] (or NULL) behind them is 0.  N <= 256, P <= 1024.
+ * The step takes one token per item and updates `state` in place (items with mask[b] = 0 keep theirs and
+ * give zeros). */
+int vmi_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N,
+                                       int dtype, size_t* bytes);
+int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, const void* delta, int64_t d_t,
+                           int64_t d_b, int delta_dtype, const float* A, const void* bm, int64_t b_t,
+                           int64_t b_b, const void* cm, int64_t c_t, int64_t c_b, const float* D,
+                           const float* delta_bias, int softplus, int dtype, const float* state_in,
+                           const void* lengths, int lengths64, void* y, float* state_out, int64_t B,
+                           int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_b, int delta_dtype,
+                       const float* A, const void* bm, int64_t b_b, const void* cm, int64_t c_b,
+                       const float* D, const float* delta_bias, int softplus, int dtype,
+                       const uint8_t* mask, float* state, void* y, int64_t B, int64_t H, int64_t P,
+                       int64_t G, int64_t N, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

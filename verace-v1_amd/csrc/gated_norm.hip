@@ -1,0 +1,399 @@
+// The norms around a block with its gate and residual scale, forward and backward, a row each:
+//
+//   r = y i1 w1, i1 = 1 / sqrt(mean(y^2) + eps1)            the norm after the block (w1 absent: r = y)
+//   s = residual + scale act(gate) r                         the residual stream
+//   n = s i2 w2, i2 = 1 / sqrt(mean(s^2) + eps2)            the norm before the next block
+//
+// and, for u = dn w2, v = dr w1, dr = dt scale act(gate):
+//   dt = ds + i2 (u - s i2^2 mean(u s))                      = dresidual
+//   dy = i1 (v - y i1^2 mean(v y)),  dgate = dt scale r act'(gate)
+//   dw1 = sum dr y i1,  dscale = sum dt act(gate) r,  dw2 = sum dn s i2        (over the rows)
+//
+// Everything between the loads and the stores is fp32; n is formed from s before s is rounded to its
+// type, and the backward forms s again from the same inputs instead of reading the rounded one.
+//
+// Bound by memory: each input is read once and each output written once.  A row is held in registers by
+// one wave (two 16-byte pieces a lane at most: rows of up to 1024 16-bit elements, no barrier), longer
+// ones by a workgroup.  The weights' gradients are kept in registers over the rows that a workgroup takes
+// and leave it as one partial row each; a second kernel adds the partials in a fixed order.
+#include <algorithm>
+#include <type_traits>
+
+#include "vmi_common.h"
+#include "vmi_dispatch.h"
+#include "vmi_vec.h"
+
+namespace vmi {
+namespace gnorm {
+
+constexpr int NTH = 256;
+
+struct Args {
+  const void *y, *res, *gate, *w1, *scale, *w2;
+  int64_t y_stride, r_stride, g_stride;  // elements between rows
+  void *s, *n;
+  float* stats;                          // [2][rows]: i1, i2 (or null)
+  const void *ds, *dn;                   // backward: gradients of s and n, contiguous (or null)
+  void *dy, *dres, *dgate;               // contiguous (or null)
+  float* partial;                        // [blocks][3][d]: dw1, dscale, dw2 (or null)
+  int64_t rows;
+  int d, silu;
+  float eps1, eps2;
+  bool vec;
+};
+
+// Sum over the G lanes of a row: a wave, or the whole workgroup (red: one float a wave; the barrier after
+// the reads lets the next sum use it again).
+template <int G> __device__ __forceinline__ float row_sum(float x, float* red) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  if constexpr (G > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = (red[0] + red[1]) + (red[2] + red[3]);
+    __syncthreads();
+  }
+  return x;
+}
+
+// act(gate) and its derivative
+template <typename T> __device__ __forceinline__ void activation(float g, bool silu, float& a, float& da) {
+  const float sg = sigmoid_for<T>(g);
+  a = silu ? g * sg : sg;
+  da = silu ? sg * (1.f + g * (1.f - sg)) : sg * (1.f - sg);
+}
+
+template <typename T, typename W, int G, int NV>
+__global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float red[NTH / 64];
+  const int lane = threadIdx.x % G, d = a.d;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (NTH / G) + threadIdx.x / G;
+  if (row >= a.rows) return;  // whole waves (G = 64) or never
+  const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+  const T* res = static_cast<const T*>(a.res) + row * a.r_stride;
+  const T* gate = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + row * a.g_stride;
+  float t[NV][N], x[NV][N], q[NV][N];
+  float ss = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = (lane + G * v) * N;
+    if (i >= d) break;
+    load_piece(y, i, d, a.vec, t[v]);
+    load_piece(res, i, d, a.vec, x[v]);
+    if (gate != nullptr) load_piece(gate, i, d, a.vec, q[v]);
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if ((lane + G * v) * N >= d) break;
+#pragma unroll
+    for (int j = 0; j < N; ++j) ss = fmaf(t[v][j], t[v][j], ss);
+  }
+  float i1 = 1.f;
+  if (a.w1 != nullptr) i1 = rsqrtf(row_sum<G>(ss, red) / d + a.eps1);
+  ss = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = (lane + G * v) * N;
+    if (i >= d) break;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (!a.vec && i + j >= d) break;
+      float r = t[v][j] * i1;
+      if (a.w1 != nullptr) r *= io<W>::load(static_cast<const W*>(a.w1), i + j);
+      if (gate != nullptr) {
+        float da;
+        activation<T>(q[v][j], a.silu, q[v][j], da);
+        r *= q[v][j];
+      }
+      t[v][j] = a.scale != nullptr ? fmaf(io<W>::load(static_cast<const W*>(a.scale), i + j), r, x[v][j])
+                                   : x[v][j] + r;
+      ss = fmaf(t[v][j], t[v][j], ss);
+    }
+    store_piece(static_cast<T*>(a.s) + row * d, i, d, a.vec, t[v]);
+  }
+  if (a.stats != nullptr && lane == 0) a.stats[row] = i1;
+  if (a.w2 == nullptr) return;
+  const float i2 = rsqrtf(row_sum<G>(ss, red) / d + a.eps2);
+  if (a.stats != nullptr && lane == 0) a.stats[a.rows + row] = i2;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = (lane + G * v) * N;
+    if (i >= d) break;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (!a.vec && i + j >= d) break;
+      t[v][j] *= i2 * io<W>::load(static_cast<const W*>(a.w2), i + j);
+    }
+    store_piece(static_cast<T*>(a.n) + row * d, i, d, a.vec, t[v]);
+  }
+}
+
+template <typename T, typename W, int G, int NV>
+__global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
+  constexpr int N = Vec<T>::N, RW = NTH / G;
+  __shared__ float red[NTH / 64];
+  __shared__ float sums[G == 64 ? 3 * 64 * NV * N : 1];
+  const int lane = threadIdx.x % G, d = a.d;
+  float b1[NV][N] = {}, bs[NV][N] = {}, b2[NV][N] = {};  // dw1, dscale, dw2
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * RW + threadIdx.x / G; row < a.rows;
+       row += static_cast<int64_t>(gridDim.x) * RW) {
+    const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+    const T* res = static_cast<const T*>(a.res) + row * a.r_stride;
+    const T* gate = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + row * a.g_stride;
+    const T* ds = a.ds == nullptr ? nullptr : static_cast<const T*>(a.ds) + row * d;
+    const T* dn = a.dn == nullptr ? nullptr : static_cast<const T*>(a.dn) + row * d;
+    const float i1 = a.w1 == nullptr ? 1.f : a.stats[row];
+    const float i2 = dn == nullptr ? 0.f : a.stats[a.rows + row];
+    float t[NV][N], yv[NV][N], q[NV][N], dt[NV][N];
+    float dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (lane + G * v) * N;
+      if (i >= d) break;
+      load_piece(y, i, d, a.vec, yv[v]);
+      if (gate != nullptr) load_piece(gate, i, d, a.vec, q[v]);
+      if (ds != nullptr) load_piece(ds, i, d, a.vec, dt[v]);
+      else
+#pragma unroll
+        for (int j = 0; j < N; ++j) dt[v][j] = 0.f;
+      if (dn == nullptr) continue;
+      float x[N], z[N];
+      load_piece(res, i, d, a.vec, x);
+      load_piece(dn, i, d, a.vec, z);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {  // s again, u = dn w2 and u . s
+        if (!a.vec && i + j >= d) break;
+        float r = yv[v][j] * i1, act = 1.f, da;
+        if (a.w1 != nullptr) r *= io<W>::load(static_cast<const W*>(a.w1), i + j);
+        if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
+        r *= act;
+        const float s = a.scale != nullptr ? fmaf(io<W>::load(static_cast<const W*>(a.scale), i + j), r, x[j]) : x[j] + r;
+        b2[v][j] = fmaf(z[j], s * i2, b2[v][j]);
+        const float u = z[j] * io<W>::load(static_cast<const W*>(a.w2), i + j);
+        dot = fmaf(u, s, dot);
+        t[v][j] = s;
+        dt[v][j] = fmaf(i2, u, dt[v][j]);
+      }
+    }
+    if (dn != nullptr) {
+      const float m = row_sum<G>(dot, red) / d * i2 * i2 * i2;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if ((lane + G * v) * N >= d) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) dt[v][j] = fmaf(-m, t[v][j], dt[v][j]);
+      }
+    }
+    dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (lane + G * v) * N;
+      if (i >= d) break;
+      if (a.dres != nullptr) store_piece(static_cast<T*>(a.dres) + row * d, i, d, a.vec, dt[v]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (!a.vec && i + j >= d) break;
+        const float w1 = a.w1 != nullptr ? io<W>::load(static_cast<const W*>(a.w1), i + j) : 1.f;
+        const float sc = a.scale != nullptr ? io<W>::load(static_cast<const W*>(a.scale), i + j) : 1.f;
+        const float yn = yv[v][j] * i1;
+        float act = 1.f, da = 0.f;
+        if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
+        const float dr = dt[v][j] * sc * act;
+        q[v][j] = dt[v][j] * sc * (yn * w1) * da;  // dgate
+        bs[v][j] = fmaf(dt[v][j] * act, yn * w1, bs[v][j]);
+        b1[v][j] = fmaf(dr, yn, b1[v][j]);
+        dt[v][j] = dr * w1;
+        dot = fmaf(dt[v][j], yv[v][j], dot);
+      }
+      if (a.dgate != nullptr) store_piece(static_cast<T*>(a.dgate) + row * d, i, d, a.vec, q[v]);
+    }
+    float m = 0.f;
+    if (a.w1 != nullptr) m = row_sum<G>(dot, red) / d * i1 * i1 * i1;
+    if (a.dy == nullptr) continue;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (lane + G * v) * N;
+      if (i >= d) break;
+#pragma unroll
+      for (int j = 0; j < N; ++j) dt[v][j] = fmaf(-m, yv[v][j], i1 * dt[v][j]);
+      store_piece(static_cast<T*>(a.dy) + row * d, i, d, a.vec, dt[v]);
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 3 * d;
+  if constexpr (G == 64) {  // the waves' sums one after the other: the same order in every run
+    constexpr int M = 64 * NV * N;
+    for (int w = 0; w < RW; ++w) {
+      if (threadIdx.x / 64 == w) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int i = (lane + 64 * v) * N + j;
+            sums[i] = (w ? sums[i] : 0.f) + b1[v][j];
+            sums[M + i] = (w ? sums[M + i] : 0.f) + bs[v][j];
+            sums[2 * M + i] = (w ? sums[2 * M + i] : 0.f) + b2[v][j];
+          }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < d; i += NTH) {
+      out[i] = sums[i];
+      out[d + i] = sums[M + i];
+      out[2 * d + i] = sums[2 * M + i];
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = (lane + G * v) * N + j;
+        if (i >= d) continue;
+        out[i] = b1[v][j];
+        out[d + i] = bs[v][j];
+        out[2 * d + i] = b2[v][j];
+      }
+  }
+}
+
+// dw[k][i] = sum of partial[b][k][i] over the blocks: 64 columns by 4 strided shares of the blocks.
+template <typename W>
+__global__ __launch_bounds__(NTH) void weights_kernel(const float* __restrict__ partial, W* dw1, W* dscale, W* dw2,
+                                                      int blocks, int d) {
+  __shared__ float part[4][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+  float s = 0.f;
+  if (col < 3 * d)
+    for (int b = share; b < blocks; b += 4) s += partial[static_cast<int64_t>(b) * 3 * d + col];
+  part[share][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (share != 0 || col >= 3 * d) return;
+  const int k = col / d, i = col - k * d, c = threadIdx.x;
+  W* dst = k == 0 ? dw1 : k == 1 ? dscale : dw2;
+  if (dst != nullptr) io<W>::store(dst, i, (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]));
+}
+
+// A wave takes rows of up to two pieces a lane, a workgroup longer ones; at most 8 pieces a lane.
+template <typename T, typename F> int by_row(int d, F&& f) {
+  const int pieces = (d + Vec<T>::N - 1) / Vec<T>::N;
+  if (pieces <= 64) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+  if (pieces <= 128) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  if (pieces <= 256) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 1>{});
+  if (pieces <= 512) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 2>{});
+  if (pieces <= 1024) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 4>{});
+  return VMI_ERR_UNSUPPORTED;
+}
+template <typename T, typename F> int by_weight(int w_dtype, int dtype, F&& f) {
+  if (w_dtype == VMI_F32) return f(float{});
+  if (w_dtype == dtype) return f(T{});
+  return VMI_ERR_UNSUPPORTED;
+}
+bool rows_fit(int64_t d, int dtype) { return d <= (dtype == VMI_F32 ? 4096 : 8192); }
+
+// Workgroups of the backward: enough to fill the card twice over, and few enough that the partials stay small.
+int backward_blocks(int64_t rows, int64_t d, int dtype) {
+  const int per = d * (dtype == VMI_F32 ? 4 : 2) <= 2048 ? NTH / 64 : 1;
+  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, 512));
+}
+
+int check(const Args& a, int dtype, int w_dtype) {
+  if (a.rows < 0 || a.d < 1 || a.silu < 0 || a.silu > 1) return VMI_ERR_INVALID_ARG;
+  if (dtype < VMI_F32 || dtype > VMI_F16 || w_dtype < VMI_F32 || w_dtype > VMI_F16) return VMI_ERR_INVALID_ARG;
+  if (a.rows > 0 && (a.y == nullptr || a.res == nullptr)) return VMI_ERR_INVALID_ARG;
+  if (!rows_fit(a.d, dtype) || a.rows > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  return VMI_OK;
+}
+bool vectors(const Args& a, int dtype) {
+  const int n = dtype == VMI_F32 ? 4 : 8;
+  return a.d % n == 0 && a.y_stride % n == 0 && a.r_stride % n == 0 && a.g_stride % n == 0 &&
+         aligned16({a.y, a.res, a.gate, a.s, a.n, a.ds, a.dn, a.dy, a.dres, a.dgate});
+}
+
+}  // namespace gnorm
+}  // namespace vmi
+
+using namespace vmi;
+using namespace vmi::gnorm;
+
+extern "C" int vmi_gated_norm(const void* y, int64_t y_stride, const void* residual, int64_t r_stride,
+                              const void* gate, int64_t g_stride, const void* w1, const void* scale,
+                              const void* w2, int dtype, int w_dtype, int gate_act, float eps1, float eps2,
+                              void* s, void* n, float* stats, int64_t rows, int64_t d, void* stream) {
+  if (d < 1 || d > INT32_MAX) return VMI_ERR_INVALID_ARG;
+  Args a{};
+  a.y = y, a.res = residual, a.gate = gate, a.w1 = w1, a.scale = scale, a.w2 = w2;
+  a.y_stride = y_stride, a.r_stride = r_stride, a.g_stride = gate == nullptr ? 0 : g_stride;
+  a.s = s, a.n = n, a.stats = stats, a.rows = rows, a.d = static_cast<int>(d), a.silu = gate_act;
+  a.eps1 = eps1, a.eps2 = eps2;
+  if (const int st = check(a, dtype, w_dtype); st != VMI_OK) return st;
+  if (rows == 0) return VMI_OK;
+  if ((w2 != nullptr) != (n != nullptr) || s == nullptr) return VMI_ERR_INVALID_ARG;
+  a.vec = vectors(a, dtype);
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    return by_weight<T>(w_dtype, dtype, [&](auto wtag) -> int {
+      using W = decltype(wtag);
+      return by_row<T>(a.d, [&](auto g, auto nv) -> int {
+        constexpr int per = NTH / decltype(g)::value;
+        hipLaunchKernelGGL((forward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
+                           dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(NTH), 0,
+                           static_cast<hipStream_t>(stream), a);
+        return hip_status(hipGetLastError());
+      });
+    });
+  });
+}
+
+extern "C" int vmi_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t d, int dtype, size_t* bytes) {
+  if (bytes == nullptr || rows < 0 || d < 1 || dtype < VMI_F32 || dtype > VMI_F16) return VMI_ERR_INVALID_ARG;
+  if (!rows_fit(d, dtype) || rows > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  *bytes = static_cast<size_t>(std::max(1, backward_blocks(rows, d, dtype))) * 3 * d * sizeof(float);
+  return VMI_OK;
+}
+
+extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* residual, int64_t r_stride,
+                                  const void* gate, int64_t g_stride, const void* w1, const void* scale,
+                                  const void* w2, int dtype, int w_dtype, int gate_act, const float* stats,
+                                  const void* ds, const void* dn, void* dy, void* dresidual, void* dgate,
+                                  void* dw1, void* dscale, void* dw2, int64_t rows, int64_t d,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (d < 1 || d > INT32_MAX) return VMI_ERR_INVALID_ARG;
+  Args a{};
+  a.y = y, a.res = residual, a.gate = gate, a.w1 = w1, a.scale = scale, a.w2 = w2;
+  a.y_stride = y_stride, a.r_stride = r_stride, a.g_stride = gate == nullptr ? 0 : g_stride;
+  a.stats = const_cast<float*>(stats), a.ds = ds, a.dn = w2 == nullptr ? nullptr : dn;
+  a.dy = dy, a.dres = dresidual, a.dgate = gate == nullptr ? nullptr : dgate;
+  a.rows = rows, a.d = static_cast<int>(d), a.silu = gate_act;
+  if (const int st = check(a, dtype, w_dtype); st != VMI_OK) return st;
+  if (rows > 0 && stats == nullptr && (w1 != nullptr || a.dn != nullptr)) return VMI_ERR_INVALID_ARG;
+  const bool weights = dw1 != nullptr || dscale != nullptr || dw2 != nullptr;
+  const int blocks = backward_blocks(rows, d, dtype);
+  if (weights && rows > 0) {
+    size_t need = 0;
+    vmi_gated_norm_bwd_workspace_bytes(rows, d, dtype, &need);
+    if (workspace == nullptr || workspace_bytes < need) return VMI_ERR_WORKSPACE;
+    a.partial = static_cast<float*>(workspace);
+  }
+  if (rows == 0 && !weights) return VMI_OK;
+  a.vec = vectors(a, dtype);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    return by_weight<T>(w_dtype, dtype, [&](auto wtag) -> int {
+      using W = decltype(wtag);
+      int rc = VMI_OK;
+      if (rows > 0)
+        rc = by_row<T>(a.d, [&](auto g, auto nv) -> int {
+          hipLaunchKernelGGL((backward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
+                             dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, st, a);
+          return hip_status(hipGetLastError());
+        });
+      if (rc != VMI_OK || !weights) return rc;
+      hipLaunchKernelGGL(weights_kernel<W>, dim3(static_cast<unsigned>((3 * d + 63) / 64)), dim3(NTH), 0, st,
+                         a.partial, static_cast<W*>(dw1), static_cast<W*>(dscale), static_cast<W*>(dw2), blocks,
+                         a.d);
+      return hip_status(hipGetLastError());
+    });
+  });
+}

@@ -8,43 +8,18 @@
 // and by memory at prefill sizes).  Sums are fp32; where the torch ops round an intermediate tensor
 // that is itself an output or a residual stream (the sums h + x), so do these; other intermediates
 // stay fp32.
-#include <initializer_list>
-
 #include "vmi_common.h"
 #include "vmi_dispatch.h"
+#include "vmi_vec.h"
 
 namespace vmi {
 namespace layer {
-
-// 16 bytes of T
-template <typename T> struct Vec {
-  static constexpr int N = 16 / sizeof(T);
-  T e[N];
-};
-template <typename T> __device__ __forceinline__ Vec<T> ldv(const T* p) {
-  return __builtin_bit_cast(Vec<T>, *reinterpret_cast<const uint4*>(p));
-}
-template <typename T> __device__ __forceinline__ void stv(T* p, const Vec<T>& v) {
-  *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, v);
-}
-template <typename T> __device__ __forceinline__ T round_to(float x) {
-  T r;
-  io<T>::store(&r, 0, x);
-  return r;
-}
-template <typename T> __device__ __forceinline__ float rounded(float x) {
-  return io<T>::to_f32(round_to<T>(x));
-}
 
 // tanh and sigmoid: the library's for an fp32 result; for a 16-bit one on v_exp_f32 and v_rcp_f32 (a
 // few 2^-24 relative), tanh as 1 - 2 / (e^2x + 1) and below 0.1, where that cancels, the series to
 // x^5 (next term 17/315 x^6 <= 6e-8 relative): 1e-6 relative at most, against 2^-11 of the result's
 // rounding.  (tanhf, expf and three full divisions an element: the activation at [8192, 2048] bf16
 // takes 34 us, so 24.)
-template <typename T> __device__ __forceinline__ float sigmoid_for(float x) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
-  return __builtin_amdgcn_rcpf(1.f + __expf(-x));
-}
 template <typename T> __device__ __forceinline__ float tanh_for(float x) {
   if constexpr (sizeof(T) == 4) return tanhf(x);
   const float x2 = x * x;
@@ -278,17 +253,6 @@ __global__ __launch_bounds__(NTH) void halting_kernel(const T* out, const T* h, 
   }
 }
 
-template <typename F> int by_type(int dtype, F&& f) {
-  if (dtype == VMI_F32) return f(float{});
-  if (dtype == VMI_BF16) return f(bf16_t{});
-  if (dtype == VMI_F16) return f(f16_t{});
-  return VMI_ERR_INVALID_ARG;
-}
-bool aligned16(std::initializer_list<const void*> ps) {
-  for (const void* p : ps)
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
-  return true;
-}
 int elem_size(int dtype) { return dtype == VMI_F32 ? 4 : 2; }
 // a row of d elements is whole 16-byte pieces and fits the registers of a workgroup
 bool row_fits(int64_t d, int dtype) {

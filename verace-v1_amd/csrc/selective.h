@@ -1,0 +1,49 @@
+// The selective state space scan's shared pieces.
+//
+//   d_t = act(delta_t + bias),  a_t = exp(d_t A),  S_t = a_t S_{t-1} + d_t x_t B_t^T,  y_t = S_t C_t + D x_t
+//
+// per sequence b and head h, S [P, N]; heads h of a group share B and C.
+#pragma once
+
+#include "vmi_common.h"
+#include "vmi_dispatch.h"
+
+namespace vmi {
+namespace sel {
+
+struct Args {
+  const void *x, *delta, *bm, *cm;          // rows [H, P], [H], [G, N], [G, N] of token t, item b
+  int64_t x_t, x_b, d_t, d_b, b_t, b_b, c_t, c_b;  // elements between tokens and between items
+  const float *A, *D, *bias;                // [H]; D, bias may be null
+  const float* state_in;                    // [B, H, P, N] or null (zeros)
+  float* state_out;                         // or null
+  void* y;                                  // [B, T, H, P] contiguous, or null
+  const void* lengths;                      // [B] int32 or int64, or null
+  const uint8_t* mask;                      // step: [B] or null
+  int lengths64, delta_dtype, softplus;
+  int B, T, H, P, G, N;
+};
+
+__device__ __forceinline__ int length_of(const void* lengths, int lengths64, int T, int b) {
+  if (lengths == nullptr) return T;
+  const int64_t n = lengths64 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
+  return static_cast<int>(n < 0 ? 0 : n > T ? T : n);
+}
+
+// The step size: softplus(z) = max(z, 0) + log1p(exp(-|z|)) with the library's functions (a few per token
+// and head), or z itself.
+__device__ __forceinline__ float step_size(float z, int softplus) {
+  if (!softplus) return z;
+  const float m = z > 0.f ? z : z != z ? z : 0.f;
+  return m + log1pf(expf(-fabsf(z)));
+}
+// d step_size / dz
+__device__ __forceinline__ float step_slope(float z, int softplus) {
+  return softplus ? 1.f / (1.f + expf(-z)) : 1.f;
+}
+
+// selective_seq.hip: token by token, any sizes with N <= 256.
+int launch_seq(const Args& a, int dtype, hipStream_t stream);
+
+}  // namespace sel
+}  // namespace vmi

@@ -1,0 +1,77 @@
+// 16-byte pieces of a row and the dispatch on an element type, shared by the element-wise kernels.
+#pragma once
+
+#include <initializer_list>
+
+#include "vmi_common.h"
+
+namespace vmi {
+
+// 16 bytes of T
+template <typename T> struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T e[N];
+};
+template <typename T> __device__ __forceinline__ Vec<T> ldv(const T* p) {
+  return __builtin_bit_cast(Vec<T>, *reinterpret_cast<const uint4*>(p));
+}
+template <typename T> __device__ __forceinline__ void stv(T* p, const Vec<T>& v) {
+  *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, v);
+}
+template <typename T> __device__ __forceinline__ T round_to(float x) {
+  T r;
+  io<T>::store(&r, 0, x);
+  return r;
+}
+template <typename T> __device__ __forceinline__ float rounded(float x) {
+  return io<T>::to_f32(round_to<T>(x));
+}
+
+// Elements i0 .. i0 + N - 1 of a row of d as fp32, zeros past its end: one 16-byte load where the rows
+// are whole aligned pieces (vec), element loads otherwise.
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* row, int i0, int d, bool vec, float (&x)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (vec) {
+    const Vec<T> v = ldv(row + i0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = io<T>::to_f32(v.e[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = i0 + j < d ? io<T>::load(row, i0 + j) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* row, int i0, int d, bool vec, const float (&x)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (vec) {
+    Vec<T> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v.e[j] = round_to<T>(x[j]);
+    stv(row + i0, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i0 + j < d) io<T>::store(row, i0 + j, x[j]);
+  }
+}
+
+// sigmoid: the library's exp and a full division for an fp32 result, v_exp_f32 and v_rcp_f32 (a few
+// 2^-24 relative) for a 16-bit one.
+template <typename T> __device__ __forceinline__ float sigmoid_for(float x) {
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
+  return __builtin_amdgcn_rcpf(1.f + __expf(-x));
+}
+template <typename F> inline int by_type(int dtype, F&& f) {
+  if (dtype == VMI_F32) return f(float{});
+  if (dtype == VMI_BF16) return f(bf16_t{});
+  if (dtype == VMI_F16) return f(f16_t{});
+  return VMI_ERR_INVALID_ARG;
+}
+inline bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  return true;
+}
+
+}  // namespace vmi

@@ -58,6 +58,16 @@ EXPORTED = (
     "vmi_mcmoe_coef",
     "vmi_norm_add",
     "vmi_halting_update",
+    "vmi_gated_norm",
+    "vmi_gated_norm_bwd_workspace_bytes",
+    "vmi_gated_norm_bwd",
+    "vmi_short_conv",
+    "vmi_short_conv_step",
+    "vmi_short_conv_bwd_workspace_bytes",
+    "vmi_short_conv_bwd",
+    "vmi_selective_scan_workspace_bytes",
+    "vmi_selective_scan_fwd",
+    "vmi_selective_step",
 )
 
 ERR_WORKSPACE = 3  # VMI_ERR_WORKSPACE
@@ -159,6 +169,26 @@ def _declare(lib):
     lib.vmi_halting_update.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, i32, i64, i64,
                                        vp]
     lib.vmi_halting_update.restype = i32
+    psz = ctypes.POINTER(sz)
+    lib.vmi_gated_norm.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, f32, f32, vp, vp, vp, i64,
+                                   i64, vp]
+    lib.vmi_gated_norm_bwd_workspace_bytes.argtypes = [i64, i64, i32, psz]
+    lib.vmi_gated_norm_bwd.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, vp,
+                                       vp, vp, vp, i64, i64, vp, sz, vp]
+    lib.vmi_short_conv.argtypes = [vp, i64, i64, vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, i64, i64, i64, i64, vp]
+    lib.vmi_short_conv_step.argtypes = [vp, i64, vp, vp, i32, i32, i32, vp, vp, vp, i64, i64, i64, vp]
+    lib.vmi_short_conv_bwd_workspace_bytes.argtypes = [i64, i64, i64, i64, psz]
+    lib.vmi_short_conv_bwd.argtypes = [vp, i64, i64, vp, vp, i32, i32, i32, vp, vp, i32, vp, i64, i64, vp, vp, vp, vp,
+                                       vp, i64, i64, i64, i64, vp, sz, vp]
+    lib.vmi_selective_scan_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i32, psz]
+    lib.vmi_selective_scan_fwd.argtypes = [vp, i64, i64, vp, i64, i64, i32, vp, vp, i64, i64, vp, i64, i64, vp, vp,
+                                           i32, i32, vp, vp, i32, vp, vp, i64, i64, i64, i64, i64, i64, vp, sz, vp]
+    lib.vmi_selective_step.argtypes = [vp, i64, vp, i64, i32, vp, vp, i64, vp, i64, vp, vp, i32, i32, vp, vp, vp, i64,
+                                       i64, i64, i64, i64, vp]
+    for name in ("gated_norm", "gated_norm_bwd_workspace_bytes", "gated_norm_bwd", "short_conv", "short_conv_step",
+                 "short_conv_bwd_workspace_bytes", "short_conv_bwd", "selective_scan_workspace_bytes",
+                 "selective_scan_fwd", "selective_step"):
+        getattr(lib, "vmi_" + name).restype = i32
 
 
 def load(path: str = LIB_PATH):

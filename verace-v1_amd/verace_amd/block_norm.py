@@ -1,0 +1,134 @@
+"""The norms either side of a block fused with its gate and residual scale (``csrc/gated_norm.hip``),
+differentiable: the training form of what :func:`verace_amd.layer_ops.norm_add` does between a layer's
+sub-blocks in inference, with a gate and a per-channel residual scale."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .hip_kernels import _ptr, _require_device, device_guard
+
+_ACT = {"sigmoid": 0, "silu": 1}
+
+
+def _rows(t: Optional[torch.Tensor], d: int) -> Optional[torch.Tensor]:
+    """t as [rows, d] with contiguous rows (a view where its rows lie at one stride)."""
+    if t is None:
+        return None
+    t = t.reshape(-1, d)
+    return t if t.stride(1) == 1 or d == 1 else t.contiguous()
+
+
+def _launch(y, residual, gate, w1, scale, w2, eps1, eps2, act, want_stats):
+    d = y.shape[-1]
+    y2, r2, g2 = _rows(y, d), _rows(residual, d), _rows(gate, d)
+    s = torch.empty(y.shape, device=y.device, dtype=y.dtype)
+    n = None if w2 is None else torch.empty_like(s)
+    stats = torch.empty(2, y2.shape[0], device=y.device, dtype=torch.float32) if want_stats else None
+    w = next((t for t in (w1, scale, w2) if t is not None), None)
+    with device_guard(y):
+        _lib.check(_lib.load().vmi_gated_norm(
+            _ptr(y2), y2.stride(0), _ptr(r2), r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), _ptr(w1),
+            _ptr(scale), _ptr(w2), _lib.dtype_code(y.dtype), _lib.dtype_code(y.dtype if w is None else w.dtype), act,
+            eps1, eps2, _ptr(s), _ptr(n), _ptr(stats), y2.shape[0], d, _lib.stream_handle(y.device)), "vmi_gated_norm")
+    return s, n, stats
+
+
+class GatedNormFunction(torch.autograd.Function):
+    """:func:`gated_norm_add` as an autograd node (the inputs and two fp32 numbers a row are kept)."""
+
+    @staticmethod
+    def forward(ctx, y, residual, gate, w1, scale, w2, eps1, eps2, act):
+        s, n, stats = _launch(y, residual, gate, w1, scale, w2, eps1, eps2, act, True)
+        ctx.save_for_backward(y, residual, gate, w1, scale, w2, stats)
+        ctx.act = act
+        ctx.set_materialize_grads(False)
+        return s, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, ds, dn):
+        y, residual, gate, w1, scale, w2, stats = ctx.saved_tensors
+        d = y.shape[-1]
+        y2, r2, g2 = _rows(y, d), _rows(residual, d), _rows(gate, d)
+        ds, dn = (None if t is None else t.contiguous() for t in (ds, dn))
+        need = ctx.needs_input_grad
+        dy, dres, dgate = (torch.empty(y.shape, device=y.device, dtype=y.dtype) if f and t is not None else None
+                           for f, t in zip(need[:3], (y, residual, gate)))
+        dw1, dscale, dw2 = (torch.empty_like(t) if f and t is not None else None
+                            for f, t in zip(need[3:6], (w1, scale, w2)))
+        w = next((t for t in (w1, scale, w2) if t is not None), None)
+        code = _lib.dtype_code(y.dtype)
+        lib = _lib.load()
+        ws, ws_bytes = None, ctypes.c_size_t(0)
+        if not (dw1 is None and dscale is None and dw2 is None):
+            _lib.check(lib.vmi_gated_norm_bwd_workspace_bytes(y2.shape[0], d, code, ctypes.byref(ws_bytes)),
+                       "vmi_gated_norm_bwd_workspace_bytes")
+            ws = torch.empty(ws_bytes.value, device=y.device, dtype=torch.uint8)
+        with device_guard(y):
+            _lib.check(lib.vmi_gated_norm_bwd(
+                _ptr(y2), y2.stride(0), _ptr(r2), r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), _ptr(w1),
+                _ptr(scale), _ptr(w2), code, _lib.dtype_code(y.dtype if w is None else w.dtype), ctx.act, _ptr(stats),
+                _ptr(ds), _ptr(dn), _ptr(dy), _ptr(dres), _ptr(dgate), _ptr(dw1), _ptr(dscale), _ptr(dw2),
+                y2.shape[0], d, _ptr(ws), ws_bytes.value, _lib.stream_handle(y.device)), "vmi_gated_norm_bwd")
+        return dy, dres, dgate, dw1, dscale, dw2, None, None, None
+
+
+def gated_norm_add(
+    y: torch.Tensor,
+    residual: torch.Tensor,
+    norm_weight: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+    scale: Optional[torch.Tensor] = None,
+    next_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    next_eps: Optional[float] = None,
+    activation: str = "silu",
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``s = residual + scale * act(gate) * rmsnorm(y; norm_weight, eps)`` and
+    ``n = rmsnorm(s; next_weight, next_eps)`` in one pass over the rows: (s, n), n None without
+    ``next_weight``.
+
+    y, residual: [..., d] of one shape and dtype (rows may be slices of a wider tensor); gate: the same,
+    or broadcastable to it, through ``activation`` ("silu" or "sigmoid"); norm_weight, scale, next_weight:
+    [d], all in y's dtype or all float32.  Each may be None and is then left out of the formula.
+    d <= 8192 (float32: 4096).  Arithmetic is fp32 and each result is rounded once; n is formed from the
+    unrounded s.  Differentiable once, in every tensor argument.
+    """
+    _require_device(y, "y")
+    if y.dim() < 1 or y.shape[-1] < 1:
+        raise RuntimeError(f"verace_amd: y must be [..., d], got {tuple(y.shape)}")
+    _lib.dtype_code(y.dtype)
+    d = y.shape[-1]
+    if d > (4096 if y.dtype == torch.float32 else 8192):
+        raise RuntimeError(f"verace_amd: rows of {d} {y.dtype} elements are too long for gated_norm_add")
+    if activation not in _ACT:
+        raise RuntimeError(f"verace_amd: activation must be one of {tuple(_ACT)}, got {activation!r}")
+    if residual.shape != y.shape:
+        raise RuntimeError(f"verace_amd: residual shape {tuple(residual.shape)} != y shape {tuple(y.shape)}")
+    if gate is not None and gate.shape != y.shape:
+        try:
+            gate = gate.expand(y.shape)
+        except RuntimeError:
+            raise RuntimeError(f"verace_amd: gate {tuple(gate.shape)} does not broadcast to {tuple(y.shape)}") from None
+    for name, t in (("residual", residual), ("gate", gate)):
+        if t is not None and (t.dtype != y.dtype or t.device != y.device):
+            raise RuntimeError(f"verace_amd: {name} must be {y.dtype} on {y.device}, got {t.dtype} on {t.device}")
+    ws = []
+    for name, t in (("norm_weight", norm_weight), ("scale", scale), ("next_weight", next_weight)):
+        if t is not None:
+            if tuple(t.shape) != (d,) or t.device != y.device or t.dtype not in (y.dtype, torch.float32):
+                raise RuntimeError(f"verace_amd: {name} must be [{d}] {y.dtype} or float32 on {y.device}, "
+                                   f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+            ws.append(t)
+    if len({t.dtype for t in ws}) > 1:
+        raise RuntimeError("verace_amd: norm_weight, scale and next_weight must have one dtype")
+    w1, sc, w2 = (None if t is None else t.contiguous() for t in (norm_weight, scale, next_weight))
+    eps1, eps2 = float(eps), float(eps if next_eps is None else next_eps)
+    act = _ACT[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, residual, gate, w1, sc, w2)):
+        return GatedNormFunction.apply(y, residual, gate, w1, sc, w2, eps1, eps2, act)
+    return _launch(y, residual, gate, w1, sc, w2, eps1, eps2, act, False)[:2]

@@ -15,6 +15,7 @@ a missing library or a failing call raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Tuple
@@ -45,6 +46,14 @@ def _mask_bytes(mask: torch.Tensor) -> torch.Tensor:
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(t: torch.Tensor):
+    """A context in which kernels are launched on t's device (nothing where it is the current one)."""
+    return _NO_GUARD if on_current_device(t) else torch.cuda.device(t.device)
 
 
 def launch_sssd_hip_scan(

@@ -1,0 +1,329 @@
+"""The selective state space scan and its short causal convolution on the gfx950 kernels
+(``csrc/selective*.hip``, ``csrc/short_conv.hip``): prompts, training and in-place single tokens.
+
+    z_t = bias + sum_j w_j x_{t - (K - 1) + j},  short_conv = act(z)
+    d_t = softplus(delta_t + delta_bias),  S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T,  y_t = S_t C_t + D x_t
+
+The recurrence beside the SSSD scan (:func:`verace_amd.sssd_scan`): the same [batch, time, heads, dim]
+layouts, fp32 states handed from call to call, a differentiable scan and an opt-in in-place step.  Every
+launcher enqueues on the current HIP stream of its tensors' device and allocates outputs and workspace
+from torch's caching allocator.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .hip_kernels import _mask_bytes, _ptr, _require_device, device_guard
+
+_ACT = {None: 0, "silu": 1}
+
+
+def _same_device(like: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise RuntimeError(f"verace_amd: {name} must be on {like.device}, got {t.device}")
+
+
+def _lengths(lengths: Optional[torch.Tensor], B: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    if lengths is None:
+        return None
+    if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"verace_amd: lengths must be [{B}] int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+    _same_device(like, lengths=lengths)
+    return lengths.contiguous()
+
+
+def _inner(t: torch.Tensor, lead: int) -> torch.Tensor:
+    """t with everything after its first ``lead`` dimensions contiguous (a copy only if it is not)."""
+    expect = 1
+    for size, stride in zip(reversed(t.shape[lead:]), reversed(t.stride()[lead:])):
+        if size != 1 and stride != expect:
+            return t.contiguous()
+        expect *= size
+    return t
+
+
+# ------------------------------------------------------------------------------------ short convolution
+
+def _conv_check(x, weight, bias, activation):
+    _require_device(x, "x")
+    _lib.dtype_code(x.dtype)
+    C = x.shape[-1]
+    if activation not in _ACT:
+        raise RuntimeError(f"verace_amd: activation must be None or 'silu', got {activation!r}")
+    if weight.dim() != 2 or weight.shape[0] != C or not 2 <= weight.shape[1] <= 4:
+        raise RuntimeError(f"verace_amd: weight must be [{C}, 2 .. 4], got {tuple(weight.shape)}")
+    if bias is not None and (tuple(bias.shape) != (C,) or bias.dtype != weight.dtype):
+        raise RuntimeError(f"verace_amd: bias must be [{C}] {weight.dtype}, got {tuple(bias.shape)} {bias.dtype}")
+    _lib.dtype_code(weight.dtype)
+    _same_device(x, weight=weight, bias=bias)
+
+
+def _launch_conv(x, weight, bias, state, lengths, act):
+    B, T, C = x.shape
+    K = weight.shape[1]
+    x, w = _inner(x, 2), weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
+    out = torch.empty(B, K - 1, C, device=x.device, dtype=x.dtype)
+    with device_guard(x):
+        _lib.check(_lib.load().vmi_short_conv(
+            _ptr(x), x.stride(1), x.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), act,
+            _ptr(state), _ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), _ptr(y), _ptr(out),
+            B, T, C, K, _lib.stream_handle(x.device)), "vmi_short_conv")
+    return y, out
+
+
+class ShortConvFunction(torch.autograd.Function):
+    """:func:`short_conv` as an autograd node (only its inputs are kept)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, act):
+        y, out = _launch_conv(x, weight, bias, state, lengths, act)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.act = act
+        ctx.set_materialize_grads(False)
+        return y, out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dout):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        B, T, C = x.shape
+        K = weight.shape[1]
+        x, w = _inner(x, 2), weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        dy = None if dy is None else _inner(dy, 2)
+        dout = None if dout is None else dout.contiguous()
+        need = ctx.needs_input_grad
+        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype) if need[0] else None
+        dw = torch.empty_like(w) if need[1] else None
+        db = torch.empty_like(b) if b is not None and need[2] else None
+        dstate = torch.empty_like(state) if state is not None and need[3] else None
+        lib = _lib.load()
+        ws, ws_bytes = None, ctypes.c_size_t(0)
+        if not (dw is None and db is None):
+            _lib.check(lib.vmi_short_conv_bwd_workspace_bytes(B, T, C, K, ctypes.byref(ws_bytes)),
+                       "vmi_short_conv_bwd_workspace_bytes")
+            ws = torch.empty(max(1, ws_bytes.value), device=x.device, dtype=torch.uint8)
+        with device_guard(x):
+            _lib.check(lib.vmi_short_conv_bwd(
+                _ptr(x), x.stride(1), x.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype),
+                ctx.act, _ptr(state), _ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), _ptr(dy),
+                0 if dy is None else dy.stride(1), 0 if dy is None else dy.stride(0), _ptr(dout), _ptr(dx), _ptr(dw),
+                _ptr(db), _ptr(dstate), B, T, C, K, _ptr(ws), ws_bytes.value, _lib.stream_handle(x.device)),
+                "vmi_short_conv_bwd")
+        return dx, dw, db, dstate, None, None
+
+
+def short_conv(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    initial_state: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+    activation: Optional[str] = "silu",
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Causal depthwise convolution over time, differentiable once.
+
+    x: [batch, seq_len, C] (rows may be slices of a wider projection); weight: [C, K], K = 2 .. 4,
+    weight[:, K - 1] on the current token; bias: [C]; initial_state: the K - 1 rows before the first,
+    [batch, K - 1, C] in x's dtype (zeros when None, never modified); lengths: [batch] on x's device,
+    how many of a right-padded sequence's rows count (values outside 0 .. seq_len are clamped); activation
+    "silu" or None.  Returns (y [batch, seq_len, C], the last K - 1 counted rows [batch, K - 1, C]); y
+    behind a sequence's length is 0 and x there is not read.
+    """
+    if x.dim() != 3:
+        raise RuntimeError(f"verace_amd: x must be [B, T, C], got {tuple(x.shape)}")
+    _conv_check(x, weight, bias, activation)
+    B, T, C = x.shape
+    lengths = _lengths(lengths, B, x)
+    state = initial_state
+    if state is not None:
+        if tuple(state.shape) != (B, weight.shape[1] - 1, C) or state.dtype != x.dtype:
+            raise RuntimeError(f"verace_amd: initial_state must be {(B, weight.shape[1] - 1, C)} {x.dtype}, "
+                               f"got {tuple(state.shape)} {state.dtype}")
+        _same_device(x, initial_state=state)
+        state = state.contiguous()
+    act = _ACT[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
+        return ShortConvFunction.apply(x, weight, bias, state, lengths, act)
+    return _launch_conv(x, weight, bias, state, lengths, act)
+
+
+def short_conv_step_(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor],
+    state: torch.Tensor,
+    activation: Optional[str] = "silu",
+    active_mask: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """One token of :func:`short_conv` per item with the state [batch, K - 1, C] (contiguous, x's dtype)
+    moved up a row in place.  x: [batch, 1, C] or [batch, C].  Items whose ``active_mask`` [batch] is off
+    keep their state and give zeros.  Returns y [batch, 1, C].  Not differentiable."""
+    _conv_check(x, weight, bias, activation)
+    B, K1, C = state.shape if state.dim() == 3 else (-1, -1, -1)
+    if K1 != weight.shape[1] - 1 or C != x.shape[-1] or state.dtype != x.dtype or not state.is_contiguous():
+        raise RuntimeError(f"verace_amd: state must be a contiguous [B, {weight.shape[1] - 1}, {x.shape[-1]}] {x.dtype} "
+                           f"tensor, got {tuple(state.shape)} {state.dtype}")
+    if tuple(x.shape) not in ((B, 1, C), (B, C)):
+        raise RuntimeError(f"verace_amd: x must hold one token for each of {B} items, got {tuple(x.shape)}")
+    _same_device(x, state=state, active_mask=active_mask)
+    x2 = _inner(x.reshape(B, C), 1)
+    mask = None if active_mask is None else _mask_bytes(active_mask.reshape(B))
+    w = weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    y = torch.empty(B, 1, C, device=x.device, dtype=x.dtype)
+    with device_guard(x):
+        _lib.check(_lib.load().vmi_short_conv_step(
+            _ptr(x2), x2.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), _ACT[activation],
+            _ptr(mask), _ptr(state), _ptr(y), B, C, K1 + 1, _lib.stream_handle(x.device)), "vmi_short_conv_step")
+    return y
+
+
+# ------------------------------------------------------------------------------------ selective scan
+
+def _head_vector(t: Optional[torch.Tensor], H: int, name: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if tuple(t.shape) != (H,):
+        raise RuntimeError(f"verace_amd: {name} must be [{H}], got {tuple(t.shape)}")
+    return t.to(torch.float32).contiguous()
+
+
+def _scan_check(x, delta, A, Bm, Cm, D, delta_bias):
+    """Shapes of x [B, T, H, P], delta [B, T, H], Bm, Cm [B, T, G, N]: (B, T, H, P, G, N)."""
+    _require_device(x, "x")
+    _lib.dtype_code(x.dtype)
+    if x.dim() != 4:
+        raise RuntimeError(f"verace_amd: x must be [B, T, H, P], got {tuple(x.shape)}")
+    B, T, H, P = x.shape
+    if delta.dim() == 4 and delta.shape[-1] == 1:
+        delta = delta.squeeze(-1)
+    if tuple(delta.shape) != (B, T, H):
+        raise RuntimeError(f"verace_amd: delta must be [B, T, H] = {(B, T, H)}, got {tuple(delta.shape)}")
+    if Bm.dim() != 4 or Bm.shape[:2] != x.shape[:2] or Cm.shape != Bm.shape:
+        raise RuntimeError(f"verace_amd: B and C must be [B, T, G, N], got {tuple(Bm.shape)}, {tuple(Cm.shape)}")
+    G, N = Bm.shape[2:]
+    if G < 1 or H % G != 0:
+        raise RuntimeError(f"verace_amd: {H} heads do not share {G} groups of B and C")
+    if not 1 <= N <= 256 or not 1 <= P <= 1024:
+        raise RuntimeError(f"verace_amd: built for head sizes 1 .. 1024 and state sizes 1 .. 256, got {P}, {N}")
+    if Bm.dtype != x.dtype or Cm.dtype != x.dtype:
+        raise RuntimeError(f"verace_amd: B and C must be {x.dtype}, got {Bm.dtype}, {Cm.dtype}")
+    _lib.dtype_code(delta.dtype)
+    _same_device(x, delta=delta, A=A, B=Bm, C=Cm, D=D, delta_bias=delta_bias)
+    return B, T, H, P, G, N
+
+
+def launch_selective_hip_scan(
+    x: torch.Tensor,
+    delta: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: Optional[torch.Tensor] = None,
+    delta_bias: Optional[torch.Tensor] = None,
+    softplus: bool = True,
+    initial_state: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`selective_scan` without autograd."""
+    b, T, H, P, G, N = _scan_check(x, delta, A, B, C, D, delta_bias)
+    lengths = _lengths(lengths, b, x)
+    if delta.dim() == 4:
+        delta = delta.squeeze(-1)
+    A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
+    state = initial_state
+    if state is not None:
+        if tuple(state.shape) != (b, H, P, N):
+            raise RuntimeError(f"verace_amd: initial_state must be {(b, H, P, N)}, got {tuple(state.shape)}")
+        _same_device(x, initial_state=state)
+        state = state.to(torch.float32).contiguous()
+    x, delta, B, C = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2)
+    y = torch.empty(b, T, H, P, device=x.device, dtype=x.dtype)
+    out = torch.empty(b, H, P, N, device=x.device, dtype=torch.float32)
+    code = _lib.dtype_code(x.dtype)
+    lib = _lib.load()
+    ws_bytes = ctypes.c_size_t(0)
+    _lib.check(lib.vmi_selective_scan_workspace_bytes(b, T, H, P, G, N, code, ctypes.byref(ws_bytes)),
+               "vmi_selective_scan_workspace_bytes")
+    ws = torch.empty(ws_bytes.value, device=x.device, dtype=torch.uint8) if ws_bytes.value else None
+    with device_guard(x):
+        _lib.check(lib.vmi_selective_scan_fwd(
+            _ptr(x), x.stride(1), x.stride(0), _ptr(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
+            _ptr(A), _ptr(B), B.stride(1), B.stride(0), _ptr(C), C.stride(1), C.stride(0), _ptr(D), _ptr(bias),
+            int(bool(softplus)), code, _ptr(state), _ptr(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), _ptr(y), _ptr(out), b, T, H, P, G, N, _ptr(ws),
+            ws_bytes.value, _lib.stream_handle(x.device)), "vmi_selective_scan_fwd")
+    return y, out
+
+
+def selective_scan(
+    x: torch.Tensor,
+    delta: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: Optional[torch.Tensor] = None,
+    delta_bias: Optional[torch.Tensor] = None,
+    softplus: bool = True,
+    initial_state: Optional[torch.Tensor] = None,
+    lengths: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Selective state space scan.
+
+    x: [batch, seq_len, num_heads, head_dim]; delta: [batch, seq_len, num_heads] (any of the three
+    dtypes); A: [num_heads] decay rates (negative for a decaying state); B, C: [batch, seq_len, groups, N]
+    in x's dtype, a group shared by num_heads / groups consecutive heads; D, delta_bias: [num_heads];
+    softplus: whether the step size is softplus(delta + delta_bias) or that sum itself; initial_state:
+    [batch, num_heads, head_dim, N], zeros when None (never modified); lengths: [batch] on x's device, how
+    many of a right-padded sequence's tokens count (values outside 0 .. seq_len are clamped).  x, delta, B
+    and C may be slices of wider rows.  head_dim <= 1024, N <= 256.  Returns (y in x's dtype, final_state
+    float32); y behind a sequence's length is 0 and nothing of the inputs there is used.
+    """
+    return launch_selective_hip_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
+
+
+def selective_step_(
+    x: torch.Tensor,
+    delta: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    state: torch.Tensor,
+    D: Optional[torch.Tensor] = None,
+    delta_bias: Optional[torch.Tensor] = None,
+    softplus: bool = True,
+    active_mask: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """One token of :func:`selective_scan` per item with ``state`` [batch, num_heads, head_dim, N] (float32,
+    contiguous) updated in place.  x: [batch, 1, num_heads, head_dim] and delta, B, C alike, or all without
+    the time dimension.  Items whose ``active_mask`` [batch] is off keep their state and give zeros.
+    Returns y [batch, 1, num_heads, head_dim].  Only for callers that own the state; not differentiable."""
+    if x.dim() == 3:
+        x, delta, B, C = x.unsqueeze(1), delta.unsqueeze(1), B.unsqueeze(1), C.unsqueeze(1)
+    b, T, H, P, G, N = _scan_check(x, delta, A, B, C, D, delta_bias)
+    if T != 1:
+        raise RuntimeError(f"verace_amd: selective_step_ takes one token per item, got {T}")
+    if delta.dim() == 4:
+        delta = delta.squeeze(-1)
+    if tuple(state.shape) != (b, H, P, N) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise RuntimeError(f"verace_amd: state must be a contiguous float32 {(b, H, P, N)} tensor, "
+                           f"got {tuple(state.shape)} {state.dtype}")
+    _same_device(x, state=state, active_mask=active_mask)
+    A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
+    x, delta, B, C = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2)
+    mask = None if active_mask is None else _mask_bytes(active_mask.reshape(b))
+    y = torch.empty(b, 1, H, P, device=x.device, dtype=x.dtype)
+    with device_guard(x):
+        _lib.check(_lib.load().vmi_selective_step(
+            _ptr(x), x.stride(0), _ptr(delta), delta.stride(0), _lib.dtype_code(delta.dtype), _ptr(A), _ptr(B),
+            B.stride(0), _ptr(C), C.stride(0), _ptr(D), _ptr(bias), int(bool(softplus)), _lib.dtype_code(x.dtype),
+            _ptr(mask), _ptr(state), _ptr(y), b, H, P, G, N, _lib.stream_handle(x.device)), "vmi_selective_step")
+    return y
