@@ -19,7 +19,7 @@ extern "C" int vmi_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t 
                                                   int dtype, size_t* bytes) {
   if (bytes == nullptr) return VMI_ERR_INVALID_ARG;
   if (const int st = check(B, T, H, P, G, N, dtype, VMI_F32); st != VMI_OK) return st;
-  *bytes = 0;
+  *bytes = chunk_workspace_bytes(B, T, H, P, N, dtype);
   return VMI_OK;
 }
 
@@ -42,7 +42,9 @@ extern "C" int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, c
   a.delta_dtype = delta_dtype, a.softplus = softplus;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.H = static_cast<int>(H), a.P = static_cast<int>(P);
   a.G = static_cast<int>(G), a.N = static_cast<int>(N);
-  return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
+  if (!use_chunk(T)) return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
+  if (workspace == nullptr || workspace_bytes < chunk_workspace_bytes(B, T, H, P, N, dtype)) return VMI_ERR_WORKSPACE;
+  return launch_chunk(a, dtype, workspace, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_b, int delta_dtype,

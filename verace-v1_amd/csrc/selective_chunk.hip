@@ -1,0 +1,432 @@
+// Chunked selective scan on the matrix cores.
+//
+// Over a chunk of L tokens with log decays c_t = A (d_1 + .. + d_t) from its start, S_0 the state there:
+//   y_t = sum_{s<=t} (C_t . B_s) e^{c_t - c_s} d_s x_s + e^{c_t} S_0 C_t + D x_t
+//   S_L = e^{c_L} S_0 + sum_s e^{c_L - c_s} d_s x_s B_s^T
+// Every exponent is a difference of one chunk, so nothing overflows that the recurrence would not.
+//
+// Launches (Sg segments of the chunks, picked by plan()):
+//   prep_kernel                d_t and c_t of every chunk (a wave each; c in fp64, kept as two floats);
+//   pass_kernel<READOUT=false> (Sg > 1) each segment's own state from zero;
+//   carry_kernel               (Sg > 1) the segments' start states;
+//   pass_kernel<READOUT=true>  every segment from its start state, with outputs.
+//
+// A workgroup of four waves takes 64 rows p of one head and walks a segment's chunks with S^T [N, 64] in
+// accumulators, 16 rows p a wave; x, B, C of the next chunk are on their way meanwhile.  S^T is directly
+// the operand of S_0 C_t.  The scores of a chunk are shared: each wave forms some of the 16 x 16 tiles on
+// or below the diagonal, and they pass through LDS as fragments.
+// With bf16 inputs the decayed scores and the carried state are rounded to bf16 where they enter y's
+// products (2^-8 of a term at most, as y's own rounding); the weighted x of the state's update enters as
+// three bf16 parts, so the state itself is carried in fp32 throughout.
+#include <algorithm>
+#include <type_traits>
+
+#include "selective_mfma.h"
+#include "vmi_vec.h"
+
+namespace vmi {
+namespace sel {
+
+constexpr int NTH = 256;
+constexpr int PB = 64;       // rows p of a workgroup
+constexpr int MAX_SEG = 64;
+
+struct Chunks {
+  Args a;
+  const float* d;            // [BH][Tp]
+  const float2* c;           // [BH][Tp]
+  float* seg_state;          // [Sg][BH][P][N]: a segment's own state, then its start state
+  float* seg_decay;          // [Sg][BH]
+  int nch, seg_chunks, nseg, pblocks;
+  bool vec_x, vec_bc, vec_state, vec_y;
+};
+
+// ------------------------------------------------------------------ step sizes and log decays
+template <int L>
+__global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d_out, float2* __restrict__ c_out,
+                                                   int nch, int64_t units) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (NTH / L) + threadIdx.x / L;
+  if (unit >= units) return;
+  const int l = threadIdx.x % L;
+  // heads fastest: neighbouring chunks of threads read neighbouring heads of the same tokens
+  const int h = static_cast<int>(unit % a.H);
+  const int64_t bc = unit / a.H;
+  const int b = static_cast<int>(bc / nch), n = static_cast<int>(bc - static_cast<int64_t>(b) * nch), t = n * L + l;
+  float d = 0.f;
+  if (t < length_of(a.lengths, a.lengths64, a.T, b))
+    d = step_size(load_scalar(a.delta, a.delta_dtype, b * a.d_b + t * a.d_t + h) + (a.bias == nullptr ? 0.f : a.bias[h]),
+                  a.softplus);
+  double c = static_cast<double>(d) * static_cast<double>(a.A[h]);
+#pragma unroll
+  for (int off = 1; off < L; off <<= 1) {
+    const double up = __shfl_up(c, off, L);
+    if (l >= off) c += up;
+  }
+  const int64_t o = (static_cast<int64_t>(b) * a.H + h) * (static_cast<int64_t>(nch) * L) + t;
+  const float hi = static_cast<float>(c);
+  d_out[o] = d;
+  // an infinite or NaN sum has no low part
+  c_out[o] = make_float2(hi, __builtin_isfinite(hi) ? static_cast<float>(c - static_cast<double>(hi)) : 0.f);
+}
+
+// ------------------------------------------------------------------ the segments
+// Score tiles (t-tile, s-tile) on or below the diagonal, dealt to the waves.
+template <int L> struct Tiles;
+template <> struct Tiles<64> {
+  static constexpr int PER = 3;
+  static __device__ __forceinline__ bool get(int wave, int i, int& tt, int& st) {
+    constexpr uint32_t T[4] = {0x00'31'30, 0x10'33'32, 0x11'21'20, 0xff'ff'22};
+    const uint32_t q = (T[wave] >> (8 * i)) & 0xff;
+    tt = q >> 4, st = q & 15;
+    return q != 0xff;
+  }
+};
+template <> struct Tiles<32> {
+  static constexpr int PER = 1;
+  static __device__ __forceinline__ bool get(int wave, int, int& tt, int& st) {
+    tt = wave != 0, st = wave == 2;
+    return wave < 3;
+  }
+};
+
+template <typename IO, typename E, int NP, int L, bool READOUT>
+__global__ __launch_bounds__(NTH) void pass_kernel(Chunks k) {
+  constexpr int NT = NP / 16, LT = L / 16, KB = L / 32, KN = NP / 32, NPART = Parts<E>::N;
+  typedef Tile<E, NP> TB;
+  typedef Tile<E, PB> TX;
+  __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Cs[READOUT ? TB::elems(L) : 8];
+  __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Ms[READOUT ? LT * KB * 64 * 8 : 8];
+  __shared__ __attribute__((aligned(16))) float2 cs[L];
+  __shared__ __attribute__((aligned(16))) float ds[L], ws[L];
+  const Args& a = k.a;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  // neighbouring workgroups go to different XCDs: give each XCD a run of consecutive heads, which share B and C
+  const uint32_t total = gridDim.x, per = total / 8, body = per * 8;
+  uint32_t id = blockIdx.x;
+  if (id < body) id = (id & 7) * per + (id >> 3);
+  const int pb = id % k.pblocks;
+  const int rest = id / k.pblocks;
+  const int seg = rest / a.H % k.nseg, h = rest % a.H, b = rest / (a.H * k.nseg);
+  if (!READOUT && seg == k.nseg - 1) return;  // nothing starts from its state
+  const int64_t bh = static_cast<int64_t>(b) * a.H + h;
+  const int p0 = pb * PB, pw = p0 + 16 * wave, grp = h / (a.H / a.G);
+  const int len = length_of(a.lengths, a.lengths64, a.T, b);
+  const int c0 = seg * k.seg_chunks, c1 = min(min(k.nch, c0 + k.seg_chunks), (len + L - 1) / L);
+  const bool live = pw < a.P;  // this wave has rows
+  const IO* x = static_cast<const IO*>(a.x) + b * a.x_b + static_cast<int64_t>(h) * a.P + p0;
+  const IO* bm = static_cast<const IO*>(a.bm) + b * a.b_b + static_cast<int64_t>(grp) * a.N;
+  const IO* cm = static_cast<const IO*>(a.cm) + b * a.c_b + static_cast<int64_t>(grp) * a.N;
+  const int64_t tp = static_cast<int64_t>(k.nch) * L;
+  const float* dp = k.d + bh * tp;
+  const float2* cp = k.c + bh * tp;
+
+  Stage<IO, E, PB, L, NTH> sx;
+  Stage<IO, E, NP, L, NTH> sb, sc;
+  float rd = 0.f;
+  float2 rc = make_float2(0.f, 0.f), rl = rc;
+  auto fetch = [&](int c) {
+    sx.fetch(x, a.x_t, c * L, len, a.P - p0, k.vec_x);
+    sb.fetch(bm, a.b_t, c * L, len, a.N, k.vec_bc);
+    if constexpr (READOUT) sc.fetch(cm, a.c_t, c * L, len, a.N, k.vec_bc);
+    if (tid < L) {
+      rd = dp[c * L + tid];
+      rc = cp[c * L + tid];
+      rl = cp[c * L + L - 1];
+    }
+  };
+  if (c0 < c1) fetch(c0);
+
+  // S^T: tile j, register r = state column n = 16 j + 4 g + r of row p = pw + l16
+  f32x4 S[NT];
+  {
+    const float* src = nullptr;
+    if (READOUT) {
+      if (seg > 0) src = k.seg_state + (static_cast<int64_t>(seg) * a.B * a.H + bh) * a.P * a.N;
+      else if (a.state_in != nullptr) src = a.state_in + bh * a.P * a.N;
+    }
+    const int p = pw + l16;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int n = 16 * j + 4 * g;
+      S[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (src == nullptr || p >= a.P || n >= a.N) continue;
+      const float* q = src + static_cast<int64_t>(p) * a.N + n;
+      if (k.vec_state) {
+        S[j] = *reinterpret_cast<const f32x4*>(q);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < a.N) S[j][r] = q[r];
+      }
+    }
+  }
+  if constexpr (READOUT) {  // the tiles right of the diagonal that a block of 32 reads stay zero
+    for (int i = tid; i < LT * KB * 64 * 8; i += NTH) Ms[i] = static_cast<E>(0.f);
+  }
+  const float Dh = a.D == nullptr ? 0.f : a.D[h];
+  double seg_c = 0.0;
+
+  for (int c = c0; c < c1; ++c) {
+    lds_barrier();  // the last chunk's readers are done
+    sx.commit(Xs);
+    sb.commit(Bs);
+    if constexpr (READOUT) sc.commit(Cs);
+    if (tid < L) {
+      cs[tid] = rc;
+      ds[tid] = rd;
+      ws[tid] = rd * decay(rl, rc);
+    }
+    lds_barrier();
+    if (c + 1 < c1) fetch(c + 1);
+
+    f32x4 acc[LT];
+    if constexpr (READOUT) {
+      // scores, transposed (rows s, column t): (C_t . B_s) e^{c_t - c_s} d_s
+#pragma unroll
+      for (int i = 0; i < Tiles<L>::PER; ++i) {
+        int tt, st;
+        if (!Tiles<L>::get(wave, i, tt, st)) continue;
+        f32x4 m = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KN; ++kb)
+          m = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), row_frag<E, NP>(Cs, 16 * tt, 32 * kb, l16, g), m);
+        const float2 ct = cs[16 * tt + l16];
+        struct alignas(8) M4 { E e[4]; } q;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int s = 16 * st + 4 * g + r;
+          const float v = m[r] * (decay(ct, cs[s]) * ds[s]);
+          q.e[r] = static_cast<E>(s <= 16 * tt + l16 ? v : 0.f);
+        }
+        *reinterpret_cast<M4*>(Ms + ((tt * KB + (st >> 1)) * 64 + lane) * 8 + 4 * (st & 1)) = q;
+      }
+      // S_0 C_t, transposed: rows p, column t
+#pragma unroll
+      for (int t = 0; t < LT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (live) {
+#pragma unroll
+        for (int kb = 0; kb < KN; ++kb) {
+          const Frag<E> s = acc_frag<E>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+          for (int t = 0; t < LT; ++t) acc[t] = mma(s, row_frag<E, NP>(Cs, 16 * t, 32 * kb, l16, g), acc[t]);
+        }
+      }
+    }
+    const float2 cl = cs[L - 1];
+    Frag<E> xf[KB];
+    if (live) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) xf[kb] = col_frag<E, PB>(Xs, 32 * kb, 16 * wave, l16, g);
+      const float dl = __expf(cl.x + cl.y);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) S[j] *= dl;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        f32x4 wx[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          wx[hf] = half(xf[kb], hf) * *reinterpret_cast<const f32x4*>(ws + 32 * kb + 16 * hf + 4 * g);
+        Frag<E> part[NPART];
+        split<E>(wx, part);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const Frag<E> bt = col_frag<E, NP>(Bs, 32 * kb, 16 * j, l16, g);
+#pragma unroll
+          for (int q = NPART - 1; q >= 0; --q) S[j] = mma(bt, part[q], S[j]);
+        }
+      }
+    }
+    if constexpr (!READOUT) {
+      seg_c += static_cast<double>(cl.x) + static_cast<double>(cl.y);
+    } else {
+      lds_barrier();  // the scores are in LDS
+      if (live) {
+#pragma unroll
+        for (int t = 0; t < LT; ++t) {
+          const float2 ct = cs[16 * t + l16];
+          acc[t] *= __expf(ct.x + ct.y);
+#pragma unroll
+          for (int kb = 0; kb <= t / 2; ++kb) {
+            const E* m = Ms + ((t * KB + kb) * 64 + lane) * 8;
+            Frag<E> f;
+            if constexpr (sizeof(E) == 2) {
+              f.v = *reinterpret_cast<const bf16x8*>(m);
+            } else {
+              f.v[0] = *reinterpret_cast<const f32x4*>(m);
+              f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
+            }
+            acc[t] = mma(xf[kb], f, acc[t]);
+          }
+          const int tok = c * L + 16 * t + l16, p = pw + 4 * g;
+          if (tok < a.T && p < a.P && a.y != nullptr) {
+            const E* xr = Xs + TX::at(16 * t + l16) + 16 * wave + 4 * g;
+            IO* y = static_cast<IO*>(a.y) + ((static_cast<int64_t>(b) * a.T + tok) * a.H + h) * a.P + p;
+            struct alignas(4 * sizeof(IO)) V4 { IO e[4]; } v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v.e[r] = round_to<IO>(fmaf(Dh, static_cast<float>(xr[r]), acc[t][r]));
+            if (k.vec_y) {
+              *reinterpret_cast<V4*>(y) = v;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (p + r < a.P) y[r] = v.e[r];
+            }
+          }
+        }
+      }
+    }
+  }
+  if constexpr (READOUT) {  // tokens of chunks behind the sequence's end
+    if (a.y != nullptr) {
+      const int z0 = max(c0, c1) * L, z1 = min(a.T, (c0 + k.seg_chunks) * L), w = min(PB, a.P - p0);
+      for (int t = z0 + tid / PB; t < z1; t += NTH / PB)
+        if (tid % PB < w)
+          io<IO>::store(static_cast<IO*>(a.y), ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * a.P + p0 + tid % PB, 0.f);
+    }
+  }
+  float* dst = nullptr;
+  if constexpr (READOUT) {
+    if (seg == k.nseg - 1) dst = a.state_out + bh * a.P * a.N;
+  } else {
+    dst = k.seg_state + (static_cast<int64_t>(seg) * a.B * a.H + bh) * a.P * a.N;
+    if (pb == 0 && tid == 0) k.seg_decay[static_cast<int64_t>(seg) * a.B * a.H + bh] = expf(static_cast<float>(seg_c));
+  }
+  if (dst == nullptr) return;
+  const int p = pw + l16;
+  if (p >= a.P) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = 16 * j + 4 * g;
+    if (n >= a.N) continue;
+    float* q = dst + static_cast<int64_t>(p) * a.N + n;
+    if (k.vec_state) {
+      *reinterpret_cast<f32x4*>(q) = S[j];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.N) q[r] = S[j][r];
+    }
+  }
+}
+
+// seg_state[s] <- start of segment s for s >= 1, from the segments' own states: four values a thread.
+__global__ __launch_bounds__(NTH) void carry_kernel(float* seg_state, const float* __restrict__ seg_decay,
+                                                    const float* __restrict__ state_in, int nseg, int64_t BH, int64_t PN,
+                                                    bool vec) {
+  const int64_t total = BH * PN, w = vec ? 4 : 1;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x) * w;
+  if (i >= total) return;
+  const int64_t bh = i / PN;
+  if (vec) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (state_in != nullptr) s = *reinterpret_cast<const f32x4*>(state_in + i);
+    f32x4 own = *reinterpret_cast<const f32x4*>(seg_state + i);
+    for (int g = 0; g + 1 < nseg; ++g) {
+      s = s * seg_decay[g * BH + bh] + own;
+      if (g + 2 < nseg) own = *reinterpret_cast<const f32x4*>(seg_state + (g + 1) * total + i);
+      *reinterpret_cast<f32x4*>(seg_state + (g + 1) * total + i) = s;
+    }
+  } else {
+    float s = state_in == nullptr ? 0.f : state_in[i], own = seg_state[i];
+    for (int g = 0; g + 1 < nseg; ++g) {
+      s = s * seg_decay[g * BH + bh] + own;
+      if (g + 2 < nseg) own = seg_state[(g + 1) * total + i];
+      seg_state[(g + 1) * total + i] = s;
+    }
+  }
+}
+
+namespace {
+
+int chunk_tokens(int dtype) { return dtype == VMI_BF16 ? 64 : 32; }
+
+struct Plan {
+  int64_t nch, tp, d_bytes, c_bytes, state_bytes, decay_bytes;
+  int pblocks, seg_chunks, nseg;
+  int64_t bytes() const { return d_bytes + c_bytes + state_bytes + decay_bytes; }
+};
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Two workgroups a compute unit; a segment costs its state's way through memory, so it keeps some chunks.
+Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
+  Plan p;
+  const int L = chunk_tokens(dtype);
+  p.nch = (T + L - 1) / L;
+  p.tp = p.nch * L;
+  p.pblocks = static_cast<int>((P + PB - 1) / PB);
+  const int64_t base = B * H * p.pblocks, want = (512 + base - 1) / base;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(MAX_SEG, p.nch / 4));
+  int64_t nseg = std::min(want, most);
+  p.seg_chunks = static_cast<int>((p.nch + nseg - 1) / nseg);
+  p.nseg = static_cast<int>((p.nch + p.seg_chunks - 1) / p.seg_chunks);
+  p.d_bytes = up16(B * H * p.tp * 4);
+  p.c_bytes = up16(B * H * p.tp * 8);
+  p.state_bytes = p.nseg > 1 ? up16(p.nseg * B * H * P * N * 4) : 0;
+  p.decay_bytes = p.nseg > 1 ? up16(p.nseg * B * H * 4) : 0;
+  return p;
+}
+
+template <typename IO, typename E, int NP, int L>
+int run(Chunks k, const Plan& p, hipStream_t stream) {
+  const Args& a = k.a;
+  const int64_t units = static_cast<int64_t>(a.B) * a.H * p.nch, prep = (units + NTH / L - 1) / (NTH / L);
+  const int64_t wgs = static_cast<int64_t>(a.B) * a.H * p.pblocks * p.nseg;
+  const int64_t BH = static_cast<int64_t>(a.B) * a.H, PN = static_cast<int64_t>(a.P) * a.N;
+  if (prep > INT32_MAX || wgs > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(prep_kernel<L>, dim3(static_cast<unsigned>(prep)), dim3(NTH), 0, stream, a,
+                     const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), units);
+  if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+  if (p.nseg > 1) {
+    hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, false>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+    if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+    const bool vec = PN % 4 == 0 && aligned16({a.state_in});
+    const int64_t blocks = (BH * PN / (vec ? 4 : 1) + NTH - 1) / NTH;
+    if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(carry_kernel, dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, stream, k.seg_state,
+                       k.seg_decay, a.state_in, p.nseg, BH, PN, vec);
+    if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+  }
+  hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, true>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+  return hip_status(hipGetLastError());
+}
+
+template <typename IO, typename E, int L> int by_state(const Chunks& k, const Plan& p, hipStream_t stream) {
+  if (k.a.N <= 32) return run<IO, E, 32, L>(k, p, stream);
+  if (k.a.N <= 64) return run<IO, E, 64, L>(k, p, stream);
+  if (k.a.N <= 128) return run<IO, E, 128, L>(k, p, stream);
+  return run<IO, E, 256, L>(k, p, stream);
+}
+
+}  // namespace
+
+bool use_chunk(int64_t T) { return T >= 16; }
+
+size_t chunk_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
+  return use_chunk(T) ? static_cast<size_t>(plan(B, T, H, P, N, dtype).bytes()) : 0;
+}
+
+int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) {
+  const Plan p = plan(a.B, a.T, a.H, a.P, a.N, dtype);
+  Chunks k{};
+  k.a = a;
+  char* w = static_cast<char*>(workspace);
+  k.c = reinterpret_cast<const float2*>(w);
+  k.d = reinterpret_cast<const float*>(w + p.c_bytes);
+  k.seg_state = reinterpret_cast<float*>(w + p.c_bytes + p.d_bytes);
+  k.seg_decay = reinterpret_cast<float*>(w + p.c_bytes + p.d_bytes + p.state_bytes);
+  k.nch = static_cast<int>(p.nch), k.seg_chunks = p.seg_chunks, k.nseg = p.nseg, k.pblocks = p.pblocks;
+  const int el = dtype == VMI_F32 ? 4 : 8;
+  k.vec_x = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && aligned16({a.x});
+  k.vec_bc = a.N % el == 0 && a.b_t % el == 0 && a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 &&
+             aligned16({a.bm, a.cm});
+  k.vec_state = a.N % 4 == 0 && aligned16({a.state_in, a.state_out});
+  k.vec_y = a.P % 4 == 0 && aligned16({a.y});
+  if (dtype == VMI_BF16) return by_state<bf16_t, __bf16, 64>(k, p, stream);
+  if (dtype == VMI_F16) return by_state<f16_t, float, 32>(k, p, stream);
+  return by_state<float, float, 32>(k, p, stream);
+}
+
+}  // namespace sel
+}  // namespace vmi
