@@ -484,6 +484,20 @@ int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, const void* 
                            const void* lengths, int lengths64, void* y, float* state_out, int64_t B,
                            int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, void* workspace,
                            size_t workspace_bytes, void* stream);
+/* Gradients, for dy (rows [H, P] at its own strides) and dstate = dL/dstate_out (NULL: zero): dx, db, dc (dtype),
+ * ddelta (delta_dtype), dA, dD, dbias [H] and dstate_in fp32; any may be NULL.  What lies behind the lengths gets
+ * zeros.  B, T >= 1. */
+int vmi_selective_scan_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G,
+                                           int64_t N, int dtype, size_t* bytes);
+int vmi_selective_scan_bwd(const void* x, int64_t x_t, int64_t x_b, const void* delta, int64_t d_t,
+                           int64_t d_b, int delta_dtype, const float* A, const void* bm, int64_t b_t,
+                           int64_t b_b, const void* cm, int64_t c_t, int64_t c_b, const float* D,
+                           const float* delta_bias, int softplus, int dtype, const float* state_in,
+                           const void* lengths, int lengths64, const void* dy, int64_t y_t, int64_t y_b,
+                           const float* dstate, void* dx, void* ddelta, float* dA, void* db, void* dc,
+                           float* dD, float* dbias, float* dstate_in, int64_t B, int64_t T, int64_t H,
+                           int64_t P, int64_t G, int64_t N, void* workspace, size_t workspace_bytes,
+                           void* stream);
 int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_b, int delta_dtype,
                        const float* A, const void* bm, int64_t b_b, const void* cm, int64_t c_b,
                        const float* D, const float* delta_bias, int softplus, int dtype,

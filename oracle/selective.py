@@ -19,6 +19,7 @@ def selective_scan(x, delta, A, B, C, D=None, delta_bias=None, softplus=True, in
     sums of the terms' absolute values: what rounding errors of the products scale with."""
     x, delta, A, B, C, D, delta_bias, S = (_d(t) for t in (x, delta, A, B, C, D, delta_bias, initial_state))
     b, T, H, P = x.shape
+    delta = delta.reshape(b, T, H)
     r = H // B.shape[2]
     on = _on(b, T, lengths, x.device)
     z = delta if delta_bias is None else delta + delta_bias

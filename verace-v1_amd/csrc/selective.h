@@ -50,5 +50,19 @@ bool use_chunk(int64_t T);
 size_t chunk_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype);
 int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream);
 
+// Step sizes and log decays of every chunk of L (32 or 64) tokens: d, c [B H][nch L].
+int launch_prep(const Args& a, int L, float* d, float2* c, int nch, hipStream_t stream);
+
+// selective_bwd.hip
+struct Grads {
+  const void* dy;            // [B, T, H, P], rows [H, P] at strides y_t, y_b
+  int64_t y_t, y_b;
+  const float* dstate;       // gradient of the final state, or null
+  void *dx, *ddelta, *db, *dc;
+  float *dA, *dD, *dbias, *dstate_in;
+};
+size_t bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype);
+int launch_bwd(const Args& a, int dtype, const Grads& q, void* workspace, hipStream_t stream);
+
 }  // namespace sel
 }  // namespace vmi

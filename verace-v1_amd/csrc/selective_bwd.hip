@@ -1,0 +1,748 @@
+// Backward of the selective scan, in chunks on the matrix cores.
+//
+// With G_t the gradient of S_t from everything after t and dy_t, over a chunk of L tokens with log decays c_t
+// from its start, S_0 the state at its start, G_L the gradient of the state at its end, and
+// dec[t,s] = e^{c_t - c_s} for s <= t:
+//   Q[t,s] = (dy_t . x_s) dec d_s,   M[t,s] = (C_t . B_s) dec d_s,   R[t,s] = (C_t . B_s)(dy_t . x_s) dec
+//   dC_t = sum_s Q[t,s] B_s + e^{c_t} S_0^T dy_t
+//   dB_s = sum_t Q[t,s] C_t + e^{c_L - c_s} d_s G_L^T x_s
+//   dx_s = sum_t M[t,s] dy_t + e^{c_L - c_s} d_s G_L B_s + D dy_s
+//   G_0  = e^{c_L} G_L + sum_t e^{c_t} dy_t C_t^T
+// The gradient of token t's log decay collects every path that crosses it, from s < t (or S_0) to u >= t (or
+// G_L); with alpha_u = e^{c_u} dy_u . S_0 C_u, beta_s = e^{c_L - c_s} x_s . G_L B_s, kappa = e^{c_L} <G_L, S_0>:
+//   g_t = kappa + sum_{u>=t} (alpha_u + sum_s R[u,s] d_s - d_u sum_v R[v,u]) + sum_{s<t} d_s beta_s
+//   dd_t = sum_u R[u,t] + beta_t + A g_t,   dA = sum d_t g_t,   ddelta = dd softplus'(.)
+// Each chunk starts from its own kappa, so nothing is accumulated over the sequence but G itself.
+//
+// Launches:
+//   prep (selective_chunk.hip), states_kernel<OWN> and carry (Sg > 1 segments), states_kernel: the S_0 and G_L of
+//     every chunk, both directions in one grid, in the order in which the main kernel's fragments read them;
+//   main_kernel: a workgroup of eight waves per chunk and block of heads of a group walks the heads with dB and
+//     dC of the chunk in accumulators (they are sums over the heads: as partials of each head they would be the
+//     largest thing moved); C . B, the same for every head, is formed once;
+//   reduce_kernel: the head blocks' dB and dC and the heads' dA, dD, dbias, in a fixed order.
+//
+// bf16 inputs: Q and M, and G_L where it enters dx, are rounded to bf16 once (2^-8 of a term, as the results);
+// S_0 and G_L enter alpha, beta, dB and dC as three bf16 parts and R stays fp32, because ddelta, dA and dbias may be
+// fp32 and are sums in which such roundings do not cancel.
+#include <algorithm>
+#include <type_traits>
+
+#include "selective_mfma.h"
+#include "vmi_vec.h"
+
+namespace vmi {
+namespace sel {
+
+constexpr int PB = 64;
+constexpr int SNT = 256;     // threads of the state passes
+constexpr int MNT = 512;     // and of the main kernel
+constexpr int BWD_MAX_SEG = 32;
+
+struct Bwd {
+  Args a;
+  const void* dy;
+  int64_t y_t, y_b;
+  const float* dstate;       // [B, H, P, N] or null
+  const float* d;            // [BH][Tp]
+  const float2* c;           // [BH][Tp]
+  float* own;                // [2][Sg][BH pblocks][NP 64]: segments' own states, then their starts
+  float *s0, *g1;            // [BH pblocks][nch][NP 64], tiles of 16 x 16 in fragment order
+  float *pb, *pc;            // [hblocks][B T][G][N] (null: dB, dC written directly)
+  float* ph;                 // [3][B nch][H]: dA, dD, dbias
+  void *dx, *ddelta, *db, *dc;
+  float *dA, *dD, *dbias, *dstate_in;
+  int nch, seg_chunks, nseg, pblocks, hblocks, hper;
+  bool vec_x, vec_dy, vec_bc, vec_dx;
+};
+
+// ------------------------------------------------------------------ S_0 and G_L of every chunk
+// Four waves, 16 rows p each: tile j, register r = row p0 + 16 wave + 4 g + r, column n = 16 j + l16.  Forward:
+// S += (d_s e^{c_L - c_s} x_s) B_s^T; reverse, chunks from the last: G += (e^{c_t} dy_t) C_t^T.
+template <typename IO, typename E, int NP, int L, bool OWN>
+__global__ __launch_bounds__(SNT) void states_kernel(Bwd k) {
+  constexpr int NT = NP / 16, KB = L / 32, NPART = Parts<E>::N;
+  typedef Tile<E, NP> TB;
+  typedef Tile<E, PB> TX;
+  __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) float ws[L];
+  __shared__ float wl;
+  const Args& a = k.a;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const bool reverse = blockIdx.y != 0;
+  const int pb = blockIdx.x % k.pblocks, rest = blockIdx.x / k.pblocks;
+  // segments in the direction's order: seg 0 is the one with the given start
+  const int h = rest % a.H, seg = rest / a.H % k.nseg, b = rest / (a.H * k.nseg);
+  if (OWN && seg == k.nseg - 1) return;
+  const int64_t bh = static_cast<int64_t>(b) * a.H + h, bhp = bh * k.pblocks + pb;
+  const int64_t BHP = static_cast<int64_t>(a.B) * a.H * k.pblocks;
+  const int p0 = pb * PB, grp = h / (a.H / a.G);
+  const int len = length_of(a.lengths, a.lengths64, a.T, b);
+  const int place = reverse ? k.nseg - 1 - seg : seg;
+  const int first = place * k.seg_chunks, last = min(min(k.nch, first + k.seg_chunks), (len + L - 1) / L);
+  const int count = max(0, last - first);
+  const IO* x = static_cast<const IO*>(reverse ? k.dy : a.x) + b * (reverse ? k.y_b : a.x_b) + static_cast<int64_t>(h) * a.P + p0;
+  const IO* bm = static_cast<const IO*>(reverse ? a.cm : a.bm) + b * (reverse ? a.c_b : a.b_b) + static_cast<int64_t>(grp) * a.N;
+  const int64_t x_t = reverse ? k.y_t : a.x_t, b_t = reverse ? a.c_t : a.b_t;
+  const bool vec_x = reverse ? k.vec_dy : k.vec_x;
+  const int64_t tp = static_cast<int64_t>(k.nch) * L;
+  const float* dp = k.d + bh * tp;
+  const float2* cp = k.c + bh * tp;
+
+  Stage<IO, E, PB, L, SNT> sx;
+  Stage<IO, E, NP, L, SNT> sb;
+  float rd = 0.f;
+  float2 rc = make_float2(0.f, 0.f), rl = rc;
+  auto chunk = [&](int i) { return reverse ? last - 1 - i : first + i; };
+  auto fetch = [&](int c) {
+    sx.fetch(x, x_t, c * L, len, a.P - p0, vec_x);
+    sb.fetch(bm, b_t, c * L, len, a.N, k.vec_bc);
+    if (tid < L) {
+      rd = dp[c * L + tid];
+      rc = cp[c * L + tid];
+      rl = cp[c * L + L - 1];
+    }
+  };
+  if (count > 0) fetch(chunk(0));
+
+  f32x4 S[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) S[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!OWN) {
+    if (seg > 0) {
+      const float* src = k.own + ((reverse ? k.nseg : 0) + seg) * BHP * (NP * PB) + bhp * (NP * PB);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) S[j] = *reinterpret_cast<const f32x4*>(src + ((j * 4 + wave) * 64 + lane) * 4);
+    } else {
+      const float* src = reverse ? k.dstate : a.state_in;
+      if (src != nullptr) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int p = p0 + 16 * wave + 4 * g + r, n = 16 * j + l16;
+            if (p < a.P && n < a.N) S[j][r] = src[(bh * a.P + p) * a.N + n];
+          }
+      }
+    }
+  }
+  for (int i = 0; i < count; ++i) {
+    const int c = chunk(i);
+    if (!OWN) {
+      float* dst = (reverse ? k.g1 : k.s0) + (bhp * k.nch + c) * (NP * PB);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(dst + ((j * 4 + wave) * 64 + lane) * 4) = S[j];
+    }
+    lds_barrier();
+    sx.commit(Xs);
+    sb.commit(Bs);
+    if (tid < L) {
+      ws[tid] = reverse ? __expf(rc.x + rc.y) : rd * decay(rl, rc);
+      if (tid == L - 1) wl = __expf(rc.x + rc.y);
+    }
+    lds_barrier();
+    if (i + 1 < count) fetch(chunk(i + 1));
+    const float dl = wl;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) S[j] *= dl;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const Frag<E> xf = col_frag<E, PB>(Xs, 32 * kb, 16 * wave, l16, g);
+      f32x4 wx[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        wx[hf] = half(xf, hf) * *reinterpret_cast<const f32x4*>(ws + 32 * kb + 16 * hf + 4 * g);
+      Frag<E> part[NPART];
+      split<E>(wx, part);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const Frag<E> bt = col_frag<E, NP>(Bs, 32 * kb, 16 * j, l16, g);
+#pragma unroll
+        for (int q = NPART - 1; q >= 0; --q) S[j] = mma(part[q], bt, S[j]);
+      }
+    }
+  }
+  if (OWN) {
+    float* dst = k.own + ((reverse ? k.nseg : 0) + seg) * BHP * (NP * PB) + bhp * (NP * PB);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(dst + ((j * 4 + wave) * 64 + lane) * 4) = S[j];
+    return;
+  }
+  if (!reverse || seg != k.nseg - 1 || k.dstate_in == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = p0 + 16 * wave + 4 * g + r, n = 16 * j + l16;
+      if (p < a.P && n < a.N) k.dstate_in[(bh * a.P + p) * a.N + n] = S[j][r];
+    }
+}
+
+// own[dir][s] <- start of the direction's segment s >= 1.  The decay of a segment is the same both ways; the
+// given starts are read in the state's layout.
+template <int NP>
+__global__ __launch_bounds__(SNT) void starts_kernel(Bwd k, int L) {
+  constexpr int SZ = NP * PB;
+  const Args& a = k.a;
+  const bool reverse = blockIdx.y != 0;
+  const int64_t BHP = static_cast<int64_t>(a.B) * a.H * k.pblocks;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * SNT + threadIdx.x;  // 16-byte piece
+  if (id >= BHP * (SZ / 4)) return;
+  const int64_t bhp = id / (SZ / 4);
+  const int e = static_cast<int>(id - bhp * (SZ / 4)), lane = e & 63, wave = (e >> 6) & 3, j = e >> 8;
+  const int64_t bh = bhp / k.pblocks;
+  const int pb = static_cast<int>(bhp - bh * k.pblocks);
+  const float* src = reverse ? k.dstate : a.state_in;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (src != nullptr)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = pb * PB + 16 * wave + 4 * (lane >> 4) + r, n = 16 * j + (lane & 15);
+      if (p < a.P && n < a.N) s[r] = src[(bh * a.P + p) * a.N + n];
+    }
+  const int64_t tp = static_cast<int64_t>(k.nch) * L;
+  const float2* cp = k.c + bh * tp;
+  float* base = k.own + (reverse ? k.nseg : 0) * BHP * SZ + bhp * SZ + e * 4;
+  f32x4 own = *reinterpret_cast<const f32x4*>(base);
+  for (int g = 0; g + 1 < k.nseg; ++g) {
+    const int place = reverse ? k.nseg - 1 - g : g;
+    double c = 0.0;
+    for (int i = place * k.seg_chunks; i < min(k.nch, (place + 1) * k.seg_chunks); ++i) {
+      const float2 v = cp[static_cast<int64_t>(i) * L + L - 1];
+      c += static_cast<double>(v.x) + static_cast<double>(v.y);
+    }
+    s = s * expf(static_cast<float>(c)) + own;
+    if (g + 2 < k.nseg) own = *reinterpret_cast<const f32x4*>(base + (g + 1) * BHP * SZ);
+    *reinterpret_cast<f32x4*>(base + (g + 1) * BHP * SZ) = s;
+  }
+}
+
+// ------------------------------------------------------------------ the chunks
+// Tile i on or below the diagonal, row by row from the last: tiles 0 .. LT - 1 are the last t-tile's.
+template <int LT> __device__ __forceinline__ bool lower_tile(int i, int& tt, int& st) {
+  tt = LT - 1;
+#pragma unroll
+  for (int r = LT; r >= 1; --r) {
+    if (i < r) {
+      st = i;
+      return true;
+    }
+    i -= r;
+    --tt;
+  }
+  return false;
+}
+
+template <typename IO, typename E, int NP, int L>
+__global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
+  constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::N;
+  constexpr int NTW = NT >= NW ? NT / NW : 1;      // n-tiles of a wave: wave, wave + 8 (or wave % NT)
+  constexpr int TS = NT >= NW ? 1 : NW / NT;       // waves that share an n-tile, each LTW of the t-tiles
+  constexpr int LTW = LT / TS;
+  constexpr int NH = NP > 128 ? 2 : 1, GR = NP / NH;  // dx takes G_L through LDS 128 state columns at a time
+  constexpr int PER = (LT * (LT + 1) / 2 + NW - 1) / NW;
+  static_assert(LT % TS == 0, "");
+  typedef Tile<E, NP> TB;
+  typedef Tile<E, PB> TX;
+  typedef Tile<E, L> TQ;
+  __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Cs[TB::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Ys[TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Qs[TQ::elems(L)];   // [t][s]
+  __shared__ __attribute__((aligned(16))) E Ms[TQ::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Gs[TX::elems(GR)];  // G_L^T [n][p]
+  __shared__ __attribute__((aligned(16))) float2 cs[L];
+  __shared__ __attribute__((aligned(16))) float ds[L], es[L], ws[L];
+  __shared__ float row_r[LT][L], col_r[LT][L];                  // sum_s R d_s by s-tile, sum_t R by t-tile
+  __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
+  const Args& a = k.a;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int hb = blockIdx.x % k.hblocks;
+  int rest = blockIdx.x / k.hblocks;
+  const int grp = rest % a.G;
+  rest /= a.G;
+  const int c = rest % k.nch, b = rest / k.nch;
+  const int hg = a.H / a.G, h0 = grp * hg + hb * k.hper, h1 = min((grp + 1) * hg, h0 + k.hper);
+  const int len = length_of(a.lengths, a.lengths64, a.T, b), t0 = c * L;
+  const int64_t tp = static_cast<int64_t>(k.nch) * L;
+  const int nt0 = NT >= NW ? wave : wave % NT, tt0 = NT >= NW ? 0 : wave / NT * LTW;
+
+  f32x4 db[NTW][LTW], dc[NTW][LTW];
+#pragma unroll
+  for (int j = 0; j < NTW; ++j)
+#pragma unroll
+    for (int t = 0; t < LTW; ++t) db[j][t] = dc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (t0 < len) {
+    {
+      Stage<IO, E, NP, L, MNT> sb, sc;
+      sb.fetch(static_cast<const IO*>(a.bm) + b * a.b_b + static_cast<int64_t>(grp) * a.N, a.b_t, t0, len, a.N, k.vec_bc);
+      sc.fetch(static_cast<const IO*>(a.cm) + b * a.c_b + static_cast<int64_t>(grp) * a.N, a.c_t, t0, len, a.N, k.vec_bc);
+      sb.commit(Bs);
+      sc.commit(Cs);
+      for (int i = tid; i < TQ::elems(L); i += MNT) Qs[i] = Ms[i] = static_cast<E>(0.f);
+    }
+    Stage<IO, E, PB, L, MNT> sx, sy;
+    float rd = 0.f;
+    float2 rc = make_float2(0.f, 0.f), rl = rc;
+    f32x4 s0[NTW][4], g1[NTW][4];
+    const int units = (h1 - h0) * k.pblocks;
+    auto fetch = [&](int u) {
+      const int h = h0 + u / k.pblocks, p0 = u % k.pblocks * PB;
+      sx.fetch(static_cast<const IO*>(a.x) + b * a.x_b + static_cast<int64_t>(h) * a.P + p0, a.x_t, t0, len, a.P - p0, k.vec_x);
+      sy.fetch(static_cast<const IO*>(k.dy) + b * k.y_b + static_cast<int64_t>(h) * a.P + p0, k.y_t, t0, len, a.P - p0, k.vec_dy);
+      if (tid < L) {
+        const int64_t o = (static_cast<int64_t>(b) * a.H + h) * tp + t0;
+        rd = k.d[o + tid];
+        rc = k.c[o + tid];
+        rl = k.c[o + L - 1];
+      }
+    };
+    auto fetch_states = [&](int u) {
+      const int64_t bhp = (static_cast<int64_t>(b) * a.H + h0) * k.pblocks + u;
+      const int64_t o = (bhp * k.nch + c) * (NP * PB) + lane * 4;
+#pragma unroll
+      for (int j = 0; j < NTW; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int64_t q = o + ((nt0 + NW * j) * 4 + w) * 256;
+          s0[j][w] = *reinterpret_cast<const f32x4*>(k.s0 + q);
+          g1[j][w] = *reinterpret_cast<const f32x4*>(k.g1 + q);
+        }
+    };
+    fetch(0);
+    fetch_states(0);
+    __syncthreads();
+    f32x4 cb[PER];  // C . B of this wave's tiles, transposed (rows s, column t)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int tt, st;
+      cb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!lower_tile<LT>(wave + NW * i, tt, st)) continue;
+#pragma unroll
+      for (int kb = 0; kb < KN; ++kb)
+        cb[i] = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), row_frag<E, NP>(Cs, 16 * tt, 32 * kb, l16, g), cb[i]);
+    }
+    double dd_sum = 0.0, g_sum = 0.0, dd_acc = 0.0;  // wave 0: over a head's row blocks
+
+    for (int u = 0; u < units; ++u) {
+      const int h = h0 + u / k.pblocks, pb = u % k.pblocks, p0 = pb * PB;
+      lds_barrier();  // the last unit's readers are done
+      sx.commit(Xs);
+      sy.commit(Ys);
+      if (tid < L) {
+        cs[tid] = rc;
+        ds[tid] = rd;
+        es[tid] = __expf(rc.x + rc.y);
+        ws[tid] = decay(rl, rc);
+      }
+      lds_barrier();
+      if (u + 1 < units) fetch(u + 1);
+      // Q, M and the sums of R
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int tt, st;
+        if (!lower_tile<LT>(wave + NW * i, tt, st)) continue;
+        f32x4 xy = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KP; ++kb)
+          xy = mma(row_frag<E, PB>(Xs, 16 * st, 32 * kb, l16, g), row_frag<E, PB>(Ys, 16 * tt, 32 * kb, l16, g), xy);
+        const int t = 16 * tt + l16;
+        const float2 ct = cs[t];
+        struct alignas(8) M4 { E e[4]; } q, m;
+        float rs = 0.f, dg = 0.f, rr[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int s = 16 * st + 4 * g + r;
+          const bool on = s <= t;
+          const float w = on ? decay(ct, cs[s]) : 0.f, wd = w * ds[s];
+          const float x0 = on ? xy[r] : 0.f, c0 = on ? cb[i][r] : 0.f;
+          q.e[r] = static_cast<E>(x0 * wd);
+          m.e[r] = static_cast<E>(c0 * wd);
+          rr[r] = c0 * x0 * w;
+          rs = fmaf(rr[r], ds[s], rs);
+          if (s == t) dg = x0;
+        }
+        const int o = TQ::at(t) + 16 * st + 4 * g;
+        *reinterpret_cast<M4*>(Qs + o) = q;
+        *reinterpret_cast<M4*>(Ms + o) = m;
+        rs += __shfl_xor(rs, 16);
+        rs += __shfl_xor(rs, 32);
+        if (g == 0) row_r[st][t] = rs;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) rr[r] = row16_sum(rr[r]);
+        if (l16 == 0) *reinterpret_cast<float4*>(&col_r[tt][16 * st + 4 * g]) = make_float4(rr[0], rr[1], rr[2], rr[3]);
+        if (tt == st) {
+#pragma unroll
+          for (int off = 32; off >= 1; off >>= 1) dg += __shfl_xor(dg, off);
+          if (lane == 0) diag[tt] = dg;
+        }
+      }
+      // S_0^T dy and G_L^T x (rows n, column t or s)
+      float kp = 0.f, al[LTW] = {}, be[LTW] = {};
+#pragma unroll
+      for (int j = 0; j < NTW; ++j) {
+        const int n = 16 * (nt0 + NW * j) + 4 * g;
+        f32x4 sy_[LTW], gx_[LTW];
+#pragma unroll
+        for (int t = 0; t < LTW; ++t) sy_[t] = gx_[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KP; ++kb) {
+          Frag<E> sp[NPART], gp[NPART];
+          {
+            const f32x4 v[2] = {s0[j][2 * kb], s0[j][2 * kb + 1]}, w[2] = {g1[j][2 * kb], g1[j][2 * kb + 1]};
+            split<E>(v, sp);
+            split<E>(w, gp);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) kp = fmaf(v[hf][r], w[hf][r], kp);
+          }
+#pragma unroll
+          for (int t = 0; t < LTW; ++t) {
+            const Frag<E> yf = row_frag<E, PB>(Ys, 16 * (tt0 + t), 32 * kb, l16, g);
+            const Frag<E> xf = row_frag<E, PB>(Xs, 16 * (tt0 + t), 32 * kb, l16, g);
+#pragma unroll
+            for (int q = NPART - 1; q >= 0; --q) {
+              sy_[t] = mma(sp[q], yf, sy_[t]);
+              gx_[t] = mma(gp[q], xf, gx_[t]);
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < LTW; ++t) {
+          const int tok = 16 * (tt0 + t) + l16;
+          const float e = es[tok], w = ws[tok], wd = w * ds[tok];
+          const E* cr = Cs + TB::at(tok) + n;
+          const E* br = Bs + TB::at(tok) + n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            sy_[t][r] *= e;
+            al[t] = fmaf(static_cast<float>(cr[r]), sy_[t][r], al[t]);
+            be[t] = fmaf(static_cast<float>(br[r]) * w, gx_[t][r], be[t]);
+            dc[j][t][r] += sy_[t][r];
+            db[j][t][r] = fmaf(wd, gx_[t][r], db[j][t][r]);
+          }
+        }
+      }
+      f32x4 dx[2];
+      const int pt = wave & 3, st0 = (wave >> 2) * (LT / 2);  // dx: p-tile, s-tiles st0 .. st0 + LT / 2 - 1
+      constexpr int DXT = LT / 2;
+#pragma unroll
+      for (int t = 0; t < DXT; ++t) dx[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int hh = 0; hh < NH; ++hh) {
+        if (hh > 0) lds_barrier();
+        if (NT >= NW || tt0 == 0) {
+          const int j = NH > 1 ? hh : 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            struct alignas(8) M4 { E e[4]; } q;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q.e[r] = static_cast<E>(g1[j][w][r]);
+            *reinterpret_cast<M4*>(Gs + TX::at(16 * nt0 + l16) + 16 * w + 4 * g) = q;
+          }
+        }
+        if (hh == 0) {
+#pragma unroll
+          for (int t = 0; t < LTW; ++t) {
+            float v = al[t], w = be[t];
+            v += __shfl_xor(v, 16), w += __shfl_xor(w, 16);
+            v += __shfl_xor(v, 32), w += __shfl_xor(w, 32);
+            if (g == 0) alpha[nt0][16 * (tt0 + t) + l16] = v, beta[nt0][16 * (tt0 + t) + l16] = w;
+          }
+#pragma unroll
+          for (int off = 32; off >= 1; off >>= 1) kp += __shfl_xor(kp, off);
+          if (lane == 0) kappa[wave] = NT >= NW || tt0 == 0 ? kp : 0.f;
+        }
+        if (hh == NH - 1 && u + 1 < units) fetch_states(u + 1);
+        lds_barrier();
+#pragma unroll
+        for (int kb = 0; kb < GR / 32; ++kb) {
+          const Frag<E> gf = col_frag<E, PB>(Gs, 32 * kb, 16 * pt, l16, g);
+#pragma unroll
+          for (int t = 0; t < DXT; ++t)
+            dx[t] = mma(gf, row_frag<E, NP>(Bs, 16 * (st0 + t), GR * hh + 32 * kb, l16, g), dx[t]);
+        }
+      }
+      // the chunk's own terms
+#pragma unroll
+      for (int j = 0; j < NTW; ++j) {
+#pragma unroll
+        for (int kb = 0; kb < KL; ++kb) {
+          const Frag<E> bf = col_frag<E, NP>(Bs, 32 * kb, 16 * (nt0 + NW * j), l16, g);
+          const Frag<E> cf = col_frag<E, NP>(Cs, 32 * kb, 16 * (nt0 + NW * j), l16, g);
+#pragma unroll
+          for (int t = 0; t < LTW; ++t) {
+            if ((tt0 + t) / 2 >= kb) dc[j][t] = mma(bf, row_frag<E, L>(Qs, 16 * (tt0 + t), 32 * kb, l16, g), dc[j][t]);
+            if ((tt0 + t) / 2 <= kb) db[j][t] = mma(cf, col_frag<E, L>(Qs, 32 * kb, 16 * (tt0 + t), l16, g), db[j][t]);
+          }
+        }
+      }
+      const float Dh = a.D == nullptr ? 0.f : a.D[h];
+#pragma unroll
+      for (int t = 0; t < DXT; ++t) {
+        const int st = st0 + t, s = 16 * st + l16;
+        dx[t] *= ws[s] * ds[s];
+#pragma unroll
+        for (int kb = 0; kb < KL; ++kb)
+          if (st / 2 <= kb) dx[t] = mma(col_frag<E, PB>(Ys, 32 * kb, 16 * pt, l16, g), col_frag<E, L>(Ms, 32 * kb, 16 * st, l16, g), dx[t]);
+        const int p = p0 + 16 * pt + 4 * g;
+        if (t0 + s < a.T && p < a.P && k.dx != nullptr) {
+          const E* yr = Ys + TX::at(s) + 16 * pt + 4 * g;
+          IO* o = static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0 + s) * a.H + h) * a.P + p;
+          struct alignas(4 * sizeof(IO)) V4 { IO e[4]; } v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v.e[r] = round_to<IO>(fmaf(Dh, static_cast<float>(yr[r]), dx[t][r]));
+          if (k.vec_dx) {
+            *reinterpret_cast<V4*>(o) = v;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (p + r < a.P) o[r] = v.e[r];
+          }
+        }
+      }
+      // a lane a token: the gradients of the step sizes (sums in fp64: they are differences)
+      if (wave == NW - 1) {
+        const bool in = lane < L;
+        const int t = in ? lane : 0;
+        const double d = in ? ds[t] : 0.f;
+        double rs = 0.0, cr = 0.0, alp = 0.0, bet = 0.0, kap = 0.0, dgs = 0.0;
+#pragma unroll
+        for (int i = 0; i < LT; ++i) {
+          if (i <= t / 16) rs += row_r[i][t];
+          if (i >= t / 16) cr += col_r[i][t];
+          dgs += diag[i];
+        }
+        constexpr int NS = NT < NW ? NT : NW;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) alp += alpha[i][t], bet += beta[i][t];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) kap += kappa[i];
+        kap *= static_cast<double>(es[L - 1]);
+        double suf = in ? alp + rs - d * cr : 0.0, pre = in ? d * bet : 0.0;
+        const double own_pre = pre;
+#pragma unroll
+        for (int off = 1; off < L; off <<= 1) {
+          const double v = __shfl_down(suf, off, 64), w = __shfl_up(pre, off, 64);
+          if (lane + off < L) suf += v;
+          if (lane >= off) pre += w;
+        }
+        const double gt = kap + suf + (pre - own_pre);
+        const double A = a.A[h];
+        if (pb == 0) dd_sum = g_sum = dd_acc = 0.0;
+        dd_acc += cr + bet + A * gt;
+        g_sum += d * gt;
+        dd_sum += dgs;
+        if (pb == k.pblocks - 1) {
+          const float slope = a.softplus ? -expm1f(-static_cast<float>(d)) : 1.f;  // sigmoid(z) = 1 - e^{-softplus(z)}
+          double dz = in && t0 + t < len ? dd_acc * static_cast<double>(slope) : 0.0;
+          if (in && t0 + t < a.T && k.ddelta != nullptr) {
+            const int64_t o = (static_cast<int64_t>(b) * a.T + t0 + t) * a.H + h;
+            const float v = static_cast<float>(dz);
+            if (a.delta_dtype == VMI_F32) io<float>::store(static_cast<float*>(k.ddelta), o, v);
+            else if (a.delta_dtype == VMI_BF16) io<bf16_t>::store(static_cast<bf16_t*>(k.ddelta), o, v);
+            else io<f16_t>::store(static_cast<f16_t*>(k.ddelta), o, v);
+          }
+          double ga = in ? g_sum : 0.0;
+#pragma unroll
+          for (int off = 32; off >= 1; off >>= 1) dz += __shfl_xor(dz, off), ga += __shfl_xor(ga, off);
+          if (lane == 0) {
+            const int64_t rows = static_cast<int64_t>(a.B) * k.nch, o = (static_cast<int64_t>(b) * k.nch + c) * a.H + h;
+            k.ph[o] = static_cast<float>(ga);
+            k.ph[rows * a.H + o] = static_cast<float>(dd_sum);
+            k.ph[2 * rows * a.H + o] = static_cast<float>(dz);
+          }
+        }
+      }
+    }
+  } else {  // behind the sequence's end
+    for (int h = h0; h < h1; ++h) {
+      const int rows = min(L, a.T - t0);
+      if (k.dx != nullptr)
+        for (int t = wave; t < rows; t += NW)
+          for (int p = lane; p < a.P; p += 64)
+            io<IO>::store(static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0 + t) * a.H + h) * a.P, p, 0.f);
+      if (tid < rows && k.ddelta != nullptr) {
+        const int64_t o = (static_cast<int64_t>(b) * a.T + t0 + tid) * a.H + h;
+        if (a.delta_dtype == VMI_F32) static_cast<float*>(k.ddelta)[o] = 0.f;
+        else static_cast<uint16_t*>(k.ddelta)[o] = 0;
+      }
+      if (tid < 3) k.ph[(tid * static_cast<int64_t>(a.B) * k.nch + static_cast<int64_t>(b) * k.nch + c) * a.H + h] = 0.f;
+    }
+  }
+  // dB, dC: rows n, column t
+#pragma unroll
+  for (int j = 0; j < NTW; ++j) {
+    const int n = 16 * (nt0 + NW * j) + 4 * g;
+#pragma unroll
+    for (int t = 0; t < LTW; ++t) {
+      const int tok = t0 + 16 * (tt0 + t) + l16;
+      if (tok >= a.T || n >= a.N) continue;
+      const int64_t o = ((static_cast<int64_t>(b) * a.T + tok) * a.G + grp) * a.N + n;
+      const int64_t part = static_cast<int64_t>(hb) * a.B * a.T * a.G * a.N;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (n + r >= a.N) continue;
+        if (k.pb != nullptr) {
+          k.pb[part + o + r] = db[j][t][r];
+          k.pc[part + o + r] = dc[j][t][r];
+        } else {
+          if (k.db != nullptr) io<IO>::store(static_cast<IO*>(k.db), o + r, db[j][t][r]);
+          if (k.dc != nullptr) io<IO>::store(static_cast<IO*>(k.dc), o + r, dc[j][t][r]);
+        }
+      }
+    }
+  }
+}
+
+// Blocks below `heads`: 64 of the 3 H head sums by four strided shares of the chunks.  The others: dB and dC
+// from the head blocks' partials.
+template <typename IO>
+__global__ __launch_bounds__(SNT) void reduce_kernel(Bwd k, int heads, int64_t elems) {
+  const Args& a = k.a;
+  if (static_cast<int>(blockIdx.x) < heads) {
+    __shared__ double part[4][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6, l = threadIdx.x & 63;
+    const int64_t rows = static_cast<int64_t>(a.B) * k.nch;
+    double s = 0.0;
+    const int which = col / a.H, h = col - which * a.H;
+    if (which < 3)
+      for (int64_t r = share; r < rows; r += 4) s += k.ph[(which * rows + r) * a.H + h];
+    part[share][l] = s;
+    __syncthreads();
+    if (share != 0 || which >= 3) return;
+    float* dst = which == 0 ? k.dA : which == 1 ? k.dD : k.dbias;
+    if (dst != nullptr) dst[h] = static_cast<float>((part[0][l] + part[1][l]) + (part[2][l] + part[3][l]));
+    return;
+  }
+  const int64_t i = static_cast<int64_t>(blockIdx.x - heads) * SNT + threadIdx.x;
+  if (i >= elems) return;
+  float vb = 0.f, vc = 0.f;
+  for (int q = 0; q < k.hblocks; ++q) {
+    vb += k.pb[q * elems + i];
+    vc += k.pc[q * elems + i];
+  }
+  if (k.db != nullptr) io<IO>::store(static_cast<IO*>(k.db), i, vb);
+  if (k.dc != nullptr) io<IO>::store(static_cast<IO*>(k.dc), i, vc);
+}
+
+namespace {
+
+int bwd_tokens(int dtype) { return dtype == VMI_BF16 ? 64 : 32; }
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+struct Plan {
+  int64_t nch, tp, c_bytes, d_bytes, own_bytes, state_bytes, part_bytes, ph_bytes;
+  int np, pblocks, seg_chunks, nseg, hblocks, hper;
+  int64_t bytes() const { return c_bytes + d_bytes + own_bytes + 2 * state_bytes + 2 * part_bytes + ph_bytes; }
+};
+
+Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
+  Plan p;
+  const int L = bwd_tokens(dtype);
+  p.np = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+  p.nch = (T + L - 1) / L;
+  p.tp = p.nch * L;
+  p.pblocks = static_cast<int>((P + PB - 1) / PB);
+  const int64_t BHP = B * H * p.pblocks, want = (512 + 2 * BHP - 1) / (2 * BHP);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(BWD_MAX_SEG, p.nch / 4));
+  const int64_t nseg = std::min(want, most);
+  p.seg_chunks = static_cast<int>((p.nch + nseg - 1) / nseg);
+  p.nseg = static_cast<int>((p.nch + p.seg_chunks - 1) / p.seg_chunks);
+  const int64_t hg = H / G, blocks = B * p.nch * G, split = std::min<int64_t>(hg, (512 + blocks - 1) / blocks);
+  p.hper = static_cast<int>((hg + split - 1) / split);
+  p.hblocks = static_cast<int>((hg + p.hper - 1) / p.hper);
+  p.c_bytes = up16(B * H * p.tp * 8);
+  p.d_bytes = up16(B * H * p.tp * 4);
+  const int64_t state = static_cast<int64_t>(p.np) * PB * 4;
+  p.own_bytes = p.nseg > 1 ? 2 * p.nseg * BHP * state : 0;
+  p.state_bytes = BHP * p.nch * state;
+  p.part_bytes = p.hblocks > 1 ? up16(p.hblocks * B * T * G * N * 4) : 0;
+  p.ph_bytes = up16(3 * B * p.nch * H * 4);
+  return p;
+}
+
+template <typename IO, typename E, int NP, int L> int run(Bwd k, const Plan& p, hipStream_t stream) {
+  const Args& a = k.a;
+  const int64_t BHP = static_cast<int64_t>(a.B) * a.H * p.pblocks, wgs = BHP * p.nseg;
+  const int64_t blocks = static_cast<int64_t>(a.B) * p.nch * a.G * p.hblocks;
+  if (wgs > INT32_MAX || blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  auto ok = [](int& st) { return (st = hip_status(hipGetLastError())) == VMI_OK; };
+  int st = launch_prep(a, L, const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), stream);
+  if (st != VMI_OK) return st;
+  const dim3 grid(static_cast<unsigned>(wgs), 2);
+  if (p.nseg > 1) {
+    hipLaunchKernelGGL((states_kernel<IO, E, NP, L, true>), grid, dim3(SNT), 0, stream, k);
+    if (!ok(st)) return st;
+    const int64_t pieces = (BHP * (NP * PB / 4) + SNT - 1) / SNT;
+    if (pieces > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(starts_kernel<NP>, dim3(static_cast<unsigned>(pieces), 2), dim3(SNT), 0, stream, k, L);
+    if (!ok(st)) return st;
+  }
+  hipLaunchKernelGGL((states_kernel<IO, E, NP, L, false>), grid, dim3(SNT), 0, stream, k);
+  if (!ok(st)) return st;
+  hipLaunchKernelGGL((main_kernel<IO, E, NP, L>), dim3(static_cast<unsigned>(blocks)), dim3(MNT), 0, stream, k);
+  if (!ok(st)) return st;
+  const int heads = (3 * a.H + 63) / 64;
+  const int64_t elems = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
+  const int64_t rb = heads + (p.hblocks > 1 ? (elems + SNT - 1) / SNT : 0);
+  if (rb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(reduce_kernel<IO>, dim3(static_cast<unsigned>(rb)), dim3(SNT), 0, stream, k, heads, elems);
+  ok(st);
+  return st;
+}
+
+template <typename IO, typename E, int L> int by_state(const Bwd& k, const Plan& p, hipStream_t stream) {
+  if (p.np == 64) return run<IO, E, 64, L>(k, p, stream);
+  if (p.np == 128) return run<IO, E, 128, L>(k, p, stream);
+  return run<IO, E, 256, L>(k, p, stream);
+}
+
+}  // namespace
+
+size_t bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
+  return static_cast<size_t>(plan(B, T, H, P, G, N, dtype).bytes());
+}
+
+int launch_bwd(const Args& a, int dtype, const Grads& q, void* workspace, hipStream_t stream) {
+  const Plan p = plan(a.B, a.T, a.H, a.P, a.G, a.N, dtype);
+  Bwd k{};
+  k.a = a;
+  k.dy = q.dy, k.y_t = q.y_t, k.y_b = q.y_b, k.dstate = q.dstate;
+  k.dx = q.dx, k.ddelta = q.ddelta, k.db = q.db, k.dc = q.dc, k.dA = q.dA, k.dD = q.dD, k.dbias = q.dbias;
+  k.dstate_in = q.dstate_in;
+  char* w = static_cast<char*>(workspace);
+  auto take = [&](int64_t bytes) {
+    char* r = w;
+    w += bytes;
+    return r;
+  };
+  k.c = reinterpret_cast<const float2*>(take(p.c_bytes));
+  k.d = reinterpret_cast<const float*>(take(p.d_bytes));
+  k.own = reinterpret_cast<float*>(take(p.own_bytes));
+  k.s0 = reinterpret_cast<float*>(take(p.state_bytes));
+  k.g1 = reinterpret_cast<float*>(take(p.state_bytes));
+  if (p.hblocks > 1) {
+    k.pb = reinterpret_cast<float*>(take(p.part_bytes));
+    k.pc = reinterpret_cast<float*>(take(p.part_bytes));
+  }
+  k.ph = reinterpret_cast<float*>(take(p.ph_bytes));
+  k.nch = static_cast<int>(p.nch), k.seg_chunks = p.seg_chunks, k.nseg = p.nseg, k.pblocks = p.pblocks;
+  k.hblocks = p.hblocks, k.hper = p.hper;
+  const int el = dtype == VMI_F32 ? 4 : 8;
+  k.vec_x = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && aligned16({a.x});
+  k.vec_dy = a.P % el == 0 && q.y_t % el == 0 && q.y_b % el == 0 && aligned16({q.dy});
+  k.vec_bc = a.N % el == 0 && a.b_t % el == 0 && a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 &&
+             aligned16({a.bm, a.cm});
+  k.vec_dx = a.P % 4 == 0 && aligned16({q.dx});
+  if (dtype == VMI_BF16) return by_state<bf16_t, __bf16, 64>(k, p, stream);
+  if (dtype == VMI_F16) return by_state<f16_t, float, 32>(k, p, stream);
+  return by_state<float, float, 32>(k, p, stream);
+}
+
+}  // namespace sel
+}  // namespace vmi

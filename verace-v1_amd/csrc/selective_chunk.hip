@@ -371,13 +371,12 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
 template <typename IO, typename E, int NP, int L>
 int run(Chunks k, const Plan& p, hipStream_t stream) {
   const Args& a = k.a;
-  const int64_t units = static_cast<int64_t>(a.B) * a.H * p.nch, prep = (units + NTH / L - 1) / (NTH / L);
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * p.pblocks * p.nseg;
   const int64_t BH = static_cast<int64_t>(a.B) * a.H, PN = static_cast<int64_t>(a.P) * a.N;
-  if (prep > INT32_MAX || wgs > INT32_MAX) return VMI_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(prep_kernel<L>, dim3(static_cast<unsigned>(prep)), dim3(NTH), 0, stream, a,
-                     const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), units);
-  if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+  if (wgs > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (const int st = launch_prep(a, L, const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), stream);
+      st != VMI_OK)
+    return st;
   if (p.nseg > 1) {
     hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, false>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
@@ -400,6 +399,15 @@ template <typename IO, typename E, int L> int by_state(const Chunks& k, const Pl
 }
 
 }  // namespace
+
+int launch_prep(const Args& a, int L, float* d, float2* c, int nch, hipStream_t stream) {
+  const int64_t units = static_cast<int64_t>(a.B) * a.H * nch, blocks = (units + NTH / L - 1) / (NTH / L);
+  if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (L == 64) hipLaunchKernelGGL(prep_kernel<64>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
+  else hipLaunchKernelGGL(prep_kernel<32>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
+  return hip_status(hipGetLastError());
+}
 
 bool use_chunk(int64_t T) { return T >= 16; }
 

@@ -28,9 +28,9 @@ Drop-in replacements for the reference's SSSD hot path:
 * ``VeraceV1Layer`` / ``VeraceV1Model`` / ``VeraceV1Config`` / ``DecodeState``
                                -- the layer harness (``backbone.py:21-210``, ACDE
                                   ``acd_engine.py:36-167``) with batched in-place decode
-* ``selective_scan`` / ``launch_selective_hip_scan`` / ``selective_step_``
-                               -- selective state space scan beside the SSSD scan, and its in-place
-                                  single-token step
+* ``selective_scan`` / ``launch_selective_hip_scan`` / ``launch_selective_hip_scan_bwd`` /
+  ``selective_step_``          -- selective state space scan beside the SSSD scan, its backward and its
+                                  in-place single-token step
 * ``short_conv`` / ``short_conv_step_``
                                -- the short causal convolution before it, and its single-token step
 * ``gated_norm_add``           -- the norms either side of a block with its gate and residual scale
@@ -55,8 +55,8 @@ from .mcmoe import ManifoldContinuousMoE, SiTUGLU
 from .backbone import (AdaptiveCognitiveDepthEngine, DecodeGraph, DecodeState, LayerDecodeState,
                        VeraceV1Config, VeraceV1Layer, VeraceV1Model)
 from .block_norm import gated_norm_add
-from .selective import (launch_selective_hip_scan, selective_scan, selective_step_, short_conv,
-                        short_conv_step_)
+from .selective import (launch_selective_hip_scan, launch_selective_hip_scan_bwd, selective_scan,
+                        selective_step_, short_conv, short_conv_step_)
 from .state_cache import SlotTable, SSSDStateCache
 
 __all__ = [
@@ -87,6 +87,7 @@ __all__ = [
     "VeraceV1Model",
     "selective_scan",
     "launch_selective_hip_scan",
+    "launch_selective_hip_scan_bwd",
     "selective_step_",
     "short_conv",
     "short_conv_step_",

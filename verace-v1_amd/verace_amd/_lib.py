@@ -68,6 +68,8 @@ EXPORTED = (
     "vmi_selective_scan_workspace_bytes",
     "vmi_selective_scan_fwd",
     "vmi_selective_step",
+    "vmi_selective_scan_bwd_workspace_bytes",
+    "vmi_selective_scan_bwd",
 )
 
 ERR_WORKSPACE = 3  # VMI_ERR_WORKSPACE
@@ -185,9 +187,13 @@ def _declare(lib):
                                            i32, i32, vp, vp, i32, vp, vp, i64, i64, i64, i64, i64, i64, vp, sz, vp]
     lib.vmi_selective_step.argtypes = [vp, i64, vp, i64, i32, vp, vp, i64, vp, i64, vp, vp, i32, i32, vp, vp, vp, i64,
                                        i64, i64, i64, i64, vp]
+    lib.vmi_selective_scan_bwd_workspace_bytes.argtypes = lib.vmi_selective_scan_workspace_bytes.argtypes
+    lib.vmi_selective_scan_bwd.argtypes = [vp, i64, i64, vp, i64, i64, i32, vp, vp, i64, i64, vp, i64, i64, vp, vp,
+                                           i32, i32, vp, vp, i32, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                           i64, i64, i64, i64, i64, i64, vp, sz, vp]
     for name in ("gated_norm", "gated_norm_bwd_workspace_bytes", "gated_norm_bwd", "short_conv", "short_conv_step",
                  "short_conv_bwd_workspace_bytes", "short_conv_bwd", "selective_scan_workspace_bytes",
-                 "selective_scan_fwd", "selective_step"):
+                 "selective_scan_fwd", "selective_step", "selective_scan_bwd_workspace_bytes", "selective_scan_bwd"):
         getattr(lib, "vmi_" + name).restype = i32
 
 

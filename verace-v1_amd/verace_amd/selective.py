@@ -264,6 +264,79 @@ def launch_selective_hip_scan(
     return y, out
 
 
+def launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D=None, delta_bias=None, softplus=True, initial_state=None,
+                                  lengths=None, d_state=None, need_d_state=True):
+    """Gradients of :func:`launch_selective_hip_scan` for dy = dL/dy [batch, seq_len, num_heads, head_dim] and
+    d_state = dL/dfinal_state (None: zero): (dx, ddelta, dA, dB, dC, dD, ddelta_bias, dinitial_state), dx, dB and
+    dC in x's dtype, ddelta in delta's, the others float32; dinitial_state None unless need_d_state."""
+    b, T, H, P, G, N = _scan_check(x, delta, A, B, C, D, delta_bias)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise RuntimeError(f"verace_amd: dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    _same_device(x, dy=dy, d_state=d_state, initial_state=initial_state)
+    lengths = _lengths(lengths, b, x)
+    shape = delta.shape
+    if delta.dim() == 4:
+        delta = delta.squeeze(-1)
+    for name, t in (("initial_state", initial_state), ("d_state", d_state)):
+        if t is not None and tuple(t.shape) != (b, H, P, N):
+            raise RuntimeError(f"verace_amd: {name} must be {(b, H, P, N)}, got {tuple(t.shape)}")
+    state, d_state = (None if t is None else t.to(torch.float32).contiguous() for t in (initial_state, d_state))
+    A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
+    x, delta, B, C, dy = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2), _inner(dy, 2)
+
+    def new(like, dtype=None):
+        return torch.empty(like.shape, device=x.device, dtype=dtype or like.dtype)
+    dx, dd, dB, dC = new(x), new(delta), new(B), new(C)
+    heads = torch.empty(3, H, device=x.device, dtype=torch.float32)
+    d0 = torch.empty(b, H, P, N, device=x.device, dtype=torch.float32) if need_d_state else None
+    if b == 0 or T == 0:
+        heads.zero_()
+        if d0 is not None:
+            d0.zero_() if d_state is None else d0.copy_(d_state)
+        return dx, dd.view(shape), heads[0], dB, dC, heads[1], heads[2], d0
+    code = _lib.dtype_code(x.dtype)
+    lib = _lib.load()
+    ws_bytes = ctypes.c_size_t(0)
+    _lib.check(lib.vmi_selective_scan_bwd_workspace_bytes(b, T, H, P, G, N, code, ctypes.byref(ws_bytes)),
+               "vmi_selective_scan_bwd_workspace_bytes")
+    ws = torch.empty(ws_bytes.value, device=x.device, dtype=torch.uint8)
+    with device_guard(x):
+        _lib.check(lib.vmi_selective_scan_bwd(
+            _ptr(x), x.stride(1), x.stride(0), _ptr(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
+            _ptr(A), _ptr(B), B.stride(1), B.stride(0), _ptr(C), C.stride(1), C.stride(0), _ptr(D), _ptr(bias),
+            int(bool(softplus)), code, _ptr(state), _ptr(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), _ptr(dy), dy.stride(1), dy.stride(0),
+            _ptr(d_state), _ptr(dx), _ptr(dd), _ptr(heads[0]), _ptr(dB), _ptr(dC), _ptr(heads[1]), _ptr(heads[2]),
+            _ptr(d0), b, T, H, P, G, N, _ptr(ws), ws_bytes.value, _lib.stream_handle(x.device)),
+            "vmi_selective_scan_bwd")
+    return dx, dd.view(shape), heads[0], dB, dC, heads[1], heads[2], d0
+
+
+class SelectiveScanFunction(torch.autograd.Function):
+    """:func:`selective_scan` as an autograd node: only the inputs are kept, the backward makes the states of
+    every chunk again."""
+
+    @staticmethod
+    def forward(ctx, x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths):
+        y, state = launch_selective_hip_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
+        ctx.save_for_backward(x, delta, A, B, C, D, delta_bias, initial_state, lengths)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, d_state):
+        x, delta, A, B, C, D, delta_bias, initial_state, lengths = ctx.saved_tensors
+        dy = torch.zeros_like(x) if dy is None else dy
+        need0 = initial_state is not None and ctx.needs_input_grad[8]
+        dx, dd, dA, dB, dC, dD, dbias, d0 = launch_selective_hip_scan_bwd(
+            x, delta, A, B, C, dy, D, delta_bias, ctx.softplus, initial_state, lengths, d_state, need0)
+        return (dx, dd, dA.to(A.dtype), dB, dC, None if D is None else dD.to(D.dtype),
+                None if delta_bias is None else dbias.to(delta_bias.dtype), None,
+                d0.to(initial_state.dtype) if need0 else None, None)
+
+
 def selective_scan(
     x: torch.Tensor,
     delta: torch.Tensor,
@@ -276,7 +349,7 @@ def selective_scan(
     initial_state: Optional[torch.Tensor] = None,
     lengths: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Selective state space scan.
+    """Selective state space scan, differentiable once in every tensor argument but ``lengths``.
 
     x: [batch, seq_len, num_heads, head_dim]; delta: [batch, seq_len, num_heads] (any of the three
     dtypes); A: [num_heads] decay rates (negative for a decaying state); B, C: [batch, seq_len, groups, N]
@@ -287,6 +360,9 @@ def selective_scan(
     and C may be slices of wider rows.  head_dim <= 1024, N <= 256.  Returns (y in x's dtype, final_state
     float32); y behind a sequence's length is 0 and nothing of the inputs there is used.
     """
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, delta, A, B, C, D, delta_bias, initial_state)):
+        return SelectiveScanFunction.apply(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
     return launch_selective_hip_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
 
 
