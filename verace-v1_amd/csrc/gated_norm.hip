@@ -39,7 +39,7 @@ struct Args {
   int64_t rows;
   int d, silu;
   float eps1, eps2;
-  bool vec;
+  bool vec, wide;
 };
 
 // Sum over the G lanes of a row: a wave, or the whole workgroup (red: one float a wave; the barrier after
@@ -54,6 +54,23 @@ template <int G> __device__ __forceinline__ float row_sum(float x, float* red) {
     __syncthreads();
   }
   return x;
+}
+
+// N weights from element i on: whole 16-byte pieces where the rows are (wide), element loads otherwise.
+template <typename W, int N> __device__ __forceinline__ void load_w(const void* base, int i, int d, bool wide, float (&x)[N]) {
+  const W* p = static_cast<const W*>(base);
+  constexpr int EL = Vec<W>::N;
+  if (wide) {
+#pragma unroll
+    for (int q = 0; q < N / EL; ++q) {
+      const Vec<W> v = ldv(p + i + q * EL);
+#pragma unroll
+      for (int j = 0; j < EL; ++j) x[q * EL + j] = io<W>::to_f32(v.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = i + j < d ? io<W>::load(p, i + j) : 0.f;
+  }
 }
 
 // act(gate) and its derivative
@@ -96,18 +113,19 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   for (int v = 0; v < NV; ++v) {
     const int i = (lane + G * v) * N;
     if (i >= d) break;
+    float w1[N], sc[N];
+    if (a.w1 != nullptr) load_w<W>(a.w1, i, d, a.wide, w1);
+    if (a.scale != nullptr) load_w<W>(a.scale, i, d, a.wide, sc);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (!a.vec && i + j >= d) break;
       float r = t[v][j] * i1;
-      if (a.w1 != nullptr) r *= io<W>::load(static_cast<const W*>(a.w1), i + j);
+      if (a.w1 != nullptr) r *= w1[j];
       if (gate != nullptr) {
         float da;
         activation<T>(q[v][j], a.silu, q[v][j], da);
         r *= q[v][j];
       }
-      t[v][j] = a.scale != nullptr ? fmaf(io<W>::load(static_cast<const W*>(a.scale), i + j), r, x[v][j])
-                                   : x[v][j] + r;
+      t[v][j] = a.scale != nullptr ? fmaf(sc[j], r, x[v][j]) : x[v][j] + r;
       ss = fmaf(t[v][j], t[v][j], ss);
     }
     store_piece(static_cast<T*>(a.s) + row * d, i, d, a.vec, t[v]);
@@ -120,11 +138,10 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   for (int v = 0; v < NV; ++v) {
     const int i = (lane + G * v) * N;
     if (i >= d) break;
+    float w2[N];
+    load_w<W>(a.w2, i, d, a.wide, w2);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (!a.vec && i + j >= d) break;
-      t[v][j] *= i2 * io<W>::load(static_cast<const W*>(a.w2), i + j);
-    }
+    for (int j = 0; j < N; ++j) t[v][j] *= i2 * w2[j];
     store_piece(static_cast<T*>(a.n) + row * d, i, d, a.vec, t[v]);
   }
 }
@@ -158,19 +175,21 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < N; ++j) dt[v][j] = 0.f;
       if (dn == nullptr) continue;
-      float x[N], z[N];
+      float x[N], z[N], w1[N], sc[N], w2[N];
       load_piece(res, i, d, a.vec, x);
       load_piece(dn, i, d, a.vec, z);
+      if (a.w1 != nullptr) load_w<W>(a.w1, i, d, a.wide, w1);
+      if (a.scale != nullptr) load_w<W>(a.scale, i, d, a.wide, sc);
+      load_w<W>(a.w2, i, d, a.wide, w2);
 #pragma unroll
       for (int j = 0; j < N; ++j) {  // s again, u = dn w2 and u . s
-        if (!a.vec && i + j >= d) break;
         float r = yv[v][j] * i1, act = 1.f, da;
-        if (a.w1 != nullptr) r *= io<W>::load(static_cast<const W*>(a.w1), i + j);
+        if (a.w1 != nullptr) r *= w1[j];
         if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
         r *= act;
-        const float s = a.scale != nullptr ? fmaf(io<W>::load(static_cast<const W*>(a.scale), i + j), r, x[j]) : x[j] + r;
+        const float s = a.scale != nullptr ? fmaf(sc[j], r, x[j]) : x[j] + r;
         b2[v][j] = fmaf(z[j], s * i2, b2[v][j]);
-        const float u = z[j] * io<W>::load(static_cast<const W*>(a.w2), i + j);
+        const float u = z[j] * w2[j];
         dot = fmaf(u, s, dot);
         t[v][j] = s;
         dt[v][j] = fmaf(i2, u, dt[v][j]);
@@ -191,11 +210,12 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
       const int i = (lane + G * v) * N;
       if (i >= d) break;
       if (a.dres != nullptr) store_piece(static_cast<T*>(a.dres) + row * d, i, d, a.vec, dt[v]);
+      float w1s[N], scs[N];
+      if (a.w1 != nullptr) load_w<W>(a.w1, i, d, a.wide, w1s);
+      if (a.scale != nullptr) load_w<W>(a.scale, i, d, a.wide, scs);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        if (!a.vec && i + j >= d) break;
-        const float w1 = a.w1 != nullptr ? io<W>::load(static_cast<const W*>(a.w1), i + j) : 1.f;
-        const float sc = a.scale != nullptr ? io<W>::load(static_cast<const W*>(a.scale), i + j) : 1.f;
+        const float w1 = a.w1 != nullptr ? w1s[j] : 1.f, sc = a.scale != nullptr ? scs[j] : 1.f;
         const float yn = yv[v][j] * i1;
         float act = 1.f, da = 0.f;
         if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
@@ -257,21 +277,25 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
   }
 }
 
-// dw[k][i] = sum of partial[b][k][i] over the blocks: 64 columns by 4 strided shares of the blocks.
+// dw[k][i] = sum of partial[b][k][i] over the blocks: 32 columns by 32 strided shares of the blocks.
 template <typename W>
-__global__ __launch_bounds__(NTH) void weights_kernel(const float* __restrict__ partial, W* dw1, W* dscale, W* dw2,
-                                                      int blocks, int d) {
-  __shared__ float part[4][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ partial, W* dw1, W* dscale, W* dw2,
+                                                       int blocks, int d) {
+  __shared__ float part[32][33];
+  const int c = threadIdx.x & 31, share = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
   float s = 0.f;
   if (col < 3 * d)
-    for (int b = share; b < blocks; b += 4) s += partial[static_cast<int64_t>(b) * 3 * d + col];
-  part[share][threadIdx.x & 63] = s;
+    for (int b = share; b < blocks; b += 32) s += partial[static_cast<int64_t>(b) * 3 * d + col];
+  part[share][c] = s;
   __syncthreads();
-  if (share != 0 || col >= 3 * d) return;
-  const int k = col / d, i = col - k * d, c = threadIdx.x;
+  s = part[c][share];  // a column's shares in 32 neighbouring lanes
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+  const int out = blockIdx.x * 32 + share;
+  if (c != 0 || out >= 3 * d) return;
+  const int k = out / d, i = out - k * d;
   W* dst = k == 0 ? dw1 : k == 1 ? dscale : dw2;
-  if (dst != nullptr) io<W>::store(dst, i, (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]));
+  if (dst != nullptr) io<W>::store(dst, i, s);
 }
 
 // A wave takes rows of up to two pieces a lane, a workgroup longer ones; at most 8 pieces a lane.
@@ -330,6 +354,7 @@ extern "C" int vmi_gated_norm(const void* y, int64_t y_stride, const void* resid
   if (rows == 0) return VMI_OK;
   if ((w2 != nullptr) != (n != nullptr) || s == nullptr) return VMI_ERR_INVALID_ARG;
   a.vec = vectors(a, dtype);
+  a.wide = a.vec && aligned16({w1, scale, w2});
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     return by_weight<T>(w_dtype, dtype, [&](auto wtag) -> int {
@@ -377,6 +402,7 @@ extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* r
   }
   if (rows == 0 && !weights) return VMI_OK;
   a.vec = vectors(a, dtype);
+  a.wide = a.vec && aligned16({w1, scale, w2});
   hipStream_t st = static_cast<hipStream_t>(stream);
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
@@ -390,7 +416,7 @@ extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* r
           return hip_status(hipGetLastError());
         });
       if (rc != VMI_OK || !weights) return rc;
-      hipLaunchKernelGGL(weights_kernel<W>, dim3(static_cast<unsigned>((3 * d + 63) / 64)), dim3(NTH), 0, st,
+      hipLaunchKernelGGL(weights_kernel<W>, dim3(static_cast<unsigned>((3 * d + 31) / 32)), dim3(1024), 0, st,
                          a.partial, static_cast<W*>(dw1), static_cast<W*>(dscale), static_cast<W*>(dw2), blocks,
                          a.d);
       return hip_status(hipGetLastError());

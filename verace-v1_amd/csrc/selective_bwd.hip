@@ -53,14 +53,14 @@ struct Bwd {
   void *dx, *ddelta, *db, *dc;
   float *dA, *dD, *dbias, *dstate_in;
   int nch, seg_chunks, nseg, pblocks, hblocks, hper;
-  bool vec_x, vec_dy, vec_bc, vec_dx;
+  bool vec, vec_dx;
 };
 
 // ------------------------------------------------------------------ S_0 and G_L of every chunk
 // Four waves, 16 rows p each: tile j, register r = row p0 + 16 wave + 4 g + r, column n = 16 j + l16.  Forward:
 // S += (d_s e^{c_L - c_s} x_s) B_s^T; reverse, chunks from the last: G += (e^{c_t} dy_t) C_t^T.
-template <typename IO, typename E, int NP, int L, bool OWN>
-__global__ __launch_bounds__(SNT) void states_kernel(Bwd k) {
+template <typename IO, typename E, int NP, int L, bool OWN, bool VEC>
+__global__ __launch_bounds__(SNT, 2) void states_kernel(Bwd k) {
   constexpr int NT = NP / 16, KB = L / 32, NPART = Parts<E>::N;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
@@ -85,19 +85,20 @@ __global__ __launch_bounds__(SNT) void states_kernel(Bwd k) {
   const IO* x = static_cast<const IO*>(reverse ? k.dy : a.x) + b * (reverse ? k.y_b : a.x_b) + static_cast<int64_t>(h) * a.P + p0;
   const IO* bm = static_cast<const IO*>(reverse ? a.cm : a.bm) + b * (reverse ? a.c_b : a.b_b) + static_cast<int64_t>(grp) * a.N;
   const int64_t x_t = reverse ? k.y_t : a.x_t, b_t = reverse ? a.c_t : a.b_t;
-  const bool vec_x = reverse ? k.vec_dy : k.vec_x;
   const int64_t tp = static_cast<int64_t>(k.nch) * L;
   const float* dp = k.d + bh * tp;
   const float2* cp = k.c + bh * tp;
 
-  Stage<IO, E, PB, L, SNT> sx;
-  Stage<IO, E, NP, L, SNT> sb;
+  Stage<IO, E, PB, L, SNT, VEC> sx;
+  Stage<IO, E, NP, L, SNT, VEC> sb;
+  sx.init(x, x_t, a.P - p0);
+  sb.init(bm, b_t, a.N);
   float rd = 0.f;
   float2 rc = make_float2(0.f, 0.f), rl = rc;
   auto chunk = [&](int i) { return reverse ? last - 1 - i : first + i; };
   auto fetch = [&](int c) {
-    sx.fetch(x, x_t, c * L, len, a.P - p0, vec_x);
-    sb.fetch(bm, b_t, c * L, len, a.N, k.vec_bc);
+    sx.fetch(c * L, len);
+    sb.fetch(c * L, len);
     if (tid < L) {
       rd = dp[c * L + tid];
       rc = cp[c * L + tid];
@@ -156,10 +157,14 @@ __global__ __launch_bounds__(SNT) void states_kernel(Bwd k) {
       Frag<E> part[NPART];
       split<E>(wx, part);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const Frag<E> bt = col_frag<E, NP>(Bs, 32 * kb, 16 * j, l16, g);
+      for (int j0 = 0; j0 < NT; j0 += 4) {  // four chains in flight
+        Frag<E> bt[4];
 #pragma unroll
-        for (int q = NPART - 1; q >= 0; --q) S[j] = mma(part[q], bt, S[j]);
+        for (int j = 0; j < 4; ++j) bt[j] = col_frag<E, NP>(Bs, 32 * kb, 16 * (j0 + j), l16, g);
+#pragma unroll
+        for (int q = NPART - 1; q >= 0; --q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) S[j0 + j] = mma(part[q], bt[j], S[j0 + j]);
       }
     }
   }
@@ -234,7 +239,7 @@ template <int LT> __device__ __forceinline__ bool lower_tile(int i, int& tt, int
   return false;
 }
 
-template <typename IO, typename E, int NP, int L>
+template <typename IO, typename E, int NP, int L, bool VEC>
 __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::N;
   constexpr int NTW = NT >= NW ? NT / NW : 1;      // n-tiles of a wave: wave, wave + 8 (or wave % NT)
@@ -277,22 +282,26 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
 
   if (t0 < len) {
     {
-      Stage<IO, E, NP, L, MNT> sb, sc;
-      sb.fetch(static_cast<const IO*>(a.bm) + b * a.b_b + static_cast<int64_t>(grp) * a.N, a.b_t, t0, len, a.N, k.vec_bc);
-      sc.fetch(static_cast<const IO*>(a.cm) + b * a.c_b + static_cast<int64_t>(grp) * a.N, a.c_t, t0, len, a.N, k.vec_bc);
+      Stage<IO, E, NP, L, MNT, VEC> sb, sc;
+      sb.init(static_cast<const IO*>(a.bm) + b * a.b_b + static_cast<int64_t>(grp) * a.N, a.b_t, a.N);
+      sc.init(static_cast<const IO*>(a.cm) + b * a.c_b + static_cast<int64_t>(grp) * a.N, a.c_t, a.N);
+      sb.fetch(t0, len);
+      sc.fetch(t0, len);
       sb.commit(Bs);
       sc.commit(Cs);
       for (int i = tid; i < TQ::elems(L); i += MNT) Qs[i] = Ms[i] = static_cast<E>(0.f);
     }
-    Stage<IO, E, PB, L, MNT> sx, sy;
+    Stage<IO, E, PB, L, MNT, VEC> sx, sy;
     float rd = 0.f;
     float2 rc = make_float2(0.f, 0.f), rl = rc;
     f32x4 s0[NTW][4], g1[NTW][4];
     const int units = (h1 - h0) * k.pblocks;
     auto fetch = [&](int u) {
       const int h = h0 + u / k.pblocks, p0 = u % k.pblocks * PB;
-      sx.fetch(static_cast<const IO*>(a.x) + b * a.x_b + static_cast<int64_t>(h) * a.P + p0, a.x_t, t0, len, a.P - p0, k.vec_x);
-      sy.fetch(static_cast<const IO*>(k.dy) + b * k.y_b + static_cast<int64_t>(h) * a.P + p0, k.y_t, t0, len, a.P - p0, k.vec_dy);
+      sx.init(static_cast<const IO*>(a.x) + b * a.x_b + static_cast<int64_t>(h) * a.P + p0, a.x_t, a.P - p0);
+      sy.init(static_cast<const IO*>(k.dy) + b * k.y_b + static_cast<int64_t>(h) * a.P + p0, k.y_t, a.P - p0);
+      sx.fetch(t0, len);
+      sy.fetch(t0, len);
       if (tid < L) {
         const int64_t o = (static_cast<int64_t>(b) * a.H + h) * tp + t0;
         rd = k.d[o + tid];
@@ -666,7 +675,7 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int 
   return p;
 }
 
-template <typename IO, typename E, int NP, int L> int run(Bwd k, const Plan& p, hipStream_t stream) {
+template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const Plan& p, hipStream_t stream) {
   const Args& a = k.a;
   const int64_t BHP = static_cast<int64_t>(a.B) * a.H * p.pblocks, wgs = BHP * p.nseg;
   const int64_t blocks = static_cast<int64_t>(a.B) * p.nch * a.G * p.hblocks;
@@ -676,16 +685,16 @@ template <typename IO, typename E, int NP, int L> int run(Bwd k, const Plan& p, 
   if (st != VMI_OK) return st;
   const dim3 grid(static_cast<unsigned>(wgs), 2);
   if (p.nseg > 1) {
-    hipLaunchKernelGGL((states_kernel<IO, E, NP, L, true>), grid, dim3(SNT), 0, stream, k);
+    hipLaunchKernelGGL((states_kernel<IO, E, NP, L, true, VEC>), grid, dim3(SNT), 0, stream, k);
     if (!ok(st)) return st;
     const int64_t pieces = (BHP * (NP * PB / 4) + SNT - 1) / SNT;
     if (pieces > INT32_MAX) return VMI_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(starts_kernel<NP>, dim3(static_cast<unsigned>(pieces), 2), dim3(SNT), 0, stream, k, L);
     if (!ok(st)) return st;
   }
-  hipLaunchKernelGGL((states_kernel<IO, E, NP, L, false>), grid, dim3(SNT), 0, stream, k);
+  hipLaunchKernelGGL((states_kernel<IO, E, NP, L, false, VEC>), grid, dim3(SNT), 0, stream, k);
   if (!ok(st)) return st;
-  hipLaunchKernelGGL((main_kernel<IO, E, NP, L>), dim3(static_cast<unsigned>(blocks)), dim3(MNT), 0, stream, k);
+  hipLaunchKernelGGL((main_kernel<IO, E, NP, L, VEC>), dim3(static_cast<unsigned>(blocks)), dim3(MNT), 0, stream, k);
   if (!ok(st)) return st;
   const int heads = (3 * a.H + 63) / 64;
   const int64_t elems = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
@@ -697,9 +706,13 @@ template <typename IO, typename E, int NP, int L> int run(Bwd k, const Plan& p, 
 }
 
 template <typename IO, typename E, int L> int by_state(const Bwd& k, const Plan& p, hipStream_t stream) {
-  if (p.np == 64) return run<IO, E, 64, L>(k, p, stream);
-  if (p.np == 128) return run<IO, E, 128, L>(k, p, stream);
-  return run<IO, E, 256, L>(k, p, stream);
+  auto go = [&](auto np) -> int {
+    constexpr int NP = decltype(np)::value;
+    return k.vec ? run<IO, E, NP, L, true>(k, p, stream) : run<IO, E, NP, L, false>(k, p, stream);
+  };
+  if (p.np == 64) return go(std::integral_constant<int, 64>{});
+  if (p.np == 128) return go(std::integral_constant<int, 128>{});
+  return go(std::integral_constant<int, 256>{});
 }
 
 }  // namespace
@@ -734,10 +747,9 @@ int launch_bwd(const Args& a, int dtype, const Grads& q, void* workspace, hipStr
   k.nch = static_cast<int>(p.nch), k.seg_chunks = p.seg_chunks, k.nseg = p.nseg, k.pblocks = p.pblocks;
   k.hblocks = p.hblocks, k.hper = p.hper;
   const int el = dtype == VMI_F32 ? 4 : 8;
-  k.vec_x = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && aligned16({a.x});
-  k.vec_dy = a.P % el == 0 && q.y_t % el == 0 && q.y_b % el == 0 && aligned16({q.dy});
-  k.vec_bc = a.N % el == 0 && a.b_t % el == 0 && a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 &&
-             aligned16({a.bm, a.cm});
+  k.vec = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && q.y_t % el == 0 && q.y_b % el == 0 &&
+          a.N % el == 0 && a.b_t % el == 0 && a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 &&
+          aligned16({a.x, q.dy, a.bm, a.cm});
   k.vec_dx = a.P % 4 == 0 && aligned16({q.dx});
   if (dtype == VMI_BF16) return by_state<bf16_t, __bf16, 64>(k, p, stream);
   if (dtype == VMI_F16) return by_state<f16_t, float, 32>(k, p, stream);

@@ -38,7 +38,7 @@ struct Chunks {
   float* seg_state;          // [Sg][BH][P][N]: a segment's own state, then its start state
   float* seg_decay;          // [Sg][BH]
   int nch, seg_chunks, nseg, pblocks;
-  bool vec_x, vec_bc, vec_state, vec_y;
+  bool vec, vec_state, vec_y;
 };
 
 // ------------------------------------------------------------------ step sizes and log decays
@@ -89,8 +89,8 @@ template <> struct Tiles<32> {
   }
 };
 
-template <typename IO, typename E, int NP, int L, bool READOUT>
-__global__ __launch_bounds__(NTH) void pass_kernel(Chunks k) {
+template <typename IO, typename E, int NP, int L, bool READOUT, bool VEC>
+__global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
   constexpr int NT = NP / 16, LT = L / 16, KB = L / 32, KN = NP / 32, NPART = Parts<E>::N;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
@@ -122,14 +122,17 @@ __global__ __launch_bounds__(NTH) void pass_kernel(Chunks k) {
   const float* dp = k.d + bh * tp;
   const float2* cp = k.c + bh * tp;
 
-  Stage<IO, E, PB, L, NTH> sx;
-  Stage<IO, E, NP, L, NTH> sb, sc;
+  Stage<IO, E, PB, L, NTH, VEC> sx;
+  Stage<IO, E, NP, L, NTH, VEC> sb, sc;
+  sx.init(x, a.x_t, a.P - p0);
+  sb.init(bm, a.b_t, a.N);
+  if constexpr (READOUT) sc.init(cm, a.c_t, a.N);
   float rd = 0.f;
   float2 rc = make_float2(0.f, 0.f), rl = rc;
   auto fetch = [&](int c) {
-    sx.fetch(x, a.x_t, c * L, len, a.P - p0, k.vec_x);
-    sb.fetch(bm, a.b_t, c * L, len, a.N, k.vec_bc);
-    if constexpr (READOUT) sc.fetch(cm, a.c_t, c * L, len, a.N, k.vec_bc);
+    sx.fetch(c * L, len);
+    sb.fetch(c * L, len);
+    if constexpr (READOUT) sc.fetch(c * L, len);
     if (tid < L) {
       rd = dp[c * L + tid];
       rc = cp[c * L + tid];
@@ -230,11 +233,16 @@ __global__ __launch_bounds__(NTH) void pass_kernel(Chunks k) {
           wx[hf] = half(xf[kb], hf) * *reinterpret_cast<const f32x4*>(ws + 32 * kb + 16 * hf + 4 * g);
         Frag<E> part[NPART];
         split<E>(wx, part);
+        constexpr int JB = NT < 4 ? NT : 4;  // chains in flight
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const Frag<E> bt = col_frag<E, NP>(Bs, 32 * kb, 16 * j, l16, g);
+        for (int j0 = 0; j0 < NT; j0 += JB) {
+          Frag<E> bt[JB];
 #pragma unroll
-          for (int q = NPART - 1; q >= 0; --q) S[j] = mma(bt, part[q], S[j]);
+          for (int j = 0; j < JB; ++j) bt[j] = col_frag<E, NP>(Bs, 32 * kb, 16 * (j0 + j), l16, g);
+#pragma unroll
+          for (int q = NPART - 1; q >= 0; --q)
+#pragma unroll
+            for (int j = 0; j < JB; ++j) S[j0 + j] = mma(bt[j], part[q], S[j0 + j]);
         }
       }
     }
@@ -368,7 +376,7 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
   return p;
 }
 
-template <typename IO, typename E, int NP, int L>
+template <typename IO, typename E, int NP, int L, bool VEC>
 int run(Chunks k, const Plan& p, hipStream_t stream) {
   const Args& a = k.a;
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * p.pblocks * p.nseg;
@@ -378,7 +386,7 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
       st != VMI_OK)
     return st;
   if (p.nseg > 1) {
-    hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, false>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+    hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, false, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
     const bool vec = PN % 4 == 0 && aligned16({a.state_in});
     const int64_t blocks = (BH * PN / (vec ? 4 : 1) + NTH - 1) / NTH;
@@ -387,15 +395,19 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
                        k.seg_decay, a.state_in, p.nseg, BH, PN, vec);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
   }
-  hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, true>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+  hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, true, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
   return hip_status(hipGetLastError());
 }
 
 template <typename IO, typename E, int L> int by_state(const Chunks& k, const Plan& p, hipStream_t stream) {
-  if (k.a.N <= 32) return run<IO, E, 32, L>(k, p, stream);
-  if (k.a.N <= 64) return run<IO, E, 64, L>(k, p, stream);
-  if (k.a.N <= 128) return run<IO, E, 128, L>(k, p, stream);
-  return run<IO, E, 256, L>(k, p, stream);
+  auto go = [&](auto np) -> int {
+    constexpr int NP = decltype(np)::value;
+    return k.vec ? run<IO, E, NP, L, true>(k, p, stream) : run<IO, E, NP, L, false>(k, p, stream);
+  };
+  if (k.a.N <= 32) return go(std::integral_constant<int, 32>{});
+  if (k.a.N <= 64) return go(std::integral_constant<int, 64>{});
+  if (k.a.N <= 128) return go(std::integral_constant<int, 128>{});
+  return go(std::integral_constant<int, 256>{});
 }
 
 }  // namespace
@@ -426,9 +438,8 @@ int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) 
   k.seg_decay = reinterpret_cast<float*>(w + p.c_bytes + p.d_bytes + p.state_bytes);
   k.nch = static_cast<int>(p.nch), k.seg_chunks = p.seg_chunks, k.nseg = p.nseg, k.pblocks = p.pblocks;
   const int el = dtype == VMI_F32 ? 4 : 8;
-  k.vec_x = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && aligned16({a.x});
-  k.vec_bc = a.N % el == 0 && a.b_t % el == 0 && a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 &&
-             aligned16({a.bm, a.cm});
+  k.vec = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && a.N % el == 0 && a.b_t % el == 0 &&
+          a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 && aligned16({a.x, a.bm, a.cm});
   k.vec_state = a.N % 4 == 0 && aligned16({a.state_in, a.state_out});
   k.vec_y = a.P % 4 == 0 && aligned16({a.y});
   if (dtype == VMI_BF16) return by_state<bf16_t, __bf16, 64>(k, p, stream);

@@ -125,38 +125,56 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// A tile's rows on their way from global memory: NTH threads hold PER 16-byte pieces each.
-template <typename IO, typename E, int W, int ROWS, int NTH> struct Stage {
+// A tile's rows on their way from global memory: NTH threads hold PER 16-byte pieces each, all of one column.
+// VEC: whole aligned pieces; else element by element.
+template <typename IO, typename E, int W, int ROWS, int NTH, bool VEC> struct Stage {
   static constexpr int EL = 16 / sizeof(IO);
   static constexpr int PR = W / EL;                       // pieces of a row
   static constexpr int PER = (ROWS * PR + NTH - 1) / NTH;
+  static constexpr int STEP = NTH / PR;                   // rows between a thread's pieces
+  static_assert(NTH % PR == 0, "");
   uint4 v[PER];
-  // rows t0 .. t0 + ROWS - 1 of `base` (row stride in elements), columns below `cols`, rows below `end`; else 0
-  __device__ __forceinline__ void fetch(const IO* base, int64_t stride, int t0, int end, int cols, bool vec) {
+  const IO* src;   // this thread's piece of row 0
+  int64_t stride;
+  int row, left;   // first row, and columns from the piece's first on
+  __device__ __forceinline__ void init(const IO* base, int64_t stride_, int cols) {
+    const int c = threadIdx.x % PR * EL;
+    row = threadIdx.x / PR, left = cols - c, stride = stride_;
+    src = base + row * stride + c;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int p = threadIdx.x + NTH * i, row = p / PR, c = (p - row * PR) * EL;
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (p >= ROWS * PR || t0 + row >= end || c >= cols) continue;
-      const IO* src = base + (t0 + row) * stride + c;
-      if (vec) {
-        v[i] = *reinterpret_cast<const uint4*>(src);
-      } else {
-        struct alignas(16) V { IO e[EL]; };
-        V q = __builtin_bit_cast(V, v[i]);
+    for (int i = 0; i < PER; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ uint4 piece(const IO* p) const {
+    if constexpr (VEC) {
+      return *reinterpret_cast<const uint4*>(p);
+    } else {
+      struct alignas(16) V { IO e[EL]; };
+      V q = __builtin_bit_cast(V, make_uint4(0, 0, 0, 0));
 #pragma unroll
-        for (int j = 0; j < EL; ++j)
-          if (c + j < cols) q.e[j] = src[j];
-        v[i] = __builtin_bit_cast(uint4, q);
-      }
+      for (int j = 0; j < EL; ++j)
+        if (j < left) q.e[j] = p[j];
+      return __builtin_bit_cast(uint4, q);
+    }
+  }
+  // rows t0 .. t0 + ROWS - 1, zeros from row `end` on
+  __device__ __forceinline__ void fetch(int t0, int end) {
+    if (left <= 0) return;
+    const IO* p = src + t0 * stride;
+    if (t0 + ROWS <= end) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (PER * NTH == ROWS * PR || row + STEP * i < ROWS) v[i] = piece(p + STEP * i * stride);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        v[i] = row + STEP * i < ROWS && t0 + row + STEP * i < end ? piece(p + STEP * i * stride) : make_uint4(0, 0, 0, 0);
     }
   }
   __device__ __forceinline__ void commit(E* tile) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int p = threadIdx.x + NTH * i, row = p / PR, c = (p - row * PR) * EL;
-      if (p >= ROWS * PR) continue;
-      E* dst = tile + Tile<E, W>::at(row) + c;
+      if (PER * NTH != ROWS * PR && row + STEP * i >= ROWS) continue;
+      E* dst = tile + Tile<E, W>::at(row + STEP * i) + threadIdx.x % PR * EL;
       if constexpr (sizeof(IO) == sizeof(E)) {
         *reinterpret_cast<uint4*>(dst) = v[i];
       } else {  // fp16 -> fp32

@@ -9,8 +9,8 @@
 //   dz = dy act'(z);  drow[t] = sum_j w[j] dz[t + (K - 1) - j] (+ the state's gradient for its rows);
 //   dw[j] = sum_t dz[t] row[t - (K - 1) + j],  dbias = sum_t dz[t]
 //
-// Bound by memory: x (and dy) read once, y (dx) written once; sums are fp32.  A thread takes one 16-byte
-// piece of the channels and slides down RUN tokens with the last K rows in registers, so the rows that
+// Bound by memory: x (and dy) read once, y (dx) written once; sums are fp32.  A thread takes four
+// channels and slides down RUN tokens with the last K rows in registers, so the rows that
 // two runs share (K - 1 of RUN) are the only ones read twice.  The weights' gradients leave a workgroup
 // as one partial row per channel and are added by a second kernel in a fixed order.
 #include <algorithm>
@@ -24,9 +24,10 @@ namespace vmi {
 namespace sconv {
 
 constexpr int NTH = 256;
+constexpr int PIECE = 4;     // channels of a thread (one, where C or an address does not divide)
 constexpr int RUN = 16;       // tokens of a thread, forward
 constexpr int BRUN = 32;      // rows of a thread, backward
-constexpr int CT = 32;        // channel pieces of a backward workgroup, by NTH / CT runs
+constexpr int CT = 64;        // channel pieces of a backward workgroup, by NTH / CT runs
 
 struct Args {
   const void *x, *w, *bias, *state_in;
@@ -40,6 +41,7 @@ struct Args {
   int64_t dy_stride, dy_batch;
   int B, T, C, w_dtype, act, lengths64;
   int pieces, runs;
+  bool wide;                   // w and bias 16-byte aligned
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
@@ -48,39 +50,60 @@ __device__ __forceinline__ int length_of(const Args& a, int b) {
   return static_cast<int>(n < 0 ? 0 : n > a.T ? a.T : n);
 }
 
-template <typename T, int N> __device__ __forceinline__ void load(const T* p, float (&x)[N]) {
-  if constexpr (N == 1) {
-    x[0] = io<T>::load(p, 0);
-  } else {
-    const Vec<T> v = ldv(p);
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = io<T>::to_f32(v.e[j]);
-  }
+// N consecutive elements as they lie in memory, N = 4 or 1.
+template <typename T, int N> struct alignas(N * sizeof(T)) Raw { T e[N]; };
+template <typename T, int N> __device__ __forceinline__ Raw<T, N> raw(const T* p) {
+  return *reinterpret_cast<const Raw<T, N>*>(p);
 }
-template <typename T, int N> __device__ __forceinline__ void store(T* p, const float (&x)[N]) {
-  if constexpr (N == 1) {
-    io<T>::store(p, 0, x[0]);
-  } else {
-    Vec<T> v;
+template <typename T, int N> __device__ __forceinline__ void widen(const Raw<T, N>& r, float (&x)[N]) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v.e[j] = round_to<T>(x[j]);
-    stv(p, v);
-  }
+  for (int j = 0; j < N; ++j) x[j] = io<T>::to_f32(r.e[j]);
+}
+template <typename T, int N> __device__ __forceinline__ void load(const T* p, float (&x)[N]) { widen<T, N>(raw<T, N>(p), x); }
+template <typename T, int N> __device__ __forceinline__ void store(T* p, const float (&x)[N]) {
+  Raw<T, N> r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r.e[j] = round_to<T>(x[j]);
+  *reinterpret_cast<Raw<T, N>*>(p) = r;
 }
 template <int N> __device__ __forceinline__ void zero(float (&x)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) x[j] = 0.f;
 }
 
+// M consecutive parameters of type W from element i on, four at a time where wide.
+template <typename W, int M>
+__device__ __forceinline__ void parameters(const void* base, int64_t i, bool wide, float (&x)[M]) {
+  const W* p = static_cast<const W*>(base) + i;
+  if (M % 4 == 0 && wide) {
+#pragma unroll
+    for (int q = 0; q < M; q += 4) {
+      const Raw<W, 4> v = raw<W, 4>(p + q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[q + j] = io<W>::to_f32(v.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < M; ++j) x[j] = io<W>::load(p, j);
+  }
+}
+template <int M>
+__device__ __forceinline__ void parameters(const void* base, int dtype, int64_t i, bool wide, float (&x)[M]) {
+  if (dtype == VMI_F32) parameters<float, M>(base, i, wide, x);
+  else if (dtype == VMI_BF16) parameters<bf16_t, M>(base, i, wide, x);
+  else parameters<f16_t, M>(base, i, wide, x);
+}
 // Weights and bias of channels c0 .. c0 + N - 1
 template <typename T, int K, int N>
 __device__ __forceinline__ void weights(const Args& a, int c0, float (&w)[K][N], float (&b)[N]) {
+  float flat[K * N];
+  parameters<K * N>(a.w, a.w_dtype, static_cast<int64_t>(c0) * K, a.wide, flat);
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
+  for (int j = 0; j < N; ++j)
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][j] = load_scalar(a.w, a.w_dtype, static_cast<int64_t>(c0 + j) * K + k);
-    b[j] = a.bias == nullptr ? 0.f : load_scalar(a.bias, a.w_dtype, c0 + j);
-  }
+    for (int k = 0; k < K; ++k) w[k][j] = flat[j * K + k];
+  if (a.bias != nullptr) parameters<N>(a.bias, a.w_dtype, c0, a.wide, b);
+  else zero(b);
 }
 
 // Row t of item b: the sequence's for t >= 0, the state's for -(K - 1) <= t < 0, zeros before.
@@ -107,12 +130,9 @@ __device__ __forceinline__ void conv(const float (&w)[K][N], const float (&b)[N]
 // Threads of run `runs` (one past the tokens') copy the final state.
 template <typename T, int K, int N>
 __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x;
-  const int64_t per = static_cast<int64_t>(a.pieces) * (a.runs + 1);
-  const int b = static_cast<int>(id / per);
-  if (b >= a.B) return;
-  const int rest = static_cast<int>(id - b * per);
-  const int run = rest / a.pieces, c0 = (rest - run * a.pieces) * N;
+  const int id = blockIdx.x * NTH + threadIdx.x, b = blockIdx.y;
+  const int run = id / a.pieces, c0 = (id - run * a.pieces) * N;
+  if (run > a.runs) return;
   const int n = length_of(a, b);
   if (run == a.runs) {
     if (a.state_out == nullptr) return;
@@ -126,7 +146,8 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   }
   const int t0 = run * RUN, t1 = min(t0 + RUN, a.T);
   T* y = static_cast<T*>(a.y) + (static_cast<int64_t>(b) * a.T + t0) * a.C + c0;
-  float w[K][N], bias[N], win[K][N], next[RUN][N];
+  float w[K][N], bias[N], win[K][N];
+  Raw<T, N> next[RUN];
   weights<T, K, N>(a, c0, w, bias);
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) {
@@ -136,7 +157,7 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   const T* xr = static_cast<const T*>(a.x) + b * a.x_batch + t0 * a.x_stride + c0;
 #pragma unroll
   for (int i = 0; i < RUN; ++i)  // every load of the run in flight at once
-    if (t0 + i < n) load<T, N>(xr + i * a.x_stride, next[i]);
+    if (t0 + i < n) next[i] = raw<T, N>(xr + i * a.x_stride);
 #pragma unroll
   for (int i = 0; i < RUN; ++i) {
     if (t0 + i >= t1) break;
@@ -146,8 +167,7 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
       for (int k = 0; k < K - 1; ++k)
 #pragma unroll
         for (int j = 0; j < N; ++j) win[k][j] = win[k + 1][j];
-#pragma unroll
-      for (int j = 0; j < N; ++j) win[K - 1][j] = next[i][j];
+      widen<T, N>(next[i], win[K - 1]);
       conv<T, K, N>(w, bias, win, z);
       if (a.act)
 #pragma unroll
@@ -161,11 +181,9 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
 
 // One token of every item: the state moves up a row.
 template <typename T, int K, int N>
-__global__ __launch_bounds__(NTH) void step_kernel(Args a) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x;
-  const int b = static_cast<int>(id / a.pieces);
-  if (b >= a.B) return;
-  const int c0 = static_cast<int>(id - static_cast<int64_t>(b) * a.pieces) * N;
+__global__ __launch_bounds__(64) void step_kernel(Args a) {
+  const int id = blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y, c0 = id * N;
+  if (id >= a.pieces) return;
   float w[K][N], bias[N], win[K][N], z[N];
   zero(z);
   if (a.mask == nullptr || a.mask[b] != 0) {
@@ -208,58 +226,76 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
       if (t0 - (K - 1) + k < n) row<T, K, N>(a, b, t0 - (K - 1) + k, c0, win[k + 1]);
       else zero(win[k + 1]);
     }
-    for (int u = t0; u < t1 + K - 1; ++u) {
+    constexpr int GRP = 8;  // tokens whose loads are in flight together
+    for (int u0 = t0; u0 < t1 + K - 1; u0 += GRP) {
+      Raw<T, N> xs[GRP], gs[GRP];
 #pragma unroll
-      for (int k = 0; k < K - 1; ++k)
+      for (int i = 0; i < GRP; ++i) {
+        const int u = u0 + i;
+        if (u < 0 || u >= n || u >= t1 + K - 1) continue;
+        xs[i] = raw<T, N>(static_cast<const T*>(a.x) + b * a.x_batch + u * a.x_stride + c0);
+        if (a.dy != nullptr) gs[i] = raw<T, N>(static_cast<const T*>(a.dy) + b * a.dy_batch + u * a.dy_stride + c0);
+      }
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          win[k][j] = win[k + 1][j];
-          dz[k][j] = dz[k + 1][j];
-        }
-      zero(dz[K - 1]);
-      if (u < n) {
-        row<T, K, N>(a, b, u, c0, win[K - 1]);
-        if (u >= 0 && a.dy != nullptr) {
-          float z[N], g[N];
-          load<T, N>(static_cast<const T*>(a.dy) + b * a.dy_batch + u * a.dy_stride + c0, g);
-          conv<T, K, N>(w, bias, win, z);
+      for (int i = 0; i < GRP; ++i) {
+        const int u = u0 + i;
+        if (u >= t1 + K - 1) break;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            if (a.act) {
-              const float sg = sigmoid_for<T>(z[j]);
-              g[j] *= sg * (1.f + z[j] * (1.f - sg));
-            }
-            dz[K - 1][j] = g[j];
+            win[k][j] = win[k + 1][j];
+            dz[k][j] = dz[k + 1][j];
           }
-          if (u < t1) {  // token u is this run's
+        zero(dz[K - 1]);
+        if (u < n) {
+          if (u < 0) {
+            row<T, K, N>(a, b, u, c0, win[K - 1]);
+          } else {
+            widen<T, N>(xs[i], win[K - 1]);
+            if (a.dy != nullptr) {
+              float z[N], g[N];
+              widen<T, N>(gs[i], g);
+              conv<T, K, N>(w, bias, win, z);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-              db[j] += dz[K - 1][j];
+              for (int j = 0; j < N; ++j) {
+                if (a.act) {
+                  const float sg = sigmoid_for<T>(z[j]);
+                  g[j] *= sg * (1.f + z[j] * (1.f - sg));
+                }
+                dz[K - 1][j] = g[j];
+              }
+              if (u < t1) {  // token u is this run's
 #pragma unroll
-              for (int k = 0; k < K; ++k) dw[k][j] = fmaf(dz[K - 1][j], win[k][j], dw[k][j]);
+                for (int j = 0; j < N; ++j) {
+                  db[j] += dz[K - 1][j];
+#pragma unroll
+                  for (int k = 0; k < K; ++k) dw[k][j] = fmaf(dz[K - 1][j], win[k][j], dw[k][j]);
+                }
+              }
             }
           }
         }
-      }
-      const int t = u - (K - 1);  // done: dz of t .. t + K - 1 are dz[0] .. dz[K - 1]
-      if (t < t0) continue;
-      float d[N];
+        const int t = u - (K - 1);  // done: dz of t .. t + K - 1 are dz[0] .. dz[K - 1]
+        if (t < t0) continue;
+        float d[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        d[j] = 0.f;
+        for (int j = 0; j < N; ++j) {
+          d[j] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) d[j] = fmaf(w[k][j], dz[K - 1 - k][j], d[j]);
-      }
-      if (a.dstate_out != nullptr && t < n && t >= n - (K - 1)) {
-        float g[N];
-        load<T, N>(static_cast<const T*>(a.dstate_out) + (static_cast<int64_t>(b) * (K - 1) + (t - n + K - 1)) * a.C + c0, g);
+          for (int k = 0; k < K; ++k) d[j] = fmaf(w[k][j], dz[K - 1 - k][j], d[j]);
+        }
+        if (a.dstate_out != nullptr && t < n && t >= n - (K - 1)) {
+          float g[N];
+          load<T, N>(static_cast<const T*>(a.dstate_out) + (static_cast<int64_t>(b) * (K - 1) + (t - n + K - 1)) * a.C + c0, g);
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] += g[j];
-      }
-      if (t >= 0) {
-        if (t < a.T && a.dx != nullptr) store<T, N>(static_cast<T*>(a.dx) + (static_cast<int64_t>(b) * a.T + t) * a.C + c0, d);
-      } else if (a.dstate_in != nullptr) {
-        store<T, N>(static_cast<T*>(a.dstate_in) + (static_cast<int64_t>(b) * (K - 1) + (t + K - 1)) * a.C + c0, d);
+          for (int j = 0; j < N; ++j) d[j] += g[j];
+        }
+        if (t >= 0) {
+          if (t < a.T && a.dx != nullptr) store<T, N>(static_cast<T*>(a.dx) + (static_cast<int64_t>(b) * a.T + t) * a.C + c0, d);
+        } else if (a.dstate_in != nullptr) {
+          store<T, N>(static_cast<T*>(a.dstate_in) + (static_cast<int64_t>(b) * (K - 1) + (t + K - 1)) * a.C + c0, d);
+        }
       }
     }
   }
@@ -311,12 +347,15 @@ template <typename T, typename F> int by_shape(const Args& a, int K, bool vec, F
     if (K == 3) return f(std::integral_constant<int, 3>{}, n);
     return f(std::integral_constant<int, 4>{}, n);
   };
-  return vec ? width(std::integral_constant<int, Vec<T>::N>{}) : width(std::integral_constant<int, 1>{});
+  return vec ? width(std::integral_constant<int, PIECE>{}) : width(std::integral_constant<int, 1>{});
 }
 bool vectors(const Args& a, int dtype) {
-  const int n = dtype == VMI_F32 ? 4 : 8;
-  return a.C % n == 0 && a.x_stride % n == 0 && a.x_batch % n == 0 && a.dy_stride % n == 0 && a.dy_batch % n == 0 &&
-         aligned16({a.x, a.state_in, a.y, a.state_out, a.dy, a.dstate_out, a.dx, a.dstate_in});
+  const size_t bytes = PIECE * (dtype == VMI_F32 ? 4 : 2);
+  for (const void* p : {a.x, a.state_in, static_cast<const void*>(a.y), static_cast<const void*>(a.state_out), a.dy,
+                        a.dstate_out, static_cast<const void*>(a.dx), static_cast<const void*>(a.dstate_in)})
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return false;
+  return a.C % PIECE == 0 && a.x_stride % PIECE == 0 && a.x_batch % PIECE == 0 && a.dy_stride % PIECE == 0 &&
+         a.dy_batch % PIECE == 0;
 }
 int check(int64_t B, int64_t T, int64_t C, int64_t K, int dtype, int w_dtype, int act) {
   if (B < 0 || T < 0 || C < 1 || K < 1 || act < 0 || act > 1) return VMI_ERR_INVALID_ARG;
@@ -348,15 +387,16 @@ extern "C" int vmi_short_conv(const void* x, int64_t x_stride, int64_t x_batch, 
   a.y = y, a.state_out = state_out, a.x_stride = x_stride, a.x_batch = x_batch;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.C = static_cast<int>(C), a.w_dtype = w_dtype, a.act = act;
   const bool vec = vectors(a, dtype);
+  a.wide = aligned16({a.w, a.bias});
   return by_type(dtype, [&](auto tag) -> int {
     using IO = decltype(tag);
-    a.pieces = vec ? a.C / Vec<IO>::N : a.C;
+    a.pieces = vec ? a.C / PIECE : a.C;
     a.runs = (a.T + RUN - 1) / RUN;
-    const int64_t blocks = (B * a.pieces * (a.runs + 1LL) + NTH - 1) / NTH;
-    if (blocks > INT32_MAX || static_cast<int64_t>(a.pieces) * (a.runs + 1LL) > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    const int64_t blocks = (a.pieces * (a.runs + 1LL) + NTH - 1) / NTH;
+    if (blocks > INT32_MAX / NTH) return VMI_ERR_UNSUPPORTED;
     return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
       hipLaunchKernelGGL((forward_kernel<IO, decltype(k)::value, decltype(n)::value>),
-                         dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, static_cast<hipStream_t>(stream), a);
+                         dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(B)), dim3(NTH), 0, static_cast<hipStream_t>(stream), a);
       return hip_status(hipGetLastError());
     });
   });
@@ -372,14 +412,13 @@ extern "C" int vmi_short_conv_step(const void* x, int64_t x_batch, const void* w
   a.x = x, a.w = w, a.bias = bias, a.mask = mask, a.state_out = state, a.y = y, a.x_batch = x_batch;
   a.B = static_cast<int>(B), a.T = 1, a.C = static_cast<int>(C), a.w_dtype = w_dtype, a.act = act;
   const bool vec = vectors(a, dtype);
+  a.wide = aligned16({a.w, a.bias});
   return by_type(dtype, [&](auto tag) -> int {
     using IO = decltype(tag);
-    a.pieces = vec ? a.C / Vec<IO>::N : a.C;
-    const int64_t blocks = (B * a.pieces + NTH - 1) / NTH;
-    if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    a.pieces = vec ? a.C / PIECE : a.C;
     return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
       hipLaunchKernelGGL((step_kernel<IO, decltype(k)::value, decltype(n)::value>),
-                         dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, static_cast<hipStream_t>(stream), a);
+                         dim3(static_cast<unsigned>((a.pieces + 63) / 64), static_cast<unsigned>(B)), dim3(64), 0, static_cast<hipStream_t>(stream), a);
       return hip_status(hipGetLastError());
     });
   });
@@ -416,12 +455,13 @@ extern "C" int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_bat
     a.partial = static_cast<float*>(workspace);
   }
   const bool vec = vectors(a, dtype);
+  a.wide = aligned16({a.w, a.bias});
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc = VMI_OK;
   if (B > 0)
     rc = by_type(dtype, [&](auto tag) -> int {
       using IO = decltype(tag);
-      a.pieces = vec ? a.C / Vec<IO>::N : a.C;
+      a.pieces = vec ? a.C / PIECE : a.C;
       a.runs = static_cast<int>(parts / B);
       return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
         hipLaunchKernelGGL((backward_kernel<IO, decltype(k)::value, decltype(n)::value>),
