@@ -69,7 +69,7 @@ __global__ __launch_bounds__(SNT, 2) void states_kernel(Bwd k) {
   __shared__ __attribute__((aligned(16))) float ws[L];
   __shared__ float wl;
   const Args& a = k.a;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const bool reverse = blockIdx.y != 0;
   const int pb = blockIdx.x % k.pblocks, rest = blockIdx.x / k.pblocks;
   // segments in the direction's order: seg 0 is the one with the given start
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   __shared__ float row_r[LT][L], col_r[LT][L];                  // sum_s R d_s by s-tile, sum_t R by t-tile
   __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
   const Args& a = k.a;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int hb = blockIdx.x % k.hblocks;
   int rest = blockIdx.x / k.hblocks;
   const int grp = rest % a.G;
@@ -502,11 +502,12 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         if (t0 + s < a.T && p < a.P && k.dx != nullptr) {
           const E* yr = Ys + TX::at(s) + 16 * pt + 4 * g;
           IO* o = static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0 + s) * a.H + h) * a.P + p;
-          struct alignas(4 * sizeof(IO)) V4 { IO e[4]; } v;
+          f32x4 q;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v.e[r] = round_to<IO>(fmaf(Dh, static_cast<float>(yr[r]), dx[t][r]));
+          for (int r = 0; r < 4; ++r) q[r] = fmaf(Dh, static_cast<float>(yr[r]), dx[t][r]);
+          const Out4<IO> v = out4<IO>(q);
           if (k.vec_dx) {
-            *reinterpret_cast<V4*>(o) = v;
+            *reinterpret_cast<Out4<IO>*>(o) = v;
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)

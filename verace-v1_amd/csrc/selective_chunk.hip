@@ -19,7 +19,6 @@
 // products (2^-8 of a term at most, as y's own rounding); the weighted x of the state's update enters as
 // three bf16 parts, so the state itself is carried in fp32 throughout.
 #include <algorithm>
-#include <type_traits>
 
 #include "selective_mfma.h"
 #include "vmi_vec.h"
@@ -28,6 +27,7 @@ namespace vmi {
 namespace sel {
 
 constexpr int NTH = 256;
+constexpr int L = 32;        // tokens of a chunk
 constexpr int PB = 64;       // rows p of a workgroup
 constexpr int MAX_SEG = 64;
 
@@ -42,27 +42,27 @@ struct Chunks {
 };
 
 // ------------------------------------------------------------------ step sizes and log decays
-template <int L>
+template <int LC>
 __global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d_out, float2* __restrict__ c_out,
                                                    int nch, int64_t units) {
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (NTH / L) + threadIdx.x / L;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (NTH / LC) + threadIdx.x / LC;
   if (unit >= units) return;
-  const int l = threadIdx.x % L;
+  const int l = threadIdx.x % LC;
   // heads fastest: neighbouring chunks of threads read neighbouring heads of the same tokens
   const int h = static_cast<int>(unit % a.H);
   const int64_t bc = unit / a.H;
-  const int b = static_cast<int>(bc / nch), n = static_cast<int>(bc - static_cast<int64_t>(b) * nch), t = n * L + l;
+  const int b = static_cast<int>(bc / nch), n = static_cast<int>(bc - static_cast<int64_t>(b) * nch), t = n * LC + l;
   float d = 0.f;
   if (t < length_of(a.lengths, a.lengths64, a.T, b))
     d = step_size(load_scalar(a.delta, a.delta_dtype, b * a.d_b + t * a.d_t + h) + (a.bias == nullptr ? 0.f : a.bias[h]),
                   a.softplus);
   double c = static_cast<double>(d) * static_cast<double>(a.A[h]);
 #pragma unroll
-  for (int off = 1; off < L; off <<= 1) {
-    const double up = __shfl_up(c, off, L);
+  for (int off = 1; off < LC; off <<= 1) {
+    const double up = __shfl_up(c, off, LC);
     if (l >= off) c += up;
   }
-  const int64_t o = (static_cast<int64_t>(b) * a.H + h) * (static_cast<int64_t>(nch) * L) + t;
+  const int64_t o = (static_cast<int64_t>(b) * a.H + h) * (static_cast<int64_t>(nch) * LC) + t;
   const float hi = static_cast<float>(c);
   d_out[o] = d;
   // an infinite or NaN sum has no low part
@@ -70,38 +70,19 @@ __global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d
 }
 
 // ------------------------------------------------------------------ the segments
-// Score tiles (t-tile, s-tile) on or below the diagonal, dealt to the waves.
-template <int L> struct Tiles;
-template <> struct Tiles<64> {
-  static constexpr int PER = 3;
-  static __device__ __forceinline__ bool get(int wave, int i, int& tt, int& st) {
-    constexpr uint32_t T[4] = {0x00'31'30, 0x10'33'32, 0x11'21'20, 0xff'ff'22};
-    const uint32_t q = (T[wave] >> (8 * i)) & 0xff;
-    tt = q >> 4, st = q & 15;
-    return q != 0xff;
-  }
-};
-template <> struct Tiles<32> {
-  static constexpr int PER = 1;
-  static __device__ __forceinline__ bool get(int wave, int, int& tt, int& st) {
-    tt = wave != 0, st = wave == 2;
-    return wave < 3;
-  }
-};
-
-template <typename IO, typename E, int NP, int L, bool READOUT, bool VEC>
-__global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
-  constexpr int NT = NP / 16, LT = L / 16, KB = L / 32, KN = NP / 32, NPART = Parts<E>::N;
+template <typename IO, typename E, int NP, bool READOUT, bool VEC>
+__global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass_kernel(Chunks k) {
+  constexpr int NT = NP / 16, LT = L / 16, KN = NP / 32, NPART = Parts<E>::N;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Cs[READOUT ? TB::elems(L) : 8];
+  __shared__ __attribute__((aligned(16))) E Cs[READOUT ? RowTile<E, NP>::elems(L) : 8];
   __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Ms[READOUT ? LT * KB * 64 * 8 : 8];
+  __shared__ __attribute__((aligned(16))) E Ms[READOUT ? LT * 64 * 8 : 8];
   __shared__ __attribute__((aligned(16))) float2 cs[L];
   __shared__ __attribute__((aligned(16))) float ds[L], ws[L];
   const Args& a = k.a;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   // neighbouring workgroups go to different XCDs: give each XCD a run of consecutive heads, which share B and C
   const uint32_t total = gridDim.x, per = total / 8, body = per * 8;
   uint32_t id = blockIdx.x;
@@ -165,8 +146,8 @@ __global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
       }
     }
   }
-  if constexpr (READOUT) {  // the tiles right of the diagonal that a block of 32 reads stay zero
-    for (int i = tid; i < LT * KB * 64 * 8; i += NTH) Ms[i] = static_cast<E>(0.f);
+  if constexpr (READOUT) {  // the tile right of the diagonal stays zero
+    for (int i = tid; i < LT * 64 * 8; i += NTH) Ms[i] = static_cast<E>(0.f);
   }
   const float Dh = a.D == nullptr ? 0.f : a.D[h];
   double seg_c = 0.0;
@@ -175,7 +156,7 @@ __global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
     lds_barrier();  // the last chunk's readers are done
     sx.commit(Xs);
     sb.commit(Bs);
-    if constexpr (READOUT) sc.commit(Cs);
+    if constexpr (READOUT) sc.commit_rows(Cs);
     if (tid < L) {
       cs[tid] = rc;
       ds[tid] = rd;
@@ -187,23 +168,22 @@ __global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
     f32x4 acc[LT];
     if constexpr (READOUT) {
       // scores, transposed (rows s, column t): (C_t . B_s) e^{c_t - c_s} d_s
-#pragma unroll
-      for (int i = 0; i < Tiles<L>::PER; ++i) {
-        int tt, st;
-        if (!Tiles<L>::get(wave, i, tt, st)) continue;
+      // three tiles on or below the diagonal, one wave each
+      if (wave < 3) {
+        const int tt = wave != 0, st = wave == 2;
         f32x4 m = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KN; ++kb)
-          m = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), row_frag<E, NP>(Cs, 16 * tt, 32 * kb, l16, g), m);
+          m = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), packed_frag<E, NP, L>(Cs, 16 * tt, 32 * kb, l16, g), m);
         const float2 ct = cs[16 * tt + l16];
-        struct alignas(8) M4 { E e[4]; } q;
+        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int s = 16 * st + 4 * g + r;
           const float v = m[r] * (decay(ct, cs[s]) * ds[s]);
           q.e[r] = static_cast<E>(s <= 16 * tt + l16 ? v : 0.f);
         }
-        *reinterpret_cast<M4*>(Ms + ((tt * KB + (st >> 1)) * 64 + lane) * 8 + 4 * (st & 1)) = q;
+        *reinterpret_cast<M4*>(Ms + (tt * 64 + lane) * 8 + 4 * st) = q;
       }
       // S_0 C_t, transposed: rows p, column t
 #pragma unroll
@@ -213,37 +193,32 @@ __global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
         for (int kb = 0; kb < KN; ++kb) {
           const Frag<E> s = acc_frag<E>(S[2 * kb], S[2 * kb + 1]);
 #pragma unroll
-          for (int t = 0; t < LT; ++t) acc[t] = mma(s, row_frag<E, NP>(Cs, 16 * t, 32 * kb, l16, g), acc[t]);
+          for (int t = 0; t < LT; ++t) acc[t] = mma(s, packed_frag<E, NP, L>(Cs, 16 * t, 32 * kb, l16, g), acc[t]);
         }
       }
     }
     const float2 cl = cs[L - 1];
-    Frag<E> xf[KB];
+    Frag<E> xf;
     if (live) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) xf[kb] = col_frag<E, PB>(Xs, 32 * kb, 16 * wave, l16, g);
+      xf = col_frag<E, PB>(Xs, 0, 16 * wave, l16, g);
       const float dl = __expf(cl.x + cl.y);
 #pragma unroll
       for (int j = 0; j < NT; ++j) S[j] *= dl;
+      f32x4 wx[2];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        f32x4 wx[2];
+      for (int hf = 0; hf < 2; ++hf) wx[hf] = half(xf, hf) * *reinterpret_cast<const f32x4*>(ws + 16 * hf + 4 * g);
+      Frag<E> part[NPART];
+      split<E>(wx, part);
+      constexpr int JB = NT < 4 ? NT : 4;  // chains in flight
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-          wx[hf] = half(xf[kb], hf) * *reinterpret_cast<const f32x4*>(ws + 32 * kb + 16 * hf + 4 * g);
-        Frag<E> part[NPART];
-        split<E>(wx, part);
-        constexpr int JB = NT < 4 ? NT : 4;  // chains in flight
+      for (int j0 = 0; j0 < NT; j0 += JB) {
+        Frag<E> bt[JB];
 #pragma unroll
-        for (int j0 = 0; j0 < NT; j0 += JB) {
-          Frag<E> bt[JB];
+        for (int j = 0; j < JB; ++j) bt[j] = col_frag<E, NP>(Bs, 0, 16 * (j0 + j), l16, g);
 #pragma unroll
-          for (int j = 0; j < JB; ++j) bt[j] = col_frag<E, NP>(Bs, 32 * kb, 16 * (j0 + j), l16, g);
+        for (int q = NPART - 1; q >= 0; --q)
 #pragma unroll
-          for (int q = NPART - 1; q >= 0; --q)
-#pragma unroll
-            for (int j = 0; j < JB; ++j) S[j0 + j] = mma(bt[j], part[q], S[j0 + j]);
-        }
+          for (int j = 0; j < JB; ++j) S[j0 + j] = mma(bt[j], part[q], S[j0 + j]);
       }
     }
     if constexpr (!READOUT) {
@@ -255,27 +230,25 @@ __global__ __launch_bounds__(NTH, 2) void pass_kernel(Chunks k) {
         for (int t = 0; t < LT; ++t) {
           const float2 ct = cs[16 * t + l16];
           acc[t] *= __expf(ct.x + ct.y);
-#pragma unroll
-          for (int kb = 0; kb <= t / 2; ++kb) {
-            const E* m = Ms + ((t * KB + kb) * 64 + lane) * 8;
-            Frag<E> f;
-            if constexpr (sizeof(E) == 2) {
-              f.v = *reinterpret_cast<const bf16x8*>(m);
-            } else {
-              f.v[0] = *reinterpret_cast<const f32x4*>(m);
-              f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
-            }
-            acc[t] = mma(xf[kb], f, acc[t]);
+          const E* m = Ms + (t * 64 + lane) * 8;
+          Frag<E> f;
+          if constexpr (sizeof(E) == 2) {
+            f.v = *reinterpret_cast<const bf16x8*>(m);
+          } else {
+            f.v[0] = *reinterpret_cast<const f32x4*>(m);
+            f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
           }
+          acc[t] = mma(xf, f, acc[t]);
           const int tok = c * L + 16 * t + l16, p = pw + 4 * g;
           if (tok < a.T && p < a.P && a.y != nullptr) {
             const E* xr = Xs + TX::at(16 * t + l16) + 16 * wave + 4 * g;
             IO* y = static_cast<IO*>(a.y) + ((static_cast<int64_t>(b) * a.T + tok) * a.H + h) * a.P + p;
-            struct alignas(4 * sizeof(IO)) V4 { IO e[4]; } v;
+            f32x4 o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v.e[r] = round_to<IO>(fmaf(Dh, static_cast<float>(xr[r]), acc[t][r]));
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(Dh, static_cast<float>(xr[r]), acc[t][r]);
+            const Out4<IO> v = out4<IO>(o);
             if (k.vec_y) {
-              *reinterpret_cast<V4*>(y) = v;
+              *reinterpret_cast<Out4<IO>*>(y) = v;
             } else {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
@@ -348,8 +321,6 @@ __global__ __launch_bounds__(NTH) void carry_kernel(float* seg_state, const floa
 
 namespace {
 
-int chunk_tokens(int dtype) { return dtype == VMI_BF16 ? 64 : 32; }
-
 struct Plan {
   int64_t nch, tp, d_bytes, c_bytes, state_bytes, decay_bytes;
   int pblocks, seg_chunks, nseg;
@@ -357,14 +328,13 @@ struct Plan {
 };
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Two workgroups a compute unit; a segment costs its state's way through memory, so it keeps some chunks.
-Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
+// Three workgroups a compute unit; a segment costs its state's way through memory, so it keeps some chunks.
+Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N) {
   Plan p;
-  const int L = chunk_tokens(dtype);
   p.nch = (T + L - 1) / L;
   p.tp = p.nch * L;
   p.pblocks = static_cast<int>((P + PB - 1) / PB);
-  const int64_t base = B * H * p.pblocks, want = (512 + base - 1) / base;
+  const int64_t base = B * H * p.pblocks, want = (768 + base - 1) / base;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(MAX_SEG, p.nch / 4));
   int64_t nseg = std::min(want, most);
   p.seg_chunks = static_cast<int>((p.nch + nseg - 1) / nseg);
@@ -376,7 +346,7 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
   return p;
 }
 
-template <typename IO, typename E, int NP, int L, bool VEC>
+template <typename IO, typename E, int NP, bool VEC>
 int run(Chunks k, const Plan& p, hipStream_t stream) {
   const Args& a = k.a;
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * p.pblocks * p.nseg;
@@ -386,7 +356,7 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
       st != VMI_OK)
     return st;
   if (p.nseg > 1) {
-    hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, false, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+    hipLaunchKernelGGL((pass_kernel<IO, E, NP, false, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
     const bool vec = PN % 4 == 0 && aligned16({a.state_in});
     const int64_t blocks = (BH * PN / (vec ? 4 : 1) + NTH - 1) / NTH;
@@ -395,14 +365,14 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
                        k.seg_decay, a.state_in, p.nseg, BH, PN, vec);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
   }
-  hipLaunchKernelGGL((pass_kernel<IO, E, NP, L, true, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
+  hipLaunchKernelGGL((pass_kernel<IO, E, NP, true, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
   return hip_status(hipGetLastError());
 }
 
-template <typename IO, typename E, int L> int by_state(const Chunks& k, const Plan& p, hipStream_t stream) {
+template <typename IO, typename E> int by_state(const Chunks& k, const Plan& p, hipStream_t stream) {
   auto go = [&](auto np) -> int {
     constexpr int NP = decltype(np)::value;
-    return k.vec ? run<IO, E, NP, L, true>(k, p, stream) : run<IO, E, NP, L, false>(k, p, stream);
+    return k.vec ? run<IO, E, NP, true>(k, p, stream) : run<IO, E, NP, false>(k, p, stream);
   };
   if (k.a.N <= 32) return go(std::integral_constant<int, 32>{});
   if (k.a.N <= 64) return go(std::integral_constant<int, 64>{});
@@ -412,11 +382,11 @@ template <typename IO, typename E, int L> int by_state(const Chunks& k, const Pl
 
 }  // namespace
 
-int launch_prep(const Args& a, int L, float* d, float2* c, int nch, hipStream_t stream) {
-  const int64_t units = static_cast<int64_t>(a.B) * a.H * nch, blocks = (units + NTH / L - 1) / (NTH / L);
+int launch_prep(const Args& a, int tokens, float* d, float2* c, int nch, hipStream_t stream) {
+  const int64_t units = static_cast<int64_t>(a.B) * a.H * nch, blocks = (units + NTH / tokens - 1) / (NTH / tokens);
   if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (L == 64) hipLaunchKernelGGL(prep_kernel<64>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
+  if (tokens == 64) hipLaunchKernelGGL(prep_kernel<64>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
   else hipLaunchKernelGGL(prep_kernel<32>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
   return hip_status(hipGetLastError());
 }
@@ -424,11 +394,11 @@ int launch_prep(const Args& a, int L, float* d, float2* c, int nch, hipStream_t 
 bool use_chunk(int64_t T) { return T >= 16; }
 
 size_t chunk_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
-  return use_chunk(T) ? static_cast<size_t>(plan(B, T, H, P, N, dtype).bytes()) : 0;
+  return use_chunk(T) ? static_cast<size_t>(plan(B, T, H, P, N).bytes()) : 0;
 }
 
 int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) {
-  const Plan p = plan(a.B, a.T, a.H, a.P, a.N, dtype);
+  const Plan p = plan(a.B, a.T, a.H, a.P, a.N);
   Chunks k{};
   k.a = a;
   char* w = static_cast<char*>(workspace);
@@ -442,9 +412,9 @@ int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) 
           a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 && aligned16({a.x, a.bm, a.cm});
   k.vec_state = a.N % 4 == 0 && aligned16({a.state_in, a.state_out});
   k.vec_y = a.P % 4 == 0 && aligned16({a.y});
-  if (dtype == VMI_BF16) return by_state<bf16_t, __bf16, 64>(k, p, stream);
-  if (dtype == VMI_F16) return by_state<f16_t, float, 32>(k, p, stream);
-  return by_state<float, float, 32>(k, p, stream);
+  if (dtype == VMI_BF16) return by_state<bf16_t, __bf16>(k, p, stream);
+  if (dtype == VMI_F16) return by_state<f16_t, float>(k, p, stream);
+  return by_state<float, float>(k, p, stream);
 }
 
 }  // namespace sel

@@ -10,6 +10,8 @@
 //     decayed sums' range, and bf16 not its 11 bits).
 #pragma once
 
+#include <type_traits>
+
 #include "selective.h"
 #include "vmi_lanes.h"
 #include "vmi_mfma.h"
@@ -53,6 +55,30 @@ __device__ __forceinline__ Frag<E> row_frag(const E* tile, int row0, int k0, int
   }
   return f;
 }
+// A tile that is only read by rows: the eight values of a lane's fragment lie side by side (one 16-byte read),
+// and the four lane groups read from quarters a multiple of the banks apart, so that a read's 16 distinct rows
+// are in distinct banks whichever lanes are served together.
+template <typename E, int W> struct RowTile {
+  static constexpr int PITCH = sizeof(E) == 2 ? (W == 32 ? 24 : W / 4 + 8) : W + 4;
+  static constexpr int elems(int rows) { return rows * PITCH * (sizeof(E) == 2 ? 4 : 1); }
+  // where the four elements from column c on (c % 4 == 0) lie in row r of a tile of ROWS
+  template <int ROWS> static __device__ __forceinline__ int at(int r, int c) {
+    if constexpr (sizeof(E) == 2) return ((c >> 2) & 3) * (ROWS * PITCH) + r * PITCH + (c >> 5) * 8 + ((c >> 4) & 1) * 4;
+    else return r * PITCH + c;
+  }
+};
+template <typename E, int W, int ROWS>
+__device__ __forceinline__ Frag<E> packed_frag(const E* tile, int row0, int k0, int l16, int g) {
+  const E* p = tile + (row0 + l16) * RowTile<E, W>::PITCH + (sizeof(E) == 2 ? g * (ROWS * RowTile<E, W>::PITCH) + k0 / 4 : k0 + 4 * g);
+  Frag<E> f;
+  if constexpr (sizeof(E) == 2) {
+    f.v = *reinterpret_cast<const bf16x8*>(p);
+  } else {
+    f.v[0] = *reinterpret_cast<const f32x4*>(p);
+    f.v[1] = *reinterpret_cast<const f32x4*>(p + 16);
+  }
+  return f;
+}
 // The fragment whose outer index is a column and whose contraction runs down the rows.
 template <typename E, int W>
 __device__ __forceinline__ Frag<E> col_frag(const E* tile, int k0, int col0, int l16, int g) {
@@ -90,32 +116,39 @@ template <typename E> struct Parts { static constexpr int N = sizeof(E) == 2 ? 3
 template <typename E>
 __device__ __forceinline__ void split(const f32x4 (&x)[2], Frag<E> (&f)[Parts<E>::N]) {
   if constexpr (sizeof(E) == 2) {
+    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+    float r[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < 8; ++i) r[i] = x[i / 4][i % 4];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[k].v[i] = static_cast<__bf16>(r[i]);  // v_cvt_pk_bf16_f32 pairs
+      if (k == 2) break;
+      const u32x4 q = __builtin_bit_cast(u32x4, f[k].v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float r = x[h][i];
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const __bf16 q = static_cast<__bf16>(r);
-          f[k].v[4 * h + i] = q;
-          r -= static_cast<float>(q);
-        }
+        r[2 * i] -= __uint_as_float(q[i] << 16);
+        r[2 * i + 1] -= __uint_as_float(q[i] & 0xffff0000u);
       }
+    }
   } else {
     f[0].v[0] = x[0], f[0].v[1] = x[1];
   }
 }
 template <typename E> __device__ __forceinline__ f32x4 half(const Frag<E>& f, int h) {
   if constexpr (sizeof(E) == 2) {
-    f32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = static_cast<float>(f.v[4 * h + i]);
-    return r;
+    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 q = __builtin_bit_cast(u32x4, f.v);
+    return f32x4{__uint_as_float(q[2 * h] << 16), __uint_as_float(q[2 * h] & 0xffff0000u),
+                 __uint_as_float(q[2 * h + 1] << 16), __uint_as_float(q[2 * h + 1] & 0xffff0000u)};
   } else {
     return f.v[h];
   }
 }
+
+// The number of this wave in its workgroup, known to be the same in all lanes.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // Orders LDS accesses only: global loads and stores stay in flight across it.
 __device__ __forceinline__ void lds_barrier() {
@@ -178,16 +211,50 @@ template <typename IO, typename E, int W, int ROWS, int NTH, bool VEC> struct St
       if constexpr (sizeof(IO) == sizeof(E)) {
         *reinterpret_cast<uint4*>(dst) = v[i];
       } else {  // fp16 -> fp32
-        const f16x8 h = __builtin_bit_cast(f16x8, v[i]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<float4*>(dst + 4 * k) =
-              make_float4(static_cast<float>(h[4 * k]), static_cast<float>(h[4 * k + 1]), static_cast<float>(h[4 * k + 2]),
-                          static_cast<float>(h[4 * k + 3]));
+        *reinterpret_cast<float4*>(dst) = wide(i, 0);
+        *reinterpret_cast<float4*>(dst + 4) = wide(i, 1);
       }
     }
   }
+  __device__ __forceinline__ void commit_rows(E* tile) const {
+    const int c = threadIdx.x % PR * EL;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (PER * NTH != ROWS * PR && row + STEP * i >= ROWS) continue;
+      const int r = row + STEP * i;
+      if constexpr (sizeof(E) == 2) {
+        *reinterpret_cast<uint2*>(tile + RowTile<E, W>::template at<ROWS>(r, c)) = make_uint2(v[i].x, v[i].y);
+        *reinterpret_cast<uint2*>(tile + RowTile<E, W>::template at<ROWS>(r, c + 4)) = make_uint2(v[i].z, v[i].w);
+      } else if constexpr (sizeof(IO) == 4) {
+        *reinterpret_cast<uint4*>(tile + RowTile<E, W>::template at<ROWS>(r, c)) = v[i];
+      } else {
+        *reinterpret_cast<float4*>(tile + RowTile<E, W>::template at<ROWS>(r, c)) = wide(i, 0);
+        *reinterpret_cast<float4*>(tile + RowTile<E, W>::template at<ROWS>(r, c + 4)) = wide(i, 1);
+      }
+    }
+  }
+  __device__ __forceinline__ float4 wide(int i, int h) const {
+    const f16x8 q = __builtin_bit_cast(f16x8, v[i]);
+    return make_float4(static_cast<float>(q[4 * h]), static_cast<float>(q[4 * h + 1]), static_cast<float>(q[4 * h + 2]),
+                       static_cast<float>(q[4 * h + 3]));
+  }
 };
+
+// fp32 -> four values of the memory type, by the conversion instructions.
+template <typename IO> struct alignas(4 * sizeof(IO)) Out4 { IO e[4]; };
+template <typename IO> __device__ __forceinline__ Out4<IO> out4(f32x4 x) {
+  if constexpr (std::is_same_v<IO, bf16_t>) {
+    bf16x4 q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q[r] = static_cast<__bf16>(x[r]);
+    return __builtin_bit_cast(Out4<IO>, q);
+  } else {
+    Out4<IO> q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q.e[r] = static_cast<IO>(x[r]);
+    return q;
+  }
+}
 
 // Log decays from a chunk's start, as two floats: their differences keep the accuracy of a small exponent.
 __device__ __forceinline__ float decay(float2 to, float2 from) { return __expf((to.x - from.x) + (to.y - from.y)); }
