@@ -20,6 +20,7 @@
 //   main_kernel: a workgroup of eight waves per chunk and block of heads of a group walks the heads with dB and
 //     dC of the chunk in accumulators (they are sums over the heads: as partials of each head they would be the
 //     largest thing moved); C . B, the same for every head, is formed once;
+//   steps_kernel: g, and from it ddelta and the chunks' shares of dA and dbias;
 //   reduce_kernel: the head blocks' dB and dC and the heads' dA, dD, dbias, in a fixed order.
 //
 // bf16 inputs: Q and M, and G_L where it enters dx, are rounded to bf16 once (2^-8 of a term, as the results);
@@ -50,6 +51,8 @@ struct Bwd {
   float *s0, *g1;            // [BH pblocks][nch][NP 64], tiles of 16 x 16 in fragment order
   float *pb, *pc;            // [hblocks][B T][G][N] (null: dB, dC written directly)
   float* ph;                 // [3][B nch][H]: dA, dD, dbias
+  float* tok;                // [4][BH pblocks][Tp]: sums of alpha, beta, rows and columns of R
+  float* chk;                // [2][BH pblocks][nch]: kappa, sum of x . dy
   void *dx, *ddelta, *db, *dc;
   float *dA, *dD, *dbias, *dstate_in;
   int nch, seg_chunks, nseg, pblocks, hblocks, hper;
@@ -334,8 +337,6 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       for (int kb = 0; kb < KN; ++kb)
         cb[i] = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), row_frag<E, NP>(Cs, 16 * tt, 32 * kb, l16, g), cb[i]);
     }
-    double dd_sum = 0.0, g_sum = 0.0, dd_acc = 0.0;  // wave 0: over a head's row blocks
-
     for (int u = 0; u < units; ++u) {
       const int h = h0 + u / k.pblocks, pb = u % k.pblocks, p0 = pb * PB;
       lds_barrier();  // the last unit's readers are done
@@ -377,15 +378,13 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const int o = TQ::at(t) + 16 * st + 4 * g;
         *reinterpret_cast<M4*>(Qs + o) = q;
         *reinterpret_cast<M4*>(Ms + o) = m;
-        rs += __shfl_xor(rs, 16);
-        rs += __shfl_xor(rs, 32);
+        rs = half_pair_sum(row_pair_sum(rs));
         if (g == 0) row_r[st][t] = rs;
 #pragma unroll
         for (int r = 0; r < 4; ++r) rr[r] = row16_sum(rr[r]);
         if (l16 == 0) *reinterpret_cast<float4*>(&col_r[tt][16 * st + 4 * g]) = make_float4(rr[0], rr[1], rr[2], rr[3]);
         if (tt == st) {
-#pragma unroll
-          for (int off = 32; off >= 1; off >>= 1) dg += __shfl_xor(dg, off);
+          dg = half_pair_sum(row_pair_sum(row16_sum(dg)));
           if (lane == 0) diag[tt] = dg;
         }
       }
@@ -457,13 +456,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         if (hh == 0) {
 #pragma unroll
           for (int t = 0; t < LTW; ++t) {
-            float v = al[t], w = be[t];
-            v += __shfl_xor(v, 16), w += __shfl_xor(w, 16);
-            v += __shfl_xor(v, 32), w += __shfl_xor(w, 32);
+            const float v = half_pair_sum(row_pair_sum(al[t])), w = half_pair_sum(row_pair_sum(be[t]));
             if (g == 0) alpha[nt0][16 * (tt0 + t) + l16] = v, beta[nt0][16 * (tt0 + t) + l16] = w;
           }
-#pragma unroll
-          for (int off = 32; off >= 1; off >>= 1) kp += __shfl_xor(kp, off);
+          kp = half_pair_sum(row_pair_sum(row16_sum(kp)));
           if (lane == 0) kappa[wave] = NT >= NW || tt0 == 0 ? kp : 0.f;
         }
         if (hh == NH - 1 && u + 1 < units) fetch_states(u + 1);
@@ -515,56 +511,27 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           }
         }
       }
-      // a lane a token: the gradients of the step sizes (sums in fp64: they are differences)
-      if (wave == NW - 1) {
-        const bool in = lane < L;
-        const int t = in ? lane : 0;
-        const double d = in ? ds[t] : 0.f;
-        double rs = 0.0, cr = 0.0, alp = 0.0, bet = 0.0, kap = 0.0, dgs = 0.0;
+      // what the step sizes' gradients are made of, for steps_kernel: the last four waves a sum each
+      {
+        const int64_t bhp = (static_cast<int64_t>(b) * a.H + h) * k.pblocks + pb, plane = static_cast<int64_t>(a.B) * a.H * k.pblocks;
+        const int which = wave - (NW - 4), t = lane % L;
+        if (which >= 0) {
+          constexpr int NS = NT < NW ? NT : NW;
+          float v = 0.f;
+          if (which < 2) {
 #pragma unroll
-        for (int i = 0; i < LT; ++i) {
-          if (i <= t / 16) rs += row_r[i][t];
-          if (i >= t / 16) cr += col_r[i][t];
-          dgs += diag[i];
-        }
-        constexpr int NS = NT < NW ? NT : NW;
+            for (int i = 0; i < NS; ++i) v += which == 0 ? alpha[i][t] : beta[i][t];
+          } else {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) alp += alpha[i][t], bet += beta[i][t];
-#pragma unroll
-        for (int i = 0; i < NW; ++i) kap += kappa[i];
-        kap *= static_cast<double>(es[L - 1]);
-        double suf = in ? alp + rs - d * cr : 0.0, pre = in ? d * bet : 0.0;
-        const double own_pre = pre;
-#pragma unroll
-        for (int off = 1; off < L; off <<= 1) {
-          const double v = __shfl_down(suf, off, 64), w = __shfl_up(pre, off, 64);
-          if (lane + off < L) suf += v;
-          if (lane >= off) pre += w;
-        }
-        const double gt = kap + suf + (pre - own_pre);
-        const double A = a.A[h];
-        if (pb == 0) dd_sum = g_sum = dd_acc = 0.0;
-        dd_acc += cr + bet + A * gt;
-        g_sum += d * gt;
-        dd_sum += dgs;
-        if (pb == k.pblocks - 1) {
-          const float slope = a.softplus ? -expm1f(-static_cast<float>(d)) : 1.f;  // sigmoid(z) = 1 - e^{-softplus(z)}
-          double dz = in && t0 + t < len ? dd_acc * static_cast<double>(slope) : 0.0;
-          if (in && t0 + t < a.T && k.ddelta != nullptr) {
-            const int64_t o = (static_cast<int64_t>(b) * a.T + t0 + t) * a.H + h;
-            const float v = static_cast<float>(dz);
-            if (a.delta_dtype == VMI_F32) io<float>::store(static_cast<float*>(k.ddelta), o, v);
-            else if (a.delta_dtype == VMI_BF16) io<bf16_t>::store(static_cast<bf16_t*>(k.ddelta), o, v);
-            else io<f16_t>::store(static_cast<f16_t*>(k.ddelta), o, v);
+            for (int i = 0; i < LT; ++i)
+              if (which == 2 ? i <= t / 16 : i >= t / 16) v += which == 2 ? row_r[i][t] : col_r[i][t];
           }
-          double ga = in ? g_sum : 0.0;
+          if (lane < L) k.tok[(which * plane + bhp) * tp + t0 + t] = v;
+          if (lane == 0 && which < 2) {
+            float s = 0.f;
 #pragma unroll
-          for (int off = 32; off >= 1; off >>= 1) dz += __shfl_xor(dz, off), ga += __shfl_xor(ga, off);
-          if (lane == 0) {
-            const int64_t rows = static_cast<int64_t>(a.B) * k.nch, o = (static_cast<int64_t>(b) * k.nch + c) * a.H + h;
-            k.ph[o] = static_cast<float>(ga);
-            k.ph[rows * a.H + o] = static_cast<float>(dd_sum);
-            k.ph[2 * rows * a.H + o] = static_cast<float>(dz);
+            for (int i = 0; i < NW; ++i) s += which == 0 ? kappa[i] : i < LT ? diag[i] : 0.f;
+            k.chk[(which * plane + bhp) * k.nch + c] = which == 0 ? s * es[L - 1] : s;
           }
         }
       }
@@ -576,12 +543,6 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         for (int t = wave; t < rows; t += NW)
           for (int p = lane; p < a.P; p += 64)
             io<IO>::store(static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0 + t) * a.H + h) * a.P, p, 0.f);
-      if (tid < rows && k.ddelta != nullptr) {
-        const int64_t o = (static_cast<int64_t>(b) * a.T + t0 + tid) * a.H + h;
-        if (a.delta_dtype == VMI_F32) static_cast<float*>(k.ddelta)[o] = 0.f;
-        else static_cast<uint16_t*>(k.ddelta)[o] = 0;
-      }
-      if (tid < 3) k.ph[(tid * static_cast<int64_t>(a.B) * k.nch + static_cast<int64_t>(b) * k.nch + c) * a.H + h] = 0.f;
     }
   }
   // dB, dC: rows n, column t
@@ -594,6 +555,11 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       if (tok >= a.T || n >= a.N) continue;
       const int64_t o = ((static_cast<int64_t>(b) * a.T + tok) * a.G + grp) * a.N + n;
       const int64_t part = static_cast<int64_t>(hb) * a.B * a.T * a.G * a.N;
+      if (k.pb != nullptr && a.N % 4 == 0) {
+        *reinterpret_cast<f32x4*>(k.pb + part + o) = db[j][t];
+        *reinterpret_cast<f32x4*>(k.pc + part + o) = dc[j][t];
+        continue;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (n + r >= a.N) continue;
@@ -607,6 +573,67 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       }
     }
   }
+}
+
+// The gradients of a chunk's step sizes, a lane a token: the sums over the tokens before and after are differences
+// of the main kernel's, and run in fp64.
+template <int L>
+__global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
+  const Args& a = k.a;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (SNT / 64) + (threadIdx.x >> 6);
+  if (unit >= units) return;
+  const int lane = threadIdx.x & 63;
+  const int h = static_cast<int>(unit % a.H);
+  const int64_t bc = unit / a.H;
+  const int b = static_cast<int>(bc / k.nch), c = static_cast<int>(bc - static_cast<int64_t>(b) * k.nch);
+  const int len = length_of(a.lengths, a.lengths64, a.T, b), t = c * L + lane;
+  const int64_t bh = static_cast<int64_t>(b) * a.H + h, tp = static_cast<int64_t>(k.nch) * L;
+  const int64_t plane = static_cast<int64_t>(a.B) * a.H * k.pblocks;
+  const bool in = lane < L && t < len;
+  double dz = 0.0, ga = 0.0, dgs = 0.0;
+  if (c * L < len) {
+    double al = 0.0, be = 0.0, rs = 0.0, cr = 0.0, kap = 0.0, d = 0.0;
+    for (int p = 0; p < k.pblocks; ++p) {
+      const int64_t row = bh * k.pblocks + p;
+      kap += k.chk[row * k.nch + c];
+      dgs += k.chk[(plane + row) * k.nch + c];
+      if (!in) continue;
+      al += k.tok[row * tp + t];
+      be += k.tok[(plane + row) * tp + t];
+      rs += k.tok[(2 * plane + row) * tp + t];
+      cr += k.tok[(3 * plane + row) * tp + t];
+    }
+    if (in) d = k.d[bh * tp + t];
+    double suf = al + rs - d * cr, pre = d * be;
+    const double own = pre;
+#pragma unroll
+    for (int off = 1; off < L; off <<= 1) {
+      const double v = __shfl_down(suf, off, 64), w = __shfl_up(pre, off, 64);
+      if (lane + off < L) suf += v;
+      if (lane >= off) pre += w;
+    }
+    const double gt = kap + suf + (pre - own);
+    // sigmoid(z) = 1 - e^{-softplus(z)}
+    const double slope = a.softplus ? static_cast<double>(-expm1f(-static_cast<float>(d))) : 1.0;
+    if (in) {
+      dz = (cr + be + static_cast<double>(a.A[h]) * gt) * slope;
+      ga = d * gt;
+    }
+  }
+  if (lane < L && t < a.T && k.ddelta != nullptr) {
+    const int64_t o = (static_cast<int64_t>(b) * a.T + t) * a.H + h;
+    const float v = static_cast<float>(dz);
+    if (a.delta_dtype == VMI_F32) io<float>::store(static_cast<float*>(k.ddelta), o, v);
+    else if (a.delta_dtype == VMI_BF16) io<bf16_t>::store(static_cast<bf16_t*>(k.ddelta), o, v);
+    else io<f16_t>::store(static_cast<f16_t*>(k.ddelta), o, v);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) dz += __shfl_xor(dz, off), ga += __shfl_xor(ga, off);
+  if (lane != 0) return;
+  const int64_t rows = static_cast<int64_t>(a.B) * k.nch, o = bc * a.H + h;
+  k.ph[o] = static_cast<float>(ga);
+  k.ph[rows * a.H + o] = static_cast<float>(dgs);
+  k.ph[2 * rows * a.H + o] = static_cast<float>(dz);
 }
 
 // Blocks below `heads`: 64 of the 3 H head sums by four strided shares of the chunks.  The others: dB and dC
@@ -629,15 +656,27 @@ __global__ __launch_bounds__(SNT) void reduce_kernel(Bwd k, int heads, int64_t e
     if (dst != nullptr) dst[h] = static_cast<float>((part[0][l] + part[1][l]) + (part[2][l] + part[3][l]));
     return;
   }
-  const int64_t i = static_cast<int64_t>(blockIdx.x - heads) * SNT + threadIdx.x;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x - heads) * SNT + threadIdx.x) * 4;
   if (i >= elems) return;
-  float vb = 0.f, vc = 0.f;
-  for (int q = 0; q < k.hblocks; ++q) {
-    vb += k.pb[q * elems + i];
-    vc += k.pc[q * elems + i];
+  const int left = static_cast<int>(elems - i < 4 ? elems - i : 4);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const float* part = which ? k.pc : k.pb;
+    IO* dst = static_cast<IO*>(which ? k.dc : k.db);
+    if (dst == nullptr) continue;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (elems % 4 == 0) {
+      for (int q = 0; q < k.hblocks; ++q) v += *reinterpret_cast<const f32x4*>(part + q * elems + i);
+      if (reinterpret_cast<uintptr_t>(dst) % (4 * sizeof(IO)) == 0) {
+        *reinterpret_cast<Out4<IO>*>(dst + i) = out4<IO>(v);
+        continue;
+      }
+    } else {
+      for (int q = 0; q < k.hblocks; ++q)
+        for (int r = 0; r < left; ++r) v[r] += part[q * elems + i + r];
+    }
+    for (int r = 0; r < left; ++r) io<IO>::store(dst, i + r, v[r]);
   }
-  if (k.db != nullptr) io<IO>::store(static_cast<IO*>(k.db), i, vb);
-  if (k.dc != nullptr) io<IO>::store(static_cast<IO*>(k.dc), i, vc);
 }
 
 namespace {
@@ -646,9 +685,9 @@ int bwd_tokens(int dtype) { return dtype == VMI_BF16 ? 64 : 32; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Plan {
-  int64_t nch, tp, c_bytes, d_bytes, own_bytes, state_bytes, part_bytes, ph_bytes;
+  int64_t nch, tp, c_bytes, d_bytes, own_bytes, state_bytes, part_bytes, ph_bytes, tok_bytes, chk_bytes;
   int np, pblocks, seg_chunks, nseg, hblocks, hper;
-  int64_t bytes() const { return c_bytes + d_bytes + own_bytes + 2 * state_bytes + 2 * part_bytes + ph_bytes; }
+  int64_t bytes() const { return c_bytes + d_bytes + own_bytes + 2 * state_bytes + 2 * part_bytes + ph_bytes + tok_bytes + chk_bytes; }
 };
 
 Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
@@ -658,12 +697,12 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int 
   p.nch = (T + L - 1) / L;
   p.tp = p.nch * L;
   p.pblocks = static_cast<int>((P + PB - 1) / PB);
-  const int64_t BHP = B * H * p.pblocks, want = (512 + 2 * BHP - 1) / (2 * BHP);
+  const int64_t BHP = B * H * p.pblocks, want = (256 + 2 * BHP - 1) / (2 * BHP);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(BWD_MAX_SEG, p.nch / 4));
   const int64_t nseg = std::min(want, most);
   p.seg_chunks = static_cast<int>((p.nch + nseg - 1) / nseg);
   p.nseg = static_cast<int>((p.nch + p.seg_chunks - 1) / p.seg_chunks);
-  const int64_t hg = H / G, blocks = B * p.nch * G, split = std::min<int64_t>(hg, (512 + blocks - 1) / blocks);
+  const int64_t hg = H / G, blocks = B * p.nch * G, split = std::min<int64_t>(hg, (256 + blocks - 1) / blocks);
   p.hper = static_cast<int>((hg + split - 1) / split);
   p.hblocks = static_cast<int>((hg + p.hper - 1) / p.hper);
   p.c_bytes = up16(B * H * p.tp * 8);
@@ -673,6 +712,8 @@ Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int 
   p.state_bytes = BHP * p.nch * state;
   p.part_bytes = p.hblocks > 1 ? up16(p.hblocks * B * T * G * N * 4) : 0;
   p.ph_bytes = up16(3 * B * p.nch * H * 4);
+  p.tok_bytes = up16(4 * BHP * p.tp * 4);
+  p.chk_bytes = up16(2 * BHP * p.nch * 4);
   return p;
 }
 
@@ -697,9 +738,13 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
   if (!ok(st)) return st;
   hipLaunchKernelGGL((main_kernel<IO, E, NP, L, VEC>), dim3(static_cast<unsigned>(blocks)), dim3(MNT), 0, stream, k);
   if (!ok(st)) return st;
+  const int64_t chunks = static_cast<int64_t>(a.B) * a.H * p.nch, sb = (chunks + SNT / 64 - 1) / (SNT / 64);
+  if (sb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(steps_kernel<L>, dim3(static_cast<unsigned>(sb)), dim3(SNT), 0, stream, k, chunks);
+  if (!ok(st)) return st;
   const int heads = (3 * a.H + 63) / 64;
   const int64_t elems = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
-  const int64_t rb = heads + (p.hblocks > 1 ? (elems + SNT - 1) / SNT : 0);
+  const int64_t rb = heads + (p.hblocks > 1 ? (elems + 4 * SNT - 1) / (4 * SNT) : 0);
   if (rb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(reduce_kernel<IO>, dim3(static_cast<unsigned>(rb)), dim3(SNT), 0, stream, k, heads, elems);
   ok(st);
@@ -745,6 +790,8 @@ int launch_bwd(const Args& a, int dtype, const Grads& q, void* workspace, hipStr
     k.pc = reinterpret_cast<float*>(take(p.part_bytes));
   }
   k.ph = reinterpret_cast<float*>(take(p.ph_bytes));
+  k.tok = reinterpret_cast<float*>(take(p.tok_bytes));
+  k.chk = reinterpret_cast<float*>(take(p.chk_bytes));
   k.nch = static_cast<int>(p.nch), k.seg_chunks = p.seg_chunks, k.nseg = p.nseg, k.pblocks = p.pblocks;
   k.hblocks = p.hblocks, k.hper = p.hper;
   const int el = dtype == VMI_F32 ? 4 : 8;
