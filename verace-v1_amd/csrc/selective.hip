@@ -1,7 +1,9 @@
 // C entry points of the selective state space scan (selective.h).
 #include <algorithm>
 
-#include "selective.h"
+#include <initializer_list>
+
+#include "selective_mfma.h"
 
 using namespace vmi;
 using namespace vmi::sel;
@@ -13,6 +15,13 @@ int check(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int 
   if (dtype < VMI_F32 || dtype > VMI_F16 || delta_dtype < VMI_F32 || delta_dtype > VMI_F16) return VMI_ERR_INVALID_ARG;
   if (N > 256 || P > 1024 || T > INT32_MAX - 4096 || B > 65535 || H > 65535 || B * H > 4194304) return VMI_ERR_UNSUPPORTED;
   return VMI_OK;
+}
+
+// The chunk kernels' lane offsets are 32 bits wide.
+bool strides_fit(std::initializer_list<int64_t> strides, int64_t H, int64_t P) {
+  for (int64_t s : strides)
+    if (s < -kMaxStride || s > kMaxStride) return false;
+  return H * P <= kMaxStride;
 }
 
 }  // namespace
@@ -44,7 +53,7 @@ extern "C" int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, c
   a.delta_dtype = delta_dtype, a.softplus = softplus;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.H = static_cast<int>(H), a.P = static_cast<int>(P);
   a.G = static_cast<int>(G), a.N = static_cast<int>(N);
-  if (!use_chunk(T)) return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
+  if (!use_chunk(T) || !strides_fit({x_t, b_t, c_t}, H, P)) return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
   if (workspace == nullptr || workspace_bytes < chunk_workspace_bytes(B, T, H, P, N, dtype)) return VMI_ERR_WORKSPACE;
   return launch_chunk(a, dtype, workspace, static_cast<hipStream_t>(stream));
 }
@@ -70,6 +79,7 @@ extern "C" int vmi_selective_scan_bwd(const void* x, int64_t x_t, int64_t x_b, c
   if (B == 0 || T == 0) return VMI_ERR_INVALID_ARG;  // nothing to differentiate
   if (A == nullptr || x == nullptr || delta == nullptr || bm == nullptr || cm == nullptr || dy == nullptr)
     return VMI_ERR_INVALID_ARG;
+  if (!strides_fit({x_t, b_t, c_t, y_t}, H, P)) return VMI_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < bwd_workspace_bytes(B, T, H, P, G, N, dtype)) return VMI_ERR_WORKSPACE;
   Args a{};
   a.x = x, a.delta = delta, a.bm = bm, a.cm = cm, a.x_t = x_t, a.x_b = x_b, a.d_t = d_t, a.d_b = d_b;

@@ -497,7 +497,8 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const int p = p0 + 16 * pt + 4 * g;
         if (t0 + s < a.T && p < a.P && k.dx != nullptr) {
           const E* yr = Ys + TX::at(s) + 16 * pt + 4 * g;
-          IO* o = static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0 + s) * a.H + h) * a.P + p;
+          // a scalar base and a lane's offset
+          IO* o = static_cast<IO*>(k.dx) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P + p0 + (s * a.H * a.P + 16 * pt + 4 * g);
           f32x4 q;
 #pragma unroll
           for (int r = 0; r < 4; ++r) q[r] = fmaf(Dh, static_cast<float>(yr[r]), dx[t][r]);

@@ -151,6 +151,10 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
   }
   const float Dh = a.D == nullptr ? 0.f : a.D[h];
   double seg_c = 0.0;
+  // where this lane's y of the chunk's first 16 tokens lies, and the way to the next 16
+  const int64_t y16 = 16 * static_cast<int64_t>(a.H) * a.P;
+  IO* y = static_cast<IO*>(a.y) + ((static_cast<int64_t>(b) * a.T + c0 * L + l16) * a.H + h) * a.P + pw + 4 * g;
+  const bool y_on = pw + 4 * g < a.P && a.y != nullptr;
 
   for (int c = c0; c < c1; ++c) {
     lds_barrier();  // the last chunk's readers are done
@@ -239,24 +243,24 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
             f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
           }
           acc[t] = mma(xf, f, acc[t]);
-          const int tok = c * L + 16 * t + l16, p = pw + 4 * g;
-          if (tok < a.T && p < a.P && a.y != nullptr) {
+          if (y_on && c * L + 16 * t + l16 < a.T) {
             const E* xr = Xs + TX::at(16 * t + l16) + 16 * wave + 4 * g;
-            IO* y = static_cast<IO*>(a.y) + ((static_cast<int64_t>(b) * a.T + tok) * a.H + h) * a.P + p;
+            IO* yt = y + t * y16;
             f32x4 o;
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(Dh, static_cast<float>(xr[r]), acc[t][r]);
             const Out4<IO> v = out4<IO>(o);
             if (k.vec_y) {
-              *reinterpret_cast<Out4<IO>*>(y) = v;
+              *reinterpret_cast<Out4<IO>*>(yt) = v;
             } else {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (p + r < a.P) y[r] = v.e[r];
+                if (pw + 4 * g + r < a.P) yt[r] = v.e[r];
             }
           }
         }
       }
+      y += LT * y16;
     }
   }
   if constexpr (READOUT) {  // tokens of chunks behind the sequence's end

@@ -158,6 +158,9 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Elements between the rows of an input at most: 64 rows of fp32 from a tile's first in 32 bits.
+constexpr int64_t kMaxStride = 1 << 23;
+
 // A tile's rows on their way from global memory: NTH threads hold PER 16-byte pieces each, all of one column.
 // VEC: whole aligned pieces; else element by element.
 template <typename IO, typename E, int W, int ROWS, int NTH, bool VEC> struct Stage {
@@ -167,13 +170,14 @@ template <typename IO, typename E, int W, int ROWS, int NTH, bool VEC> struct St
   static constexpr int STEP = NTH / PR;                   // rows between a thread's pieces
   static_assert(NTH % PR == 0, "");
   uint4 v[PER];
-  const IO* src;   // this thread's piece of row 0
+  const IO* src;   // row 0, the same in all lanes
   int64_t stride;
+  uint32_t off;    // this thread's piece from there (kMaxStride keeps it in 32 bits)
   int row, left;   // first row, and columns from the piece's first on
   __device__ __forceinline__ void init(const IO* base, int64_t stride_, int cols) {
     const int c = threadIdx.x % PR * EL;
-    row = threadIdx.x / PR, left = cols - c, stride = stride_;
-    src = base + row * stride + c;
+    row = threadIdx.x / PR, left = cols - c, stride = stride_, src = base;
+    off = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) + c;
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = make_uint4(0, 0, 0, 0);
   }
@@ -192,15 +196,15 @@ template <typename IO, typename E, int W, int ROWS, int NTH, bool VEC> struct St
   // rows t0 .. t0 + ROWS - 1, zeros from row `end` on
   __device__ __forceinline__ void fetch(int t0, int end) {
     if (left <= 0) return;
-    const IO* p = src + t0 * stride;
+    const IO* p = src + t0 * stride;  // a scalar base and a lane's offset to every load
     if (t0 + ROWS <= end) {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (PER * NTH == ROWS * PR || row + STEP * i < ROWS) v[i] = piece(p + STEP * i * stride);
+        if (PER * NTH == ROWS * PR || row + STEP * i < ROWS) v[i] = piece(p + STEP * i * stride + off);
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        v[i] = row + STEP * i < ROWS && t0 + row + STEP * i < end ? piece(p + STEP * i * stride) : make_uint4(0, 0, 0, 0);
+        v[i] = row + STEP * i < ROWS && t0 + row + STEP * i < end ? piece(p + STEP * i * stride + off) : make_uint4(0, 0, 0, 0);
     }
   }
   __device__ __forceinline__ void commit(E* tile) const {
