@@ -21,6 +21,7 @@
 
 #include "vmi_common.h"
 #include "vmi_dispatch.h"
+#include "vmi_lanes.h"
 #include "vmi_vec.h"
 
 namespace vmi {
@@ -42,15 +43,15 @@ struct Args {
   bool vec, wide;
 };
 
-// Sum over the G lanes of a row: a wave, or the whole workgroup (red: one float a wave; the barrier after
+// Sum over the G lanes of a row: a wave, two of a workgroup's four, or all (red: one float a wave; the barrier after
 // the reads lets the next sum use it again).
 template <int G> __device__ __forceinline__ float row_sum(float x, float* red) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  x = half_pair_sum(row_pair_sum(row16_sum(x)));
   if constexpr (G > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[wave] = x;
     __syncthreads();
-    x = (red[0] + red[1]) + (red[2] + red[3]);
+    x = G == 128 ? red[wave & ~1] + red[wave | 1] : (red[0] + red[1]) + (red[2] + red[3]);
     __syncthreads();
   }
   return x;
@@ -73,11 +74,10 @@ template <typename W, int N> __device__ __forceinline__ void load_w(const void* 
   }
 }
 
-// act(gate) and its derivative
-template <typename T> __device__ __forceinline__ void activation(float g, bool silu, float& a, float& da) {
-  const float sg = sigmoid_for<T>(g);
-  a = silu ? g * sg : sg;
-  da = silu ? sg * (1.f + g * (1.f - sg)) : sg * (1.f - sg);
+// act(gate) and its derivative, from the gate and its sigmoid
+__device__ __forceinline__ float activation(float g, float sg, bool silu) { return silu ? g * sg : sg; }
+__device__ __forceinline__ float slope(float g, float sg, bool silu) {
+  return silu ? sg * (1.f + g * (1.f - sg)) : sg * (1.f - sg);
 }
 
 template <typename T, typename W, int G, int NV>
@@ -120,11 +120,7 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
     for (int j = 0; j < N; ++j) {
       float r = t[v][j] * i1;
       if (a.w1 != nullptr) r *= w1[j];
-      if (gate != nullptr) {
-        float da;
-        activation<T>(q[v][j], a.silu, q[v][j], da);
-        r *= q[v][j];
-      }
+      if (gate != nullptr) r *= activation(q[v][j], sigmoid_for<T>(q[v][j]), a.silu);
       t[v][j] = a.scale != nullptr ? fmaf(sc[j], r, x[v][j]) : x[v][j] + r;
       ss = fmaf(t[v][j], t[v][j], ss);
     }
@@ -146,56 +142,97 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   }
 }
 
-template <typename T, typename W, int G, int NV>
-__global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
+// N elements from i on as they lie in memory.
+template <typename T, bool VEC> __device__ __forceinline__ Vec<T> raw(const T* row, int i, int d) {
+  if constexpr (VEC) {
+    return ldv(row + i);
+  } else {
+    Vec<T> v;
+#pragma unroll
+    for (int j = 0; j < Vec<T>::N; ++j) v.e[j] = i + j < d ? row[i + j] : round_to<T>(0.f);
+    return v;
+  }
+}
+template <typename T> __device__ __forceinline__ void widen(const Vec<T>& v, float (&x)[Vec<T>::N]) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N; ++j) x[j] = io<T>::to_f32(v.e[j]);
+}
+
+// A workgroup takes NTH / G rows at a time, the next ones' inputs on their way meanwhile.
+template <typename T, typename W, int G, int NV, bool VEC>
+__global__ __launch_bounds__(NTH, NV == 1 ? 3 : 1) void backward_kernel(Args a) {
   constexpr int N = Vec<T>::N, RW = NTH / G;
   __shared__ float red[NTH / 64];
-  __shared__ float sums[G == 64 ? 3 * 64 * NV * N : 1];
+  __shared__ float sums[RW > 1 ? 3 * G * NV * N : 1];
   const int lane = threadIdx.x % G, d = a.d;
   float b1[NV][N] = {}, bs[NV][N] = {}, b2[NV][N] = {};  // dw1, dscale, dw2
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * RW + threadIdx.x / G; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * RW) {
-    const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
-    const T* res = static_cast<const T*>(a.res) + row * a.r_stride;
-    const T* gate = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + row * a.g_stride;
-    const T* ds = a.ds == nullptr ? nullptr : static_cast<const T*>(a.ds) + row * d;
-    const T* dn = a.dn == nullptr ? nullptr : static_cast<const T*>(a.dn) + row * d;
-    const float i1 = a.w1 == nullptr ? 1.f : a.stats[row];
-    const float i2 = dn == nullptr ? 0.f : a.stats[a.rows + row];
-    float t[NV][N], yv[NV][N], q[NV][N], dt[NV][N];
+  const bool has_gate = a.gate != nullptr, has_s = a.ds != nullptr, has_n = a.dn != nullptr;
+  Vec<T> ry[NV], rr[NV], rg[NV], rs[NV], rn[NV];
+  float r1 = 1.f, r2 = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (lane + G * v) * N;
+      if (i >= d) break;
+      ry[v] = raw<T, VEC>(static_cast<const T*>(a.y) + row * a.y_stride, i, d);
+      if (has_gate) rg[v] = raw<T, VEC>(static_cast<const T*>(a.gate) + row * a.g_stride, i, d);
+      if (has_s) rs[v] = raw<T, VEC>(static_cast<const T*>(a.ds) + row * d, i, d);
+      if (has_n) {
+        rr[v] = raw<T, VEC>(static_cast<const T*>(a.res) + row * a.r_stride, i, d);
+        rn[v] = raw<T, VEC>(static_cast<const T*>(a.dn) + row * d, i, d);
+      }
+    }
+    if (a.w1 != nullptr) r1 = a.stats[row];
+    if (has_n) r2 = a.stats[a.rows + row];
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * RW, mine = threadIdx.x / G;
+  fetch(static_cast<int64_t>(blockIdx.x) * RW + mine);
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RW; row0 < a.rows; row0 += step) {
+    const int64_t row = row0 + mine;
+    const bool on = row < a.rows;  // the others take part in the barriers
+    const float i1 = r1, i2 = r2;
+    float t[NV][N], yv[NV][N], q[NV][N], sg[NV][N], dt[NV][N], x[NV][N], z[NV][N];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      widen<T>(ry[v], yv[v]);
+      widen<T>(rg[v], q[v]);
+      widen<T>(rs[v], dt[v]);
+      widen<T>(rr[v], x[v]);
+      widen<T>(rn[v], z[v]);
+      if (!has_s)
+#pragma unroll
+        for (int j = 0; j < N; ++j) dt[v][j] = 0.f;
+    }
+    fetch(row + step);
     float dot = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (lane + G * v) * N;
       if (i >= d) break;
-      load_piece(y, i, d, a.vec, yv[v]);
-      if (gate != nullptr) load_piece(gate, i, d, a.vec, q[v]);
-      if (ds != nullptr) load_piece(ds, i, d, a.vec, dt[v]);
-      else
+      if (!on) break;
+      if (has_gate)
 #pragma unroll
-        for (int j = 0; j < N; ++j) dt[v][j] = 0.f;
-      if (dn == nullptr) continue;
-      float x[N], z[N], w1[N], sc[N], w2[N];
-      load_piece(res, i, d, a.vec, x);
-      load_piece(dn, i, d, a.vec, z);
+        for (int j = 0; j < N; ++j) sg[v][j] = sigmoid_for<T>(q[v][j]);
+      if (!has_n) continue;
+      float w1[N], sc[N], w2[N];
       if (a.w1 != nullptr) load_w<W>(a.w1, i, d, a.wide, w1);
       if (a.scale != nullptr) load_w<W>(a.scale, i, d, a.wide, sc);
       load_w<W>(a.w2, i, d, a.wide, w2);
 #pragma unroll
       for (int j = 0; j < N; ++j) {  // s again, u = dn w2 and u . s
-        float r = yv[v][j] * i1, act = 1.f, da;
+        float r = yv[v][j] * i1;
         if (a.w1 != nullptr) r *= w1[j];
-        if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
-        r *= act;
-        const float s = a.scale != nullptr ? fmaf(sc[j], r, x[j]) : x[j] + r;
-        b2[v][j] = fmaf(z[j], s * i2, b2[v][j]);
-        const float u = z[j] * w2[j];
+        if (has_gate) r *= activation(q[v][j], sg[v][j], a.silu);
+        const float s = a.scale != nullptr ? fmaf(sc[j], r, x[v][j]) : x[v][j] + r;
+        b2[v][j] = fmaf(z[v][j], s * i2, b2[v][j]);
+        const float u = z[v][j] * w2[j];
         dot = fmaf(u, s, dot);
         t[v][j] = s;
         dt[v][j] = fmaf(i2, u, dt[v][j]);
       }
     }
-    if (dn != nullptr) {
+    if (has_n) {
       const float m = row_sum<G>(dot, red) / d * i2 * i2 * i2;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -208,8 +245,8 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (lane + G * v) * N;
-      if (i >= d) break;
-      if (a.dres != nullptr) store_piece(static_cast<T*>(a.dres) + row * d, i, d, a.vec, dt[v]);
+      if (i >= d || !on) break;
+      if (a.dres != nullptr) store_piece(static_cast<T*>(a.dres) + row * d, i, d, VEC, dt[v]);
       float w1s[N], scs[N];
       if (a.w1 != nullptr) load_w<W>(a.w1, i, d, a.wide, w1s);
       if (a.scale != nullptr) load_w<W>(a.scale, i, d, a.wide, scs);
@@ -218,7 +255,7 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
         const float w1 = a.w1 != nullptr ? w1s[j] : 1.f, sc = a.scale != nullptr ? scs[j] : 1.f;
         const float yn = yv[v][j] * i1;
         float act = 1.f, da = 0.f;
-        if (gate != nullptr) activation<T>(q[v][j], a.silu, act, da);
+        if (has_gate) act = activation(q[v][j], sg[v][j], a.silu), da = slope(q[v][j], sg[v][j], a.silu);
         const float dr = dt[v][j] * sc * act;
         q[v][j] = dt[v][j] * sc * (yn * w1) * da;  // dgate
         bs[v][j] = fmaf(dt[v][j] * act, yn * w1, bs[v][j]);
@@ -226,31 +263,31 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
         dt[v][j] = dr * w1;
         dot = fmaf(dt[v][j], yv[v][j], dot);
       }
-      if (a.dgate != nullptr) store_piece(static_cast<T*>(a.dgate) + row * d, i, d, a.vec, q[v]);
+      if (a.dgate != nullptr) store_piece(static_cast<T*>(a.dgate) + row * d, i, d, VEC, q[v]);
     }
     float m = 0.f;
     if (a.w1 != nullptr) m = row_sum<G>(dot, red) / d * i1 * i1 * i1;
-    if (a.dy == nullptr) continue;
+    if (a.dy == nullptr || !on) continue;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (lane + G * v) * N;
       if (i >= d) break;
 #pragma unroll
       for (int j = 0; j < N; ++j) dt[v][j] = fmaf(-m, yv[v][j], i1 * dt[v][j]);
-      store_piece(static_cast<T*>(a.dy) + row * d, i, d, a.vec, dt[v]);
+      store_piece(static_cast<T*>(a.dy) + row * d, i, d, VEC, dt[v]);
     }
   }
   if (a.partial == nullptr) return;
   float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 3 * d;
-  if constexpr (G == 64) {  // the waves' sums one after the other: the same order in every run
-    constexpr int M = 64 * NV * N;
+  if constexpr (RW > 1) {  // the rows' sums one after the other: the same order in every run
+    constexpr int M = G * NV * N;
     for (int w = 0; w < RW; ++w) {
-      if (threadIdx.x / 64 == w) {
+      if (mine == w) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const int i = (lane + 64 * v) * N + j;
+            const int i = (lane + G * v) * N + j;
             sums[i] = (w ? sums[i] : 0.f) + b1[v][j];
             sums[M + i] = (w ? sums[M + i] : 0.f) + bs[v][j];
             sums[2 * M + i] = (w ? sums[2 * M + i] : 0.f) + b2[v][j];
@@ -299,10 +336,11 @@ __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__
 }
 
 // A wave takes rows of up to two pieces a lane, a workgroup longer ones; at most 8 pieces a lane.
-template <typename T, typename F> int by_row(int d, F&& f) {
+template <typename T, bool BACKWARD, typename F> int by_row(int d, F&& f) {
   const int pieces = (d + Vec<T>::N - 1) / Vec<T>::N;
   if (pieces <= 64) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-  if (pieces <= 128) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  // two waves a row: one leaves 232 registers and no room for the next row's loads (220 us at 32768 rows of 1024)
+  if (pieces <= 128) return f(std::integral_constant<int, BACKWARD ? 128 : 64>{}, std::integral_constant<int, BACKWARD ? 1 : 2>{});
   if (pieces <= 256) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 1>{});
   if (pieces <= 512) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 2>{});
   if (pieces <= 1024) return f(std::integral_constant<int, NTH>{}, std::integral_constant<int, 4>{});
@@ -315,10 +353,11 @@ template <typename T, typename F> int by_weight(int w_dtype, int dtype, F&& f) {
 }
 bool rows_fit(int64_t d, int dtype) { return d <= (dtype == VMI_F32 ? 4096 : 8192); }
 
-// Workgroups of the backward: enough to fill the card twice over, and few enough that the partials stay small.
+// Workgroups of the backward: enough to fill the card, and few enough that the partials stay small.
 int backward_blocks(int64_t rows, int64_t d, int dtype) {
-  const int per = d * (dtype == VMI_F32 ? 4 : 2) <= 2048 ? NTH / 64 : 1;
-  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, 512));
+  const int64_t bytes = d * (dtype == VMI_F32 ? 4 : 2);
+  const int per = bytes <= 1024 ? 4 : bytes <= 2048 ? 2 : 1;
+  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, 768));
 }
 
 int check(const Args& a, int dtype, int w_dtype) {
@@ -359,7 +398,7 @@ extern "C" int vmi_gated_norm(const void* y, int64_t y_stride, const void* resid
     using T = decltype(tag);
     return by_weight<T>(w_dtype, dtype, [&](auto wtag) -> int {
       using W = decltype(wtag);
-      return by_row<T>(a.d, [&](auto g, auto nv) -> int {
+      return by_row<T, false>(a.d, [&](auto g, auto nv) -> int {
         constexpr int per = NTH / decltype(g)::value;
         hipLaunchKernelGGL((forward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
                            dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(NTH), 0,
@@ -410,9 +449,11 @@ extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* r
       using W = decltype(wtag);
       int rc = VMI_OK;
       if (rows > 0)
-        rc = by_row<T>(a.d, [&](auto g, auto nv) -> int {
-          hipLaunchKernelGGL((backward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
-                             dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, st, a);
+        rc = by_row<T, true>(a.d, [&](auto g, auto nv) -> int {
+          constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+          const dim3 grid(static_cast<unsigned>(blocks));
+          if (a.vec) hipLaunchKernelGGL((backward_kernel<T, W, G, NV, true>), grid, dim3(NTH), 0, st, a);
+          else hipLaunchKernelGGL((backward_kernel<T, W, G, NV, false>), grid, dim3(NTH), 0, st, a);
           return hip_status(hipGetLastError());
         });
       if (rc != VMI_OK || !weights) return rc;

@@ -41,14 +41,19 @@ __device__ __forceinline__ void load_piece(const T* row, int i0, int d, bool vec
     for (int j = 0; j < N; ++j) x[j] = i0 + j < d ? io<T>::load(row, i0 + j) : 0.f;
   }
 }
+// The compiler's own type of a memory type.
+template <typename T> struct native { typedef T type; };
+template <> struct native<bf16_t> { typedef __bf16 type; };
 template <typename T>
 __device__ __forceinline__ void store_piece(T* row, int i0, int d, bool vec, const float (&x)[Vec<T>::N]) {
   constexpr int N = Vec<T>::N;
   if (vec) {
-    Vec<T> v;
+    typename native<T>::type e[N];  // by the conversion instructions, two at a time
 #pragma unroll
-    for (int j = 0; j < N; ++j) v.e[j] = round_to<T>(x[j]);
-    stv(row + i0, v);
+    for (int j = 0; j < N; ++j) e[j] = static_cast<typename native<T>::type>(x[j]);
+    uint4 v;
+    __builtin_memcpy(&v, e, 16);
+    *reinterpret_cast<uint4*>(row + i0) = v;
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)

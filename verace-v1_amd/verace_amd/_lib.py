@@ -229,5 +229,11 @@ def check(status: int, what: str) -> None:
         raise RuntimeError(f"verace_amd: {what} failed: {msg} (status {status}, hipError {hip})")
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream of a device as the library takes it (torch.cuda.current_stream without the object)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index)
+
+
 def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)

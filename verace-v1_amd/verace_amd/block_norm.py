@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hip_kernels import _ptr, _require_device, device_guard
+from .hip_kernels import _require_device, address, device_guard
 
 _ACT = {"sigmoid": 0, "silu": 1}
 
@@ -18,7 +18,8 @@ def _rows(t: Optional[torch.Tensor], d: int) -> Optional[torch.Tensor]:
     """t as [rows, d] with contiguous rows (a view where its rows lie at one stride)."""
     if t is None:
         return None
-    t = t.reshape(-1, d)
+    if t.dim() != 2:
+        t = t.reshape(-1, d)
     return t if t.stride(1) == 1 or d == 1 else t.contiguous()
 
 
@@ -31,9 +32,9 @@ def _launch(y, residual, gate, w1, scale, w2, eps1, eps2, act, want_stats):
     w = next((t for t in (w1, scale, w2) if t is not None), None)
     with device_guard(y):
         _lib.check(_lib.load().vmi_gated_norm(
-            _ptr(y2), y2.stride(0), _ptr(r2), r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), _ptr(w1),
-            _ptr(scale), _ptr(w2), _lib.dtype_code(y.dtype), _lib.dtype_code(y.dtype if w is None else w.dtype), act,
-            eps1, eps2, _ptr(s), _ptr(n), _ptr(stats), y2.shape[0], d, _lib.stream_handle(y.device)), "vmi_gated_norm")
+            address(y2), y2.stride(0), address(r2), r2.stride(0), address(g2), 0 if g2 is None else g2.stride(0), address(w1),
+            address(scale), address(w2), _lib.dtype_code(y.dtype), _lib.dtype_code(y.dtype if w is None else w.dtype), act,
+            eps1, eps2, address(s), address(n), address(stats), y2.shape[0], d, _lib.raw_stream(y.device)), "vmi_gated_norm")
     return s, n, stats
 
 
@@ -70,10 +71,10 @@ class GatedNormFunction(torch.autograd.Function):
             ws = torch.empty(ws_bytes.value, device=y.device, dtype=torch.uint8)
         with device_guard(y):
             _lib.check(lib.vmi_gated_norm_bwd(
-                _ptr(y2), y2.stride(0), _ptr(r2), r2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), _ptr(w1),
-                _ptr(scale), _ptr(w2), code, _lib.dtype_code(y.dtype if w is None else w.dtype), ctx.act, _ptr(stats),
-                _ptr(ds), _ptr(dn), _ptr(dy), _ptr(dres), _ptr(dgate), _ptr(dw1), _ptr(dscale), _ptr(dw2),
-                y2.shape[0], d, _ptr(ws), ws_bytes.value, _lib.stream_handle(y.device)), "vmi_gated_norm_bwd")
+                address(y2), y2.stride(0), address(r2), r2.stride(0), address(g2), 0 if g2 is None else g2.stride(0), address(w1),
+                address(scale), address(w2), code, _lib.dtype_code(y.dtype if w is None else w.dtype), ctx.act, address(stats),
+                address(ds), address(dn), address(dy), address(dres), address(dgate), address(dw1), address(dscale), address(dw2),
+                y2.shape[0], d, address(ws), ws_bytes.value, _lib.raw_stream(y.device)), "vmi_gated_norm_bwd")
         return dy, dres, dgate, dw1, dscale, dw2, None, None, None
 
 
@@ -99,33 +100,35 @@ def gated_norm_add(
     unrounded s.  Differentiable once, in every tensor argument.
     """
     _require_device(y, "y")
-    if y.dim() < 1 or y.shape[-1] < 1:
-        raise RuntimeError(f"verace_amd: y must be [..., d], got {tuple(y.shape)}")
-    _lib.dtype_code(y.dtype)
-    d = y.shape[-1]
-    if d > (4096 if y.dtype == torch.float32 else 8192):
-        raise RuntimeError(f"verace_amd: rows of {d} {y.dtype} elements are too long for gated_norm_add")
+    shape, dtype, device = y.shape, y.dtype, y.device
+    if len(shape) < 1 or shape[-1] < 1:
+        raise RuntimeError(f"verace_amd: y must be [..., d], got {tuple(shape)}")
+    _lib.dtype_code(dtype)
+    d = shape[-1]
+    if d > (4096 if dtype == torch.float32 else 8192):
+        raise RuntimeError(f"verace_amd: rows of {d} {dtype} elements are too long for gated_norm_add")
     if activation not in _ACT:
         raise RuntimeError(f"verace_amd: activation must be one of {tuple(_ACT)}, got {activation!r}")
-    if residual.shape != y.shape:
-        raise RuntimeError(f"verace_amd: residual shape {tuple(residual.shape)} != y shape {tuple(y.shape)}")
-    if gate is not None and gate.shape != y.shape:
+    if residual.shape != shape:
+        raise RuntimeError(f"verace_amd: residual shape {tuple(residual.shape)} != y shape {tuple(shape)}")
+    if gate is not None and gate.shape != shape:
         try:
-            gate = gate.expand(y.shape)
+            gate = gate.expand(shape)
         except RuntimeError:
-            raise RuntimeError(f"verace_amd: gate {tuple(gate.shape)} does not broadcast to {tuple(y.shape)}") from None
+            raise RuntimeError(f"verace_amd: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
     for name, t in (("residual", residual), ("gate", gate)):
-        if t is not None and (t.dtype != y.dtype or t.device != y.device):
-            raise RuntimeError(f"verace_amd: {name} must be {y.dtype} on {y.device}, got {t.dtype} on {t.device}")
-    ws = []
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise RuntimeError(f"verace_amd: {name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+    w_dtype = None
     for name, t in (("norm_weight", norm_weight), ("scale", scale), ("next_weight", next_weight)):
-        if t is not None:
-            if tuple(t.shape) != (d,) or t.device != y.device or t.dtype not in (y.dtype, torch.float32):
-                raise RuntimeError(f"verace_amd: {name} must be [{d}] {y.dtype} or float32 on {y.device}, "
-                                   f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-            ws.append(t)
-    if len({t.dtype for t in ws}) > 1:
-        raise RuntimeError("verace_amd: norm_weight, scale and next_weight must have one dtype")
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != d or t.device != device or t.dtype not in (dtype, torch.float32):
+            raise RuntimeError(f"verace_amd: {name} must be [{d}] {dtype} or float32 on {device}, "
+                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if w_dtype is not None and t.dtype != w_dtype:
+            raise RuntimeError("verace_amd: norm_weight, scale and next_weight must have one dtype")
+        w_dtype = t.dtype
     w1, sc, w2 = (None if t is None else t.contiguous() for t in (norm_weight, scale, next_weight))
     eps1, eps2 = float(eps), float(eps if next_eps is None else next_eps)
     act = _ACT[activation]

@@ -48,6 +48,11 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def address(t: Optional[torch.Tensor]) -> Optional[int]:
+    """A tensor's device pointer as a plain number (None: absent)."""
+    return None if t is None else t.data_ptr()
+
+
 _NO_GUARD = contextlib.nullcontext()
 
 

@@ -17,15 +17,16 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hip_kernels import _mask_bytes, _ptr, _require_device, device_guard
+from .hip_kernels import _mask_bytes, _require_device, address, device_guard
 
 _ACT = {None: 0, "silu": 1}
 
 
 def _same_device(like: torch.Tensor, **tensors) -> None:
+    device = like.device
     for name, t in tensors.items():
-        if t is not None and t.device != like.device:
-            raise RuntimeError(f"verace_amd: {name} must be on {like.device}, got {t.device}")
+        if t is not None and t.device != device:
+            raise RuntimeError(f"verace_amd: {name} must be on {device}, got {t.device}")
 
 
 def _lengths(lengths: Optional[torch.Tensor], B: int, like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -39,6 +40,8 @@ def _lengths(lengths: Optional[torch.Tensor], B: int, like: torch.Tensor) -> Opt
 
 def _inner(t: torch.Tensor, lead: int) -> torch.Tensor:
     """t with everything after its first ``lead`` dimensions contiguous (a copy only if it is not)."""
+    if t.is_contiguous():
+        return t
     expect = 1
     for size, stride in zip(reversed(t.shape[lead:]), reversed(t.stride()[lead:])):
         if size != 1 and stride != expect:
@@ -72,9 +75,9 @@ def _launch_conv(x, weight, bias, state, lengths, act):
     out = torch.empty(B, K - 1, C, device=x.device, dtype=x.dtype)
     with device_guard(x):
         _lib.check(_lib.load().vmi_short_conv(
-            _ptr(x), x.stride(1), x.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), act,
-            _ptr(state), _ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), _ptr(y), _ptr(out),
-            B, T, C, K, _lib.stream_handle(x.device)), "vmi_short_conv")
+            address(x), x.stride(1), x.stride(0), address(w), address(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), act,
+            address(state), address(lengths), int(lengths is not None and lengths.dtype == torch.int64), address(y), address(out),
+            B, T, C, K, _lib.raw_stream(x.device)), "vmi_short_conv")
     return y, out
 
 
@@ -112,10 +115,10 @@ class ShortConvFunction(torch.autograd.Function):
             ws = torch.empty(max(1, ws_bytes.value), device=x.device, dtype=torch.uint8)
         with device_guard(x):
             _lib.check(lib.vmi_short_conv_bwd(
-                _ptr(x), x.stride(1), x.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype),
-                ctx.act, _ptr(state), _ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), _ptr(dy),
-                0 if dy is None else dy.stride(1), 0 if dy is None else dy.stride(0), _ptr(dout), _ptr(dx), _ptr(dw),
-                _ptr(db), _ptr(dstate), B, T, C, K, _ptr(ws), ws_bytes.value, _lib.stream_handle(x.device)),
+                address(x), x.stride(1), x.stride(0), address(w), address(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype),
+                ctx.act, address(state), address(lengths), int(lengths is not None and lengths.dtype == torch.int64), address(dy),
+                0 if dy is None else dy.stride(1), 0 if dy is None else dy.stride(0), address(dout), address(dx), address(dw),
+                address(db), address(dstate), B, T, C, K, address(ws), ws_bytes.value, _lib.raw_stream(x.device)),
                 "vmi_short_conv_bwd")
         return dx, dw, db, dstate, None, None
 
@@ -181,8 +184,8 @@ def short_conv_step_(
     y = torch.empty(B, 1, C, device=x.device, dtype=x.dtype)
     with device_guard(x):
         _lib.check(_lib.load().vmi_short_conv_step(
-            _ptr(x2), x2.stride(0), _ptr(w), _ptr(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), _ACT[activation],
-            _ptr(mask), _ptr(state), _ptr(y), B, C, K1 + 1, _lib.stream_handle(x.device)), "vmi_short_conv_step")
+            address(x2), x2.stride(0), address(w), address(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), _ACT[activation],
+            address(mask), address(state), address(y), B, C, K1 + 1, _lib.raw_stream(x.device)), "vmi_short_conv_step")
     return y
 
 
@@ -191,8 +194,10 @@ def short_conv_step_(
 def _head_vector(t: Optional[torch.Tensor], H: int, name: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if tuple(t.shape) != (H,):
+    if t.dim() != 1 or t.shape[0] != H:
         raise RuntimeError(f"verace_amd: {name} must be [{H}], got {tuple(t.shape)}")
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
     return t.to(torch.float32).contiguous()
 
 
@@ -203,13 +208,12 @@ def _scan_check(x, delta, A, Bm, Cm, D, delta_bias):
     if x.dim() != 4:
         raise RuntimeError(f"verace_amd: x must be [B, T, H, P], got {tuple(x.shape)}")
     B, T, H, P = x.shape
-    if delta.dim() == 4 and delta.shape[-1] == 1:
-        delta = delta.squeeze(-1)
-    if tuple(delta.shape) != (B, T, H):
-        raise RuntimeError(f"verace_amd: delta must be [B, T, H] = {(B, T, H)}, got {tuple(delta.shape)}")
-    if Bm.dim() != 4 or Bm.shape[:2] != x.shape[:2] or Cm.shape != Bm.shape:
-        raise RuntimeError(f"verace_amd: B and C must be [B, T, G, N], got {tuple(Bm.shape)}, {tuple(Cm.shape)}")
-    G, N = Bm.shape[2:]
+    ds, bs = delta.shape, Bm.shape
+    if ds != (B, T, H) and ds != (B, T, H, 1):
+        raise RuntimeError(f"verace_amd: delta must be [B, T, H] = {(B, T, H)}, got {tuple(ds)}")
+    if len(bs) != 4 or bs[0] != B or bs[1] != T or Cm.shape != bs:
+        raise RuntimeError(f"verace_amd: B and C must be [B, T, G, N], got {tuple(bs)}, {tuple(Cm.shape)}")
+    G, N = bs[2], bs[3]
     if G < 1 or H % G != 0:
         raise RuntimeError(f"verace_amd: {H} heads do not share {G} groups of B and C")
     if not 1 <= N <= 256 or not 1 <= P <= 1024:
@@ -256,11 +260,11 @@ def launch_selective_hip_scan(
     ws = torch.empty(ws_bytes.value, device=x.device, dtype=torch.uint8) if ws_bytes.value else None
     with device_guard(x):
         _lib.check(lib.vmi_selective_scan_fwd(
-            _ptr(x), x.stride(1), x.stride(0), _ptr(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
-            _ptr(A), _ptr(B), B.stride(1), B.stride(0), _ptr(C), C.stride(1), C.stride(0), _ptr(D), _ptr(bias),
-            int(bool(softplus)), code, _ptr(state), _ptr(lengths),
-            int(lengths is not None and lengths.dtype == torch.int64), _ptr(y), _ptr(out), b, T, H, P, G, N, _ptr(ws),
-            ws_bytes.value, _lib.stream_handle(x.device)), "vmi_selective_scan_fwd")
+            address(x), x.stride(1), x.stride(0), address(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
+            address(A), address(B), B.stride(1), B.stride(0), address(C), C.stride(1), C.stride(0), address(D), address(bias),
+            int(bool(softplus)), code, address(state), address(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), address(y), address(out), b, T, H, P, G, N, address(ws),
+            ws_bytes.value, _lib.raw_stream(x.device)), "vmi_selective_scan_fwd")
     return y, out
 
 
@@ -302,12 +306,12 @@ def launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D=None, delta_bias=None
     ws = torch.empty(ws_bytes.value, device=x.device, dtype=torch.uint8)
     with device_guard(x):
         _lib.check(lib.vmi_selective_scan_bwd(
-            _ptr(x), x.stride(1), x.stride(0), _ptr(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
-            _ptr(A), _ptr(B), B.stride(1), B.stride(0), _ptr(C), C.stride(1), C.stride(0), _ptr(D), _ptr(bias),
-            int(bool(softplus)), code, _ptr(state), _ptr(lengths),
-            int(lengths is not None and lengths.dtype == torch.int64), _ptr(dy), dy.stride(1), dy.stride(0),
-            _ptr(d_state), _ptr(dx), _ptr(dd), _ptr(heads[0]), _ptr(dB), _ptr(dC), _ptr(heads[1]), _ptr(heads[2]),
-            _ptr(d0), b, T, H, P, G, N, _ptr(ws), ws_bytes.value, _lib.stream_handle(x.device)),
+            address(x), x.stride(1), x.stride(0), address(delta), delta.stride(1), delta.stride(0), _lib.dtype_code(delta.dtype),
+            address(A), address(B), B.stride(1), B.stride(0), address(C), C.stride(1), C.stride(0), address(D), address(bias),
+            int(bool(softplus)), code, address(state), address(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), address(dy), dy.stride(1), dy.stride(0),
+            address(d_state), address(dx), address(dd), address(heads[0]), address(dB), address(dC), address(heads[1]), address(heads[2]),
+            address(d0), b, T, H, P, G, N, address(ws), ws_bytes.value, _lib.raw_stream(x.device)),
             "vmi_selective_scan_bwd")
     return dx, dd.view(shape), heads[0], dB, dC, heads[1], heads[2], d0
 
@@ -399,7 +403,7 @@ def selective_step_(
     y = torch.empty(b, 1, H, P, device=x.device, dtype=x.dtype)
     with device_guard(x):
         _lib.check(_lib.load().vmi_selective_step(
-            _ptr(x), x.stride(0), _ptr(delta), delta.stride(0), _lib.dtype_code(delta.dtype), _ptr(A), _ptr(B),
-            B.stride(0), _ptr(C), C.stride(0), _ptr(D), _ptr(bias), int(bool(softplus)), _lib.dtype_code(x.dtype),
-            _ptr(mask), _ptr(state), _ptr(y), b, H, P, G, N, _lib.stream_handle(x.device)), "vmi_selective_step")
+            address(x), x.stride(0), address(delta), delta.stride(0), _lib.dtype_code(delta.dtype), address(A), address(B),
+            B.stride(0), address(C), C.stride(0), address(D), address(bias), int(bool(softplus)), _lib.dtype_code(x.dtype),
+            address(mask), address(state), address(y), b, H, P, G, N, _lib.raw_stream(x.device)), "vmi_selective_step")
     return y
