@@ -80,7 +80,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
   __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
   __shared__ __attribute__((aligned(16))) E Ms[READOUT ? LT * 64 * 8 : 8];
   __shared__ __attribute__((aligned(16))) float2 cs[L];
-  __shared__ __attribute__((aligned(16))) float ds[L], ws[L];
+  __shared__ __attribute__((aligned(16))) float ds[L], ws[L], es[L];
   const Args& a = k.a;
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   // neighbouring workgroups go to different XCDs: give each XCD a run of consecutive heads, which share B and C
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
     if (tid < L) {
       cs[tid] = rc;
       ds[tid] = rd;
+      es[tid] = __expf(rc.x + rc.y);
       ws[tid] = rd * decay(rl, rc);
     }
     lds_barrier();
@@ -201,11 +202,10 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
         }
       }
     }
-    const float2 cl = cs[L - 1];
     Frag<E> xf;
     if (live) {
       xf = col_frag<E, PB>(Xs, 0, 16 * wave, l16, g);
-      const float dl = __expf(cl.x + cl.y);
+      const float dl = es[L - 1];
 #pragma unroll
       for (int j = 0; j < NT; ++j) S[j] *= dl;
       f32x4 wx[2];
@@ -226,14 +226,13 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
       }
     }
     if constexpr (!READOUT) {
-      seg_c += static_cast<double>(cl.x) + static_cast<double>(cl.y);
+      seg_c += static_cast<double>(cs[L - 1].x) + static_cast<double>(cs[L - 1].y);
     } else {
       lds_barrier();  // the scores are in LDS
       if (live) {
 #pragma unroll
         for (int t = 0; t < LT; ++t) {
-          const float2 ct = cs[16 * t + l16];
-          acc[t] *= __expf(ct.x + ct.y);
+          acc[t] *= es[16 * t + l16];
           const E* m = Ms + (t * 64 + lane) * 8;
           Frag<E> f;
           if constexpr (sizeof(E) == 2) {

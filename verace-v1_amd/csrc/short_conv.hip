@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64) void step_kernel(Args a) {
 // first.  The pass goes down u = t0 .. t0 + BRUN + K - 2: z and dz of token u need rows u - (K - 1) .. u,
 // and row u - (K - 1) is done once dz of u is known.
 template <typename T, int K, int N>
-__global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
+__global__ __launch_bounds__(NTH, 3) void backward_kernel(Args a) {
   constexpr int RW = NTH / CT;
   __shared__ float sums[RW][K + 1][CT * N];
   const int piece = blockIdx.x * CT + threadIdx.x % CT, worker = threadIdx.x / CT;
@@ -226,7 +226,8 @@ __global__ __launch_bounds__(NTH) void backward_kernel(Args a) {
       if (t0 - (K - 1) + k < n) row<T, K, N>(a, b, t0 - (K - 1) + k, c0, win[k + 1]);
       else zero(win[k + 1]);
     }
-    constexpr int GRP = 8;  // tokens whose loads are in flight together
+    constexpr int GRP = 4;  // tokens whose loads are in flight together
+#pragma unroll 1
     for (int u0 = t0; u0 < t1 + K - 1; u0 += GRP) {
       Raw<T, N> xs[GRP], gs[GRP];
 #pragma unroll
