@@ -256,13 +256,15 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   typedef Tile<E, L> TQ;
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
   __shared__ __attribute__((aligned(16))) E Cs[TB::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Ys[TX::elems(L)];
+  // x, dy and the log decays of a unit while the next one's arrive
+  constexpr bool XROWS = NP <= 128;  // x by lane group (12 KB of 10); at 256 state columns LDS is full
+  __shared__ __attribute__((aligned(16))) E Xb[2][XROWS ? RowTile<E, PB>::elems(L) : TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Yb[2][TX::elems(L)];
+  __shared__ __attribute__((aligned(16))) float2 cb2[2][L];
+  __shared__ __attribute__((aligned(16))) float db2[2][L], eb2[2][L], wb2[2][L];
   __shared__ __attribute__((aligned(16))) E Qs[TQ::elems(L)];   // [t][s]
   __shared__ __attribute__((aligned(16))) E Ms[TQ::elems(L)];
   __shared__ __attribute__((aligned(16))) E Gs[TX::elems(GR)];  // G_L^T [n][p]
-  __shared__ __attribute__((aligned(16))) float2 cs[L];
-  __shared__ __attribute__((aligned(16))) float ds[L], es[L], ws[L];
   __shared__ float row_r[LT][L], col_r[LT][L];                  // sum_s R d_s by s-tile, sum_t R by t-tile
   __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
   const Args& a = k.a;
@@ -324,9 +326,26 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           g1[j][w] = *reinterpret_cast<const f32x4*>(k.g1 + q);
         }
     };
+    auto x_frag = [&](const E* tile, int row0, int k0) {
+      if constexpr (XROWS) return packed_frag<E, PB, L>(tile, row0, k0, l16, g);
+      else return row_frag<E, PB>(tile, row0, k0, l16, g);
+    };
+    auto commit = [&](int u) {
+      if constexpr (XROWS) sx.commit_rows(Xb[u & 1]);
+      else sx.commit(Xb[u & 1]);
+      sy.commit(Yb[u & 1]);
+      if (tid < L) {
+        cb2[u & 1][tid] = rc;
+        db2[u & 1][tid] = rd;
+        eb2[u & 1][tid] = __expf(rc.x + rc.y);
+        wb2[u & 1][tid] = decay(rl, rc);
+      }
+    };
     fetch(0);
     fetch_states(0);
-    __syncthreads();
+    commit(0);
+    if (units > 1) fetch(1);
+    lds_barrier();
     f32x4 cb[PER];  // C . B of this wave's tiles, transposed (rows s, column t)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -339,17 +358,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
     }
     for (int u = 0; u < units; ++u) {
       const int h = h0 + u / k.pblocks, pb = u % k.pblocks, p0 = pb * PB;
-      lds_barrier();  // the last unit's readers are done
-      sx.commit(Xs);
-      sy.commit(Ys);
-      if (tid < L) {
-        cs[tid] = rc;
-        ds[tid] = rd;
-        es[tid] = __expf(rc.x + rc.y);
-        ws[tid] = decay(rl, rc);
-      }
-      lds_barrier();
-      if (u + 1 < units) fetch(u + 1);
+      const E *Xs = Xb[u & 1], *Ys = Yb[u & 1];
+      const float2* cs = cb2[u & 1];
+      const float *ds = db2[u & 1], *es = eb2[u & 1], *ws = wb2[u & 1];
+      if (u > 0) lds_barrier();  // the last unit's readers of Q, M and G_L are done; this one's inputs are there
       // Q, M and the sums of R
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -358,7 +370,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         f32x4 xy = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KP; ++kb)
-          xy = mma(row_frag<E, PB>(Xs, 16 * st, 32 * kb, l16, g), row_frag<E, PB>(Ys, 16 * tt, 32 * kb, l16, g), xy);
+          xy = mma(x_frag(Xs, 16 * st, 32 * kb), row_frag<E, PB>(Ys, 16 * tt, 32 * kb, l16, g), xy);
         const int t = 16 * tt + l16;
         const float2 ct = cs[t];
         struct alignas(8) M4 { E e[4]; } q, m;
@@ -411,7 +423,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
 #pragma unroll
           for (int t = 0; t < LTW; ++t) {
             const Frag<E> yf = row_frag<E, PB>(Ys, 16 * (tt0 + t), 32 * kb, l16, g);
-            const Frag<E> xf = row_frag<E, PB>(Xs, 16 * (tt0 + t), 32 * kb, l16, g);
+            const Frag<E> xf = x_frag(Xs, 16 * (tt0 + t), 32 * kb);
 #pragma unroll
             for (int q = NPART - 1; q >= 0; --q) {
               sy_[t] = mma(sp[q], yf, sy_[t]);
@@ -464,6 +476,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         }
         if (hh == NH - 1 && u + 1 < units) fetch_states(u + 1);
         lds_barrier();
+        if (hh == NH - 1 && u + 1 < units) {  // into the other buffers: the unit before this one is done with them
+          commit(u + 1);
+          if (u + 2 < units) fetch(u + 2);
+        }
 #pragma unroll
         for (int kb = 0; kb < GR / 32; ++kb) {
           const Frag<E> gf = col_frag<E, PB>(Gs, 32 * kb, 16 * pt, l16, g);
