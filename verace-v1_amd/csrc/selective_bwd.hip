@@ -56,7 +56,8 @@ struct Bwd {
   void *dx, *ddelta, *db, *dc;
   float *dA, *dD, *dbias, *dstate_in;
   int nch, seg_chunks, nseg, pblocks, hblocks, hper;
-  bool vec, vec_dx;
+  const float* Dz;           // D, or anything as long without one
+  bool vec, vec_dx, has_d;
 };
 
 // ------------------------------------------------------------------ S_0 and G_L of every chunk
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   __shared__ __attribute__((aligned(16))) E Xb[2][XROWS ? RowTile<E, PB>::elems(L) : TX::elems(L)];
   __shared__ __attribute__((aligned(16))) E Yb[2][TX::elems(L)];
   __shared__ __attribute__((aligned(16))) float2 cb2[2][L];
-  __shared__ __attribute__((aligned(16))) float db2[2][L], eb2[2][L], wb2[2][L];
+  __shared__ __attribute__((aligned(16))) float db2[2][L], eb2[2][L], wb2[2][L], dh2[2];
   __shared__ __attribute__((aligned(16))) E Qs[TQ::elems(L)];   // [t][s]
   __shared__ __attribute__((aligned(16))) E Ms[TQ::elems(L)];
   __shared__ __attribute__((aligned(16))) E Gs[TX::elems(GR)];  // G_L^T [n][p]
@@ -297,8 +298,8 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       for (int i = tid; i < TQ::elems(L); i += MNT) Qs[i] = Ms[i] = static_cast<E>(0.f);
     }
     Stage<IO, E, PB, L, MNT, VEC> sx, sy;
-    float rd = 0.f;
-    float2 rc = make_float2(0.f, 0.f), rl = rc;
+    float rd, rD;
+    float2 rc, rl;
     f32x4 s0[NTW][4], g1[NTW][4];
     const int units = (h1 - h0) * k.pblocks;
     auto fetch = [&](int u) {
@@ -307,12 +308,11 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       sy.init(static_cast<const IO*>(k.dy) + b * k.y_b + static_cast<int64_t>(h) * a.P + p0, k.y_t, a.P - p0);
       sx.fetch(t0, len);
       sy.fetch(t0, len);
-      if (tid < L) {
-        const int64_t o = (static_cast<int64_t>(b) * a.H + h) * tp + t0;
-        rd = k.d[o + tid];
-        rc = k.c[o + tid];
-        rl = k.c[o + L - 1];
-      }
+      const int64_t o = (static_cast<int64_t>(b) * a.H + h) * tp + t0;  // every lane, so that no value is merged
+      rd = k.d[o + tid % L];
+      rc = k.c[o + tid % L];
+      rl = k.c[o + L - 1];
+      rD = k.Dz[h];
     };
     auto fetch_states = [&](int u) {
       const int64_t bhp = (static_cast<int64_t>(b) * a.H + h0) * k.pblocks + u;
@@ -335,6 +335,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       else sx.commit(Xb[u & 1]);
       sy.commit(Yb[u & 1]);
       if (tid < L) {
+        if (tid == 0) dh2[u & 1] = rD;
         cb2[u & 1][tid] = rc;
         db2[u & 1][tid] = rd;
         eb2[u & 1][tid] = __expf(rc.x + rc.y);
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
     fetch(0);
     fetch_states(0);
     commit(0);
-    if (units > 1) fetch(1);
+    fetch(units > 1 ? 1 : 0);
     lds_barrier();
     f32x4 cb[PER];  // C . B of this wave's tiles, transposed (rows s, column t)
 #pragma unroll
@@ -362,6 +363,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       const float2* cs = cb2[u & 1];
       const float *ds = db2[u & 1], *es = eb2[u & 1], *ws = wb2[u & 1];
       if (u > 0) lds_barrier();  // the last unit's readers of Q, M and G_L are done; this one's inputs are there
+      const float Dh = k.has_d ? dh2[u & 1] : 0.f;
       // Q, M and the sums of R
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -371,21 +373,23 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
 #pragma unroll
         for (int kb = 0; kb < KP; ++kb)
           xy = mma(x_frag(Xs, 16 * st, 32 * kb), row_frag<E, PB>(Ys, 16 * tt, 32 * kb, l16, g), xy);
-        const int t = 16 * tt + l16;
+        const int t = 16 * tt + l16, s0_ = 16 * st + 4 * g;
         const float2 ct = cs[t];
-        struct alignas(8) M4 { E e[4]; } q, m;
+        const f32x4 c01 = *reinterpret_cast<const f32x4*>(cs + s0_), c23 = *reinterpret_cast<const f32x4*>(cs + s0_ + 2);
+        const f32x4 dv = *reinterpret_cast<const f32x4*>(ds + s0_);
+        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q, m;
         float rs = 0.f, dg = 0.f, rr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int s = 16 * st + 4 * g + r;
-          const bool on = s <= t;
-          const float w = on ? decay(ct, cs[s]) : 0.f, wd = w * ds[s];
-          const float x0 = on ? xy[r] : 0.f, c0 = on ? cb[i][r] : 0.f;
-          q.e[r] = static_cast<E>(x0 * wd);
-          m.e[r] = static_cast<E>(c0 * wd);
-          rr[r] = c0 * x0 * w;
-          rs = fmaf(rr[r], ds[s], rs);
-          if (s == t) dg = x0;
+          const bool on = s0_ + r <= t;
+          const float2 from = make_float2((r < 2 ? c01 : c23)[2 * (r & 1)], (r < 2 ? c01 : c23)[2 * (r & 1) + 1]);
+          const float w = decay(ct, from), wd = w * dv[r];
+          const float xq = xy[r] * wd, cm_ = cb[i][r] * wd, xc = cb[i][r] * xy[r] * w;  // off the triangle: dropped, not added
+          q.e[r] = static_cast<E>(on ? xq : 0.f);
+          m.e[r] = static_cast<E>(on ? cm_ : 0.f);
+          rr[r] = on ? xc : 0.f;
+          rs = fmaf(rr[r], dv[r], rs);
+          dg = s0_ + r == t ? xy[r] : dg;
         }
         const int o = TQ::at(t) + 16 * st + 4 * g;
         *reinterpret_cast<M4*>(Qs + o) = q;
@@ -474,11 +478,11 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           kp = half_pair_sum(row_pair_sum(row16_sum(kp)));
           if (lane == 0) kappa[wave] = NT >= NW || tt0 == 0 ? kp : 0.f;
         }
-        if (hh == NH - 1 && u + 1 < units) fetch_states(u + 1);
+        if (hh == NH - 1) fetch_states(u + 1 < units ? u + 1 : u);
         lds_barrier();
         if (hh == NH - 1 && u + 1 < units) {  // into the other buffers: the unit before this one is done with them
           commit(u + 1);
-          if (u + 2 < units) fetch(u + 2);
+          fetch(u + 2 < units ? u + 2 : u + 1);  // always, and the states too: a load under a condition is waited for where its value merges
         }
 #pragma unroll
         for (int kb = 0; kb < GR / 32; ++kb) {
@@ -502,7 +506,6 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           }
         }
       }
-      const float Dh = a.D == nullptr ? 0.f : a.D[h];
 #pragma unroll
       for (int t = 0; t < DXT; ++t) {
         const int st = st0 + t, s = 16 * st + l16;
@@ -540,8 +543,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
             for (int i = 0; i < NS; ++i) v += which == 0 ? alpha[i][t] : beta[i][t];
           } else {
 #pragma unroll
-            for (int i = 0; i < LT; ++i)
-              if (which == 2 ? i <= t / 16 : i >= t / 16) v += which == 2 ? row_r[i][t] : col_r[i][t];
+            for (int i = 0; i < LT; ++i) {  // (slots of tiles right of the diagonal hold nothing)
+              const float w = which == 2 ? row_r[i][t] : col_r[i][t];
+              v += (which == 2 ? i <= t / 16 : i >= t / 16) ? w : 0.f;
+            }
           }
           if (lane < L) k.tok[(which * plane + bhp) * tp + t0 + t] = v;
           if (lane == 0 && which < 2) {
@@ -791,6 +796,7 @@ int launch_bwd(const Args& a, int dtype, const Grads& q, void* workspace, hipStr
   k.dy = q.dy, k.y_t = q.y_t, k.y_b = q.y_b, k.dstate = q.dstate;
   k.dx = q.dx, k.ddelta = q.ddelta, k.db = q.db, k.dc = q.dc, k.dA = q.dA, k.dD = q.dD, k.dbias = q.dbias;
   k.dstate_in = q.dstate_in;
+  k.has_d = a.D != nullptr, k.Dz = k.has_d ? a.D : a.A;
   char* w = static_cast<char*>(workspace);
   auto take = [&](int64_t bytes) {
     char* r = w;
