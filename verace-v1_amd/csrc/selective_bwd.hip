@@ -409,45 +409,43 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
 #pragma unroll
       for (int j = 0; j < NTW; ++j) {
         const int n = 16 * (nt0 + NW * j) + 4 * g;
-        f32x4 sy_[LTW], gx_[LTW];
 #pragma unroll
-        for (int t = 0; t < LTW; ++t) sy_[t] = gx_[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < KP; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < KP; ++kb) {
-          Frag<E> sp[NPART], gp[NPART];
-          {
-            const f32x4 v[2] = {s0[j][2 * kb], s0[j][2 * kb + 1]}, w[2] = {g1[j][2 * kb], g1[j][2 * kb + 1]};
-            split<E>(v, sp);
-            split<E>(w, gp);
+          for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
+            for (int r = 0; r < 4; ++r) kp = fmaf(s0[j][2 * kb + hf][r], g1[j][2 * kb + hf][r], kp);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) kp = fmaf(v[hf][r], w[hf][r], kp);
+        for (int which = 0; which < 2; ++which) {  // one after the other: the registers of one
+          f32x4 prod[LTW];
+#pragma unroll
+          for (int t = 0; t < LTW; ++t) prod[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kb = 0; kb < KP; ++kb) {
+            Frag<E> part[NPART], f[LTW];
+#pragma unroll
+            for (int t = 0; t < LTW; ++t)
+              f[t] = which ? x_frag(Xs, 16 * (tt0 + t), 32 * kb) : row_frag<E, PB>(Ys, 16 * (tt0 + t), 32 * kb, l16, g);
+            const f32x4 v[2] = {which ? g1[j][2 * kb] : s0[j][2 * kb], which ? g1[j][2 * kb + 1] : s0[j][2 * kb + 1]};
+            split<E>(v, part);
+#pragma unroll
+            for (int q = NPART - 1; q >= 0; --q)
+#pragma unroll
+              for (int t = 0; t < LTW; ++t) prod[t] = mma(part[q], f[t], prod[t]);
           }
 #pragma unroll
           for (int t = 0; t < LTW; ++t) {
-            const Frag<E> yf = row_frag<E, PB>(Ys, 16 * (tt0 + t), 32 * kb, l16, g);
-            const Frag<E> xf = x_frag(Xs, 16 * (tt0 + t), 32 * kb);
+            const int tok = 16 * (tt0 + t) + l16;
+            const E* row = (which ? Bs : Cs) + TB::at(tok) + n;
+            const float w = which ? ws[tok] : es[tok], d = which ? ds[tok] : 1.f;
+            f32x4& sum = which ? db[j][t] : dc[j][t];
+            float& dot = which ? be[t] : al[t];
 #pragma unroll
-            for (int q = NPART - 1; q >= 0; --q) {
-              sy_[t] = mma(sp[q], yf, sy_[t]);
-              gx_[t] = mma(gp[q], xf, gx_[t]);
+            for (int r = 0; r < 4; ++r) {
+              const float v = prod[t][r] * w;
+              dot = fmaf(static_cast<float>(row[r]), v, dot);
+              sum[r] = fmaf(d, v, sum[r]);
             }
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < LTW; ++t) {
-          const int tok = 16 * (tt0 + t) + l16;
-          const float e = es[tok], w = ws[tok], wd = w * ds[tok];
-          const E* cr = Cs + TB::at(tok) + n;
-          const E* br = Bs + TB::at(tok) + n;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            sy_[t][r] *= e;
-            al[t] = fmaf(static_cast<float>(cr[r]), sy_[t][r], al[t]);
-            be[t] = fmaf(static_cast<float>(br[r]) * w, gx_[t][r], be[t]);
-            dc[j][t][r] += sy_[t][r];
-            db[j][t][r] = fmaf(wd, gx_[t][r], db[j][t][r]);
           }
         }
       }
