@@ -151,3 +151,108 @@ def test_no_tokens_and_no_items(device):
     assert float(selective_scan(**d)[1].abs().sum()) == 0.0
     d, _ = inputs(device, 0, 5, 2, 16, 1, 16, torch.float32)
     assert selective_scan(**d)[0].shape == (0, 5, 2, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_non_finite_tokens_reach_no_earlier_one(device, dtype, bad):
+    """A NaN or an infinity in a token's x, delta, B or C leaves every earlier token's y as it is, and the
+    other heads' (x, delta) and channels' (x)."""
+    from verace_amd import selective_scan
+    d, state = inputs(device, 2, 100, 4, 32, 2, 64, dtype, seed=30)
+    y0, S0 = selective_scan(**d, initial_state=state)
+    ym, Sm = ref.selective_scan(**d, initial_state=state, magnitude=True)
+    # the chunk of such a token is summed in another order: both results are within check()'s bound of the exact
+    # one, and so within twice that of each other
+    bound = 2 * (torch.finfo(dtype).eps / 2 * y0.double().abs() +
+                 ((8 * 100 + 64 + 16) * U + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)) * ym)
+
+    def same(y, part):
+        return bool(((y.double() - y0.double()).abs() <= bound)[part].all())
+    for k in ("x", "delta", "B", "C"):
+        e = {n: None if v is None else v.clone() for n, v in d.items()}
+        at = {"x": (1, 45, 2, 7), "delta": (1, 45, 2), "B": (1, 45, 1, 7), "C": (1, 45, 1, 7)}[k]
+        e[k][at] = bad
+        y, S = selective_scan(**e, initial_state=state)
+        assert torch.equal(y[0], y0[0]) and torch.equal(S[0], S0[0]), k
+        assert same(y, (1, slice(0, 45))), k
+        assert not bool(torch.isfinite(y[1, 45, 2]).all()), k
+        assert torch.equal(y[1, :, :2], y0[1, :, :2]), k           # the first group's heads
+        if k in ("x", "delta"):
+            assert torch.equal(y[1, :, 3], y0[1, :, 3]), k         # the other head of the group
+        if k == "x":
+            keep = [p for p in range(32) if p != 7]
+            assert same(y, (1, slice(None), 2, keep)) and torch.equal(S[1, 2][keep], S0[1, 2][keep])
+        if k == "C":
+            assert torch.equal(y[1, 46:], y0[1, 46:]) and torch.equal(S, S0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strong_decays(device, dtype):
+    """Log decays of hundreds a token and of none at all: differences of a chunk's sums keep their accuracy."""
+    from verace_amd import selective_scan
+    d, state = inputs(device, 1, 150, 4, 32, 1, 32, dtype, seed=31, delta_dtype=torch.float32)
+    d["A"] = torch.tensor([-1e-6, -3.0, -200.0, -1e4], device=device)
+    check(selective_scan(**d, initial_state=state), d, state)
+
+
+def test_graph_replays(device):
+    """Scan, convolution, norm and both steps captured in one graph with states updated in place: each replay,
+    between eager work, gives the eager bits."""
+    from verace_amd import gated_norm_add, selective_scan, selective_step_, short_conv, short_conv_step_
+    g = torch.Generator(device).manual_seed(40)
+
+    def r(*s):
+        return torch.randn(*s, generator=g, device=device).to(torch.bfloat16)
+    B, H, P, N = 2, 4, 64, 128
+    x, w, b, cs = r(B, 300, H * P), r(H * P, 4), r(H * P), r(B, 3, H * P)
+    delta, Bm, Cm = r(B, 300, H), r(B, 300, 1, N), r(B, 300, 1, N)
+    A, nw = -torch.rand(H, generator=g, device=device), r(H * P)
+    S = torch.randn(B, H, P, N, generator=g, device=device)
+    tok = r(B, 1, H * P)
+
+    def run(cs, S):
+        y, last = short_conv(x, w, b)
+        o, fin = selective_scan(y.view(B, 300, H, P), delta, A, Bm, Cm)
+        s, n = gated_norm_add(o.reshape(B, 300, H * P), x, nw, y, nw, nw)
+        t = short_conv_step_(tok, w, b, cs)
+        z = selective_step_(t.view(B, 1, H, P), delta[:, :1], A, Bm[:, :1], Cm[:, :1], S)
+        return last, fin, s, n, t, z
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(cs.clone(), S.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    cs1, S1, cs2, S2 = cs.clone(), S.clone(), cs.clone(), S.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(cs1, S1)
+    cs1.copy_(cs), S1.copy_(S)
+    for i in range(4):
+        x.add_(0.125 * i)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, run(cs2, S2)):
+            assert torch.equal(p, q), i
+        assert torch.equal(cs1, cs2) and torch.equal(S1, S2)
+
+
+def test_other_streams_at_once(device):
+    """Two calls on two streams at the same time, each with its own workspace."""
+    from verace_amd import selective_scan
+    d1, s1 = inputs(device, 1, 700, 4, 64, 1, 128, torch.bfloat16, seed=50)
+    d2, s2 = inputs(device, 2, 500, 2, 64, 2, 64, torch.float32, seed=51)
+    want1, want2 = selective_scan(**d1, initial_state=s1), selective_scan(**d2, initial_state=s2)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got1, got2 = [], []
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            got1.append(selective_scan(**d1, initial_state=s1))
+        with torch.cuda.stream(b):
+            got2.append(selective_scan(**d2, initial_state=s2))
+    torch.cuda.synchronize()
+    for got, want in ((got1, want1), (got2, want2)):
+        for y, S in got:
+            assert torch.equal(y, want[0]) and torch.equal(S, want[1])

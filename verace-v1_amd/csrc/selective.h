@@ -46,7 +46,7 @@ __device__ __forceinline__ float step_slope(float z, int softplus) {
 int launch_seq(const Args& a, int dtype, hipStream_t stream);
 
 // selective_chunk.hip: in chunks on the matrix cores, given the workspace; from use_chunk() tokens on.
-bool use_chunk(int64_t T);
+bool use_chunk(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype);
 size_t chunk_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype);
 int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream);
 

@@ -1,6 +1,5 @@
 // C entry points of the selective state space scan (selective.h).
 #include <algorithm>
-
 #include <initializer_list>
 
 #include "selective_mfma.h"
@@ -53,7 +52,8 @@ extern "C" int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, c
   a.delta_dtype = delta_dtype, a.softplus = softplus;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.H = static_cast<int>(H), a.P = static_cast<int>(P);
   a.G = static_cast<int>(G), a.N = static_cast<int>(N);
-  if (!use_chunk(T) || !strides_fit({x_t, b_t, c_t}, H, P)) return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
+  if (!use_chunk(B, T, H, P, N, dtype) || !strides_fit({x_t, b_t, c_t}, H, P))
+    return launch_seq(a, dtype, static_cast<hipStream_t>(stream));
   if (workspace == nullptr || workspace_bytes < chunk_workspace_bytes(B, T, H, P, N, dtype)) return VMI_ERR_WORKSPACE;
   return launch_chunk(a, dtype, workspace, static_cast<hipStream_t>(stream));
 }

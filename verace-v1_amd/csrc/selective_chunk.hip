@@ -70,6 +70,18 @@ __global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d
 }
 
 // ------------------------------------------------------------------ the segments
+// acc[r] += sum_{s<=t} M[t,s] x[s, r] for a chunk with values that a product with a zero does not drop.
+template <typename E>
+__device__ __forceinline__ void add_in_order(const E* m, const E* x, int t, int l16, f32x4& acc) {
+#pragma unroll 1
+  for (int s = 0; s <= t; ++s) {
+    const float w = static_cast<float>(m[(l16 + 16 * ((s >> 2) & 3)) * 8 + 4 * (s >> 4) + (s & 3)]);
+    const E* row = x + Tile<E, PB>::at(s);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] = fmaf(w, static_cast<float>(row[r]), acc[r]);
+  }
+}
+
 template <typename IO, typename E, int NP, bool READOUT, bool VEC>
 __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass_kernel(Chunks k) {
   constexpr int NT = NP / 16, LT = L / 16, KN = NP / 32, NPART = Parts<E>::N;
@@ -230,18 +242,26 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
     } else {
       lds_barrier();  // the scores are in LDS
       if (live) {
+        // a NaN or an infinity among this wave's x (0 times it is NaN): token by token, so that no earlier one sees it
+        const f32x4 z0 = half(xf, 0) * 0.f, z1 = half(xf, 1) * 0.f;
+        const float z = ((z0[0] + z0[1]) + (z0[2] + z0[3])) + ((z1[0] + z1[1]) + (z1[2] + z1[3]));
+        const bool odd = __any(z != z);
 #pragma unroll
         for (int t = 0; t < LT; ++t) {
           acc[t] *= es[16 * t + l16];
-          const E* m = Ms + (t * 64 + lane) * 8;
-          Frag<E> f;
-          if constexpr (sizeof(E) == 2) {
-            f.v = *reinterpret_cast<const bf16x8*>(m);
+          if (odd) {
+            add_in_order<E>(Ms + t * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
           } else {
-            f.v[0] = *reinterpret_cast<const f32x4*>(m);
-            f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
+            const E* m = Ms + (t * 64 + lane) * 8;
+            Frag<E> f;
+            if constexpr (sizeof(E) == 2) {
+              f.v = *reinterpret_cast<const bf16x8*>(m);
+            } else {
+              f.v[0] = *reinterpret_cast<const f32x4*>(m);
+              f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
+            }
+            acc[t] = mma(xf, f, acc[t]);
           }
-          acc[t] = mma(xf, f, acc[t]);
           if (y_on && c * L + 16 * t + l16 < a.T) {
             const E* xr = Xs + TX::at(16 * t + l16) + 16 * wave + 4 * g;
             IO* yt = y + t * y16;
@@ -394,10 +414,15 @@ int launch_prep(const Args& a, int tokens, float* d, float2* c, int nch, hipStre
   return hip_status(hipGetLastError());
 }
 
-bool use_chunk(int64_t T) { return T >= 16; }
+// us of a call, token by token / in chunks (H32 P64 N128): bf16 B64 T4 41 / 42, T8 64 / 42; B8 T8 17.5 / 19.5,
+// T12 23 / 19.5; B1 T12 18 / 19.8, T15 22 / 19.8.  fp32 B64 T12 67 / 60; B1 T15 19 / 20.  Many tokens' states
+// make a token by token call wait on memory, so the chunks pay sooner.
+bool use_chunk(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
+  return T >= (dtype == VMI_BF16 && B * H * P * N >= (1 << 22) ? 5 : 12);
+}
 
 size_t chunk_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
-  return use_chunk(T) ? static_cast<size_t>(plan(B, T, H, P, N).bytes()) : 0;
+  return use_chunk(B, T, H, P, N, dtype) ? static_cast<size_t>(plan(B, T, H, P, N).bytes()) : 0;
 }
 
 int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) {
