@@ -106,3 +106,44 @@ def test_c_refusals(lib):
     assert lib.vmi_short_conv(one, 8, 8, one, null, 0, 0, 1, one, null, 0, one, one, 1, 1, 8, 4, null) == 4
     assert lib.vmi_gated_norm(one, 8, one, 8, null, 0, null, null, one, 0, 0, 1, 0.0, 0.0, one, null, null, 1, 8, null) == 1
     assert lib.vmi_gated_norm(one, 8, one, 8, null, 0, null, null, null, 1, 2, 1, 0.0, 0.0, one, null, null, 1, 8, null) == 2
+
+
+def test_traced_shapes():
+    """Fake HIP tensors go through the registered operators: shapes and dtypes, gradients, refusals; no kernel runs."""
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        bf = torch.bfloat16
+        x, delta, bm = _e(2, 40, 4, 16, dtype=bf), _e(2, 40, 4), _e(2, 40, 2, 8, dtype=bf)
+        y, state = va.selective_scan(x, delta, _e(4), bm, bm, _e(4), lengths=_e(2, dtype=torch.int32))
+        assert y.shape == x.shape and y.dtype == bf and state.shape == (2, 4, 16, 8) and state.dtype == torch.float32
+        c, last = va.short_conv(y.flatten(2), _e(64, 4, dtype=bf), _e(64, dtype=bf))
+        assert c.shape == (2, 40, 64) and last.shape == (2, 3, 64) and last.dtype == bf
+        s, n = va.gated_norm_add(c, c, _e(64), c, None, _e(64))
+        assert s.shape == n.shape == c.shape and n.dtype == bf
+        assert va.gated_norm_add(c, c, _e(64))[1] is None
+        grads = torch.ops.verace.selective_scan_bwd(x, delta, _e(4), bm, bm, y, None, None, True, None, None, None)
+        for g, t in zip(grads, (x, delta, _e(4), bm, bm, _e(4), _e(4), _e(0))):
+            assert g.shape == t.shape and g.dtype == t.dtype
+        with torch.no_grad():
+            assert va.selective_step_(x[:, 0], delta[:, 0], _e(4), bm[:, 0], bm[:, 0], state).shape == (2, 1, 4, 16)
+            assert va.short_conv_step_(c[:, 0], _e(64, 4), None, last).shape == (2, 1, 64)
+
+
+def test_gradient_operator_refusals():
+    ops = torch.ops.verace
+    x, y = torch.zeros(2, 5, 8), torch.zeros(3, 8)
+    for call in (lambda: ops.short_conv_bwd(x, torch.zeros(8, 4), None, None, None, "silu", x[:, :4], None),
+                 lambda: ops.gated_norm_bwd(y, y, None, None, None, None, torch.zeros(2, 2), "silu", y, None),
+                 lambda: ops.selective_scan_bwd(x.view(2, 5, 2, 4), x[..., :2], torch.zeros(2), x.view(2, 5, 2, 4),
+                                                x.view(2, 5, 2, 4), x, None, None, True, None, None, None)):
+        with pytest.raises(RuntimeError, match="verace_amd"):
+            call()
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        from verace_amd import block_norm, selective
+        z = _e(2, 5, 8)
+        with pytest.raises(RuntimeError, match="dy must be"):
+            selective._launch_conv_bwd(z, _e(8, 4), None, None, None, 1, _e(2, 4, 8), None, (True,) * 4)
+        with pytest.raises(RuntimeError, match="d_last must be"):
+            selective._launch_conv_bwd(z, _e(8, 4), None, None, None, 1, None, _e(2, 4, 8), (True,) * 4)
+        for stats, ds in ((_e(2, 2), _e(3, 8)), (_e(2, 3), _e(3, 4)), (_e(3, 2).t(), _e(3, 8))):
+            with pytest.raises(RuntimeError, match="must be"):
+                block_norm._launch_bwd(_e(3, 8), _e(3, 8), None, None, None, None, stats, 1, ds, None, (True,) * 6)

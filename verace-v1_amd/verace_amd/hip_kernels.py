@@ -56,6 +56,17 @@ def address(t: Optional[torch.Tensor]) -> Optional[int]:
 _NO_GUARD = contextlib.nullcontext()
 
 
+def traced(x: torch.Tensor) -> bool:
+    """Whether torch.compile or FakeTensor tracing runs the caller: the registered operators (ops.py) then take
+    the launchers' place."""
+    if torch.compiler.is_compiling():
+        return True
+    if type(x) is torch.Tensor:
+        return False
+    from torch._subclasses.fake_tensor import FakeTensor
+    return isinstance(x, FakeTensor)
+
+
 def device_guard(t: torch.Tensor):
     """A context in which kernels are launched on t's device (nothing where it is the current one)."""
     return _NO_GUARD if on_current_device(t) else torch.cuda.device(t.device)

@@ -17,18 +17,26 @@ Replaces, for tracing purposes, the reference's Triton launcher ``launch_sssd_tr
 * ``verace::cham_step_fused_(proj, h, h_real!, h_imag!, r_real!?, r_imag!?, mask?) -> out`` --
   :func:`cham_step_fused_` (mutates the states).
 * ``verace::ns_retraction(h_real, h_imag, steps) -> (real, imag)``.
+* ``verace::selective_scan(x, delta, A, B, C, D?, delta_bias?, softplus, state?, lengths?) -> (y, state_T)`` --
+  differentiable through ``verace::selective_scan_bwd``; ``verace::selective_step_(..., state!, ...) -> y``.
+* ``verace::short_conv(x, weight, bias?, state?, lengths?, activation?) -> (y, last rows)`` -- differentiable through
+  ``verace::short_conv_bwd``; ``verace::short_conv_step_(x, weight, bias?, state!, activation?, mask?) -> y``.
+* ``verace::gated_norm(y, residual, gate?, w1?, scale?, w2?, eps, next_eps, activation) -> (s, n, stats)`` -- differentiable
+  through ``verace::gated_norm_bwd`` (n empty without w2).
 
 The eager module path calls the launchers directly (no dispatcher overhead in a decode loop);
 :class:`~verace_amd.SSSDAttention` switches to these operators while ``torch.compile`` traces.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 
+from . import block_norm as bn
 from . import hip_kernels as hk
+from . import selective as sel
 
 
 @torch.library.custom_op("verace::sssd_scan", mutates_args=())
@@ -189,3 +197,173 @@ def ns_retraction(h_real: Tensor, h_imag: Tensor, steps: int) -> Tuple[Tensor, T
 def _ns_fake(h_real, h_imag, steps):
     return (h_real.new_empty(h_real.shape, dtype=torch.float32),
             h_real.new_empty(h_real.shape, dtype=torch.float32))
+
+
+# ------------------------------------------------------------------------------------ selective state space layer
+
+@torch.library.custom_op("verace::selective_scan", mutates_args=())
+def selective_scan(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                   delta_bias: Optional[Tensor], softplus: bool, state: Optional[Tensor],
+                   lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    return sel.launch_selective_hip_scan(x, delta, A, B, C, D, delta_bias, softplus, state, lengths)
+
+
+@selective_scan.register_fake
+def _selective_scan_fake(x, delta, A, B, C, D, delta_bias, softplus, state, lengths):
+    b, T, H, P = x.shape
+    return x.new_empty((b, T, H, P)), x.new_empty((b, H, P, B.shape[-1]), dtype=torch.float32)
+
+
+@torch.library.custom_op("verace::selective_scan_bwd", mutates_args=())
+def selective_scan_bwd(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, dy: Tensor, D: Optional[Tensor],
+                       delta_bias: Optional[Tensor], softplus: bool, state: Optional[Tensor],
+                       lengths: Optional[Tensor], d_state: Optional[Tensor]) -> List[Tensor]:
+    *grads, d0 = sel.launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D, delta_bias, softplus, state, lengths,
+                                                   d_state, state is not None)
+    # separate storages: the three head vectors are rows of one tensor
+    out = [g.clone() if i in (2, 5, 6) else g for i, g in enumerate(grads)]
+    return out + [x.new_empty((0,), dtype=torch.float32) if d0 is None else d0]
+
+
+@selective_scan_bwd.register_fake
+def _selective_scan_bwd_fake(x, delta, A, B, C, dy, D, delta_bias, softplus, state, lengths, d_state):
+    H = x.shape[2]
+    heads = [x.new_empty((H,), dtype=torch.float32) for _ in range(3)]
+    d0 = x.new_empty((0,) if state is None else state.shape, dtype=torch.float32)
+    return [x.new_empty(x.shape), delta.new_empty(delta.shape), heads[0], B.new_empty(B.shape), C.new_empty(C.shape),
+            heads[1], heads[2], d0]
+
+
+def _selective_setup(ctx, inputs, output):
+    x, delta, A, B, C, D, delta_bias, softplus, state, lengths = inputs
+    ctx.save_for_backward(x, delta, A, B, C, D, delta_bias, state, lengths)
+    ctx.softplus = softplus
+
+
+def _selective_backward(ctx, dy, d_state):
+    x, delta, A, B, C, D, delta_bias, state, lengths = ctx.saved_tensors
+    dy = torch.zeros_like(x) if dy is None else dy
+    dx, dd, dA, dB, dC, dD, dbias, d0 = torch.ops.verace.selective_scan_bwd(
+        x, delta, A, B, C, dy, D, delta_bias, ctx.softplus, state, lengths, d_state)
+    return (dx, dd, dA.to(A.dtype), dB, dC, None if D is None else dD.to(D.dtype),
+            None if delta_bias is None else dbias.to(delta_bias.dtype), None,
+            None if state is None else d0.to(state.dtype), None)
+
+
+selective_scan.register_autograd(_selective_backward, setup_context=_selective_setup)
+
+
+@torch.library.custom_op("verace::selective_step_", mutates_args=("state",))
+def selective_step_(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tensor, D: Optional[Tensor],
+                    delta_bias: Optional[Tensor], softplus: bool, active_mask: Optional[Tensor]) -> Tensor:
+    return sel.selective_step_(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+
+
+@selective_step_.register_fake
+def _selective_step_fake(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask):
+    b, H, P, _ = state.shape
+    return x.new_empty((b, 1, H, P))
+
+
+@torch.library.custom_op("verace::short_conv", mutates_args=())
+def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Optional[Tensor], lengths: Optional[Tensor],
+               activation: Optional[str]) -> Tuple[Tensor, Tensor]:
+    return sel.short_conv(x, weight, bias, state, lengths, activation)
+
+
+@short_conv.register_fake
+def _short_conv_fake(x, weight, bias, state, lengths, activation):
+    B, _, C = x.shape
+    return x.new_empty(x.shape), x.new_empty((B, weight.shape[1] - 1, C))
+
+
+def _or_empty(like: Tensor, grads) -> List[Tensor]:
+    return [like.new_empty((0,)) if g is None else g for g in grads]
+
+
+def _new_like(like: Tensor, tensors) -> List[Tensor]:
+    return _or_empty(like, [None if t is None else t.new_empty(t.shape) for t in tensors])
+
+
+@torch.library.custom_op("verace::short_conv_bwd", mutates_args=())
+def short_conv_bwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Optional[Tensor],
+                   lengths: Optional[Tensor], activation: Optional[str], dy: Optional[Tensor],
+                   d_last: Optional[Tensor]) -> List[Tensor]:
+    lengths, state = sel._conv_args(x, weight, bias, state, lengths, activation)
+    return _or_empty(x, sel._launch_conv_bwd(x, weight, bias, state, lengths, sel._ACT[activation], dy, d_last, (True,) * 4))
+
+
+@short_conv_bwd.register_fake
+def _short_conv_bwd_fake(x, weight, bias, state, lengths, activation, dy, d_last):
+    return _new_like(x, (x, weight, bias, state))
+
+
+def _conv_setup(ctx, inputs, output):
+    x, weight, bias, state, lengths, ctx.activation = inputs
+    ctx.save_for_backward(x, weight, bias, state, lengths)
+
+
+def _conv_backward(ctx, dy, d_last):
+    x, weight, bias, state, lengths = ctx.saved_tensors
+    dx, dw, db, ds = torch.ops.verace.short_conv_bwd(x, weight, bias, state, lengths, ctx.activation, dy, d_last)
+    return dx, dw, None if bias is None else db, None if state is None else ds, None, None
+
+
+short_conv.register_autograd(_conv_backward, setup_context=_conv_setup)
+
+
+@torch.library.custom_op("verace::short_conv_step_", mutates_args=("state",))
+def short_conv_step_(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Tensor, activation: Optional[str],
+                     active_mask: Optional[Tensor]) -> Tensor:
+    return sel.short_conv_step_(x, weight, bias, state, activation, active_mask)
+
+
+@short_conv_step_.register_fake
+def _short_conv_step_fake(x, weight, bias, state, activation, active_mask):
+    return x.new_empty((state.shape[0], 1, state.shape[2]))
+
+
+@torch.library.custom_op("verace::gated_norm", mutates_args=())
+def gated_norm(y: Tensor, residual: Tensor, gate: Optional[Tensor], w1: Optional[Tensor], scale: Optional[Tensor],
+               w2: Optional[Tensor], eps: float, next_eps: float, activation: str) -> Tuple[Tensor, Tensor, Tensor]:
+    args = bn._checked(y, residual, gate, w1, scale, w2, activation)
+    s, n, stats = bn._launch(*args, eps, next_eps, bn._ACT[activation], True)
+    for row, w in zip(stats, (w1, w2)):  # not written without that norm
+        if w is None:
+            row.zero_()
+    return s, y.new_empty((0,)) if n is None else n, stats
+
+
+@gated_norm.register_fake
+def _gated_norm_fake(y, residual, gate, w1, scale, w2, eps, next_eps, activation):
+    rows = y.numel() // y.shape[-1]
+    return (y.new_empty(y.shape), y.new_empty((0,) if w2 is None else y.shape),
+            y.new_empty((2, rows), dtype=torch.float32))
+
+
+@torch.library.custom_op("verace::gated_norm_bwd", mutates_args=())
+def gated_norm_bwd(y: Tensor, residual: Tensor, gate: Optional[Tensor], w1: Optional[Tensor], scale: Optional[Tensor],
+                   w2: Optional[Tensor], stats: Tensor, activation: str, ds: Optional[Tensor],
+                   dn: Optional[Tensor]) -> List[Tensor]:
+    args = bn._checked(y, residual, gate, w1, scale, w2, activation)
+    return _or_empty(y, bn._launch_bwd(*args, stats, bn._ACT[activation], ds, dn, (True,) * 6))
+
+
+@gated_norm_bwd.register_fake
+def _gated_norm_bwd_fake(y, residual, gate, w1, scale, w2, stats, activation, ds, dn):
+    return _new_like(y, (y, residual, gate, w1, scale, w2))
+
+
+def _norm_setup(ctx, inputs, output):
+    y, residual, gate, w1, scale, w2, _, _, ctx.activation = inputs
+    ctx.save_for_backward(y, residual, gate, w1, scale, w2, output[2])
+
+
+def _norm_backward(ctx, ds, dn, _):
+    y, residual, gate, w1, scale, w2, stats = ctx.saved_tensors
+    given = (y, residual, gate, w1, scale, w2)
+    grads = torch.ops.verace.gated_norm_bwd(*given, stats, ctx.activation, ds, None if w2 is None else dn)
+    return (*(None if t is None else g for t, g in zip(given, grads)), None, None, None)
+
+
+gated_norm.register_autograd(_norm_backward, setup_context=_norm_setup)

@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hip_kernels import _mask_bytes, _require_device, address, device_guard
+from .hip_kernels import _mask_bytes, _require_device, address, device_guard, traced
 
 _ACT = {None: 0, "silu": 1}
 
@@ -27,6 +27,13 @@ def _same_device(like: torch.Tensor, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise RuntimeError(f"verace_amd: {name} must be on {device}, got {t.device}")
+
+
+def _grad_check(like: torch.Tensor, shape, **grads) -> None:
+    for name, t in grads.items():
+        if t is not None and (t.shape != shape or t.dtype != like.dtype or t.device != like.device):
+            raise RuntimeError(f"verace_amd: {name} must be {tuple(shape)} {like.dtype} on {like.device}, "
+                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def _lengths(lengths: Optional[torch.Tensor], B: int, like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -66,6 +73,22 @@ def _conv_check(x, weight, bias, activation):
     _same_device(x, weight=weight, bias=bias)
 
 
+def _conv_args(x, weight, bias, state, lengths, activation):
+    """The lengths and the initial state of a call as the launchers take them."""
+    if x.dim() != 3:
+        raise RuntimeError(f"verace_amd: x must be [B, T, C], got {tuple(x.shape)}")
+    _conv_check(x, weight, bias, activation)
+    B, T, C = x.shape
+    lengths = _lengths(lengths, B, x)
+    if state is not None:
+        if tuple(state.shape) != (B, weight.shape[1] - 1, C) or state.dtype != x.dtype:
+            raise RuntimeError(f"verace_amd: initial_state must be {(B, weight.shape[1] - 1, C)} {x.dtype}, "
+                               f"got {tuple(state.shape)} {state.dtype}")
+        _same_device(x, initial_state=state)
+        state = state.contiguous()
+    return lengths, state
+
+
 def _launch_conv(x, weight, bias, state, lengths, act):
     B, T, C = x.shape
     K = weight.shape[1]
@@ -79,6 +102,36 @@ def _launch_conv(x, weight, bias, state, lengths, act):
             address(state), address(lengths), int(lengths is not None and lengths.dtype == torch.int64), address(y), address(out),
             B, T, C, K, _lib.raw_stream(x.device)), "vmi_short_conv")
     return y, out
+
+
+def _launch_conv_bwd(x, weight, bias, state, lengths, act, dy, dout, need):
+    """(dx, dweight, dbias, dstate) for dL/dy and dL/dlast rows (either may be None), None where not needed."""
+    B, T, C = x.shape
+    K = weight.shape[1]
+    _grad_check(x, x.shape, dy=dy)
+    _grad_check(x, (B, K - 1, C), d_last=dout)
+    x, w = _inner(x, 2), weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    dy = None if dy is None else _inner(dy, 2)
+    dout = None if dout is None else dout.contiguous()
+    dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype) if need[0] else None
+    dw = torch.empty_like(w) if need[1] else None
+    db = torch.empty_like(b) if b is not None and need[2] else None
+    dstate = torch.empty_like(state) if state is not None and need[3] else None
+    lib = _lib.load()
+    ws, ws_bytes = None, ctypes.c_size_t(0)
+    if not (dw is None and db is None):
+        _lib.check(lib.vmi_short_conv_bwd_workspace_bytes(B, T, C, K, ctypes.byref(ws_bytes)),
+                   "vmi_short_conv_bwd_workspace_bytes")
+        ws = torch.empty(max(1, ws_bytes.value), device=x.device, dtype=torch.uint8)
+    with device_guard(x):
+        _lib.check(lib.vmi_short_conv_bwd(
+            address(x), x.stride(1), x.stride(0), address(w), address(b), _lib.dtype_code(x.dtype),
+            _lib.dtype_code(w.dtype), act, address(state), address(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), address(dy), 0 if dy is None else dy.stride(1),
+            0 if dy is None else dy.stride(0), address(dout), address(dx), address(dw), address(db), address(dstate),
+            B, T, C, K, address(ws), ws_bytes.value, _lib.raw_stream(x.device)), "vmi_short_conv_bwd")
+    return dx, dw, db, dstate
 
 
 class ShortConvFunction(torch.autograd.Function):
@@ -96,31 +149,7 @@ class ShortConvFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dout):
         x, weight, bias, state, lengths = ctx.saved_tensors
-        B, T, C = x.shape
-        K = weight.shape[1]
-        x, w = _inner(x, 2), weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        dy = None if dy is None else _inner(dy, 2)
-        dout = None if dout is None else dout.contiguous()
-        need = ctx.needs_input_grad
-        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype) if need[0] else None
-        dw = torch.empty_like(w) if need[1] else None
-        db = torch.empty_like(b) if b is not None and need[2] else None
-        dstate = torch.empty_like(state) if state is not None and need[3] else None
-        lib = _lib.load()
-        ws, ws_bytes = None, ctypes.c_size_t(0)
-        if not (dw is None and db is None):
-            _lib.check(lib.vmi_short_conv_bwd_workspace_bytes(B, T, C, K, ctypes.byref(ws_bytes)),
-                       "vmi_short_conv_bwd_workspace_bytes")
-            ws = torch.empty(max(1, ws_bytes.value), device=x.device, dtype=torch.uint8)
-        with device_guard(x):
-            _lib.check(lib.vmi_short_conv_bwd(
-                address(x), x.stride(1), x.stride(0), address(w), address(b), _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype),
-                ctx.act, address(state), address(lengths), int(lengths is not None and lengths.dtype == torch.int64), address(dy),
-                0 if dy is None else dy.stride(1), 0 if dy is None else dy.stride(0), address(dout), address(dx), address(dw),
-                address(db), address(dstate), B, T, C, K, address(ws), ws_bytes.value, _lib.raw_stream(x.device)),
-                "vmi_short_conv_bwd")
-        return dx, dw, db, dstate, None, None
+        return (*_launch_conv_bwd(x, weight, bias, state, lengths, ctx.act, dy, dout, ctx.needs_input_grad[:4]), None, None)
 
 
 def short_conv(
@@ -140,18 +169,9 @@ def short_conv(
     "silu" or None.  Returns (y [batch, seq_len, C], the last K - 1 counted rows [batch, K - 1, C]); y
     behind a sequence's length is 0 and x there is not read.
     """
-    if x.dim() != 3:
-        raise RuntimeError(f"verace_amd: x must be [B, T, C], got {tuple(x.shape)}")
-    _conv_check(x, weight, bias, activation)
-    B, T, C = x.shape
-    lengths = _lengths(lengths, B, x)
-    state = initial_state
-    if state is not None:
-        if tuple(state.shape) != (B, weight.shape[1] - 1, C) or state.dtype != x.dtype:
-            raise RuntimeError(f"verace_amd: initial_state must be {(B, weight.shape[1] - 1, C)} {x.dtype}, "
-                               f"got {tuple(state.shape)} {state.dtype}")
-        _same_device(x, initial_state=state)
-        state = state.contiguous()
+    lengths, state = _conv_args(x, weight, bias, initial_state, lengths, activation)
+    if traced(x):
+        return torch.ops.verace.short_conv(x, weight, bias, state, lengths, activation)
     act = _ACT[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
         return ShortConvFunction.apply(x, weight, bias, state, lengths, act)
@@ -177,6 +197,8 @@ def short_conv_step_(
     if tuple(x.shape) not in ((B, 1, C), (B, C)):
         raise RuntimeError(f"verace_amd: x must hold one token for each of {B} items, got {tuple(x.shape)}")
     _same_device(x, state=state, active_mask=active_mask)
+    if traced(x):
+        return torch.ops.verace.short_conv_step_(x, weight, bias, state, activation, active_mask)
     x2 = _inner(x.reshape(B, C), 1)
     mask = None if active_mask is None else _mask_bytes(active_mask.reshape(B))
     w = weight.contiguous()
@@ -225,6 +247,15 @@ def _scan_check(x, delta, A, Bm, Cm, D, delta_bias):
     return B, T, H, P, G, N
 
 
+def _state_check(x: torch.Tensor, state: Optional[torch.Tensor], N: int, name: str = "initial_state") -> None:
+    if state is not None:
+        want = (x.shape[0], x.shape[2], x.shape[3], N)
+        if tuple(state.shape) != want:
+            raise RuntimeError(f"verace_amd: {name} must be {want}, got {tuple(state.shape)}")
+        if state.device != x.device:
+            raise RuntimeError(f"verace_amd: {name} must be on {x.device}, got {state.device}")
+
+
 def launch_selective_hip_scan(
     x: torch.Tensor,
     delta: torch.Tensor,
@@ -243,12 +274,8 @@ def launch_selective_hip_scan(
     if delta.dim() == 4:
         delta = delta.squeeze(-1)
     A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
-    state = initial_state
-    if state is not None:
-        if tuple(state.shape) != (b, H, P, N):
-            raise RuntimeError(f"verace_amd: initial_state must be {(b, H, P, N)}, got {tuple(state.shape)}")
-        _same_device(x, initial_state=state)
-        state = state.to(torch.float32).contiguous()
+    _state_check(x, initial_state, N)
+    state = None if initial_state is None else initial_state.to(torch.float32).contiguous()
     x, delta, B, C = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2)
     y = torch.empty(b, T, H, P, device=x.device, dtype=x.dtype)
     out = torch.empty(b, H, P, N, device=x.device, dtype=torch.float32)
@@ -274,16 +301,13 @@ def launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D=None, delta_bias=None
     d_state = dL/dfinal_state (None: zero): (dx, ddelta, dA, dB, dC, dD, ddelta_bias, dinitial_state), dx, dB and
     dC in x's dtype, ddelta in delta's, the others float32; dinitial_state None unless need_d_state."""
     b, T, H, P, G, N = _scan_check(x, delta, A, B, C, D, delta_bias)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise RuntimeError(f"verace_amd: dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    _same_device(x, dy=dy, d_state=d_state, initial_state=initial_state)
+    _grad_check(x, x.shape, dy=dy)
     lengths = _lengths(lengths, b, x)
     shape = delta.shape
     if delta.dim() == 4:
         delta = delta.squeeze(-1)
-    for name, t in (("initial_state", initial_state), ("d_state", d_state)):
-        if t is not None and tuple(t.shape) != (b, H, P, N):
-            raise RuntimeError(f"verace_amd: {name} must be {(b, H, P, N)}, got {tuple(t.shape)}")
+    _state_check(x, initial_state, N)
+    _state_check(x, d_state, N, "d_state")
     state, d_state = (None if t is None else t.to(torch.float32).contiguous() for t in (initial_state, d_state))
     A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
     x, delta, B, C, dy = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2), _inner(dy, 2)
@@ -364,6 +388,13 @@ def selective_scan(
     and C may be slices of wider rows.  head_dim <= 1024, N <= 256.  Returns (y in x's dtype, final_state
     float32); y behind a sequence's length is 0 and nothing of the inputs there is used.
     """
+    if traced(x):
+        _scan_check(x, delta, A, B, C, D, delta_bias)
+        _state_check(x, initial_state, B.shape[-1])
+        for name, t in (("A", A), ("D", D), ("delta_bias", delta_bias)):
+            _head_vector(t, x.shape[2], name)
+        return torch.ops.verace.selective_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state,
+                                               _lengths(lengths, x.shape[0], x))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, delta, A, B, C, D, delta_bias, initial_state)):
         return SelectiveScanFunction.apply(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
@@ -398,6 +429,8 @@ def selective_step_(
                            f"got {tuple(state.shape)} {state.dtype}")
     _same_device(x, state=state, active_mask=active_mask)
     A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
+    if traced(x):
+        return torch.ops.verace.selective_step_(x, delta, A, B, C, state, D, bias, softplus, active_mask)
     x, delta, B, C = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2)
     mask = None if active_mask is None else _mask_bytes(active_mask.reshape(b))
     y = torch.empty(b, 1, H, P, device=x.device, dtype=x.dtype)
