@@ -10,12 +10,15 @@
 //   G_0  = e^{c_L} G_L + sum_t e^{c_t} dy_t C_t^T
 // The gradient of token t's log decay collects every path that crosses it, from s < t (or S_0) to u >= t (or
 // G_L); with alpha_u = e^{c_u} dy_u . S_0 C_u, beta_s = e^{c_L - c_s} x_s . G_L B_s, kappa = e^{c_L} <G_L, S_0>:
-//   g_t = kappa + sum_{u>=t} (alpha_u + sum_s R[u,s] d_s - d_u sum_v R[v,u]) + sum_{s<t} d_s beta_s
+//   g_t = kappa + sum_{u>=t} alpha_u + sum_{s<t} d_s beta_s + sum_{u>=t, s<t} R[u,s] d_s
 //   dd_t = sum_u R[u,t] + beta_t + A g_t,   dA = sum d_t g_t,   ddelta = dd softplus'(.)
-// Each chunk starts from its own kappa, so nothing is accumulated over the sequence but G itself.
+// Each chunk starts from its own kappa, so nothing is accumulated over the sequence but G itself.  The double sum is
+// formed as it stands, tile by tile (16 x 16): as running differences of R's row and column sums it would carry every
+// rounding back over the chunk (B4 T2048 H32 P64 N128, decays up to e^-1.6 a token: dbias off by 2.2e-6 of its norm
+// that way, 1.3e-7 this way; 293 and 298 us for forward and backward).
 //
 // Launches:
-//   prep (selective_chunk.hip), states_kernel<OWN> and carry (Sg > 1 segments), states_kernel: the S_0 and G_L of
+//   prep (selective_chunk.hip), states_kernel<OWN> and starts_kernel (more than one segment), states_kernel: the S_0 and G_L of
 //     every chunk, both directions in one grid, in the order in which the main kernel's fragments read them;
 //   main_kernel: a workgroup of eight waves per chunk and block of heads of a group walks the heads with dB and
 //     dC of the chunk in accumulators (they are sums over the heads: as partials of each head they would be the
@@ -51,7 +54,7 @@ struct Bwd {
   float *s0, *g1;            // [BH pblocks][nch][NP 64], tiles of 16 x 16 in fragment order
   float *pb, *pc;            // [hblocks][B T][G][N] (null: dB, dC written directly)
   float* ph;                 // [3][B nch][H]: dA, dD, dbias
-  float* tok;                // [4][BH pblocks][Tp]: sums of alpha, beta, rows and columns of R
+  float* tok;                // [4][BH pblocks][Tp]: alpha, beta, g's sum of R d, sum_u R[u, t]
   float* chk;                // [2][BH pblocks][nch]: kappa, sum of x . dy
   void *dx, *ddelta, *db, *dc;
   float *dA, *dD, *dbias, *dstate_in;
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   __shared__ __attribute__((aligned(16))) E Qs[TQ::elems(L)];   // [t][s]
   __shared__ __attribute__((aligned(16))) E Ms[TQ::elems(L)];
   __shared__ __attribute__((aligned(16))) E Gs[TX::elems(GR)];  // G_L^T [n][p]
-  __shared__ float row_r[LT][L], col_r[LT][L];                  // sum_s R d_s by s-tile, sum_t R by t-tile
+  __shared__ float row_r[LT][L], col_r[LT][L];                  // sums of R d_s (below) by s-tile, sum_t R by t-tile
   __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
   const Args& a = k.a;
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -378,7 +381,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const f32x4 c01 = *reinterpret_cast<const f32x4*>(cs + s0_), c23 = *reinterpret_cast<const f32x4*>(cs + s0_ + 2);
         const f32x4 dv = *reinterpret_cast<const f32x4*>(ds + s0_);
         struct alignas(4 * sizeof(E)) M4 { E e[4]; } q, m;
-        float rs = 0.f, dg = 0.f, rr[4];
+        float dg = 0.f, rr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const bool on = s0_ + r <= t;
@@ -388,16 +391,22 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           q.e[r] = static_cast<E>(on ? xq : 0.f);
           m.e[r] = static_cast<E>(on ? cm_ : 0.f);
           rr[r] = on ? xc : 0.f;
-          rs = fmaf(rr[r], dv[r], rs);
           dg = s0_ + r == t ? xy[r] : dg;
         }
         const int o = TQ::at(t) + 16 * st + 4 * g;
         *reinterpret_cast<M4*>(Qs + o) = q;
         *reinterpret_cast<M4*>(Ms + o) = m;
+        // left of the diagonal the rows' sums, in a tile on it each token's sum over the paths that cross it
+        float rs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float from_t = row16_suffix(rr[r]);  // sum over the tokens from t on
+          const float v = tt != st ? rr[r] : s0_ + r < t ? from_t : 0.f;
+          rs = fmaf(v, dv[r], rs);
+          rr[r] = from_t;
+        }
         rs = half_pair_sum(row_pair_sum(rs));
         if (g == 0) row_r[st][t] = rs;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) rr[r] = row16_sum(rr[r]);
         if (l16 == 0) *reinterpret_cast<float4*>(&col_r[tt][16 * st + 4 * g]) = make_float4(rr[0], rr[1], rr[2], rr[3]);
         if (tt == st) {
           dg = half_pair_sum(row_pair_sum(row16_sum(dg)));
@@ -536,14 +545,32 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         if (which >= 0) {
           constexpr int NS = NT < NW ? NT : NW;
           float v = 0.f;
-          if (which < 2) {
+          if (which == 2) {
+            const int tile = t / 16;
+            float row = 0.f, col = 0.f;
+#pragma unroll
+            for (int i = 0; i < LT; ++i) {
+              row += i < tile ? row_r[i][t] : 0.f;
+              col += i > tile ? col_r[i][t] : 0.f;
+            }
+            col *= ds[t];
+            v = row_r[tile][t] + row16_suffix(row) + row16_before(col);
+#pragma unroll
+            for (int m = 1; m < LT - 1; ++m) {  // the tiles wholly across tile m
+              float over = 0.f;
+#pragma unroll
+              for (int i = 0; i < m; ++i) over += tile > m ? row_r[i][t] : 0.f;
+              over = half_pair_sum(row_pair_sum(row16_sum(over)));
+              v += tile == m ? over : 0.f;
+            }
+          } else if (which < 2) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) v += which == 0 ? alpha[i][t] : beta[i][t];
           } else {
 #pragma unroll
             for (int i = 0; i < LT; ++i) {  // (slots of tiles right of the diagonal hold nothing)
-              const float w = which == 2 ? row_r[i][t] : col_r[i][t];
-              v += (which == 2 ? i <= t / 16 : i >= t / 16) ? w : 0.f;
+              const float w = col_r[i][t];
+              v += i >= t / 16 ? w : 0.f;
             }
           }
           if (lane < L) k.tok[(which * plane + bhp) * tp + t0 + t] = v;
@@ -595,8 +622,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   }
 }
 
-// The gradients of a chunk's step sizes, a lane a token: the sums over the tokens before and after are differences
-// of the main kernel's, and run in fp64.
+// The gradients of a chunk's step sizes, a lane a token.
 template <int L>
 __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
   const Args& a = k.a;
@@ -612,7 +638,7 @@ __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
   const bool in = lane < L && t < len;
   double dz = 0.0, ga = 0.0, dgs = 0.0;
   if (c * L < len) {
-    double al = 0.0, be = 0.0, rs = 0.0, cr = 0.0, kap = 0.0, d = 0.0;
+    double al = 0.0, be = 0.0, in_g = 0.0, cr = 0.0, kap = 0.0, d = 0.0;
     for (int p = 0; p < k.pblocks; ++p) {
       const int64_t row = bh * k.pblocks + p;
       kap += k.chk[row * k.nch + c];
@@ -620,11 +646,11 @@ __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
       if (!in) continue;
       al += k.tok[row * tp + t];
       be += k.tok[(plane + row) * tp + t];
-      rs += k.tok[(2 * plane + row) * tp + t];
+      in_g += k.tok[(2 * plane + row) * tp + t];
       cr += k.tok[(3 * plane + row) * tp + t];
     }
     if (in) d = k.d[bh * tp + t];
-    double suf = al + rs - d * cr, pre = d * be;
+    double suf = al, pre = d * be;
     const double own = pre;
 #pragma unroll
     for (int off = 1; off < L; off <<= 1) {
@@ -632,7 +658,7 @@ __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
       if (lane + off < L) suf += v;
       if (lane >= off) pre += w;
     }
-    const double gt = kap + suf + (pre - own);
+    const double gt = kap + in_g + suf + (pre - own);
     // sigmoid(z) = 1 - e^{-softplus(z)}
     const double slope = a.softplus ? static_cast<double>(-expm1f(-static_cast<float>(d))) : 1.0;
     if (in) {

@@ -16,6 +16,22 @@ __device__ __forceinline__ float row16_sum(float x) {
   x += dpp_f32<0x140>(x);  // row_mirror
   return x;
 }
+// Over the 16 lanes of a DPP row: a lane's sum of itself and the lanes after it, and of the lanes before it.
+__device__ __forceinline__ float row16_suffix(float x) {
+  x += dpp_f32<0x101>(x);  // row_shl:1, zeros from behind the row
+  x += dpp_f32<0x102>(x);
+  x += dpp_f32<0x104>(x);
+  x += dpp_f32<0x108>(x);
+  return x;
+}
+__device__ __forceinline__ float row16_before(float x) {
+  x = dpp_f32<0x111>(x);   // row_shr:1
+  x += dpp_f32<0x111>(x);
+  x += dpp_f32<0x112>(x);
+  x += dpp_f32<0x114>(x);
+  x += dpp_f32<0x118>(x);
+  return x;
+}
 // Sum of the two 16-lane rows of each 32-lane half: v_permlane16_swap exchanges rows 1
 // and 0 (3 and 2) between its two operands, so the two results add to row0 + row1.
 __device__ __forceinline__ float row_pair_sum(float x) {
