@@ -180,7 +180,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
       ws[tid] = rd * decay(rl, rc);
     }
     lds_barrier();
-    if (c + 1 < c1) fetch(c + 1);
+    fetch(c + 1 < c1 ? c + 1 : c);
 
     f32x4 acc[LT];
     if constexpr (READOUT) {
@@ -242,26 +242,23 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
     } else {
       lds_barrier();  // the scores are in LDS
       if (live) {
-        // a NaN or an infinity among this wave's x (0 times it is NaN): token by token, so that no earlier one sees it
-        const f32x4 z0 = half(xf, 0) * 0.f, z1 = half(xf, 1) * 0.f;
-        const float z = ((z0[0] + z0[1]) + (z0[2] + z0[3])) + ((z1[0] + z1[1]) + (z1[2] + z1[3]));
-        const bool odd = __any(z != z);
 #pragma unroll
         for (int t = 0; t < LT; ++t) {
           acc[t] *= es[16 * t + l16];
-          if (odd) {
-            add_in_order<E>(Ms + t * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
+          const E* m = Ms + (t * 64 + lane) * 8;
+          Frag<E> f;
+          if constexpr (sizeof(E) == 2) {
+            f.v = *reinterpret_cast<const bf16x8*>(m);
           } else {
-            const E* m = Ms + (t * 64 + lane) * 8;
-            Frag<E> f;
-            if constexpr (sizeof(E) == 2) {
-              f.v = *reinterpret_cast<const bf16x8*>(m);
-            } else {
-              f.v[0] = *reinterpret_cast<const f32x4*>(m);
-              f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
-            }
-            acc[t] = mma(xf, f, acc[t]);
+            f.v[0] = *reinterpret_cast<const f32x4*>(m);
+            f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
           }
+          const f32x4 sum = mma(xf, f, acc[t]);
+          // a NaN or an infinity in x times a masked score's 0: in order, so that no earlier token sees it
+          if (__builtin_isunordered(sum[0], sum[1]) || __builtin_isunordered(sum[2], sum[3]))
+            add_in_order<E>(Ms + t * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
+          else
+            acc[t] = sum;
           if (y_on && c * L + 16 * t + l16 < a.T) {
             const E* xr = Xs + TX::at(16 * t + l16) + 16 * wave + 4 * g;
             IO* yt = y + t * y16;
