@@ -643,13 +643,15 @@ __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
       const int64_t row = bh * k.pblocks + p;
       kap += k.chk[row * k.nch + c];
       dgs += k.chk[(plane + row) * k.nch + c];
-      if (!in) continue;
-      al += k.tok[row * tp + t];
-      be += k.tok[(plane + row) * tp + t];
-      in_g += k.tok[(2 * plane + row) * tp + t];
-      cr += k.tok[(3 * plane + row) * tp + t];
+      const float* tok = k.tok + row * tp + c * L + lane % L;
+      const float v[4] = {tok[0], tok[plane * tp], tok[2 * plane * tp], tok[3 * plane * tp]};
+      al += in ? v[0] : 0.f;
+      be += in ? v[1] : 0.f;
+      in_g += in ? v[2] : 0.f;
+      cr += in ? v[3] : 0.f;
     }
-    if (in) d = k.d[bh * tp + t];
+    const float dt = k.d[bh * tp + c * L + lane % L];
+    d = in ? dt : 0.f;
     double suf = al, pre = d * be;
     const double own = pre;
 #pragma unroll
@@ -682,24 +684,26 @@ __global__ __launch_bounds__(SNT) void steps_kernel(Bwd k, int64_t units) {
   k.ph[2 * rows * a.H + o] = static_cast<float>(dz);
 }
 
-// Blocks below `heads`: 64 of the 3 H head sums by four strided shares of the chunks.  The others: dB and dC
+// Blocks below `heads`: 16 of the 3 H head sums by 16 strided shares of the chunks.  The others: dB and dC
 // from the head blocks' partials.
 template <typename IO>
 __global__ __launch_bounds__(SNT) void reduce_kernel(Bwd k, int heads, int64_t elems) {
   const Args& a = k.a;
   if (static_cast<int>(blockIdx.x) < heads) {
-    __shared__ double part[4][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6, l = threadIdx.x & 63;
+    constexpr int COLS = 16, SHARES = SNT / COLS;
+    __shared__ double part[SHARES][COLS];
+    const int l = threadIdx.x % COLS, share = threadIdx.x / COLS, col = blockIdx.x * COLS + l;
     const int64_t rows = static_cast<int64_t>(a.B) * k.nch;
     double s = 0.0;
     const int which = col / a.H, h = col - which * a.H;
     if (which < 3)
-      for (int64_t r = share; r < rows; r += 4) s += k.ph[(which * rows + r) * a.H + h];
+      for (int64_t r = share; r < rows; r += SHARES) s += k.ph[(which * rows + r) * a.H + h];
     part[share][l] = s;
     __syncthreads();
     if (share != 0 || which >= 3) return;
     float* dst = which == 0 ? k.dA : which == 1 ? k.dD : k.dbias;
-    if (dst != nullptr) dst[h] = static_cast<float>((part[0][l] + part[1][l]) + (part[2][l] + part[3][l]));
+    for (int i = 1; i < SHARES; ++i) s += part[i][l];
+    if (dst != nullptr) dst[h] = static_cast<float>(s);
     return;
   }
   const int64_t i = (static_cast<int64_t>(blockIdx.x - heads) * SNT + threadIdx.x) * 4;
@@ -788,7 +792,7 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
   if (sb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(steps_kernel<L>, dim3(static_cast<unsigned>(sb)), dim3(SNT), 0, stream, k, chunks);
   if (!ok(st)) return st;
-  const int heads = (3 * a.H + 63) / 64;
+  const int heads = (3 * a.H + 15) / 16;
   const int64_t elems = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
   const int64_t rb = heads + (p.hblocks > 1 ? (elems + 4 * SNT - 1) / (4 * SNT) : 0);
   if (rb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
