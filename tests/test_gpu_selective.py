@@ -57,6 +57,18 @@ def test_forward(device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,P,N", [(300, 64, 64), (530, 33, 20), (700, 64, 128), (705, 20, 7)])
+def test_segments(device, T, P, N, dtype):
+    """Long enough to be cut into segments, few (the last pass joins them) and more (a kernel does); sequences that
+    end in the first segment, inside a later one and before the first token."""
+    from verace_amd import selective_scan
+    d, state = inputs(device, 3, T, 2, P, 1, N, dtype, seed=40)
+    check(selective_scan(**d, initial_state=state), d, state)
+    lengths = torch.tensor([T - 170, 0, 5], device=device)
+    check(selective_scan(**d, lengths=lengths), d, None, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_options(device, dtype):
     """Without D or bias, the step size itself, fp32 step sizes, growing states, no decay."""
     from verace_amd import selective_scan

@@ -8,7 +8,7 @@
 // Launches (Sg segments of the chunks, picked by plan()):
 //   prep_kernel                d_t and c_t of every chunk (a wave each; c in fp64, kept as two floats);
 //   pass_kernel<READOUT=false> (Sg > 1) each segment's own state from zero;
-//   carry_kernel               (Sg > 1) the segments' start states;
+//   carry_kernel               (Sg > MAX_FOLD) the segments' start states;
 //   pass_kernel<READOUT=true>  every segment from its start state, with outputs.
 //
 // A workgroup of four waves takes 64 rows p of one head and walks a segment's chunks with S^T [N, 64] in
@@ -30,15 +30,19 @@ constexpr int NTH = 256;
 constexpr int L = 32;        // tokens of a chunk
 constexpr int PB = 64;       // rows p of a workgroup
 constexpr int MAX_SEG = 64;
+// Up to here a workgroup of the last pass runs over the earlier segments' states itself, from here on carry_kernel does,
+// a read for each state in place of one for each pair (T2048 H32 P64 N128, carried / run over, us: 3 segments 121 /
+// 115, 6 73 / 73, 8 62 / 66).
+constexpr int MAX_FOLD = 4;
 
 struct Chunks {
   Args a;
   const float* d;            // [BH][Tp]
   const float2* c;           // [BH][Tp]
-  float* seg_state;          // [Sg][BH][P][N]: a segment's own state, then its start state
+  float* seg_state;          // [Sg][BH][P][N]: a segment's own state, then (Sg > MAX_FOLD) its start state
   float* seg_decay;          // [Sg][BH]
   int nch, seg_chunks, nseg, pblocks;
-  bool vec, vec_state, vec_y;
+  bool vec, vec_state, vec_y, fold;
 };
 
 // ------------------------------------------------------------------ step sizes and log decays
@@ -136,26 +140,31 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
 
   // S^T: tile j, register r = state column n = 16 j + 4 g + r of row p = pw + l16
   f32x4 S[NT];
-  {
-    const float* src = nullptr;
-    if (READOUT) {
-      if (seg > 0) src = k.seg_state + (static_cast<int64_t>(seg) * a.B * a.H + bh) * a.P * a.N;
-      else if (a.state_in != nullptr) src = a.state_in + bh * a.P * a.N;
-    }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) S[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (READOUT) {
     const int p = pw + l16;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    auto load = [&](const float* src, int j) {
       const int n = 16 * j + 4 * g;
-      S[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (src == nullptr || p >= a.P || n >= a.N) continue;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (p >= a.P || n >= a.N) return v;
       const float* q = src + static_cast<int64_t>(p) * a.N + n;
-      if (k.vec_state) {
-        S[j] = *reinterpret_cast<const f32x4*>(q);
-      } else {
+      if (k.vec_state) return *reinterpret_cast<const f32x4*>(q);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < a.N) S[j][r] = q[r];
-      }
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.N) v[r] = q[r];
+      return v;
+    };
+    const int64_t BH = static_cast<int64_t>(a.B) * a.H, PN = static_cast<int64_t>(a.P) * a.N;
+    if ((seg == 0 || k.fold) && a.state_in != nullptr)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) S[j] = load(a.state_in + bh * PN, j);
+    // the segments before this one, or its start state alone
+#pragma unroll 2
+    for (int s = k.fold ? 0 : seg; s < (k.fold ? seg : seg + min(seg, 1)); ++s) {
+      const float dec = k.fold ? k.seg_decay[s * BH + bh] : 0.f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) S[j] = S[j] * dec + load(k.seg_state + (s * BH + bh) * PN, j);
     }
   }
   if constexpr (READOUT) {  // the tile right of the diagonal stays zero
@@ -378,6 +387,8 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
   if (p.nseg > 1) {
     hipLaunchKernelGGL((pass_kernel<IO, E, NP, false, VEC>), dim3(static_cast<unsigned>(wgs)), dim3(NTH), 0, stream, k);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+  }
+  if (p.nseg > 1 && !k.fold) {
     const bool vec = PN % 4 == 0 && aligned16({a.state_in});
     const int64_t blocks = (BH * PN / (vec ? 4 : 1) + NTH - 1) / NTH;
     if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
@@ -436,6 +447,7 @@ int launch_chunk(const Args& a, int dtype, void* workspace, hipStream_t stream) 
   k.vec = a.P % el == 0 && a.x_t % el == 0 && a.x_b % el == 0 && a.N % el == 0 && a.b_t % el == 0 &&
           a.b_b % el == 0 && a.c_t % el == 0 && a.c_b % el == 0 && aligned16({a.x, a.bm, a.cm});
   k.vec_state = a.N % 4 == 0 && aligned16({a.state_in, a.state_out});
+  k.fold = p.nseg <= MAX_FOLD;
   k.vec_y = a.P % 4 == 0 && aligned16({a.y});
   if (dtype == VMI_BF16) return by_state<bf16_t, __bf16>(k, p, stream);
   if (dtype == VMI_F16) return by_state<f16_t, float>(k, p, stream);
