@@ -57,7 +57,7 @@ def test_forward(device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("T,P,N", [(300, 64, 64), (530, 33, 20), (700, 64, 128), (705, 20, 7)])
+@pytest.mark.parametrize("T,P,N", [(150, 33, 20), (230, 64, 128), (300, 64, 64), (530, 33, 20), (700, 64, 128), (705, 20, 7)])
 def test_segments(device, T, P, N, dtype):
     """Long enough to be cut into segments, few (the last pass joins them) and more (a kernel does); sequences that
     end in the first segment, inside a later one and before the first token."""

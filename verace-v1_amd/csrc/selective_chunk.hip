@@ -357,14 +357,16 @@ struct Plan {
 };
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Three workgroups a compute unit; a segment costs its state's way through memory, so it keeps some chunks.
+// Three workgroups a compute unit; a segment costs its state's way through memory, so it keeps four chunks, or two
+// while every workgroup has a compute unit to itself and the chunks' own latency is what counts (fp32 N64, four / two:
+// B3 T777 H8 34.7 / 29.1 us, B1 T512 H8 27.4 / 22.5; with 640 workgroups B4 T300 H32 N128 45 / 60).
 Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N) {
   Plan p;
   p.nch = (T + L - 1) / L;
   p.tp = p.nch * L;
   p.pblocks = static_cast<int>((P + PB - 1) / PB);
   const int64_t base = B * H * p.pblocks, want = (768 + base - 1) / base;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(MAX_SEG, p.nch / 4));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(MAX_SEG, std::max(p.nch / 4, std::min(p.nch / 2, 256 / base))));
   int64_t nseg = std::min(want, most);
   p.seg_chunks = static_cast<int>((p.nch + nseg - 1) / nseg);
   p.nseg = static_cast<int>((p.nch + p.seg_chunks - 1) / p.seg_chunks);
