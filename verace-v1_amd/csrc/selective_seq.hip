@@ -3,7 +3,7 @@
 // Rows p of a head's state are independent: y[p] = sum_n S[p, n] C[n].  LPR lanes hold a row, four values
 // each, and a wave takes 64 / LPR rows IT times over; the state stays in registers over the tokens.  The
 // step is bound by the state's read and write (nontemporal, as every decode state here: it is touched once
-// a token): at B64 H32 P64 N128 134 MB.
+// a token): at B64 H32 P64 N128 134 MB in 26.2 us, 5.1 TB/s.
 #include <type_traits>
 
 #include "selective.h"

@@ -37,7 +37,8 @@ Drop-in replacements for the reference's SSSD hot path:
 * ``HAS_HIP``                  <- ``verace_v1.serving.triton_kernels.HAS_TRITON``
 
 ``torch.ops.verace.{sssd_scan, sssd_scan_bwd, sssd_step_, sssd_scan_fused, cham_scan, cham_step_,
-ns_retraction}`` are the same launchers registered as torch operators with fake kernels and
+ns_retraction, selective_scan, selective_scan_bwd, selective_step_, short_conv, short_conv_bwd,
+short_conv_step_, gated_norm, gated_norm_bwd}`` are the same launchers registered as torch operators with fake kernels and
 autograd (``ops.py``), for FakeTensor / meta tracing and ``torch.compile``.
 
 All compute runs in ``libverace_sssd.so`` (C ABI: ``include/verace_sssd.h``).
