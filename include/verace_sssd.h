@@ -475,7 +475,7 @@ int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_batch, const v
  * convolution; y [B, T, H, P] (or NULL) behind them is 0.  N <= 256, P <= 1024, H / G whole.
  * fp32 and fp16 inputs run in fp32; with bf16 inputs the terms of y are rounded to bf16 once more (2^-8 of a
  * term), the states are not.  A NaN or an infinity in a token reaches no earlier one.  Calls of a few tokens, and
- * rows further than 2^23 elements apart, run token by token.
+ * rows that lie backwards or more than 2^23 elements apart, run token by token.
  * The step takes one token per item and updates `state` in place (items with mask[b] = 0 keep theirs and
  * give zeros). */
 int vmi_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N,
@@ -489,7 +489,8 @@ int vmi_selective_scan_fwd(const void* x, int64_t x_t, int64_t x_b, const void* 
                            size_t workspace_bytes, void* stream);
 /* Gradients, for dy (rows [H, P] at its own strides) and dstate = dL/dstate_out (NULL: zero): dx, db, dc (dtype),
  * ddelta (delta_dtype), dA, dD, dbias [H] and dstate_in fp32; any may be NULL.  What lies behind the lengths gets
- * zeros.  B, T >= 1; rows at most 2^23 elements apart.  Sums run in a fixed order: the same bits every time. */
+ * zeros.  B, T >= 1; rows 0 .. 2^23 elements apart (otherwise VMI_ERR_UNSUPPORTED).  Sums run in a
+ * fixed order: the same bits every time. */
 int vmi_selective_scan_bwd_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G,
                                            int64_t N, int dtype, size_t* bytes);
 int vmi_selective_scan_bwd(const void* x, int64_t x_t, int64_t x_b, const void* delta, int64_t d_t,

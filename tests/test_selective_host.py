@@ -147,3 +147,11 @@ def test_gradient_operator_refusals():
         for stats, ds in ((_e(2, 2), _e(3, 8)), (_e(2, 3), _e(3, 4)), (_e(3, 2).t(), _e(3, 8))):
             with pytest.raises(RuntimeError, match="must be"):
                 block_norm._launch_bwd(_e(3, 8), _e(3, 8), None, None, None, None, stats, 1, ds, None, (True,) * 6)
+
+
+def test_backward_refuses_far_and_backward_rows(lib):
+    one, null = ctypes.c_void_p(64), None
+    for x_t, b_t, y_t in ((-8, 8, 8), (8, -8, 8), (8, 8, -8), ((1 << 23) + 1, 8, 8), (8, (1 << 23) + 1, 8)):
+        assert lib.vmi_selective_scan_bwd(one, x_t, 64, one, 1, 8, 0, one, one, b_t, 64, one, 8, 64, null, null, 1, 0, null,
+                                          null, 0, one, y_t, 64, null, one, one, one, one, one, null, null, null,
+                                          1, 8, 1, 8, 1, 8, one, 1 << 40, null) == 2

@@ -16,10 +16,10 @@ int check(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int 
   return VMI_OK;
 }
 
-// The chunk kernels' lane offsets are 32 bits wide.
+// The chunk kernels' lane offsets are 32 bits wide and count up.
 bool strides_fit(std::initializer_list<int64_t> strides, int64_t H, int64_t P) {
   for (int64_t s : strides)
-    if (s < -kMaxStride || s > kMaxStride) return false;
+    if (s < 0 || s > kMaxStride) return false;
   return H * P <= kMaxStride;
 }
 
