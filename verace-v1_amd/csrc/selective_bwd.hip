@@ -204,7 +204,8 @@ __global__ __launch_bounds__(SNT) void starts_kernel(Bwd k, int L) {
   const bool reverse = blockIdx.y != 0;
   const int64_t BHP = static_cast<int64_t>(a.B) * a.H * k.pblocks;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * SNT + threadIdx.x;  // 16-byte piece
-  if (id >= BHP * (SZ / 4)) return;
+  if (id >= BHP * (SZ / 4)) return;  // whole workgroups: SZ / 4 is a multiple of SNT
+  static_assert(SZ / 4 % SNT == 0, "");
   const int64_t bhp = id / (SZ / 4);
   const int e = static_cast<int>(id - bhp * (SZ / 4)), lane = e & 63, wave = (e >> 6) & 3, j = e >> 8;
   const int64_t bh = bhp / k.pblocks;
@@ -223,11 +224,13 @@ __global__ __launch_bounds__(SNT) void starts_kernel(Bwd k, int L) {
   f32x4 own = *reinterpret_cast<const f32x4*>(base);
   for (int g = 0; g + 1 < k.nseg; ++g) {
     const int place = reverse ? k.nseg - 1 - g : g;
-    double c = 0.0;
-    for (int i = place * k.seg_chunks; i < min(k.nch, (place + 1) * k.seg_chunks); ++i) {
+    double c = 0.0;  // the same in all lanes: a wave's pieces are of one state
+    for (int i = place * k.seg_chunks + lane; i < min(k.nch, (place + 1) * k.seg_chunks); i += 64) {
       const float2 v = cp[static_cast<int64_t>(i) * L + L - 1];
       c += static_cast<double>(v.x) + static_cast<double>(v.y);
     }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off);
     s = s * expf(static_cast<float>(c)) + own;
     if (g + 2 < k.nseg) own = *reinterpret_cast<const f32x4*>(base + (g + 1) * BHP * SZ);
     *reinterpret_cast<f32x4*>(base + (g + 1) * BHP * SZ) = s;
