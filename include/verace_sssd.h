@@ -473,8 +473,8 @@ int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_batch, const v
  * *_b (elements); head h uses group h / (H / G); A, D, delta_bias [H] fp32 (D, delta_bias may be NULL).
  * state_in [B, H, P, N] (NULL: zeros) is not written and must not be state_out.  lengths as for the
  * convolution; y [B, T, H, P] (or NULL) behind them is 0.  N <= 256, P <= 1024, H / G whole.
- * fp32 and fp16 inputs run in fp32; with bf16 inputs the terms of y are rounded to bf16 once more (2^-8 of a
- * term), the states are not.  A NaN or an infinity in a token reaches no earlier one.  Calls of a few tokens, and
+ * fp32 and fp16 inputs run in fp32; with bf16 inputs the terms of y are two bf16 parts (2^-16 of a term), the
+ * states fp32 sums.  A NaN or an infinity in a token reaches no earlier one.  Calls of a few tokens, and
  * rows that lie backwards or more than 2^23 elements apart, run token by token.
  * The step takes one token per item and updates `state` in place (items with mask[b] = 0 keep theirs and
  * give zeros). */

@@ -1,0 +1,36 @@
+"""The selective scan's bf16 results against the 64-bit recurrence term by term: the products' operands that are not
+inputs (decayed scores, the carried state) are taken in two bf16 parts.
+
+Tolerances: those of test_gpu_selective.py with the bf16 terms' budget cut to what two parts leave of a value: each part
+is off by at most 2^-8 of what it rounds, so two by 2^-16.  A term of y carries one such operand."""
+import pytest
+import torch
+
+from oracle import selective as ref
+
+from test_gpu_selective import U, inputs
+
+pytestmark = pytest.mark.gpu
+TERM = 2.0 ** -16
+SHAPES = [(2, 16, 2, 64, 1, 64), (2, 40, 4, 16, 2, 16), (1, 64, 2, 64, 1, 128), (1, 70, 2, 33, 1, 20), (1, 48, 2, 128, 1, 256),
+          (1, 100, 2, 40, 1, 130)]
+
+
+def near(got, want, m, budget, what):
+    h = torch.finfo(got.dtype).eps / 2
+    err = (got.double() - want).abs()
+    bad = err > h * want.abs() + budget * m.view(want.shape)
+    assert not bool(bad.any()), (what, int(bad.sum()), float(((err - h * want.abs()) / m.view(want.shape).clamp_min(1e-30)).max()), budget)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward(device, shape, dtype):
+    from verace_amd import selective_scan
+    d, state = inputs(device, *shape, dtype, seed=60)
+    T, N = shape[1], shape[5]
+    for s0 in (None, state):
+        y, _ = selective_scan(**d, initial_state=s0)
+        y64, _ = ref.selective_scan(**d, initial_state=s0)
+        m, _ = ref.selective_scan(**d, initial_state=s0, magnitude=True)
+        near(y, y64, m, (8 * T + N + 16) * U + (TERM if dtype == torch.bfloat16 else 0.0), "y")

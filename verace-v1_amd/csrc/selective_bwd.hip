@@ -72,7 +72,7 @@ struct Bwd {
 // S += (d_s e^{c_L - c_s} x_s) B_s^T; reverse, chunks from the last: G += (e^{c_t} dy_t) C_t^T.
 template <typename IO, typename E, int NP, int L, bool OWN, bool VEC>
 __global__ __launch_bounds__(SNT, 2) void states_kernel(Bwd k) {
-  constexpr int NT = NP / 16, KB = L / 32, NPART = Parts<E>::N;
+  constexpr int NT = NP / 16, KB = L / 32, NPART = Parts<E>::ALL;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
@@ -255,7 +255,7 @@ template <int LT> __device__ __forceinline__ bool lower_tile(int i, int& tt, int
 
 template <typename IO, typename E, int NP, int L, bool VEC>
 __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
-  constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::N;
+  constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::ALL;
   constexpr int NTW = NT >= NW ? NT / NW : 1;      // n-tiles of a wave: wave, wave + 8 (or wave % NT)
   constexpr int TS = NT >= NW ? 1 : NW / NT;       // waves that share an n-tile, each LTW of the t-tiles
   constexpr int LTW = LT / TS;

@@ -15,13 +15,12 @@
 // accumulators, 16 rows p a wave; x, B, C of the next chunk are on their way meanwhile.  S^T is directly
 // the operand of S_0 C_t.  The scores of a chunk are shared: each wave forms some of the 16 x 16 tiles on
 // or below the diagonal, and they pass through LDS as fragments.
-// With bf16 inputs the decayed scores and the carried state are rounded to bf16 where they enter y's
-// products (2^-8 of a term at most, as y's own rounding); the weighted x of the state's update enters as
-// three bf16 parts, so the state itself is carried in fp32 throughout.
+// With bf16 inputs the decayed scores and the carried state enter y's products as two bf16 parts (2^-16 of a term at
+// most: y is off by its own rounding and no more; one part each puts its distance to 64 bits from 1.66e-3 to 2.1e-3 and
+// saves 7 of 76 us), the weighted x of the state's update as three, so the state itself is carried in fp32 throughout.
 //
-// Bound by instruction issue: B4 T2048 H32 P64 N128 bf16, 69 us (76 MB would move in 15): outputs 41.5, own states
-// 22.9, carry 7.7, prep 5.5; of the outputs' 80k clocks a SIMD 37k issue VALU and 19k matrix instructions.  Three
-// workgroups a compute unit; four (128 registers) measured 75 us, a chunk of 64 tokens in the own pass the same as 32.
+// Bound by instruction issue: B4 T2048 H32 P64 N128 bf16, 76 us (76 MB would move in 15); each launch by itself under the
+// profiler: outputs 48.3, own states 22.4, carry 7.3, prep 5.6.  Three workgroups a compute unit.
 #include <algorithm>
 
 #include "selective_mfma.h"
@@ -80,10 +79,13 @@ __global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d
 // ------------------------------------------------------------------ the segments
 // acc[r] += sum_{s<=t} M[t,s] x[s, r] for a chunk with values that a product with a zero does not drop.
 template <typename E>
-__device__ __forceinline__ void add_in_order(const E* m, const E* x, int t, int l16, f32x4& acc) {
+__device__ __forceinline__ void add_in_order(const E* m, int part, const E* x, int t, int l16, f32x4& acc) {
 #pragma unroll 1
   for (int s = 0; s <= t; ++s) {
-    const float w = static_cast<float>(m[(l16 + 16 * ((s >> 2) & 3)) * 8 + 4 * (s >> 4) + (s & 3)]);
+    float w = 0.f;
+#pragma unroll
+    for (int i = Parts<E>::TERM - 1; i >= 0; --i)
+      w += static_cast<float>(m[i * part + (l16 + 16 * ((s >> 2) & 3)) * 8 + 4 * (s >> 4) + (s & 3)]);
     const E* row = x + Tile<E, PB>::at(s);
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] = fmaf(w, static_cast<float>(row[r]), acc[r]);
@@ -92,13 +94,13 @@ __device__ __forceinline__ void add_in_order(const E* m, const E* x, int t, int 
 
 template <typename IO, typename E, int NP, bool READOUT, bool VEC>
 __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass_kernel(Chunks k) {
-  constexpr int NT = NP / 16, LT = L / 16, KN = NP / 32, NPART = Parts<E>::N;
+  constexpr int NT = NP / 16, LT = L / 16, KN = NP / 32, NPART = Parts<E>::ALL, TERM = Parts<E>::TERM;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
   __shared__ __attribute__((aligned(16))) E Cs[READOUT ? RowTile<E, NP>::elems(L) : 8];
   __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Ms[READOUT ? LT * 64 * 8 : 8];
+  __shared__ __attribute__((aligned(16))) E Ms[TERM][READOUT ? LT * 64 * 8 : 8];
   __shared__ __attribute__((aligned(16))) float2 cs[L];
   __shared__ __attribute__((aligned(16))) float ds[L], ws[L], es[L];
   const Args& a = k.a;
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
     }
   }
   if constexpr (READOUT) {  // the tile right of the diagonal stays zero
-    for (int i = tid; i < LT * 64 * 8; i += NTH) Ms[i] = static_cast<E>(0.f);
+    for (int i = tid; i < TERM * LT * 64 * 8; i += NTH) Ms[0][i] = static_cast<E>(0.f);
   }
   const float Dh = a.D == nullptr ? 0.f : a.D[h];
   double seg_c = 0.0;
@@ -206,14 +208,20 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
         for (int kb = 0; kb < KN; ++kb)
           m = mma(row_frag<E, NP>(Bs, 16 * st, 32 * kb, l16, g), packed_frag<E, NP, L>(Cs, 16 * tt, 32 * kb, l16, g), m);
         const float2 ct = cs[16 * tt + l16];
-        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q;
+        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q[TERM];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int s = 16 * st + 4 * g + r;
-          const float v = m[r] * (decay(ct, cs[s]) * ds[s]);
-          q.e[r] = static_cast<E>(s <= 16 * tt + l16 ? v : 0.f);
+          float v = m[r] * (decay(ct, cs[s]) * ds[s]);
+          v = s <= 16 * tt + l16 ? v : 0.f;
+#pragma unroll
+          for (int i = 0; i < TERM; ++i) {
+            q[i].e[r] = static_cast<E>(v);
+            v -= static_cast<float>(q[i].e[r]);
+          }
         }
-        *reinterpret_cast<M4*>(Ms + (tt * 64 + lane) * 8 + 4 * st) = q;
+#pragma unroll
+        for (int i = 0; i < TERM; ++i) *reinterpret_cast<M4*>(Ms[i] + (tt * 64 + lane) * 8 + 4 * st) = q[i];
       }
       // S_0 C_t, transposed: rows p, column t
 #pragma unroll
@@ -221,9 +229,15 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
       if (live) {
 #pragma unroll
         for (int kb = 0; kb < KN; ++kb) {
-          const Frag<E> s = acc_frag<E>(S[2 * kb], S[2 * kb + 1]);
+          const f32x4 s[2] = {S[2 * kb], S[2 * kb + 1]};
+          Frag<E> sp[TERM], cf[LT];
+          split<E>(s, sp);
 #pragma unroll
-          for (int t = 0; t < LT; ++t) acc[t] = mma(s, packed_frag<E, NP, L>(Cs, 16 * t, 32 * kb, l16, g), acc[t]);
+          for (int t = 0; t < LT; ++t) cf[t] = packed_frag<E, NP, L>(Cs, 16 * t, 32 * kb, l16, g);
+#pragma unroll
+          for (int i = TERM - 1; i >= 0; --i)
+#pragma unroll
+            for (int t = 0; t < LT; ++t) acc[t] = mma(sp[i], cf[t], acc[t]);
         }
       }
     }
@@ -258,18 +272,22 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
 #pragma unroll
         for (int t = 0; t < LT; ++t) {
           acc[t] *= es[16 * t + l16];
-          const E* m = Ms + (t * 64 + lane) * 8;
-          Frag<E> f;
-          if constexpr (sizeof(E) == 2) {
-            f.v = *reinterpret_cast<const bf16x8*>(m);
-          } else {
-            f.v[0] = *reinterpret_cast<const f32x4*>(m);
-            f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
+          f32x4 sum = acc[t];
+#pragma unroll
+          for (int i = TERM - 1; i >= 0; --i) {
+            const E* m = Ms[i] + (t * 64 + lane) * 8;
+            Frag<E> f;
+            if constexpr (sizeof(E) == 2) {
+              f.v = *reinterpret_cast<const bf16x8*>(m);
+            } else {
+              f.v[0] = *reinterpret_cast<const f32x4*>(m);
+              f.v[1] = *reinterpret_cast<const f32x4*>(m + 4);
+            }
+            sum = mma(xf, f, sum);
           }
-          const f32x4 sum = mma(xf, f, acc[t]);
           // a NaN or an infinity in x times a masked score's 0: in order, so that no earlier token sees it
           if (__builtin_isunordered(sum[0], sum[1]) || __builtin_isunordered(sum[2], sum[3]))
-            add_in_order<E>(Ms + t * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
+            add_in_order<E>(Ms[0] + t * 64 * 8, LT * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
           else
             acc[t] = sum;
           if (y_on && c * L + 16 * t + l16 < a.T) {

@@ -99,43 +99,47 @@ __device__ __forceinline__ Frag<E> col_frag(const E* tile, int k0, int col0, int
   return f;
 }
 
-// Two accumulator tiles (contraction indexes k0 + 4g + r and k0 + 16 + 4g + r) as a fragment, rounded once.
-template <typename E> __device__ __forceinline__ Frag<E> acc_frag(f32x4 a, f32x4 b) {
-  Frag<E> f;
-  if constexpr (sizeof(E) == 2) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.v[i] = static_cast<__bf16>(a[i]), f.v[4 + i] = static_cast<__bf16>(b[i]);
-  } else {
-    f.v[0] = a, f.v[1] = b;
-  }
-  return f;
-}
-
-// The parts of eight fp32 values: three bf16 parts hold all 24 bits, fp32 is its own part.
-template <typename E> struct Parts { static constexpr int N = sizeof(E) == 2 ? 3 : 1; };
-template <typename E>
-__device__ __forceinline__ void split(const f32x4 (&x)[2], Frag<E> (&f)[Parts<E>::N]) {
+// The parts that eight fp32 values are multiplied in: ALL hold their 24 bits (three of bf16), TERM is what a term of a
+// 16-bit result takes (two: off by 2^-16 of it).  fp32 is its own part.
+template <typename E> struct Parts {
+  static constexpr int ALL = sizeof(E) == 2 ? 3 : 1;
+  static constexpr int TERM = sizeof(E) == 2 ? 2 : 1;
+};
+template <typename E, int M>
+__device__ __forceinline__ void split(const f32x4 (&x)[2], Frag<E> (&f)[M]) {
   if constexpr (sizeof(E) == 2) {
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    // v - (its bf16) is exact, in one v_dot2 with a pair and (-1, 0) or (0, -1); a pair with an infinity gives NaN for
+    // both, and both belong to one row of the product
+    uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+    asm volatile("" : "+s"(first), "+s"(second));  // not as inline constants, whose place in a pair is the encoding's
     float r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = x[i / 4][i % 4];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < M; ++k) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[k].v[i] = static_cast<__bf16>(r[i]);  // v_cvt_pk_bf16_f32 pairs
-      if (k == 2) break;
+      if (k == M - 1) break;
       const u32x4 q = __builtin_bit_cast(u32x4, f[k].v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        r[2 * i] -= __uint_as_float(q[i] << 16);
-        r[2 * i + 1] -= __uint_as_float(q[i] & 0xffff0000u);
+        const uint32_t both = q[i];
+        const bf16x2 pair = __builtin_bit_cast(bf16x2, both);
+        r[2 * i] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, first), r[2 * i], false);
+        r[2 * i + 1] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, second), r[2 * i + 1], false);
       }
     }
   } else {
     f[0].v[0] = x[0], f[0].v[1] = x[1];
   }
 }
+// Half a fragment (four values side by side) as it is, to an aligned place.
+__device__ __forceinline__ void put_half(__bf16* o, const Frag<__bf16>& f, int h) {
+  *reinterpret_cast<bf16x4*>(o) = h ? __builtin_shufflevector(f.v, f.v, 4, 5, 6, 7) : __builtin_shufflevector(f.v, f.v, 0, 1, 2, 3);
+}
+__device__ __forceinline__ void put_half(float* o, const Frag<float>& f, int h) { *reinterpret_cast<f32x4*>(o) = f.v[h]; }
 template <typename E> __device__ __forceinline__ f32x4 half(const Frag<E>& f, int h) {
   if constexpr (sizeof(E) == 2) {
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
