@@ -26,13 +26,14 @@
 //   steps_kernel: g, and from it ddelta and the chunks' shares of dA and dbias;
 //   reduce_kernel: the head blocks' dB and dC and the heads' dA, dD, dbias, in a fixed order.
 //
-// bf16 inputs: Q and M, and G_L where it enters dx, are rounded to bf16 once (2^-8 of a term, as the results);
+// bf16 inputs: Q and M, and G_L where it enters dx, are two bf16 parts (2^-16 of a term: dx, dB and dC are off by their
+// own rounding and no more; one part each saves 28 us below and puts their distance to 64 bits from 1.66e-3 to 2.3e-3);
 // S_0 and G_L enter alpha, beta, dB and dC as three bf16 parts and R stays fp32, because ddelta, dA and dbias may be
 // fp32 and are sums in which such roundings do not cancel.
 //
-// B4 T2048 H32 P64 N128 bf16, us: main 119 (one workgroup a compute unit, two waves a SIMD: VALU 104k and matrix 38k of
-// 247k clocks, the rest latency), states 77 (268 MB of S_0 and G_L written: 57 at the copy rate), steps 7.5, prep 6,
-// reduce 5.8.  A chunk of 64 halves the states' traffic against 32.
+// B4 T2048 H32 P64 N128 bf16, us: main 146 (one workgroup a compute unit, two waves a SIMD), states 77 (268 MB of S_0 and
+// G_L written: 57 at the copy rate), steps 7.5, prep 7, reduce 5.9.  A chunk of 64 halves the states' traffic against 32;
+// above 128 state columns its accumulators and parts fit neither the registers nor LDS, so there it is 32.
 #include <algorithm>
 #include <type_traits>
 
@@ -255,11 +256,11 @@ template <int LT> __device__ __forceinline__ bool lower_tile(int i, int& tt, int
 
 template <typename IO, typename E, int NP, int L, bool VEC>
 __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
-  constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::ALL;
+  constexpr int NW = MNT / 64, NT = NP / 16, LT = L / 16, KL = L / 32, KN = NP / 32, KP = PB / 32, NPART = Parts<E>::ALL, TERM = Parts<E>::TERM;
   constexpr int NTW = NT >= NW ? NT / NW : 1;      // n-tiles of a wave: wave, wave + 8 (or wave % NT)
   constexpr int TS = NT >= NW ? 1 : NW / NT;       // waves that share an n-tile, each LTW of the t-tiles
   constexpr int LTW = LT / TS;
-  constexpr int NH = NP > 128 ? 2 : 1, GR = NP / NH;  // dx takes G_L through LDS 128 state columns at a time
+  constexpr int GR = NP < 128 / TERM ? NP : 128 / TERM, NH = NP / GR;  // dx takes G_L through LDS GR state columns at a time
   constexpr int PER = (LT * (LT + 1) / 2 + NW - 1) / NW;
   static_assert(LT % TS == 0, "");
   typedef Tile<E, NP> TB;
@@ -268,14 +269,14 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
   __shared__ __attribute__((aligned(16))) E Cs[TB::elems(L)];
   // x, dy and the log decays of a unit while the next one's arrive
-  constexpr bool XROWS = NP <= 128;  // x by lane group (12 KB of 10); at 256 state columns LDS is full
+  constexpr bool XROWS = NP <= 128 || sizeof(E) == 2;  // x by lane group (12 KB of 10); where LDS is full, not
   __shared__ __attribute__((aligned(16))) E Xb[2][XROWS ? RowTile<E, PB>::elems(L) : TX::elems(L)];
   __shared__ __attribute__((aligned(16))) E Yb[2][TX::elems(L)];
   __shared__ __attribute__((aligned(16))) float2 cb2[2][L];
   __shared__ __attribute__((aligned(16))) float db2[2][L], eb2[2][L], wb2[2][L], dh2[2];
-  __shared__ __attribute__((aligned(16))) E Qs[TQ::elems(L)];   // [t][s]
-  __shared__ __attribute__((aligned(16))) E Ms[TQ::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Gs[TX::elems(GR)];  // G_L^T [n][p]
+  __shared__ __attribute__((aligned(16))) E Qs[TERM][TQ::elems(L)];   // [t][s]
+  __shared__ __attribute__((aligned(16))) E Ms[TERM][TQ::elems(L)];
+  __shared__ __attribute__((aligned(16))) E Gs[TERM][TX::elems(GR)];  // G_L^T [n][p]
   __shared__ float row_r[LT][L], col_r[LT][L];                  // sums of R d_s (below) by s-tile, sum_t R by t-tile
   __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
   const Args& a = k.a;
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       sc.fetch(t0, len);
       sb.commit(Bs);
       sc.commit(Cs);
-      for (int i = tid; i < TQ::elems(L); i += MNT) Qs[i] = Ms[i] = static_cast<E>(0.f);
+      for (int i = tid; i < TERM * TQ::elems(L); i += MNT) Qs[0][i] = Ms[0][i] = static_cast<E>(0.f);
     }
     Stage<IO, E, PB, L, MNT, VEC> sx, sy;
     float rd, rD;
@@ -387,22 +388,30 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const float2 ct = cs[t];
         const f32x4 c01 = *reinterpret_cast<const f32x4*>(cs + s0_), c23 = *reinterpret_cast<const f32x4*>(cs + s0_ + 2);
         const f32x4 dv = *reinterpret_cast<const f32x4*>(ds + s0_);
-        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q, m;
+        struct alignas(4 * sizeof(E)) M4 { E e[4]; } q[TERM], m[TERM];
         float dg = 0.f, rr[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const bool on = s0_ + r <= t;
           const float2 from = make_float2((r < 2 ? c01 : c23)[2 * (r & 1)], (r < 2 ? c01 : c23)[2 * (r & 1) + 1]);
           const float w = decay(ct, from), wd = w * dv[r];
-          const float xq = xy[r] * wd, cm_ = cb[i][r] * wd, xc = cb[i][r] * xy[r] * w;  // off the triangle: dropped, not added
-          q.e[r] = static_cast<E>(on ? xq : 0.f);
-          m.e[r] = static_cast<E>(on ? cm_ : 0.f);
+          float xq = xy[r] * wd, cm_ = cb[i][r] * wd;
+          const float xc = cb[i][r] * xy[r] * w;  // off the triangle: dropped, not added
+          xq = on ? xq : 0.f, cm_ = on ? cm_ : 0.f;
+#pragma unroll
+          for (int k = 0; k < TERM; ++k) {
+            q[k].e[r] = static_cast<E>(xq), m[k].e[r] = static_cast<E>(cm_);
+            xq -= static_cast<float>(q[k].e[r]), cm_ -= static_cast<float>(m[k].e[r]);
+          }
           rr[r] = on ? xc : 0.f;
           dg = s0_ + r == t ? xy[r] : dg;
         }
         const int o = TQ::at(t) + 16 * st + 4 * g;
-        *reinterpret_cast<M4*>(Qs + o) = q;
-        *reinterpret_cast<M4*>(Ms + o) = m;
+#pragma unroll
+        for (int k = 0; k < TERM; ++k) {
+          *reinterpret_cast<M4*>(Qs[k] + o) = q[k];
+          *reinterpret_cast<M4*>(Ms[k] + o) = m[k];
+        }
         // left of the diagonal the rows' sums, in a tile on it each token's sum over the paths that cross it
         float rs = 0.f;
 #pragma unroll
@@ -473,14 +482,21 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
 #pragma unroll
       for (int hh = 0; hh < NH; ++hh) {
         if (hh > 0) lds_barrier();
-        if (NT >= NW || tt0 == 0) {
-          const int j = NH > 1 ? hh : 0;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            struct alignas(8) M4 { E e[4]; } q;
+        for (int j = 0; j < NTW; ++j) {
+          const int tile = nt0 + NW * j;
+          if (tile / (GR / 16) != hh || (NT < NW && tt0 != 0)) continue;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) q.e[r] = static_cast<E>(g1[j][w][r]);
-            *reinterpret_cast<M4*>(Gs + TX::at(16 * nt0 + l16) + 16 * w + 4 * g) = q;
+          for (int w = 0; w < 4; w += 2) {
+            const f32x4 v[2] = {g1[j][w], g1[j][w + 1]};
+            Frag<E> part[TERM];
+            split<E>(v, part);
+#pragma unroll
+            for (int k = 0; k < TERM; ++k) {
+              E* o = Gs[k] + TX::at(16 * (tile % (GR / 16)) + l16) + 16 * w + 4 * g;
+              put_half(o, part[k], 0);
+              put_half(o + 16, part[k], 1);
+            }
           }
         }
         if (hh == 0) {
@@ -500,10 +516,15 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         }
 #pragma unroll
         for (int kb = 0; kb < GR / 32; ++kb) {
-          const Frag<E> gf = col_frag<E, PB>(Gs, 32 * kb, 16 * pt, l16, g);
+          Frag<E> gf[TERM], bf[DXT];
 #pragma unroll
-          for (int t = 0; t < DXT; ++t)
-            dx[t] = mma(gf, row_frag<E, NP>(Bs, 16 * (st0 + t), GR * hh + 32 * kb, l16, g), dx[t]);
+          for (int i = 0; i < TERM; ++i) gf[i] = col_frag<E, PB>(Gs[i], 32 * kb, 16 * pt, l16, g);
+#pragma unroll
+          for (int t = 0; t < DXT; ++t) bf[t] = row_frag<E, NP>(Bs, 16 * (st0 + t), GR * hh + 32 * kb, l16, g);
+#pragma unroll
+          for (int i = TERM - 1; i >= 0; --i)
+#pragma unroll
+            for (int t = 0; t < DXT; ++t) dx[t] = mma(gf[i], bf[t], dx[t]);
         }
       }
       // the chunk's own terms
@@ -514,10 +535,12 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           const Frag<E> bf = col_frag<E, NP>(Bs, 32 * kb, 16 * (nt0 + NW * j), l16, g);
           const Frag<E> cf = col_frag<E, NP>(Cs, 32 * kb, 16 * (nt0 + NW * j), l16, g);
 #pragma unroll
-          for (int t = 0; t < LTW; ++t) {
-            if ((tt0 + t) / 2 >= kb) dc[j][t] = mma(bf, row_frag<E, L>(Qs, 16 * (tt0 + t), 32 * kb, l16, g), dc[j][t]);
-            if ((tt0 + t) / 2 <= kb) db[j][t] = mma(cf, col_frag<E, L>(Qs, 32 * kb, 16 * (tt0 + t), l16, g), db[j][t]);
-          }
+          for (int i = TERM - 1; i >= 0; --i)
+#pragma unroll
+            for (int t = 0; t < LTW; ++t) {
+              if ((tt0 + t) / 2 >= kb) dc[j][t] = mma(bf, row_frag<E, L>(Qs[i], 16 * (tt0 + t), 32 * kb, l16, g), dc[j][t]);
+              if ((tt0 + t) / 2 <= kb) db[j][t] = mma(cf, col_frag<E, L>(Qs[i], 32 * kb, 16 * (tt0 + t), l16, g), db[j][t]);
+            }
         }
       }
 #pragma unroll
@@ -525,8 +548,12 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const int st = st0 + t, s = 16 * st + l16;
         dx[t] *= ws[s] * ds[s];
 #pragma unroll
-        for (int kb = 0; kb < KL; ++kb)
-          if (st / 2 <= kb) dx[t] = mma(col_frag<E, PB>(Ys, 32 * kb, 16 * pt, l16, g), col_frag<E, L>(Ms, 32 * kb, 16 * st, l16, g), dx[t]);
+        for (int kb = 0; kb < KL; ++kb) {
+          if (st / 2 > kb) continue;
+          const Frag<E> yf = col_frag<E, PB>(Ys, 32 * kb, 16 * pt, l16, g);
+#pragma unroll
+          for (int i = TERM - 1; i >= 0; --i) dx[t] = mma(yf, col_frag<E, L>(Ms[i], 32 * kb, 16 * st, l16, g), dx[t]);
+        }
         const int p = p0 + 16 * pt + 4 * g;
         if (t0 + s < a.T && p < a.P && k.dx != nullptr) {
           const E* yr = Ys + TX::at(s) + 16 * pt + 4 * g;
@@ -738,7 +765,7 @@ __global__ __launch_bounds__(SNT) void reduce_kernel(Bwd k, int heads, int64_t e
 
 namespace {
 
-int bwd_tokens(int dtype) { return dtype == VMI_BF16 ? 64 : 32; }
+int bwd_tokens(int dtype, int64_t N) { return dtype == VMI_BF16 && N <= 128 ? 64 : 32; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Plan {
@@ -749,7 +776,7 @@ struct Plan {
 
 Plan plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
   Plan p;
-  const int L = bwd_tokens(dtype);
+  const int L = bwd_tokens(dtype, N);
   p.np = N <= 64 ? 64 : N <= 128 ? 128 : 256;
   p.nch = (T + L - 1) / L;
   p.tp = p.nch * L;
@@ -808,9 +835,10 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
   return st;
 }
 
-template <typename IO, typename E, int L> int by_state(const Bwd& k, const Plan& p, hipStream_t stream) {
+// Chunks of MOST tokens up to 128 state columns, of 32 above.
+template <typename IO, typename E, int MOST> int by_state(const Bwd& k, const Plan& p, hipStream_t stream) {
   auto go = [&](auto np) -> int {
-    constexpr int NP = decltype(np)::value;
+    constexpr int NP = decltype(np)::value, L = NP > 128 ? 32 : MOST;
     return k.vec ? run<IO, E, NP, L, true>(k, p, stream) : run<IO, E, NP, L, false>(k, p, stream);
   };
   if (p.np == 64) return go(std::integral_constant<int, 64>{});

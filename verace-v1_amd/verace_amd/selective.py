@@ -388,8 +388,8 @@ def selective_scan(
     and C may be slices of wider rows.  head_dim <= 1024, N <= 256.  Returns (y in x's dtype, final_state
     float32); y behind a sequence's length is 0 and nothing of the inputs there is used.
 
-    bf16: each term of y is taken to 2^-16 of itself, each term of the gradients of x, B and C carries one more rounding to
-    bf16; the states and the other gradients are fp32 sums of the inputs as they are.  A NaN or an infinity in a token reaches no earlier output, but in
+    bf16: each term of y and of the gradients of x, B and C is taken to 2^-16 of itself; the states and the other gradients
+    are fp32 sums of the inputs as they are.  A NaN or an infinity in a token reaches no earlier output, but in
     the backward the gradients of its chunk's other tokens and of earlier ones.  The backward takes rows up to 2^23
     elements apart.
     """
