@@ -562,6 +562,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           f32x4 q;
 #pragma unroll
           for (int r = 0; r < 4; ++r) q[r] = fmaf(Dh, static_cast<float>(yr[r]), dx[t][r]);
+          if (t0 + L > len) {  // behind the length 0, whatever a NaN made of the zeros there
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[r] = t0 + s < len ? q[r] : 0.f;
+          }
           const Out4<IO> v = out4<IO>(q);
           if (k.vec_dx) {
             *reinterpret_cast<Out4<IO>*>(o) = v;
@@ -634,6 +638,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
     for (int t = 0; t < LTW; ++t) {
       const int tok = t0 + 16 * (tt0 + t) + l16;
       if (tok >= a.T || n >= a.N) continue;
+      if (tok >= len) db[j][t] = dc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
       const int64_t o = ((static_cast<int64_t>(b) * a.T + tok) * a.G + grp) * a.N + n;
       const int64_t part = static_cast<int64_t>(hb) * a.B * a.T * a.G * a.N;
       if (k.pb != nullptr && a.N % 4 == 0) {

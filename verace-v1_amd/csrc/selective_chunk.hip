@@ -296,6 +296,10 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
             f32x4 o;
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(Dh, static_cast<float>(xr[r]), acc[t][r]);
+            if (c * L + L > len) {  // behind the length 0, whatever a NaN made of the zeros there
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[r] = c * L + 16 * t + l16 < len ? o[r] : 0.f;
+            }
             const Out4<IO> v = out4<IO>(o);
             if (k.vec_y) {
               *reinterpret_cast<Out4<IO>*>(yt) = v;
