@@ -294,6 +294,7 @@ __global__ __launch_bounds__(NTH, 3) void backward_kernel(Args a) {
           for (int j = 0; j < N; ++j) d[j] += g[j];
         }
         if (t >= 0) {
+          if (t >= n) zero(d);  // whatever the weights are
           if (t < a.T && a.dx != nullptr) store<T, N>(static_cast<T*>(a.dx) + (static_cast<int64_t>(b) * a.T + t) * a.C + c0, d);
         } else if (a.dstate_in != nullptr) {
           store<T, N>(static_cast<T*>(a.dstate_in) + (static_cast<int64_t>(b) * (K - 1) + (t + K - 1)) * a.C + c0, d);
