@@ -210,8 +210,9 @@ template <typename T, int K, int N>
 __global__ __launch_bounds__(NTH, 3) void backward_kernel(Args a) {
   constexpr int RW = NTH / CT;
   __shared__ float sums[RW][K + 1][CT * N];
-  const int piece = blockIdx.x * CT + threadIdx.x % CT, worker = threadIdx.x / CT;
-  const int part = blockIdx.y, b = part / a.runs, run = (part - b * a.runs) * RW + worker;
+  const int cols = (a.pieces + CT - 1) / CT, part = blockIdx.x / cols, block = blockIdx.x - part * cols;
+  const int piece = block * CT + threadIdx.x % CT, worker = threadIdx.x / CT;
+  const int b = part / a.runs, run = (part - b * a.runs) * RW + worker;
   const int c0 = piece * N;
   const bool on = piece < a.pieces;
   float dw[K][N] = {}, db[N] = {};
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(NTH, 3) void backward_kernel(Args a) {
   }
   __syncthreads();
   for (int i = threadIdx.x; i < (K + 1) * CT * N; i += NTH) {
-    const int k = i / (CT * N), c = i - k * (CT * N), ch = blockIdx.x * CT * N + c;
+    const int k = i / (CT * N), c = i - k * (CT * N), ch = block * CT * N + c;
     if (ch >= a.C) continue;
     float s = 0.f;
 #pragma unroll
@@ -449,7 +450,7 @@ extern "C" int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_bat
   a.dy_batch = dy == nullptr ? 0 : dy_batch;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.C = static_cast<int>(C), a.w_dtype = w_dtype, a.act = act;
   const int64_t parts = backward_parts(B, T, K);
-  if (parts > 65535) return VMI_ERR_UNSUPPORTED;
+  if (parts > INT32_MAX) return VMI_ERR_UNSUPPORTED;
   const bool weights = dw != nullptr || dbias != nullptr;
   if (weights && B > 0) {
     size_t need = 0;
@@ -466,10 +467,11 @@ extern "C" int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_bat
       using IO = decltype(tag);
       a.pieces = vec ? a.C / PIECE : a.C;
       a.runs = static_cast<int>(parts / B);
+      const int64_t blocks = parts * ((a.pieces + CT - 1) / CT);
+      if (blocks > INT32_MAX / NTH) return VMI_ERR_UNSUPPORTED;  // as many elements as no card holds
       return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
         hipLaunchKernelGGL((backward_kernel<IO, decltype(k)::value, decltype(n)::value>),
-                           dim3(static_cast<unsigned>((a.pieces + CT - 1) / CT), static_cast<unsigned>(parts)),
-                           dim3(NTH), 0, s, a);
+                           dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, s, a);
         return hip_status(hipGetLastError());
       });
     });
