@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hip_kernels import _require_device, address, device_guard, traced
+from .hip_kernels import _require_device, address, device_guard, refuse_tangents, traced
 
 _ACT = {"sigmoid": 0, "silu": 1}
 
@@ -148,6 +148,7 @@ def gated_norm_add(
     unrounded s.  Differentiable once, in every tensor argument.
     """
     y, residual, gate, w1, sc, w2 = _checked(y, residual, gate, norm_weight, scale, next_weight, activation)
+    refuse_tangents(y, residual, gate, w1, sc, w2)
     if traced(y):
         s, n, _ = torch.ops.verace.gated_norm(y, residual, gate, w1, sc, w2, eps, eps if next_eps is None else next_eps,
                                               activation)

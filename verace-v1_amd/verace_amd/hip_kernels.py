@@ -57,14 +57,20 @@ _NO_GUARD = contextlib.nullcontext()
 
 
 def traced(x: torch.Tensor) -> bool:
-    """Whether torch.compile or FakeTensor tracing runs the caller: the registered operators (ops.py) then take
-    the launchers' place."""
-    if torch.compiler.is_compiling():
-        return True
-    if type(x) is torch.Tensor:
-        return False
-    from torch._subclasses.fake_tensor import FakeTensor
-    return isinstance(x, FakeTensor)
+    """Whether something sees the operators that the caller runs: torch.compile, torch.jit.trace, a dispatch or function
+    mode, a tensor subclass (FakeTensor among them).  The registered operators (ops.py) then take the launchers' place."""
+    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
+            or torch._C._len_torch_dispatch_stack() != 0 or torch._C._len_torch_function_stack() != 0
+            or type(x) not in (torch.Tensor, torch.nn.Parameter))
+
+
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives, which neither the launchers nor the registered operators carry, raise."""
+    if torch.autograd.forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("verace_amd: no forward-mode derivative of this operator")
 
 
 def device_guard(t: torch.Tensor):

@@ -256,7 +256,7 @@ selective_scan.register_autograd(_selective_backward, setup_context=_selective_s
 @torch.library.custom_op("verace::selective_step_", mutates_args=("state",))
 def selective_step_(x: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tensor, D: Optional[Tensor],
                     delta_bias: Optional[Tensor], softplus: bool, active_mask: Optional[Tensor]) -> Tensor:
-    return sel.selective_step_(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+    return sel._launch_selective_step(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
 
 
 @selective_step_.register_fake
@@ -268,7 +268,8 @@ def _selective_step_fake(x, delta, A, B, C, state, D, delta_bias, softplus, acti
 @torch.library.custom_op("verace::short_conv", mutates_args=())
 def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Optional[Tensor], lengths: Optional[Tensor],
                activation: Optional[str]) -> Tuple[Tensor, Tensor]:
-    return sel.short_conv(x, weight, bias, state, lengths, activation)
+    lengths, state = sel._conv_args(x, weight, bias, state, lengths, activation)
+    return sel._launch_conv(x, weight, bias, state, lengths, sel._ACT[activation])
 
 
 @short_conv.register_fake
@@ -315,7 +316,7 @@ short_conv.register_autograd(_conv_backward, setup_context=_conv_setup)
 @torch.library.custom_op("verace::short_conv_step_", mutates_args=("state",))
 def short_conv_step_(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Tensor, activation: Optional[str],
                      active_mask: Optional[Tensor]) -> Tensor:
-    return sel.short_conv_step_(x, weight, bias, state, activation, active_mask)
+    return sel._launch_conv_step(x, weight, bias, state, activation, active_mask)
 
 
 @short_conv_step_.register_fake

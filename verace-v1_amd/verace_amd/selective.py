@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hip_kernels import _mask_bytes, _require_device, address, device_guard, traced
+from .hip_kernels import _mask_bytes, _require_device, address, device_guard, refuse_tangents, traced
 
 _ACT = {None: 0, "silu": 1}
 
@@ -170,6 +170,7 @@ def short_conv(
     behind a sequence's length is 0 and x there is not read.
     """
     lengths, state = _conv_args(x, weight, bias, initial_state, lengths, activation)
+    refuse_tangents(x, weight, bias, state)
     if traced(x):
         return torch.ops.verace.short_conv(x, weight, bias, state, lengths, activation)
     act = _ACT[activation]
@@ -189,6 +190,15 @@ def short_conv_step_(
     """One token of :func:`short_conv` per item with the state [batch, K - 1, C] (contiguous, x's dtype)
     moved up a row in place.  x: [batch, 1, C] or [batch, C].  Items whose ``active_mask`` [batch] is off
     keep their state and give zeros.  Returns y [batch, 1, C].  Not differentiable."""
+    refuse_tangents(x, weight, bias, state)
+    if traced(x):
+        _conv_step_check(x, weight, bias, state, activation, active_mask)
+        return torch.ops.verace.short_conv_step_(x, weight, bias, state, activation, active_mask)
+    return _launch_conv_step(x, weight, bias, state, activation, active_mask)
+
+
+def _conv_step_check(x, weight, bias, state, activation, active_mask):
+    """(B, K - 1, C) of a step's arguments."""
     _conv_check(x, weight, bias, activation)
     B, K1, C = state.shape if state.dim() == 3 else (-1, -1, -1)
     if K1 != weight.shape[1] - 1 or C != x.shape[-1] or state.dtype != x.dtype or not state.is_contiguous():
@@ -197,8 +207,11 @@ def short_conv_step_(
     if tuple(x.shape) not in ((B, 1, C), (B, C)):
         raise RuntimeError(f"verace_amd: x must hold one token for each of {B} items, got {tuple(x.shape)}")
     _same_device(x, state=state, active_mask=active_mask)
-    if traced(x):
-        return torch.ops.verace.short_conv_step_(x, weight, bias, state, activation, active_mask)
+    return B, K1, C
+
+
+def _launch_conv_step(x, weight, bias, state, activation, active_mask):
+    B, K1, C = _conv_step_check(x, weight, bias, state, activation, active_mask)
     x2 = _inner(x.reshape(B, C), 1)
     mask = None if active_mask is None else _mask_bytes(active_mask.reshape(B))
     w = weight.contiguous()
@@ -393,6 +406,7 @@ def selective_scan(
     the backward the gradients of its chunk's other tokens and of earlier ones.  The backward takes rows up to 2^23
     elements apart.
     """
+    refuse_tangents(x, delta, A, B, C, D, delta_bias, initial_state)
     if traced(x):
         _scan_check(x, delta, A, B, C, D, delta_bias)
         _state_check(x, initial_state, B.shape[-1])
@@ -422,6 +436,15 @@ def selective_step_(
     contiguous) updated in place.  x: [batch, 1, num_heads, head_dim] and delta, B, C alike, or all without
     the time dimension.  Items whose ``active_mask`` [batch] is off keep their state and give zeros.
     Returns y [batch, 1, num_heads, head_dim].  Only for callers that own the state; not differentiable."""
+    refuse_tangents(x, delta, A, B, C, state, D, delta_bias)
+    if traced(x):
+        x, delta, A, B, C, D, delta_bias = _step_check(x, delta, A, B, C, state, D, delta_bias, active_mask)[:7]
+        return torch.ops.verace.selective_step_(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+    return _launch_selective_step(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+
+
+def _step_check(x, delta, A, B, C, state, D, delta_bias, active_mask):
+    """x, delta, A, B, C, D, delta_bias of a step as the launcher takes them, and the sizes."""
     if x.dim() == 3:
         x, delta, B, C = x.unsqueeze(1), delta.unsqueeze(1), B.unsqueeze(1), C.unsqueeze(1)
     b, T, H, P, G, N = _scan_check(x, delta, A, B, C, D, delta_bias)
@@ -434,8 +457,11 @@ def selective_step_(
                            f"got {tuple(state.shape)} {state.dtype}")
     _same_device(x, state=state, active_mask=active_mask)
     A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
-    if traced(x):
-        return torch.ops.verace.selective_step_(x, delta, A, B, C, state, D, bias, softplus, active_mask)
+    return x, delta, A, B, C, D, bias, (b, H, P, G, N)
+
+
+def _launch_selective_step(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask):
+    x, delta, A, B, C, D, bias, (b, H, P, G, N) = _step_check(x, delta, A, B, C, state, D, delta_bias, active_mask)
     x, delta, B, C = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2)
     mask = None if active_mask is None else _mask_bytes(active_mask.reshape(b))
     y = torch.empty(b, 1, H, P, device=x.device, dtype=x.dtype)
