@@ -45,6 +45,12 @@ def _lengths(lengths: Optional[torch.Tensor], B: int, like: torch.Tensor) -> Opt
     return lengths.contiguous()
 
 
+def _own_state(state: torch.Tensor) -> None:
+    """A state that a step may overwrite: not one that autograd follows."""
+    if state.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("verace_amd: a state that requires grad cannot be updated in place (use the prompt form, or no_grad)")
+
+
 def _inner(t: torch.Tensor, lead: int) -> torch.Tensor:
     """t with everything after its first ``lead`` dimensions contiguous (a copy only if it is not)."""
     if t.is_contiguous():
@@ -189,12 +195,16 @@ def short_conv_step_(
 ) -> torch.Tensor:
     """One token of :func:`short_conv` per item with the state [batch, K - 1, C] (contiguous, x's dtype)
     moved up a row in place.  x: [batch, 1, C] or [batch, C].  Items whose ``active_mask`` [batch] is off
-    keep their state and give zeros.  Returns y [batch, 1, C].  Not differentiable."""
+    keep their state and give zeros.  Returns y [batch, 1, C].  Not differentiable; a backward of a call that
+    took this state raises, as after any in-place operation."""
     refuse_tangents(x, weight, bias, state)
+    _own_state(state)
     if traced(x):
         _conv_step_check(x, weight, bias, state, activation, active_mask)
         return torch.ops.verace.short_conv_step_(x, weight, bias, state, activation, active_mask)
-    return _launch_conv_step(x, weight, bias, state, activation, active_mask)
+    y = _launch_conv_step(x, weight, bias, state, activation, active_mask)
+    torch.autograd.graph.increment_version(state)
+    return y
 
 
 def _conv_step_check(x, weight, bias, state, activation, active_mask):
@@ -435,12 +445,16 @@ def selective_step_(
     """One token of :func:`selective_scan` per item with ``state`` [batch, num_heads, head_dim, N] (float32,
     contiguous) updated in place.  x: [batch, 1, num_heads, head_dim] and delta, B, C alike, or all without
     the time dimension.  Items whose ``active_mask`` [batch] is off keep their state and give zeros.
-    Returns y [batch, 1, num_heads, head_dim].  Only for callers that own the state; not differentiable."""
+    Returns y [batch, 1, num_heads, head_dim].  Only for callers that own the state; not differentiable, and a backward
+    of a call that took this state raises, as after any in-place operation."""
     refuse_tangents(x, delta, A, B, C, state, D, delta_bias)
+    _own_state(state)
     if traced(x):
         x, delta, A, B, C, D, delta_bias = _step_check(x, delta, A, B, C, state, D, delta_bias, active_mask)[:7]
         return torch.ops.verace.selective_step_(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
-    return _launch_selective_step(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+    y = _launch_selective_step(x, delta, A, B, C, state, D, delta_bias, softplus, active_mask)
+    torch.autograd.graph.increment_version(state)
+    return y
 
 
 def _step_check(x, delta, A, B, C, state, D, delta_bias, active_mask):
