@@ -63,6 +63,14 @@ def _inner(t: torch.Tensor, lead: int) -> torch.Tensor:
     return t
 
 
+_MAX_ROW = 1 << 23  # elements between tokens that the chunk kernels' 32-bit offsets reach
+
+
+def _near(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where its tokens lie further apart than the backward takes."""
+    return t if t.stride(1) <= _MAX_ROW else t.clone(memory_format=torch.contiguous_format)
+
+
 # ------------------------------------------------------------------------------------ short convolution
 
 def _conv_check(x, weight, bias, activation):
@@ -333,7 +341,8 @@ def launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D=None, delta_bias=None
     _state_check(x, d_state, N, "d_state")
     state, d_state = (None if t is None else t.to(torch.float32).contiguous() for t in (initial_state, d_state))
     A, D, bias = (_head_vector(t, H, n) for t, n in ((A, "A"), (D, "D"), (delta_bias, "delta_bias")))
-    x, delta, B, C, dy = _inner(x, 2), _inner(delta, 2), _inner(B, 2), _inner(C, 2), _inner(dy, 2)
+    x, B, C, dy = (_near(_inner(t, 2)) for t in (x, B, C, dy))
+    delta = _inner(delta, 2)
 
     def new(like, dtype=None):
         return torch.empty(like.shape, device=x.device, dtype=dtype or like.dtype)
@@ -363,12 +372,18 @@ def launch_selective_hip_scan_bwd(x, delta, A, B, C, dy, D=None, delta_bias=None
     return dx, dd.view(shape), heads[0], dB, dC, heads[1], heads[2], d0
 
 
+def _rows_fit(x: torch.Tensor, B: torch.Tensor) -> None:
+    if x.dim() == 4 and B.dim() == 4 and max(x.shape[2] * x.shape[3], B.shape[2] * B.shape[3]) > _MAX_ROW:
+        raise RuntimeError(f"verace_amd: selective_scan is differentiable up to {_MAX_ROW} elements a token in x, B and C")
+
+
 class SelectiveScanFunction(torch.autograd.Function):
     """:func:`selective_scan` as an autograd node: only the inputs are kept, the backward makes the states of
     every chunk again."""
 
     @staticmethod
     def forward(ctx, x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths):
+        _rows_fit(x, B)
         y, state = launch_selective_hip_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state, lengths)
         ctx.save_for_backward(x, delta, A, B, C, D, delta_bias, initial_state, lengths)
         ctx.softplus = softplus
@@ -413,8 +428,8 @@ def selective_scan(
 
     bf16: each term of y and of the gradients of x, B and C is taken to 2^-16 of itself; the states and the other gradients
     are fp32 sums of the inputs as they are.  A NaN or an infinity in a token reaches no earlier output, but in
-    the backward the gradients of its chunk's other tokens and of earlier ones.  The backward takes rows up to 2^23
-    elements apart.
+    the backward the gradients of its chunk's other tokens and of earlier ones.  Tokens more than 2^23 elements apart run
+    token by token, and the backward takes a copy of them; a token of more than 2^23 elements has no backward.
     """
     refuse_tangents(x, delta, A, B, C, D, delta_bias, initial_state)
     if traced(x):
@@ -422,6 +437,9 @@ def selective_scan(
         _state_check(x, initial_state, B.shape[-1])
         for name, t in (("A", A), ("D", D), ("delta_bias", delta_bias)):
             _head_vector(t, x.shape[2], name)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                           for t in (x, delta, A, B, C, D, delta_bias, initial_state)):
+            _rows_fit(x, B)
         return torch.ops.verace.selective_scan(x, delta, A, B, C, D, delta_bias, softplus, initial_state,
                                                _lengths(lengths, x.shape[0], x))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
