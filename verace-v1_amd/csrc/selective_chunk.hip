@@ -60,10 +60,14 @@ __global__ __launch_bounds__(NTH) void prep_kernel(Args a, float* __restrict__ d
   const int64_t bc = unit / a.H;
   const int b = static_cast<int>(bc / nch), n = static_cast<int>(bc - static_cast<int64_t>(b) * nch), t = n * LC + l;
   float d = 0.f;
-  if (t < length_of(a.lengths, a.lengths64, a.T, b))
+  double c = 0.0;
+  if (t < length_of(a.lengths, a.lengths64, a.T, b)) {
     d = step_size(load_scalar(a.delta, a.delta_dtype, b * a.d_b + t * a.d_t + h) + (a.bias == nullptr ? 0.f : a.bias[h]),
                   a.softplus);
-  double c = static_cast<double>(d) * static_cast<double>(a.A[h]);
+    c = static_cast<double>(d) * static_cast<double>(a.A[h]);
+    // e^-10000 is 0 like e^-inf, and a chunk's sums of it stay finite: an infinite one has no differences (a NaN stays one)
+    if (c < -1e4) c = -1e4;
+  }
 #pragma unroll
   for (int off = 1; off < LC; off <<= 1) {
     const double up = __shfl_up(c, off, LC);
