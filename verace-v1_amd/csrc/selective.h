@@ -7,6 +7,7 @@
 
 #include "vmi_common.h"
 #include "vmi_dispatch.h"
+#include "vmi_vec.h"
 
 namespace vmi {
 namespace sel {
@@ -24,12 +25,6 @@ struct Args {
   int B, T, H, P, G, N;
 };
 
-__device__ __forceinline__ int length_of(const void* lengths, int lengths64, int T, int b) {
-  if (lengths == nullptr) return T;
-  const int64_t n = lengths64 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
-  return static_cast<int>(n < 0 ? 0 : n > T ? T : n);
-}
-
 // The step size: softplus(z) = max(z, 0) + log1p(exp(-|z|)) with the library's functions (a few per token
 // and head), or z itself.
 __device__ __forceinline__ float step_size(float z, int softplus) {
@@ -37,10 +32,9 @@ __device__ __forceinline__ float step_size(float z, int softplus) {
   const float m = z > 0.f ? z : z != z ? z : 0.f;
   return m + log1pf(expf(-fabsf(z)));
 }
-// d step_size / dz
-__device__ __forceinline__ float step_slope(float z, int softplus) {
-  return softplus ? 1.f / (1.f + expf(-z)) : 1.f;
-}
+
+// Workspace pieces start at multiples of 16 bytes.
+inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // selective_seq.hip: token by token, any sizes with N <= 256.
 int launch_seq(const Args& a, int dtype, hipStream_t stream);

@@ -38,7 +38,6 @@
 #include <type_traits>
 
 #include "selective_mfma.h"
-#include "vmi_vec.h"
 
 namespace vmi {
 namespace sel {
@@ -771,7 +770,6 @@ __global__ __launch_bounds__(SNT) void reduce_kernel(Bwd k, int heads, int64_t e
 namespace {
 
 int bwd_tokens(int dtype, int64_t N) { return dtype == VMI_BF16 && N <= 128 ? 64 : 32; }
-int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Plan {
   int64_t nch, tp, c_bytes, d_bytes, own_bytes, state_bytes, part_bytes, ph_bytes, tok_bytes, chk_bytes;

@@ -24,7 +24,6 @@
 #include <algorithm>
 
 #include "selective_mfma.h"
-#include "vmi_vec.h"
 
 namespace vmi {
 namespace sel {
@@ -385,7 +384,6 @@ struct Plan {
   int pblocks, seg_chunks, nseg;
   int64_t bytes() const { return d_bytes + c_bytes + state_bytes + decay_bytes; }
 };
-int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // Three workgroups a compute unit; a segment costs its state's way through memory, so it keeps four chunks, or two
 // while every workgroup has a compute unit to itself and the chunks' own latency is what counts (fp32 N64, four / two:

@@ -7,7 +7,6 @@
 #include <type_traits>
 
 #include "selective.h"
-#include "vmi_vec.h"
 
 namespace vmi {
 namespace sel {

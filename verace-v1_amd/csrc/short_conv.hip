@@ -45,12 +45,6 @@ struct Args {
   bool wide;                   // w and bias 16-byte aligned
 };
 
-__device__ __forceinline__ int length_of(const Args& a, int b) {
-  if (a.lengths == nullptr) return a.T;
-  const int64_t n = a.lengths64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
-  return static_cast<int>(n < 0 ? 0 : n > a.T ? a.T : n);
-}
-
 // N consecutive elements as they lie in memory, N = 4 or 1.
 template <typename T, int N> struct alignas(N * sizeof(T)) Raw { T e[N]; };
 template <typename T, int N> __device__ __forceinline__ Raw<T, N> raw(const T* p) {
@@ -134,7 +128,7 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   const int id = blockIdx.x * NTH + threadIdx.x, b = blockIdx.y;
   const int run = id / a.pieces, c0 = (id - run * a.pieces) * N;
   if (run > a.runs) return;
-  const int n = length_of(a, b);
+  const int n = length_of(a.lengths, a.lengths64, a.T, b);
   if (run == a.runs) {
     if (a.state_out == nullptr) return;
     float x[N];
@@ -218,7 +212,7 @@ __global__ __launch_bounds__(NTH, 3) void backward_kernel(Args a) {
   float dw[K][N] = {}, db[N] = {};
   const int t0 = run * BRUN - (K - 1), t1 = min(t0 + BRUN, a.T);  // rows of this run
   if (on && t0 < a.T) {
-    const int n = length_of(a, b);
+    const int n = length_of(a.lengths, a.lengths64, a.T, b);
     float w[K][N], bias[N], win[K][N], dz[K][N];
     weights<T, K, N>(a, c0, w, bias);
 #pragma unroll

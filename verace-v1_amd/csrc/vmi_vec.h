@@ -61,6 +61,13 @@ __device__ __forceinline__ void store_piece(T* row, int i0, int d, bool vec, con
   }
 }
 
+// How many of item b's T tokens count: its length within 0 .. T, or all.
+__device__ __forceinline__ int length_of(const void* lengths, int lengths64, int T, int b) {
+  if (lengths == nullptr) return T;
+  const int64_t n = lengths64 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
+  return static_cast<int>(n < 0 ? 0 : n > T ? T : n);
+}
+
 // sigmoid: the library's exp and a full division for an fp32 result, v_exp_f32 and v_rcp_f32 (a few
 // 2^-24 relative) for a 16-bit one.
 template <typename T> __device__ __forceinline__ float sigmoid_for(float x) {
