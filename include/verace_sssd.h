@@ -474,8 +474,10 @@ int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_batch, const v
  * state_in [B, H, P, N] (NULL: zeros) is not written and must not be state_out.  lengths as for the
  * convolution; y [B, T, H, P] (or NULL) behind them is 0.  N <= 256, P <= 1024, H / G whole.
  * fp32 and fp16 inputs run in fp32; with bf16 inputs the terms of y are two bf16 parts (2^-16 of a term), the
- * states fp32 sums.  A NaN or an infinity in a token reaches no earlier one.  Calls of a few tokens, and
- * rows that lie backwards or more than 2^23 elements apart, run token by token.
+ * states fp32 sums.  A NaN or an infinity in a token reaches no earlier one, and nothing behind the length.  Log
+ * decays below -10000 a token count as -10000 (both give 0); growth by e^88 or more over a chunk or a segment of
+ * chunks gives NaN.  Calls of a few tokens, and rows that lie backwards or more than 2^23 elements apart, run token
+ * by token.
  * The step takes one token per item and updates `state` in place (items with mask[b] = 0 keep theirs and
  * give zeros). */
 int vmi_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N,

@@ -16,7 +16,9 @@
 // one wave (two 16-byte pieces a lane at most: rows of up to 1024 16-bit elements, no barrier), longer
 // ones by a workgroup.  The weights' gradients are kept in registers over the rows that a workgroup takes
 // and leave it as one partial row each; a second kernel adds the partials in a fixed order.  bf16 rows of 1024:
-// forward 18.8 us at 84 MB (4.5 TB/s), 79 us and backward 164 us at 872 MB together (3.6 TB/s).
+// forward 18.8 us at 84 MB (4.5 TB/s), 79 us and backward 164 us at 872 MB together (3.6 TB/s).  The 16-bit backward holds
+// five inputs of a row and the next one's: three workgroups a compute unit leave 168 registers for rows of up to 2048
+// elements, and 10 to 28 spill (unaligned rows 37 to 70); above 4096 about 95 (250).
 #include <algorithm>
 #include <type_traits>
 

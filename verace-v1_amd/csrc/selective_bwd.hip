@@ -27,13 +27,15 @@
 //   reduce_kernel: the head blocks' dB and dC and the heads' dA, dD, dbias, in a fixed order.
 //
 // bf16 inputs: Q and M, and G_L where it enters dx, are two bf16 parts (2^-16 of a term: dx, dB and dC are off by their
-// own rounding and no more; one part each saves 28 us below and puts their distance to 64 bits from 1.66e-3 to 2.3e-3);
+// own rounding and no more; one part each saves 25 us below and puts their distance to 64 bits from 1.66e-3 to 2.3e-3);
 // S_0 and G_L enter alpha, beta, dB and dC as three bf16 parts and R stays fp32, because ddelta, dA and dbias may be
 // fp32 and are sums in which such roundings do not cancel.
 //
-// B4 T2048 H32 P64 N128 bf16, us: main 146 (one workgroup a compute unit, two waves a SIMD), states 77 (268 MB of S_0 and
-// G_L written: 57 at the copy rate), steps 7.5, prep 7, reduce 5.9.  A chunk of 64 halves the states' traffic against 32;
-// above 128 state columns its accumulators and parts fit neither the registers nor LDS, so there it is 32.
+// B4 T2048 H32 P64 N128 bf16, us: main 143 (one workgroup a compute unit, two waves a SIMD: of 303k clocks VALU 115k, matrix
+// 50k; LDS 124k a compute unit, 44k of them bank conflicts), states 78 (268 MB of S_0 and G_L written: 57 at the copy rate),
+// steps 7.6, prep 6.2, reduce 5.7.  A chunk of 64 halves the states' traffic against 32; above 128 state columns its
+// accumulators and parts fit neither the registers nor LDS (193 spilled registers with one part; 18 in chunks of 32), so
+// there it is 32 (forward and backward at B2 T2048 H32 P64 N256 482 us for 504).
 #include <algorithm>
 #include <type_traits>
 

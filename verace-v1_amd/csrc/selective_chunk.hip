@@ -17,10 +17,12 @@
 // or below the diagonal, and they pass through LDS as fragments.
 // With bf16 inputs the decayed scores and the carried state enter y's products as two bf16 parts (2^-16 of a term at
 // most: y is off by its own rounding and no more; one part each puts its distance to 64 bits from 1.66e-3 to 2.1e-3 and
-// saves 7 of 76 us), the weighted x of the state's update as three, so the state itself is carried in fp32 throughout.
+// saves 4 of 73 us), the weighted x of the state's update as three, so the state itself is carried in fp32 throughout.
 //
-// Bound by instruction issue: B4 T2048 H32 P64 N128 bf16, 76 us (76 MB would move in 15); each launch by itself under the
-// profiler: outputs 48.3, own states 22.4, carry 7.3, prep 5.6.  Three workgroups a compute unit.
+// Bound by instruction issue: B4 T2048 H32 P64 N128 bf16, 73 us (76 MB would move in 15).  Under the profiler, which counts
+// each launch by itself: outputs 55 (of its 104k clocks a SIMD 49k issue VALU and 24k matrix instructions), own states 22.6,
+// prep 5.4.  Three workgroups a compute unit.  At 256 state columns the pass with outputs spills: 44 to 50 registers in
+// fp32, 2 to 4 in the 16-bit types.
 #include <algorithm>
 
 #include "selective_mfma.h"
@@ -33,9 +35,9 @@ constexpr int L = 32;        // tokens of a chunk
 constexpr int PB = 64;       // rows p of a workgroup
 constexpr int MAX_SEG = 64;
 // Up to here a workgroup of the last pass runs over the earlier segments' states itself, from here on carry_kernel does,
-// a read for each state in place of one for each pair (T2048 H32 P64 N128, carried / run over, us: 3 segments 121 /
-// 115, 6 73 / 73, 8 62 / 66).
-constexpr int MAX_FOLD = 4;
+// a read for each state in place of one for each pair (bf16 T2048 H32 P64 N128, carried / run over, us: 3 segments 120 /
+// 114, 6 75 / 73, 8 65 / 68, 12 54 / 62).
+constexpr int MAX_FOLD = 6;
 
 struct Chunks {
   Args a;
@@ -452,8 +454,8 @@ int launch_prep(const Args& a, int tokens, float* d, float2* c, int nch, hipStre
   return hip_status(hipGetLastError());
 }
 
-// us of a call, token by token / in chunks (H32 P64 N128): bf16 B64 T4 41 / 42, T8 64 / 42; B8 T8 17.5 / 19.5,
-// T12 23 / 19.5; B1 T12 18 / 19.8, T15 22 / 19.8.  fp32 B64 T12 67 / 60; B1 T15 19 / 20.  Many tokens' states
+// us of a call from a held state, token by token / in chunks (H32 P64 N128): bf16 B64 T4 41 / 38, T8 65 / 38; B8 T8 17 /
+// 20, T12 24 / 20; B1 T12 18 / 20, T15 22 / 21.  fp32 B64 T12 71 / 57; B1 T15 19 / 20.  Many tokens' states
 // make a token by token call wait on memory, so the chunks pay sooner.
 bool use_chunk(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
   return T >= (dtype == VMI_BF16 && B * H * P * N >= (1 << 22) ? 5 : 12);
