@@ -34,7 +34,7 @@
 // B4 T2048 H32 P64 N128 bf16, us: main 143 (one workgroup a compute unit, two waves a SIMD: of 303k clocks VALU 115k, matrix
 // 50k; LDS 124k a compute unit, 44k of them bank conflicts), states 78 (268 MB of S_0 and G_L written: 57 at the copy rate),
 // steps 7.6, prep 6.2, reduce 5.7.  A chunk of 64 halves the states' traffic against 32; above 128 state columns its
-// accumulators and parts fit neither the registers nor LDS (193 spilled registers with one part; 18 in chunks of 32), so
+// accumulators and parts fit neither the registers nor LDS (193 spilled registers with one part; 5 in chunks of 32), so
 // there it is 32 (forward and backward at B2 T2048 H32 P64 N256 482 us for 504).
 #include <algorithm>
 #include <type_traits>
@@ -489,9 +489,10 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           if (tile / (GR / 16) != hh || (NT < NW && tt0 != 0)) continue;
 #pragma unroll
           for (int w = 0; w < 4; w += 2) {
-            const f32x4 v[2] = {g1[j][w], g1[j][w + 1]};
+            f32x4 v[2] = {g1[j][w], g1[j][w + 1]};
+            asm volatile("" : "+v"(v[0]), "+v"(v[1]));  // rounded again: the products' parts held until here would spill
             Frag<E> part[TERM];
-            split<E>(v, part);
+            split<E, TERM, true>(v, part);
 #pragma unroll
             for (int k = 0; k < TERM; ++k) {
               E* o = Gs[k] + TX::at(16 * (tile % (GR / 16)) + l16) + 16 * w + 4 * g;

@@ -105,7 +105,8 @@ template <typename E> struct Parts {
   static constexpr int ALL = sizeof(E) == 2 ? 3 : 1;
   static constexpr int TERM = sizeof(E) == 2 ? 2 : 1;
 };
-template <typename E, int M>
+// ALONE: the values are rows of different results, so none may see another's NaN.
+template <typename E, int M, bool ALONE = false>
 __device__ __forceinline__ void split(const f32x4 (&x)[2], Frag<E> (&f)[M]) {
   if constexpr (sizeof(E) == 2) {
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -126,6 +127,11 @@ __device__ __forceinline__ void split(const f32x4 (&x)[2], Frag<E> (&f)[M]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t both = q[i];
+        if constexpr (ALONE) {
+          r[2 * i] -= __uint_as_float(both << 16);
+          r[2 * i + 1] -= __uint_as_float(both & 0xffff0000u);
+          continue;
+        }
         const bf16x2 pair = __builtin_bit_cast(bf16x2, both);
         r[2 * i] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, first), r[2 * i], false);
         r[2 * i + 1] = __builtin_amdgcn_fdot2_f32_bf16(pair, __builtin_bit_cast(bf16x2, second), r[2 * i + 1], false);

@@ -427,8 +427,9 @@ def selective_scan(
     float32); y behind a sequence's length is 0 and nothing of the inputs there is used.
 
     bf16: each term of y and of the gradients of x, B and C is taken to 2^-16 of itself; the states and the other gradients
-    are fp32 sums of the inputs as they are.  A NaN or an infinity in a token reaches no earlier output, but in
-    the backward the gradients of its chunk's other tokens and of earlier ones.  Tokens more than 2^23 elements apart run
+    are fp32 sums of the inputs as they are.  A NaN or an infinity in a token reaches no earlier output and no
+    other row of its head (bf16: an infinity may come out as NaN), but in the backward the gradients of its chunk's other
+    tokens and of earlier ones.  Tokens more than 2^23 elements apart run
     token by token, and the backward takes a copy of them; a token of more than 2^23 elements has no backward.
     """
     refuse_tangents(x, delta, A, B, C, D, delta_bias, initial_state)
