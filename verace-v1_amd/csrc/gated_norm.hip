@@ -40,7 +40,7 @@ struct Args {
   const void *ds, *dn;                   // backward: gradients of s and n, contiguous (or null)
   void *dy, *dres, *dgate;               // contiguous (or null)
   float* partial;                        // [blocks][3][d]: dw1, dscale, dw2 (or null)
-  int64_t rows;
+  int64_t rows, row0;                    // row0: the launch's first
   int d, silu;
   float eps1, eps2;
   bool vec, wide;
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(NTH) void forward_kernel(Args a) {
   constexpr int N = Vec<T>::N;
   __shared__ float red[NTH / 64];
   const int lane = threadIdx.x % G, d = a.d;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (NTH / G) + threadIdx.x / G;
+  const int64_t row = a.row0 + static_cast<int64_t>(blockIdx.x) * (NTH / G) + threadIdx.x / G;
   if (row >= a.rows) return;  // whole waves (G = 64) or never
   const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
   const T* res = static_cast<const T*>(a.res) + row * a.r_stride;
@@ -403,10 +403,15 @@ extern "C" int vmi_gated_norm(const void* y, int64_t y_stride, const void* resid
       using W = decltype(wtag);
       return by_row<T, false>(a.d, [&](auto g, auto nv) -> int {
         constexpr int per = NTH / decltype(g)::value;
-        hipLaunchKernelGGL((forward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
-                           dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(NTH), 0,
-                           static_cast<hipStream_t>(stream), a);
-        return hip_status(hipGetLastError());
+        constexpr int64_t most = (UINT32_MAX / NTH) * static_cast<int64_t>(per);  // rows of a launch
+        for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
+          const int64_t n = std::min(most, rows - a.row0);
+          hipLaunchKernelGGL((forward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
+                             dim3(static_cast<unsigned>((n + per - 1) / per)), dim3(NTH), 0,
+                             static_cast<hipStream_t>(stream), a);
+          if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+        }
+        return VMI_OK;
       });
     });
   });

@@ -811,7 +811,7 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
   const Args& a = k.a;
   const int64_t BHP = static_cast<int64_t>(a.B) * a.H * p.pblocks, wgs = BHP * p.nseg;
   const int64_t blocks = static_cast<int64_t>(a.B) * p.nch * a.G * p.hblocks;
-  if (wgs > INT32_MAX || blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(wgs, SNT) || !grid_fits(blocks, MNT)) return VMI_ERR_UNSUPPORTED;
   auto ok = [](int& st) { return (st = hip_status(hipGetLastError())) == VMI_OK; };
   int st = launch_prep(a, L, const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), stream);
   if (st != VMI_OK) return st;
@@ -820,7 +820,7 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
     hipLaunchKernelGGL((states_kernel<IO, E, NP, L, true, VEC>), grid, dim3(SNT), 0, stream, k);
     if (!ok(st)) return st;
     const int64_t pieces = (BHP * (NP * PB / 4) + SNT - 1) / SNT;
-    if (pieces > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    if (!grid_fits(pieces, SNT)) return VMI_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(starts_kernel<NP>, dim3(static_cast<unsigned>(pieces), 2), dim3(SNT), 0, stream, k, L);
     if (!ok(st)) return st;
   }
@@ -829,13 +829,13 @@ template <typename IO, typename E, int NP, int L, bool VEC> int run(Bwd k, const
   hipLaunchKernelGGL((main_kernel<IO, E, NP, L, VEC>), dim3(static_cast<unsigned>(blocks)), dim3(MNT), 0, stream, k);
   if (!ok(st)) return st;
   const int64_t chunks = static_cast<int64_t>(a.B) * a.H * p.nch, sb = (chunks + SNT / 64 - 1) / (SNT / 64);
-  if (sb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(sb, SNT)) return VMI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(steps_kernel<L>, dim3(static_cast<unsigned>(sb)), dim3(SNT), 0, stream, k, chunks);
   if (!ok(st)) return st;
   const int heads = (3 * a.H + 15) / 16;
   const int64_t elems = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
   const int64_t rb = heads + (p.hblocks > 1 ? (elems + 4 * SNT - 1) / (4 * SNT) : 0);
-  if (rb > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(rb, SNT)) return VMI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(reduce_kernel<IO>, dim3(static_cast<unsigned>(rb)), dim3(SNT), 0, stream, k, heads, elems);
   ok(st);
   return st;

@@ -412,7 +412,7 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
   const Args& a = k.a;
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * p.pblocks * p.nseg;
   const int64_t BH = static_cast<int64_t>(a.B) * a.H, PN = static_cast<int64_t>(a.P) * a.N;
-  if (wgs > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(wgs, NTH)) return VMI_ERR_UNSUPPORTED;
   if (const int st = launch_prep(a, L, const_cast<float*>(k.d), const_cast<float2*>(k.c), static_cast<int>(p.nch), stream);
       st != VMI_OK)
     return st;
@@ -423,7 +423,7 @@ int run(Chunks k, const Plan& p, hipStream_t stream) {
   if (p.nseg > 1 && !k.fold) {
     const bool vec = PN % 4 == 0 && aligned16({a.state_in});
     const int64_t blocks = (BH * PN / (vec ? 4 : 1) + NTH - 1) / NTH;
-    if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+    if (!grid_fits(blocks, NTH)) return VMI_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(carry_kernel, dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, stream, k.seg_state,
                        k.seg_decay, a.state_in, p.nseg, BH, PN, vec);
     if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
@@ -447,7 +447,7 @@ template <typename IO, typename E> int by_state(const Chunks& k, const Plan& p, 
 
 int launch_prep(const Args& a, int tokens, float* d, float2* c, int nch, hipStream_t stream) {
   const int64_t units = static_cast<int64_t>(a.B) * a.H * nch, blocks = (units + NTH / tokens - 1) / (NTH / tokens);
-  if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(blocks, NTH)) return VMI_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (tokens == 64) hipLaunchKernelGGL(prep_kernel<64>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
   else hipLaunchKernelGGL(prep_kernel<32>, grid, dim3(NTH), 0, stream, a, d, c, nch, units);
@@ -458,6 +458,8 @@ int launch_prep(const Args& a, int tokens, float* d, float2* c, int nch, hipStre
 // 20, T12 24 / 20; B1 T12 18 / 20, T15 22 / 21.  fp32 B64 T12 71 / 57; B1 T15 19 / 20.  Many tokens' states
 // make a token by token call wait on memory, so the chunks pay sooner.
 bool use_chunk(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype) {
+  // (segments only multiply the first where it is small)
+  if (!grid_fits(B * H * ((P + PB - 1) / PB), NTH) || !grid_fits(B * H * ((T + L - 1) / L) / (NTH / L) + 1, NTH)) return false;
   return T >= (dtype == VMI_BF16 && B * H * P * N >= (1 << 22) ? 5 : 12);
 }
 

@@ -121,7 +121,7 @@ int launch_seq(const Args& a, int dtype, hipStream_t stream) {
       constexpr int rows = 64 / decltype(lpr)::value * decltype(it)::value;
       const int blocks_p = (a.P + rows - 1) / rows;
       const int64_t units = static_cast<int64_t>(a.B) * a.H * blocks_p, wgs = (units + NTH / 64 - 1) / (NTH / 64);
-      if (wgs > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+      if (!grid_fits(wgs, NTH)) return VMI_ERR_UNSUPPORTED;
       hipLaunchKernelGGL((seq_kernel<T, decltype(lpr)::value, decltype(it)::value>), dim3(static_cast<unsigned>(wgs)),
                          dim3(NTH), 0, stream, a, blocks_p, units, vec_state, vec_bc);
       return hip_status(hipGetLastError());

@@ -391,7 +391,7 @@ extern "C" int vmi_short_conv(const void* x, int64_t x_stride, int64_t x_batch, 
     a.pieces = vec ? a.C / PIECE : a.C;
     a.runs = (a.T + RUN - 1) / RUN;
     const int64_t blocks = (a.pieces * (a.runs + 1LL) + NTH - 1) / NTH;
-    if (blocks > INT32_MAX / NTH) return VMI_ERR_UNSUPPORTED;
+    if (blocks > INT32_MAX / NTH) return VMI_ERR_UNSUPPORTED;  // an item's pieces are counted in 31 bits
     return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
       hipLaunchKernelGGL((forward_kernel<IO, decltype(k)::value, decltype(n)::value>),
                          dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(B)), dim3(NTH), 0, static_cast<hipStream_t>(stream), a);
@@ -462,7 +462,7 @@ extern "C" int vmi_short_conv_bwd(const void* x, int64_t x_stride, int64_t x_bat
       a.pieces = vec ? a.C / PIECE : a.C;
       a.runs = static_cast<int>(parts / B);
       const int64_t blocks = parts * ((a.pieces + CT - 1) / CT);
-      if (blocks > INT32_MAX / NTH) return VMI_ERR_UNSUPPORTED;  // as many elements as no card holds
+      if (!grid_fits(blocks, NTH)) return VMI_ERR_UNSUPPORTED;  // 2^37 elements and more
       return by_shape<IO>(a, static_cast<int>(K), vec, [&](auto k, auto n) -> int {
         hipLaunchKernelGGL((backward_kernel<IO, decltype(k)::value, decltype(n)::value>),
                            dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, s, a);

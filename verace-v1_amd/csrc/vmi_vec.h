@@ -80,6 +80,9 @@ template <typename F> inline int by_type(int dtype, F&& f) {
   if (dtype == VMI_F16) return f(f16_t{});
   return VMI_ERR_INVALID_ARG;
 }
+// Whether a grid dimension holds this many workgroups of so many threads.  Its threads are counted in 32 bits: a larger
+// launch is cut to what is left of their number, without an error.
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
 inline bool aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
