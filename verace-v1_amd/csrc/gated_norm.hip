@@ -403,15 +403,13 @@ extern "C" int vmi_gated_norm(const void* y, int64_t y_stride, const void* resid
       using W = decltype(wtag);
       return by_row<T, false>(a.d, [&](auto g, auto nv) -> int {
         constexpr int per = NTH / decltype(g)::value;
-        constexpr int64_t most = (UINT32_MAX / NTH) * static_cast<int64_t>(per);  // rows of a launch
-        for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
-          const int64_t n = std::min(most, rows - a.row0);
+        return in_launches(rows, NTH, per, [&](int64_t row0, int64_t n) -> int {
+          a.row0 = row0;
           hipLaunchKernelGGL((forward_kernel<T, W, decltype(g)::value, decltype(nv)::value>),
                              dim3(static_cast<unsigned>((n + per - 1) / per)), dim3(NTH), 0,
                              static_cast<hipStream_t>(stream), a);
-          if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
-        }
-        return VMI_OK;
+          return hip_status(hipGetLastError());
+        });
       });
     });
   });

@@ -273,13 +273,12 @@ extern "C" int vmi_situ_glu(const void* gate, const void* up, int dtype, float b
     using T = decltype(tag);
     constexpr int N = Vec<T>::N;
     if (n % N != 0 || !aligned16({gate, up, out})) return VMI_ERR_UNSUPPORTED;
-    const int64_t nvec = n / N, blocks = (nvec + 255) / 256;
-    if (blocks > INT32_MAX) return VMI_ERR_UNSUPPORTED;
-    if (n == 0) return VMI_OK;
-    hipLaunchKernelGGL(situ_glu_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(gate),
-                       static_cast<const T*>(up), static_cast<T*>(out), beta1, beta2, nvec);
-    return hip_status(hipGetLastError());
+    return in_launches(n / N, 256, 256, [&](int64_t i, int64_t nvec) -> int {
+      hipLaunchKernelGGL(situ_glu_kernel<T>, dim3(static_cast<unsigned>((nvec + 255) / 256)), dim3(256), 0,
+                         static_cast<hipStream_t>(stream), advance<const T>(gate, i * N), advance<const T>(up, i * N),
+                         advance<T>(out, i * N), beta1, beta2, nvec);
+      return hip_status(hipGetLastError());
+    });
   });
 }
 
@@ -294,13 +293,14 @@ extern "C" int vmi_mcmoe_coef(const void* logits, const void* sigma, const void*
     if (components > 64 || rank % Vec<T>::N != 0 || rank > 4096 || !aligned16({sigma, vproj, coef}))
       return VMI_ERR_UNSUPPORTED;
     if (n > INT32_MAX) return VMI_ERR_UNSUPPORTED;
-    if (n == 0) return VMI_OK;
-    hipLaunchKernelGGL(mcmoe_coef_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(64 * GW), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(logits),
-                       static_cast<const T*>(sigma), static_cast<const T*>(vproj),
-                       static_cast<T*>(coef), static_cast<int>(top_k),
-                       static_cast<int>(components), static_cast<int>(rank));
-    return hip_status(hipGetLastError());
+    const int64_t row = components * rank;
+    return in_launches(n, 64 * GW, 1, [&](int64_t t, int64_t count) -> int {
+      hipLaunchKernelGGL(mcmoe_coef_kernel<T>, dim3(static_cast<unsigned>(count)), dim3(64 * GW), 0,
+                         static_cast<hipStream_t>(stream), advance<const T>(logits, t * components),
+                         advance<const T>(sigma, t * row), advance<const T>(vproj, t * row), advance<T>(coef, t * row),
+                         static_cast<int>(top_k), static_cast<int>(components), static_cast<int>(rank));
+      return hip_status(hipGetLastError());
+    });
   });
 }
 
@@ -314,13 +314,14 @@ extern "C" int vmi_norm_add(const void* a, const void* w1, float eps1, const voi
     using T = decltype(tag);
     if (!row_fits(d, dtype) || rows > INT32_MAX || !aligned16({a, w1, c, b, sum, w2, out}))
       return VMI_ERR_UNSUPPORTED;
-    if (rows == 0) return VMI_OK;
-    hipLaunchKernelGGL(norm_add_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(NTH), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(a),
-                       static_cast<const T*>(w1), eps1, static_cast<const T*>(c),
-                       static_cast<const T*>(b), static_cast<T*>(sum), static_cast<const T*>(w2), eps2,
-                       static_cast<T*>(out), static_cast<int>(d));
-    return hip_status(hipGetLastError());
+    return in_launches(rows, NTH, 1, [&](int64_t row, int64_t n) -> int {
+      const int64_t o = row * d;
+      hipLaunchKernelGGL(norm_add_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(NTH), 0,
+                         static_cast<hipStream_t>(stream), advance<const T>(a, o), static_cast<const T*>(w1), eps1,
+                         advance<const T>(c, o), advance<const T>(b, o), advance<T>(sum, o),
+                         static_cast<const T*>(w2), eps2, advance<T>(out, o), static_cast<int>(d));
+      return hip_status(hipGetLastError());
+    });
   });
 }
 
@@ -336,12 +337,14 @@ extern "C" int vmi_halting_update(const void* out, const void* h, void* h_next, 
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     if (!row_fits(d, dtype) || rows > INT32_MAX || !aligned16({out, h, h_next, w, final_h})) return VMI_ERR_UNSUPPORTED;
-    if (rows == 0) return VMI_OK;
-    hipLaunchKernelGGL(halting_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(NTH), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(out), static_cast<const T*>(h),
-                       static_cast<T*>(h_next), static_cast<const T*>(w), static_cast<const T*>(bias), static_cast<T*>(acc),
-                       static_cast<T*>(depth), active, still, static_cast<T*>(final_h), threshold,
-                       mode, static_cast<int>(d));
-    return hip_status(hipGetLastError());
+    return in_launches(rows, NTH, 1, [&](int64_t row, int64_t n) -> int {
+      const int64_t o = row * d;
+      hipLaunchKernelGGL(halting_kernel<T>, dim3(static_cast<unsigned>(n)), dim3(NTH), 0,
+                         static_cast<hipStream_t>(stream), advance<const T>(out, o), advance<const T>(h, o),
+                         advance<T>(h_next, o), static_cast<const T*>(w), static_cast<const T*>(bias), advance<T>(acc, row),
+                         advance<T>(depth, row), active + row, advance<uint8_t>(still, row), advance<T>(final_h, o), threshold,
+                         mode, static_cast<int>(d));
+      return hip_status(hipGetLastError());
+    });
   });
 }

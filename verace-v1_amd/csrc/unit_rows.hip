@@ -10,6 +10,7 @@
 // alignment take element loads.
 #include "vmi_common.h"
 #include "vmi_dispatch.h"
+#include "vmi_vec.h"
 
 namespace vmi {
 namespace unit {
@@ -98,16 +99,18 @@ hipError_t launch(const void* x, const void* g, void* out, int64_t rows, int D, 
   while (G < 64 && 4 * G < D) G *= 2;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out);
   const bool vec = D % 4 == 0 && bits % 16 == 0;
-  const int64_t per = NTH / G, blocks = (rows + per - 1) / per;
-  if (backward)
-    hipLaunchKernelGGL((unit_rows_kernel<X, Y, true>), dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0,
-                       stream, static_cast<const X*>(x), static_cast<const Y*>(g), static_cast<X*>(out),
-                       nullptr, rows, D, G, eps, vec);
-  else
-    hipLaunchKernelGGL((unit_rows_kernel<X, Y, false>), dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0,
-                       stream, static_cast<const X*>(x), nullptr, nullptr, static_cast<Y*>(out), rows, D,
-                       G, eps, vec);
-  return hipGetLastError();
+  const int64_t per = NTH / G;
+  return static_cast<hipError_t>(in_launches(rows, NTH, per, [&](int64_t row, int64_t n) -> int {
+    const unsigned blocks = static_cast<unsigned>((n + per - 1) / per);
+    const int64_t o = row * D;
+    if (backward)
+      hipLaunchKernelGGL((unit_rows_kernel<X, Y, true>), dim3(blocks), dim3(NTH), 0, stream, advance<const X>(x, o),
+                         advance<const Y>(g, o), advance<X>(out, o), nullptr, n, D, G, eps, vec);
+    else
+      hipLaunchKernelGGL((unit_rows_kernel<X, Y, false>), dim3(blocks), dim3(NTH), 0, stream, advance<const X>(x, o),
+                         nullptr, nullptr, advance<Y>(out, o), n, D, G, eps, vec);
+    return hipGetLastError();
+  }));
 }
 
 int run(const void* x, int x_dtype, const void* g, int y_dtype, void* out, int64_t rows, int64_t D,

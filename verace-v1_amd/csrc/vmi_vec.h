@@ -83,6 +83,17 @@ template <typename F> inline int by_type(int dtype, F&& f) {
 // Whether a grid dimension holds this many workgroups of so many threads.  Its threads are counted in 32 bits: a larger
 // launch is cut to what is left of their number, without an error.
 inline bool grid_fits(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
+// f(first, count) over n units in runs that a grid holds, `per` of them a workgroup of so many threads.
+template <typename F> inline int in_launches(int64_t n, int threads, int64_t per, F&& f) {
+  const int64_t most = UINT32_MAX / threads * per;
+  for (int64_t i = 0; i < n; i += most)
+    if (const int st = f(i, n - i < most ? n - i : most); st != 0) return st;
+  return 0;
+}
+// p, `elements` further on (null stays null).
+template <typename T> inline T* advance(const void* p, int64_t elements) {
+  return p == nullptr ? nullptr : static_cast<T*>(const_cast<void*>(p)) + elements;
+}
 inline bool aligned16(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
