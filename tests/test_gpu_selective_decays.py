@@ -58,8 +58,7 @@ def test_gradients(device, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_an_infinite_step(device, dtype):
-    """It forgets the state before it and adds nothing where x is zero... which is 0 times infinity: NaN from there on in
-    its head, as in the recurrence, and nothing else changes."""
+    """Its head's outputs and states are not finite from there on, as in the recurrence; nothing else changes."""
     from verace_amd import selective_scan
     d, state = inputs(device, 1, 100, 2, 32, 1, 32, dtype, seed=113, delta_dtype=torch.float32)
     d["delta"][0, 40, 1] = float("inf")
