@@ -267,6 +267,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
   typedef Tile<E, L> TQ;
+  constexpr int QE = TQ::elems(L), GE = TX::elems(GR);
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
   __shared__ __attribute__((aligned(16))) E Cs[TB::elems(L)];
   // x, dy and the log decays of a unit while the next one's arrive
@@ -275,9 +276,9 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
   __shared__ __attribute__((aligned(16))) E Yb[2][TX::elems(L)];
   __shared__ __attribute__((aligned(16))) float2 cb2[2][L];
   __shared__ __attribute__((aligned(16))) float db2[2][L], eb2[2][L], wb2[2][L], dh2[2];
-  __shared__ __attribute__((aligned(16))) E Qs[TERM][TQ::elems(L)];   // [t][s]
-  __shared__ __attribute__((aligned(16))) E Ms[TERM][TQ::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Gs[TERM][TX::elems(GR)];  // G_L^T [n][p]
+  __shared__ __attribute__((aligned(16))) E Qs[TERM * QE];            // [t][s], part by part
+  __shared__ __attribute__((aligned(16))) E Ms[TERM * QE];
+  __shared__ __attribute__((aligned(16))) E Gs[TERM * GE];            // G_L^T [n][p]
   __shared__ float row_r[LT][L], col_r[LT][L];                  // sums of R d_s (below) by s-tile, sum_t R by t-tile
   __shared__ float alpha[NW][L], beta[NW][L], kappa[NW], diag[LT];
   const Args& a = k.a;
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
       sc.fetch(t0, len);
       sb.commit(Bs);
       sc.commit(Cs);
-      for (int i = tid; i < TERM * TQ::elems(L); i += MNT) Qs[0][i] = Ms[0][i] = static_cast<E>(0.f);
+      for (int i = tid; i < TERM * QE; i += MNT) Qs[i] = Ms[i] = static_cast<E>(0.f);
     }
     Stage<IO, E, PB, L, MNT, VEC> sx, sy;
     float rd, rD;
@@ -410,8 +411,8 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         const int o = TQ::at(t) + 16 * st + 4 * g;
 #pragma unroll
         for (int k = 0; k < TERM; ++k) {
-          *reinterpret_cast<M4*>(Qs[k] + o) = q[k];
-          *reinterpret_cast<M4*>(Ms[k] + o) = m[k];
+          *reinterpret_cast<M4*>(Qs + k * QE + o) = q[k];
+          *reinterpret_cast<M4*>(Ms + k * QE + o) = m[k];
         }
         // left of the diagonal the rows' sums, in a tile on it each token's sum over the paths that cross it
         float rs = 0.f;
@@ -495,7 +496,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
             split<E, TERM, true>(v, part);
 #pragma unroll
             for (int k = 0; k < TERM; ++k) {
-              E* o = Gs[k] + TX::at(16 * (tile % (GR / 16)) + l16) + 16 * w + 4 * g;
+              E* o = Gs + k * GE + TX::at(16 * (tile % (GR / 16)) + l16) + 16 * w + 4 * g;
               put_half(o, part[k], 0);
               put_half(o + 16, part[k], 1);
             }
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
         for (int kb = 0; kb < GR / 32; ++kb) {
           Frag<E> gf[TERM], bf[DXT];
 #pragma unroll
-          for (int i = 0; i < TERM; ++i) gf[i] = col_frag<E, PB>(Gs[i], 32 * kb, 16 * pt, l16, g);
+          for (int i = 0; i < TERM; ++i) gf[i] = col_frag<E, PB>(Gs + i * GE, 32 * kb, 16 * pt, l16, g);
 #pragma unroll
           for (int t = 0; t < DXT; ++t) bf[t] = row_frag<E, NP>(Bs, 16 * (st0 + t), GR * hh + 32 * kb, l16, g);
 #pragma unroll
@@ -540,8 +541,8 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           for (int i = TERM - 1; i >= 0; --i)
 #pragma unroll
             for (int t = 0; t < LTW; ++t) {
-              if ((tt0 + t) / 2 >= kb) dc[j][t] = mma(bf, row_frag<E, L>(Qs[i], 16 * (tt0 + t), 32 * kb, l16, g), dc[j][t]);
-              if ((tt0 + t) / 2 <= kb) db[j][t] = mma(cf, col_frag<E, L>(Qs[i], 32 * kb, 16 * (tt0 + t), l16, g), db[j][t]);
+              if ((tt0 + t) / 2 >= kb) dc[j][t] = mma(bf, row_frag<E, L>(Qs + i * QE, 16 * (tt0 + t), 32 * kb, l16, g), dc[j][t]);
+              if ((tt0 + t) / 2 <= kb) db[j][t] = mma(cf, col_frag<E, L>(Qs + i * QE, 32 * kb, 16 * (tt0 + t), l16, g), db[j][t]);
             }
         }
       }
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(MNT) void main_kernel(Bwd k) {
           if (st / 2 > kb) continue;
           const Frag<E> yf = col_frag<E, PB>(Ys, 32 * kb, 16 * pt, l16, g);
 #pragma unroll
-          for (int i = TERM - 1; i >= 0; --i) dx[t] = mma(yf, col_frag<E, L>(Ms[i], 32 * kb, 16 * st, l16, g), dx[t]);
+          for (int i = TERM - 1; i >= 0; --i) dx[t] = mma(yf, col_frag<E, L>(Ms + i * QE, 32 * kb, 16 * st, l16, g), dx[t]);
         }
         const int p = p0 + 16 * pt + 4 * g;
         if (t0 + s < a.T && p < a.P && k.dx != nullptr) {

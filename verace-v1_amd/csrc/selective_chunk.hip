@@ -102,10 +102,11 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
   constexpr int NT = NP / 16, LT = L / 16, KN = NP / 32, NPART = Parts<E>::ALL, TERM = Parts<E>::TERM;
   typedef Tile<E, NP> TB;
   typedef Tile<E, PB> TX;
+  constexpr int MS = READOUT ? LT * 64 * 8 : 8;  // a part of the scores
   __shared__ __attribute__((aligned(16))) E Bs[TB::elems(L)];
   __shared__ __attribute__((aligned(16))) E Cs[READOUT ? RowTile<E, NP>::elems(L) : 8];
   __shared__ __attribute__((aligned(16))) E Xs[TX::elems(L)];
-  __shared__ __attribute__((aligned(16))) E Ms[TERM][READOUT ? LT * 64 * 8 : 8];
+  __shared__ __attribute__((aligned(16))) E Ms[TERM * MS];
   __shared__ __attribute__((aligned(16))) float2 cs[L];
   __shared__ __attribute__((aligned(16))) float ds[L], ws[L], es[L];
   const Args& a = k.a;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
     }
   }
   if constexpr (READOUT) {  // the tile right of the diagonal stays zero
-    for (int i = tid; i < TERM * LT * 64 * 8; i += NTH) Ms[0][i] = static_cast<E>(0.f);
+    for (int i = tid; i < TERM * MS; i += NTH) Ms[i] = static_cast<E>(0.f);
   }
   const float Dh = a.D == nullptr ? 0.f : a.D[h];
   double seg_c = 0.0;
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
           }
         }
 #pragma unroll
-        for (int i = 0; i < TERM; ++i) *reinterpret_cast<M4*>(Ms[i] + (tt * 64 + lane) * 8 + 4 * st) = q[i];
+        for (int i = 0; i < TERM; ++i) *reinterpret_cast<M4*>(Ms + i * MS + (tt * 64 + lane) * 8 + 4 * st) = q[i];
       }
       // S_0 C_t, transposed: rows p, column t
 #pragma unroll
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
           f32x4 sum = acc[t];
 #pragma unroll
           for (int i = TERM - 1; i >= 0; --i) {
-            const E* m = Ms[i] + (t * 64 + lane) * 8;
+            const E* m = Ms + i * MS + (t * 64 + lane) * 8;
             Frag<E> f;
             if constexpr (sizeof(E) == 2) {
               f.v = *reinterpret_cast<const bf16x8*>(m);
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(NTH, sizeof(E) == 2 && NP <= 128 ? 3 : 2) void pass
           }
           // a NaN or an infinity in x times a masked score's 0: in order, so that no earlier token sees it
           if (__builtin_isunordered(sum[0], sum[1]) || __builtin_isunordered(sum[2], sum[3]))
-            add_in_order<E>(Ms[0] + t * 64 * 8, LT * 64 * 8, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
+            add_in_order<E>(Ms + t * 64 * 8, MS, Xs + 16 * wave + 4 * g, 16 * t + l16, l16, acc[t]);
           else
             acc[t] = sum;
           if (y_on && c * L + 16 * t + l16 < a.T) {
