@@ -21,6 +21,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch._C import _get_tracing_state, _len_torch_dispatch_stack, _len_torch_function_stack
 
 from . import _lib
 
@@ -54,14 +55,14 @@ def address(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 _NO_GUARD = contextlib.nullcontext()
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def traced(x: torch.Tensor) -> bool:
     """Whether something sees the operators that the caller runs: torch.compile, torch.jit.trace, a dispatch or function
     mode, a tensor subclass (FakeTensor among them).  The registered operators (ops.py) then take the launchers' place."""
-    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
-            or torch._C._len_torch_dispatch_stack() != 0 or torch._C._len_torch_function_stack() != 0
-            or type(x) not in (torch.Tensor, torch.nn.Parameter))
+    return (torch.compiler.is_compiling() or _get_tracing_state() is not None or _len_torch_dispatch_stack() != 0
+            or _len_torch_function_stack() != 0 or type(x) not in _PLAIN)
 
 
 def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
