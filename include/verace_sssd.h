@@ -428,7 +428,8 @@ int vmi_halting_update(const void* out, const void* h, void* h_next, const void*
  * stats (NULL or [2][rows] floats) receives the two reciprocal roots for the backward.  d <= 8192 (F32: 4096).
  *
  * Backward: ds, dn (either may be NULL: zero) give dy, dresidual, dgate [rows, d] and dw1, dscale, dw2 [d]
- * (any may be NULL: not wanted; a workspace of the queried size is needed for the last three). */
+ * (any may be NULL: not wanted; a workspace of the queried size is needed for the last three).  gate_act + 2: dgate
+ * is fp32, for a gate whose gradient is summed further (one that was broadcast). */
 int vmi_gated_norm(const void* y, int64_t y_stride, const void* residual, int64_t r_stride,
                    const void* gate, int64_t g_stride, const void* w1, const void* scale, const void* w2,
                    int dtype, int w_dtype, int gate_act, float eps1, float eps2, void* s, void* n,

@@ -161,8 +161,21 @@ template <typename T> __device__ __forceinline__ void widen(const Vec<T>& v, flo
   for (int j = 0; j < Vec<T>::N; ++j) x[j] = io<T>::to_f32(v.e[j]);
 }
 
+template <bool VEC, int N> __device__ __forceinline__ void store_wide(float* row, int i, int d, const float (&x)[N]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < N; q += 4) *reinterpret_cast<float4*>(row + i + q) = make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j < d) row[i + j] = x[j];
+  }
+}
+
 // A workgroup takes NTH / G rows at a time, the next ones' inputs on their way meanwhile.
-template <typename T, typename W, int G, int NV, bool VEC>
+// DG32: dgate is fp32.  (A template, not a branch: that one spills three more registers, 249 us for 242 at 32768 rows of
+// 1024.)
+template <typename T, typename W, int G, int NV, bool VEC, bool DG32>
 __global__ __launch_bounds__(NTH, NV == 1 ? 3 : 1) void backward_kernel(Args a) {
   constexpr int N = Vec<T>::N, RW = NTH / G;
   __shared__ float red[NTH / 64];
@@ -266,7 +279,10 @@ __global__ __launch_bounds__(NTH, NV == 1 ? 3 : 1) void backward_kernel(Args a) 
         dt[v][j] = dr * w1;
         dot = fmaf(dt[v][j], yv[v][j], dot);
       }
-      if (a.dgate != nullptr) store_piece(static_cast<T*>(a.dgate) + row * d, i, d, VEC, q[v]);
+      if (a.dgate != nullptr) {
+        if constexpr (DG32) store_wide<VEC>(static_cast<float*>(a.dgate) + row * d, i, d, q[v]);
+        else store_piece(static_cast<T*>(a.dgate) + row * d, i, d, VEC, q[v]);
+      }
     }
     float m = 0.f;
     if (a.w1 != nullptr) m = row_sum<G>(dot, red) / d * i1 * i1 * i1;
@@ -434,7 +450,8 @@ extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* r
   a.y_stride = y_stride, a.r_stride = r_stride, a.g_stride = gate == nullptr ? 0 : g_stride;
   a.stats = const_cast<float*>(stats), a.ds = ds, a.dn = w2 == nullptr ? nullptr : dn;
   a.dy = dy, a.dres = dresidual, a.dgate = gate == nullptr ? nullptr : dgate;
-  a.rows = rows, a.d = static_cast<int>(d), a.silu = gate_act;
+  a.rows = rows, a.d = static_cast<int>(d), a.silu = gate_act & ~2;
+  const bool dgate32 = gate_act & 2;
   if (const int st = check(a, dtype, w_dtype); st != VMI_OK) return st;
   if (rows > 0 && stats == nullptr && (w1 != nullptr || a.dn != nullptr)) return VMI_ERR_INVALID_ARG;
   const bool weights = dw1 != nullptr || dscale != nullptr || dw2 != nullptr;
@@ -458,9 +475,14 @@ extern "C" int vmi_gated_norm_bwd(const void* y, int64_t y_stride, const void* r
         rc = by_row<T, true>(a.d, [&](auto g, auto nv) -> int {
           constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
           const dim3 grid(static_cast<unsigned>(blocks));
-          if (a.vec) hipLaunchKernelGGL((backward_kernel<T, W, G, NV, true>), grid, dim3(NTH), 0, st, a);
-          else hipLaunchKernelGGL((backward_kernel<T, W, G, NV, false>), grid, dim3(NTH), 0, st, a);
-          return hip_status(hipGetLastError());
+          auto go = [&](auto vec, auto wide) -> int {
+            hipLaunchKernelGGL((backward_kernel<T, W, G, NV, decltype(vec)::value, decltype(wide)::value>), grid, dim3(NTH), 0,
+                               st, a);
+            return hip_status(hipGetLastError());
+          };
+          if constexpr (sizeof(T) == 2)
+            if (dgate32) return a.vec ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
+          return a.vec ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
         });
       if (rc != VMI_OK || !weights) return rc;
       hipLaunchKernelGGL(weights_kernel<W>, dim3(static_cast<unsigned>((3 * d + 31) / 32)), dim3(1024), 0, st,

@@ -39,7 +39,7 @@ def _checked(y, residual, gate, norm_weight, scale, next_weight, activation):
         raise RuntimeError(f"verace_amd: residual shape {tuple(residual.shape)} != y shape {tuple(shape)}")
     if gate is not None and gate.shape != shape:
         try:
-            gate = gate.expand(shape)
+            gate.expand(shape)
         except RuntimeError:
             raise RuntimeError(f"verace_amd: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
     for name, t in (("residual", residual), ("gate", gate)):
@@ -58,9 +58,13 @@ def _checked(y, residual, gate, norm_weight, scale, next_weight, activation):
     return (y, residual, gate, *(None if t is None else t.contiguous() for t in (norm_weight, scale, next_weight)))
 
 
+def _gate_rows(gate: Optional[torch.Tensor], y: torch.Tensor) -> Optional[torch.Tensor]:
+    return None if gate is None else _rows(gate if gate.shape == y.shape else gate.expand(y.shape), y.shape[-1])
+
+
 def _launch(y, residual, gate, w1, scale, w2, eps1, eps2, act, want_stats):
     d = y.shape[-1]
-    y2, r2, g2 = _rows(y, d), _rows(residual, d), _rows(gate, d)
+    y2, r2, g2 = _rows(y, d), _rows(residual, d), _gate_rows(gate, y)
     s = torch.empty(y.shape, device=y.device, dtype=y.dtype)
     n = None if w2 is None else torch.empty_like(s)
     stats = torch.empty(2, y2.shape[0], device=y.device, dtype=torch.float32) if want_stats else None
@@ -76,7 +80,7 @@ def _launch(y, residual, gate, w1, scale, w2, eps1, eps2, act, want_stats):
 def _launch_bwd(y, residual, gate, w1, scale, w2, stats, act, ds, dn, need):
     """(dy, dresidual, dgate, dw1, dscale, dw2) for dL/ds and dL/dn (either may be None), None where not needed."""
     d = y.shape[-1]
-    y2, r2, g2 = _rows(y, d), _rows(residual, d), _rows(gate, d)
+    y2, r2, g2 = _rows(y, d), _rows(residual, d), _gate_rows(gate, y)
     for name, t in (("ds", ds), ("dn", None if w2 is None else dn)):
         if t is not None and (t.shape != y.shape or t.dtype != y.dtype or t.device != y.device):
             raise RuntimeError(f"verace_amd: {name} must be {tuple(y.shape)} {y.dtype} on {y.device}, "
@@ -87,6 +91,9 @@ def _launch_bwd(y, residual, gate, w1, scale, w2, stats, act, ds, dn, need):
     ds, dn = (None if t is None else t.contiguous() for t in (ds, dn))
     dy, dres, dgate = (torch.empty(y.shape, device=y.device, dtype=y.dtype) if f and t is not None else None
                        for f, t in zip(need[:3], (y, residual, gate)))
+    shared = dgate is not None and gate.shape != y.shape  # summed in fp32 over what the gate was broadcast to
+    if shared:
+        dgate = torch.empty(y.shape, device=y.device, dtype=torch.float32)
     dw1, dscale, dw2 = (torch.empty_like(t) if f and t is not None else None
                         for f, t in zip(need[3:6], (w1, scale, w2)))
     w = next((t for t in (w1, scale, w2) if t is not None), None)
@@ -100,10 +107,12 @@ def _launch_bwd(y, residual, gate, w1, scale, w2, stats, act, ds, dn, need):
     with device_guard(y):
         _lib.check(lib.vmi_gated_norm_bwd(
             address(y2), y2.stride(0), address(r2), r2.stride(0), address(g2), 0 if g2 is None else g2.stride(0),
-            address(w1), address(scale), address(w2), code, _lib.dtype_code(y.dtype if w is None else w.dtype), act,
+            address(w1), address(scale), address(w2), code, _lib.dtype_code(y.dtype if w is None else w.dtype), act | 2 * shared,
             address(stats), address(ds), address(dn), address(dy), address(dres), address(dgate), address(dw1),
             address(dscale), address(dw2), y2.shape[0], d, address(ws), ws_bytes.value, _lib.raw_stream(y.device)),
             "vmi_gated_norm_bwd")
+    if shared:
+        dgate = dgate.sum_to_size(gate.shape).to(gate.dtype)
     return dy, dres, dgate, dw1, dscale, dw2
 
 
@@ -142,7 +151,7 @@ def gated_norm_add(
     ``next_weight``.
 
     y, residual: [..., d] of one shape and dtype (rows may be slices of a wider tensor); gate: the same,
-    or broadcastable to it, through ``activation`` ("silu" or "sigmoid"); norm_weight, scale, next_weight:
+    or broadcastable to it (its gradient is then summed in fp32), through ``activation`` ("silu" or "sigmoid"); norm_weight, scale, next_weight:
     [d], all in y's dtype or all float32.  Each may be None and is then left out of the formula.
     d <= 8192 (float32: 4096).  Arithmetic is fp32 and each result is rounded once; n is formed from the
     unrounded s.  Differentiable once, in every tensor argument.
