@@ -43,7 +43,8 @@ extern "C" {
 enum vmi_dtype {
   VMI_F32 = 0,
   VMI_BF16 = 1,
-  VMI_F16 = 2
+  VMI_F16 = 2,
+  VMI_E4M3 = 3                 /* rows of the feed-forward products only, with a float32 scale each */
 };
 
 /* Status codes returned by every entry point (0 = success). */
@@ -510,6 +511,44 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
                        const float* D, const float* delta_bias, int softplus, int dtype,
                        const uint8_t* mask, float* state, void* y, int64_t B, int64_t H, int64_t P,
                        int64_t G, int64_t N, void* stream);
+
+/* Feed-forward products.  x [M, K], weights [N, K] (nn.Linear's layout), rows ldx, ldw, ... elements apart: rows start on 16
+ * bytes, and where K (N for dy) is no whole number of 16-byte pieces the rest of a row's last piece holds zeros.  A row is
+ * less than 2^24 bytes from the next; M, N, K <= 2^30.  dtype: of x and the weights; VMI_E4M3 takes a float32 scale for each
+ * row of both (the values are scale * e4m3), and bias, residual and out are then of out_dtype; otherwise out_dtype is dtype.
+ * Sums are fp32; each result is rounded once.  K = 0 is a sum of nothing.
+ *   vmi_linear_add:   out = residual + act(x w^T + bias); bias [N], residual (rows ldr apart) may be NULL;
+ *                     act 0: none, 1: z sigmoid(z), 2: z Phi(z).  out may be residual.
+ *   vmi_gated_linear: out = a(x w_gate^T) b(x w_up^T); act 1: a(z) = z sigmoid(z), b(z) = z;
+ *                     3: a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2).  ldg = ldu.
+ * Gradients from the inputs alone, for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
+ * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */
+int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
+                   const float* w_scale, int dtype, const void* bias, const void* residual, int64_t ldr,
+                   int act, void* out, int64_t ldo, int out_dtype, int64_t M, int64_t N, int64_t K,
+                   void* stream);
+int vmi_linear_add_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, size_t* bytes);
+int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const void* bias,
+                       int act, const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M,
+                       int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale, const void* w_gate, int64_t ldg,
+                     const float* gate_scale, const void* w_up, int64_t ldu, const float* up_scale, int dtype,
+                     int act, float beta1, float beta2, void* out, int64_t ldo, int out_dtype, int64_t M,
+                     int64_t F, int64_t K, void* stream);
+int vmi_gated_linear_bwd_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype, size_t* bytes);
+int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up,
+                         int64_t ldu, int dtype, int act, float beta1, float beta2, const void* dh,
+                         int64_t lddh, void* dx, void* dw, int64_t M, int64_t F, int64_t K, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm with the residual's addition and a result in 8 bits:
+ *   s = a + residual,  n = s w / sqrt(mean s^2 + eps) (norm = 0: n = s w),
+ *   scale = max(max|n| / 448, 2^-126),  q = e4m3(n / scale), each rounded once from 64 bits
+ * over rows of d elements, a_stride and r_stride apart; residual, w [d] (dtype or float32) and sum (s, dtype) may be NULL;
+ * sum, q [rows, d] and scale [rows] are contiguous.  A row with a NaN or an infinity in s w has NaN for scale and q. */
+int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* residual, int64_t r_stride, const void* w,
+                       int dtype, int w_dtype, int norm, float eps, void* sum, void* q, float* scale,
+                       int64_t rows, int64_t d, void* stream);
 
 #ifdef __cplusplus
 }

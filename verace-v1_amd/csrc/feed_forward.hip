@@ -1,0 +1,289 @@
+// The C entries of the feed-forward operators, and the two small kernels beside their products: the sum of the shares of a
+// weight's gradient and the sum of a gradient over its rows.
+//
+//   y = residual + act(x W^T + b)                              2 M N K operations
+//   h = act(x Wg^T) lin(x Wu^T)                                4 M F K
+// backward, from the inputs alone (nothing is kept by the forward):
+//   dz = dy act'(x W^T + b), dx = dz W, dW = dz^T x, db = sum dz
+//   [dg du] likewise, dx = dg Wg + du Wu, [dWg; dWu] = [dg du]^T x
+// dz is rounded once to x's type, as the matrix cores take it; products are summed in fp32.
+#include "feed_forward.h"
+
+using namespace vmi;
+using namespace vmi::prod;
+
+namespace {
+
+constexpr int NTH = 256;
+
+// out = the sum of `splits` partial results of n elements.
+template <typename T>
+__global__ __launch_bounds__(NTH) void join_kernel(const float* partial, T* out, int64_t n, int splits) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x) * 4;
+  if (i >= n) return;
+  float s[4], t[4];
+  const bool vec = n % 4 == 0;
+  load_cols<float, 4>(partial, i, n, vec, s);
+  for (int k = 1; k < splits; ++k) {
+    load_cols<float, 4>(partial + k * n, i, n, vec, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += t[j];
+  }
+  store_cols<T, 4>(out, i, n, vec, s);
+}
+
+// Column sums of [rows, n]: workgroup (b, s) those of 64 columns over the s-th share of the rows, 4 rows at a time.
+template <typename T>
+__global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, int rows, int n, int share, float* partial) {
+  __shared__ float part[4][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r0 = threadIdx.x >> 6;
+  const int first = blockIdx.y * share, last = rows - first < share ? rows : first + share;
+  float s = 0.f;
+  if (c < n)
+    for (int r = first + r0; r < last; r += 4) s += io<T>::load(x + r * ld, c);
+  part[r0][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (r0 == 0 && c < n) partial[static_cast<int64_t>(blockIdx.y) * n + c] = part[0][c & 63] + part[1][c & 63] + part[2][c & 63] + part[3][c & 63];
+}
+template <typename T>
+__global__ __launch_bounds__(NTH) void columns_join_kernel(const float* partial, int shares, int n, T* out) {
+  const int c = blockIdx.x * NTH + threadIdx.x;
+  if (c >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < shares; ++k) s += partial[static_cast<int64_t>(k) * n + c];
+  io<T>::store(out, c, s);
+}
+
+int product(int dtype, Kind kind, const Args& p, hipStream_t stream) {
+  switch (dtype) {
+    case VMI_BF16: return product_bf16(kind, p, stream);
+    case VMI_F16: return product_f16(kind, p, stream);
+    case VMI_F32: return product_f32(kind, p, stream);
+    case VMI_E4M3: return product_e4m3(kind, p, stream);
+  }
+  return VMI_ERR_INVALID_ARG;
+}
+
+int64_t size_of(int dtype) { return dtype == VMI_F32 ? 4 : dtype == VMI_E4M3 ? 1 : 2; }
+int64_t whole(int64_t n, int dtype) {  // elements of the 16-byte pieces that hold n
+  const int64_t e = 16 / size_of(dtype);
+  return (n + e - 1) / e * e;
+}
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// A matrix whose rows the tiles load in 16-byte pieces: a tile's rows lie within 31 bits of its first.
+int rows_status(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+  if (rows == 0 || cols == 0) return VMI_OK;
+  if (p == nullptr || ld < cols) return VMI_ERR_INVALID_ARG;
+  const int64_t size = size_of(dtype);
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || ld * size % 16 != 0 || ld < whole(cols, dtype)) return VMI_ERR_UNSUPPORTED;
+  return ld * size >= (INT64_C(1) << 24) ? VMI_ERR_UNSUPPORTED : VMI_OK;
+}
+bool sizes_ok(int64_t m, int64_t n, int64_t k) {
+  const int64_t most = INT64_C(1) << 30;
+  return m >= 0 && n >= 0 && k >= 0 && m <= most && n <= most && k <= most;
+}
+bool out_vectors(const void* out, int64_t ldo, const void* other, int64_t ldother, int64_t size) {
+  return aligned16({out, other}) && ldo * size % 16 == 0 && (other == nullptr || ldother * size % 16 == 0);
+}
+int first_error(std::initializer_list<int> status) {
+  for (int s : status)
+    if (s != VMI_OK) return s;
+  return VMI_OK;
+}
+
+// Shares of dW's contraction: as many as fill the compute units once with tiles of 256 x 128, each of 512 rows at least.
+struct Shares {
+  int n, length;
+};
+Shares weight_shares(int64_t rows, int64_t cols, int64_t k) {
+  const int64_t t = tiles(rows, cols, 256, 128);
+  int64_t n = t == 0 ? 1 : 256 / t;
+  const int64_t most = (k + 511) / 512;
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  int64_t length = ((k + n - 1) / n + 127) / 128 * 128;
+  if (length < 128) length = 128;
+  n = (k + length - 1) / length;
+  return {static_cast<int>(n < 1 ? 1 : n), static_cast<int>(length)};
+}
+// dW [segments * valid, cols] = dz^T x over m rows.
+int weight_gradient(const void* dz, int64_t lddz, int segments, int64_t seg, int64_t valid, const void* x, int64_t ldx,
+                    int dtype, int64_t m, int64_t cols, void* dw, float* partial, hipStream_t stream) {
+  if (valid == 0 || cols == 0) return VMI_OK;
+  const Shares s = weight_shares(segments * seg, cols, m);
+  Args p{};
+  p.a = dz, p.lda = lddz, p.b = x, p.ldb = ldx;
+  p.m = static_cast<int>(segments * seg), p.n = static_cast<int>(cols), p.k = static_cast<int>(m);
+  p.splits = s.n, p.split_k = s.length, p.seg = static_cast<int>(seg), p.seg_valid = static_cast<int>(valid);
+  p.out = dw, p.ldo = cols, p.partial = s.n > 1 ? partial : nullptr;
+  p.vec = out_vectors(dw, cols, nullptr, 0, size_of(dtype));
+  if (const int st = product(dtype, DW, p, stream); st != VMI_OK || s.n == 1) return st;
+  const int64_t n = segments * valid * cols, blocks = (n + 4 * NTH - 1) / (4 * NTH);
+  if (!grid_fits(blocks, NTH)) return VMI_ERR_UNSUPPORTED;
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(NTH), 0, stream, partial, static_cast<T*>(dw), n,
+                       s.n);
+    return hip_status(hipGetLastError());
+  });
+}
+size_t weight_bytes(int64_t rows, int64_t valid, int64_t cols, int64_t m) {
+  const Shares s = weight_shares(rows, cols, m);
+  return s.n > 1 ? align256(static_cast<size_t>(s.n) * valid * cols * 4) : 0;
+}
+int column_shares(int64_t m, int64_t n) {
+  const int64_t t = (n + 63) / 64, want = t == 0 ? 1 : (1024 + t - 1) / t, most = (m + 63) / 64;
+  const int64_t s = want < most ? want : most;
+  return static_cast<int>(s < 1 ? 1 : s);
+}
+bool gate_act(int act) { return act == ACT_SILU || act == ACT_SITU; }
+bool linear_act(int act) { return act == ACT_NONE || act == ACT_SILU || act == ACT_GELU; }
+
+}  // namespace
+
+extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
+                              int dtype, const void* bias, const void* residual, int64_t ldr, int act, void* out, int64_t ldo,
+                              int out_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  if (!sizes_ok(M, N, K) || !linear_act(act) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
+    return VMI_ERR_INVALID_ARG;
+  if (dtype != VMI_E4M3 && out_dtype != dtype) return VMI_ERR_INVALID_ARG;
+  if (M == 0 || N == 0) return VMI_OK;
+  if (out == nullptr || ldo < N || (residual != nullptr && ldr < N) || (dtype == VMI_E4M3 && (x_scale == nullptr || w_scale == nullptr)))
+    return VMI_ERR_INVALID_ARG;
+  if (const int st = first_error({rows_status(x, M, K, ldx, dtype), rows_status(w, N, K, ldw, dtype)}); st != VMI_OK) return st;
+  Args p{};
+  p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.xs = x_scale, p.ws = w_scale;
+  p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
+  p.bias = bias, p.other = residual, p.ldother = ldr, p.act = act, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
+  p.vec = out_vectors(out, ldo, residual, ldr, size_of(out_dtype));
+  return product(dtype, LINEAR, p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale, const void* w_gate, int64_t ldg,
+                                const float* gate_scale, const void* w_up, int64_t ldu, const float* up_scale, int dtype, int act,
+                                float beta1, float beta2, void* out, int64_t ldo, int out_dtype, int64_t M, int64_t F, int64_t K,
+                                void* stream) {
+  if (!sizes_ok(M, F, K) || !gate_act(act) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
+    return VMI_ERR_INVALID_ARG;
+  if (dtype != VMI_E4M3 && out_dtype != dtype) return VMI_ERR_INVALID_ARG;
+  if (M == 0 || F == 0) return VMI_OK;
+  if (out == nullptr || ldo < F || (dtype == VMI_E4M3 && (x_scale == nullptr || gate_scale == nullptr || up_scale == nullptr)))
+    return VMI_ERR_INVALID_ARG;
+  if (ldg != ldu) return VMI_ERR_UNSUPPORTED;
+  if (const int st = first_error({rows_status(x, M, K, ldx, dtype), rows_status(w_gate, F, K, ldg, dtype),
+                                  rows_status(w_up, F, K, ldu, dtype)});
+      st != VMI_OK)
+    return st;
+  Args p{};
+  p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.xs = x_scale, p.ws = gate_scale, p.ws2 = up_scale;
+  p.m = static_cast<int>(M), p.n = static_cast<int>(F), p.k = static_cast<int>(K);
+  p.act = act, p.beta1 = beta1, p.beta2 = beta2, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
+  p.vec = out_vectors(out, ldo, nullptr, 0, size_of(out_dtype));
+  return product(dtype, GATED, p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int vmi_linear_add_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, size_t* bytes) {
+  if (bytes == nullptr || !sizes_ok(M, N, K) || !linear_act(act) || dtype < 0 || dtype > VMI_F16) return VMI_ERR_INVALID_ARG;
+  const int64_t n = whole(N, dtype);
+  size_t b = act == ACT_NONE ? 0 : align256(static_cast<size_t>(M) * n * size_of(dtype));
+  b += weight_bytes(n, N, K, M);
+  *bytes = b + align256(static_cast<size_t>(column_shares(M, N)) * N * 4);
+  return VMI_OK;
+}
+
+extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const void* bias, int act,
+                                  const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M, int64_t N, int64_t K,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  if (const int st = vmi_linear_add_bwd_workspace_bytes(M, N, K, dtype, act, &need); st != VMI_OK) return st;
+  if (workspace_bytes < need || (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+    return VMI_ERR_WORKSPACE;
+  if (const int st = first_error({rows_status(x, M, K, ldx, dtype), rows_status(w, N, K, ldw, dtype), rows_status(dy, M, N, lddy, dtype)});
+      st != VMI_OK)
+    return st;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t size = size_of(dtype), n = whole(N, dtype);
+  char* at = static_cast<char*>(workspace);
+  const void* dz = dy;
+  int64_t lddz = lddy;
+  if (act != ACT_NONE) {
+    dz = at, lddz = n;
+    at += align256(static_cast<size_t>(M) * n * size);
+    if (M > 0 && N > 0) {
+      Args p{};
+      p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
+      p.bias = bias, p.other = dy, p.ldother = lddy, p.act = act, p.out = const_cast<void*>(dz), p.ldo = lddz;
+      p.vec = out_vectors(dz, lddz, dy, lddy, size);
+      if (const int st = product(dtype, LINEAR_DZ, p, s); st != VMI_OK) return st;
+    }
+  }
+  float* partial = reinterpret_cast<float*>(at);
+  at += weight_bytes(n, N, K, M);
+  if (dx != nullptr && M > 0 && K > 0) {
+    Args p{};
+    p.a = dz, p.lda = lddz, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(K), p.k = static_cast<int>(N);
+    p.out = dx, p.ldo = K, p.vec = out_vectors(dx, K, nullptr, 0, size);
+    if (const int st = product(dtype, DX, p, s); st != VMI_OK) return st;
+  }
+  if (dw != nullptr)
+    if (const int st = weight_gradient(dz, lddz, 1, n, N, x, ldx, dtype, M, K, dw, partial, s); st != VMI_OK) return st;
+  if (db != nullptr && N > 0) {
+    const int shares = column_shares(M, N);
+    const int share = static_cast<int>((M + shares - 1) / shares);
+    float* sums = reinterpret_cast<float*>(at);
+    return by_type(dtype, [&](auto tag) -> int {
+      using T = decltype(tag);
+      hipLaunchKernelGGL(columns_kernel<T>, dim3(static_cast<unsigned>((N + 63) / 64), static_cast<unsigned>(shares)), dim3(NTH), 0, s,
+                         static_cast<const T*>(dz), lddz, static_cast<int>(M), static_cast<int>(N), share, sums);
+      hipLaunchKernelGGL(columns_join_kernel<T>, dim3(static_cast<unsigned>((N + NTH - 1) / NTH)), dim3(NTH), 0, s, sums, shares,
+                         static_cast<int>(N), static_cast<T*>(db));
+      return hip_status(hipGetLastError());
+    });
+  }
+  return VMI_OK;
+}
+
+extern "C" int vmi_gated_linear_bwd_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype, size_t* bytes) {
+  if (bytes == nullptr || !sizes_ok(M, F, K) || dtype < 0 || dtype > VMI_F16) return VMI_ERR_INVALID_ARG;
+  const int64_t f = whole(F, dtype);
+  *bytes = align256(static_cast<size_t>(M) * 2 * f * size_of(dtype)) + weight_bytes(2 * f, 2 * F, K, M);
+  return VMI_OK;
+}
+
+extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
+                                    int dtype, int act, float beta1, float beta2, const void* dh, int64_t lddh, void* dx,
+                                    void* dw, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+  size_t need = 0;
+  if (const int st = vmi_gated_linear_bwd_workspace_bytes(M, F, K, dtype, &need); st != VMI_OK) return st;
+  if (!gate_act(act)) return VMI_ERR_INVALID_ARG;
+  if (workspace_bytes < need || (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+    return VMI_ERR_WORKSPACE;
+  if (ldg != ldu) return VMI_ERR_UNSUPPORTED;
+  if (const int st = first_error({rows_status(x, M, K, ldx, dtype), rows_status(w_gate, F, K, ldg, dtype),
+                                  rows_status(w_up, F, K, ldu, dtype)});
+      st != VMI_OK)
+    return st;
+  if (M > 0 && F > 0 && (dh == nullptr || lddh < F)) return VMI_ERR_INVALID_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t size = size_of(dtype), f = whole(F, dtype), lddz = 2 * f;
+  char* dz = static_cast<char*>(workspace);
+  float* partial = reinterpret_cast<float*>(dz + align256(static_cast<size_t>(M) * lddz * size));
+  if (M > 0 && F > 0) {
+    Args p{};
+    p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.m = static_cast<int>(M), p.n = static_cast<int>(F);
+    p.k = static_cast<int>(K), p.other = dh, p.ldother = lddh, p.act = act, p.beta1 = beta1, p.beta2 = beta2;
+    p.out = dz, p.ldo = lddz, p.second = f, p.vec = out_vectors(dz, lddz, dh, lddh, size);
+    if (const int st = product(dtype, GATED_DZ, p, s); st != VMI_OK) return st;
+  }
+  if (dx != nullptr && M > 0 && K > 0) {
+    Args p{};
+    p.a = dz, p.lda = lddz, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.second = f;
+    p.m = static_cast<int>(M), p.n = static_cast<int>(K), p.k = static_cast<int>(F);
+    p.out = dx, p.ldo = K, p.vec = out_vectors(dx, K, nullptr, 0, size);
+    if (const int st = product(dtype, DX, p, s); st != VMI_OK) return st;
+  }
+  if (dw != nullptr) return weight_gradient(dz, lddz, 2, f, F, x, ldx, dtype, M, K, dw, partial, s);
+  return VMI_OK;
+}

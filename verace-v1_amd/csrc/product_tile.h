@@ -1,0 +1,328 @@
+// Tiles of matrix products for gfx950: C[m][n] = sum_k A(m, k) B(n, k) with fp32 accumulators, for bf16, fp16, fp32 and
+// e4m3 operands, each stored with k contiguous in a row (weights [N, K], activations [M, K]) or with m (n) contiguous
+// (the same tensors in a backward pass).  The epilogue gets the accumulators.
+//
+// A tile has two pieces of HM rows of A and two of HN rows of B; 128 bytes of k are a step.  A step's four pieces lie in one
+// of two LDS stages, filled by direct loads two steps ahead, a piece a phase.  A phase reads one piece into registers, issues the
+// loads of the piece that went free a phase ago, and multiplies A's piece with B's:
+//
+//     phase   reads             loads of step t + 2   product
+//       0     A0                B0                    A0 B0
+//       1     B1                A0                    A0 B1
+//       2     A1                B1                    A1 B0
+//       3     B0 of step t + 1  A1                    A1 B1
+//
+// A barrier ends the reading and the multiplying half of each phase.  With two waves a SIMD the halves of the workgroup go
+// one half-phase apart, so one wave of a SIMD multiplies while the other reads (STAGGER).  A wave waits for its own loads
+// of a piece at the end of the reading half before the one that reads it, one barrier ahead of every reader, with the six
+// pieces issued later still in flight: about 3000 clocks to cover the latency of HBM.
+//
+// LDS is read at 16 bytes a lane (k contiguous), by transposing reads of 8 (m contiguous, 16 bits) or 4 bytes a lane (fp32),
+// and its 16-byte slots are permuted so that the lanes of an access fall in distinct banks.  The direct loads write LDS in
+// lane order, so the permutation is made by the addresses that they read.  Loads outside the operands return zeros: their
+// offset lies beyond the buffer's size.
+#pragma once
+
+#include "vmi_common.h"
+#include "vmi_mfma.h"
+
+namespace vmi {
+namespace prod {
+
+struct e4m3 {
+  uint8_t bits;
+};
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+// Sixteen rows of each operand over 128 bytes of k: lane l holds row l % 16, and of each half (64 bytes) the 16 bytes at
+// 16 * (l / 16) (fp32: every fourth k of them).  The order of k is the same in both operands and otherwise free.
+typedef i32x8 Frag;
+
+template <typename E> __device__ __forceinline__ f32x4 mma(Frag b, Frag a, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mma<__bf16>(Frag b, Frag a, f32x4 c) {
+  c = mfma_t<__bf16>::mma16(__builtin_bit_cast(bf16x8, (i32x4)b.lo), __builtin_bit_cast(bf16x8, (i32x4)a.lo), c);
+  return mfma_t<__bf16>::mma16(__builtin_bit_cast(bf16x8, (i32x4)b.hi), __builtin_bit_cast(bf16x8, (i32x4)a.hi), c);
+}
+template <> __device__ __forceinline__ f32x4 mma<_Float16>(Frag b, Frag a, f32x4 c) {
+  c = mfma_t<_Float16>::mma16(__builtin_bit_cast(f16x8, (i32x4)b.lo), __builtin_bit_cast(f16x8, (i32x4)a.lo), c);
+  return mfma_t<_Float16>::mma16(__builtin_bit_cast(f16x8, (i32x4)b.hi), __builtin_bit_cast(f16x8, (i32x4)a.hi), c);
+}
+template <> __device__ __forceinline__ f32x4 mma<float>(Frag b, Frag a, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (int)b[e]), __builtin_bit_cast(float, (int)a[e]), c, 0, 0, 0);
+  return c;
+}
+template <> __device__ __forceinline__ f32x4 mma<e4m3>(Frag b, Frag a, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 0, 0, 0);  // both e4m3, no block scales
+}
+
+constexpr unsigned kOutside = 0x80000000u;  // an offset past every buffer
+
+__device__ __forceinline__ unsigned lds_offset(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));
+}
+// 64 lanes x 16 bytes from base + off straight into LDS at `lds` (the wave's, uniform), zeros where off is kOutside.  As an
+// asm block so that the compiler adds no waits of its own around LDS reads; it has no register results.
+__device__ __forceinline__ void load_lds(const char* base, unsigned off, unsigned lds) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const i32x4 srd = {static_cast<int>(b), static_cast<int>(b >> 32), static_cast<int>(kOutside - 16), 0x20000};
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(lds), "v"(off), "s"(srd) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads_and_lds() {
+  static_assert(N < 64);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));  // vmcnt(N), lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// HM, HN: rows of a piece; WM x WN waves, each with MF x NF fragments of 16 x 16 of each of the four products.
+template <int HM_, int HN_, int WM_, int WN_> struct Shape {
+  static constexpr int HM = HM_, HN = HN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
+  static constexpr int MF = HM / (16 * WM), NF = HN / (16 * WN);
+  static constexpr int LA = HM * 8 / THREADS, LB = HN * 8 / THREADS;  // loads of a thread for a piece
+  static constexpr int A_BYTES = HM * 128, B_BYTES = HN * 128, STAGE = 2 * (A_BYTES + B_BYTES);
+  static constexpr int FLIGHT = 3 * (LA + LB);  // the loads of six pieces
+  static constexpr bool STAGGER = WM * WN == 8;
+  static_assert(LA >= 1 && LB >= 1 && MF >= 1 && NF >= 1);
+};
+
+// One operand: `MN` where its m (n) is contiguous in memory.
+struct Matrix {
+  const char* p;
+  int64_t ld;  // bytes
+};
+
+// A thread's loads of one piece of an operand.  H rows (columns) of the piece, of which `inside` are in the operand.
+// PERM: the order in which B's columns go to fragments (see column_of).
+template <typename E, bool MN, int H, int L, int THREADS, int XF, bool PERM> struct Loader {
+  static constexpr int SIZE = sizeof(E), KT = 128 / SIZE, RB = MN ? H * SIZE : 128, SLOTS = RB / 16;
+  unsigned off[L];
+  int k[L];  // the first k of the load within a step, in elements
+
+  __device__ __forceinline__ static int swizzle(int row) {
+    if constexpr (!MN) return (row >> 1) & 7;
+    else if constexpr (SIZE == 4) return ((row >> 2) & (SLOTS >= 16 ? 3 : 1)) << 2;
+    else if constexpr (SLOTS >= 16) return ((row & 3) << 2) | (((row >> 3) & 1) << 1);
+    else if constexpr (SLOTS == 8) return (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) << 1;
+    else return ((row >> 3) & 1) << 1;
+  }
+  __device__ __forceinline__ void init(int tid, unsigned ld, int inside) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int c = i * THREADS + tid, row = c / SLOTS, slot = (c % SLOTS) ^ swizzle(row);
+      if constexpr (MN) {
+        const int x = slot * (16 / SIZE);
+        k[i] = row;
+        off[i] = x < inside ? row * ld + slot * 16 : kOutside;
+      } else {
+        int x = row;
+        if constexpr (PERM) {
+          const int r = row % (16 * XF), j = r / 16, q = r % 16;
+          x = row - r + (q / 4) * 4 * XF + j * 4 + q % 4;
+        }
+        k[i] = slot * (16 / SIZE);
+        off[i] = x < inside ? x * ld + slot * 16 : kOutside;
+      }
+    }
+  }
+  // left: how many k there are from the step's first on
+  __device__ __forceinline__ void issue(const char* base, int left, unsigned lds) const {
+#pragma unroll
+    for (int i = 0; i < L; ++i) load_lds(base, k[i] < left ? off[i] : kOutside, lds + i * THREADS * 16);
+  }
+};
+
+// Reads XF fragments of a piece; `first`: the wave's first row (column) of the piece.
+template <typename E, bool MN, int H, int XF> struct Reader {
+  static constexpr int SIZE = sizeof(E), RB = H * SIZE;
+  unsigned at[MN ? XF : 2];
+  __device__ __forceinline__ void init(int lane, int first) {
+    const int i = lane & 15, q = lane >> 4;
+    if constexpr (!MN) {
+      const int x = (i >> 1) & 7;
+      at[0] = (first + i) * 128 + ((q ^ x) << 4);
+      at[1] = at[0] ^ 64;
+    } else if constexpr (SIZE == 2) {
+      // lane 4 e + p of a group of 16 addresses row k = 8 q + e and the 4 columns at 4 p
+      const int e = i >> 2, p = i & 3, k = 8 * q + e;
+#pragma unroll
+      for (int f = 0; f < XF; ++f) {
+        const int c4 = (first + f * 16) / 4 + p;
+        at[f] = k * RB + (((c4 >> 1) ^ Loader<E, MN, H, 1, 64, 1, false>::swizzle(k)) << 4) + (c4 & 1) * 8;
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < XF; ++f) {
+        const int c = first + f * 16 + i;
+        at[f] = 4 * q * RB + (((c >> 2) ^ Loader<E, MN, H, 1, 64, 1, false>::swizzle(4 * q)) << 4) + (c & 3) * 4;
+      }
+    }
+  }
+  __device__ __forceinline__ void read(const char* piece, Frag (&f)[XF]) const {
+    if constexpr (!MN) {
+#pragma unroll
+      for (int x = 0; x < XF; ++x) {
+        f[x].lo = *reinterpret_cast<const i32x4*>(piece + at[0] + x * 2048);
+        f[x].hi = *reinterpret_cast<const i32x4*>(piece + at[1] + x * 2048);
+      }
+    } else if constexpr (SIZE == 2) {
+#pragma unroll
+      for (int x = 0; x < XF; ++x) {
+        i16x4 v[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)  // k + 32 * (h / 2) + 4 * (h % 2)
+          v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_i16x4*)(piece + at[x] + (32 * (h / 2) + 4 * (h % 2)) * RB));
+        typedef short i16x8 __attribute__((ext_vector_type(8)));
+        f[x].lo = __builtin_bit_cast(i32x4, (i16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        f[x].hi = __builtin_bit_cast(i32x4, (i16x8)__builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < XF; ++x)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          f[x][e] = *reinterpret_cast<const int*>(piece + at[x] + ((e / 4) * 16 + e % 4) * RB);
+    }
+  }
+};
+
+// A tile's operands: two pieces of A and two of B at their first k, and (SEGMENTS == 2) again the second part of k.
+struct Operands {
+  const char* a[2];
+  const char* b[2];
+  int64_t a_step, b_step;    // bytes from one step of k to the next
+  unsigned lda, ldb;         // bytes
+  int a_inside[2], b_inside[2];
+  int k;                     // elements of k (of each segment)
+  const char* a2[2];
+  const char* b2[2];
+};
+
+template <typename S> struct Acc {
+  f32x4 v[2][2][S::MF][S::NF];
+};
+
+template <typename E, bool AMN, bool BMN, typename S, int SEGMENTS>
+__device__ __forceinline__ void tile_product(Operands& o, char* lds, Acc<S>& acc) {
+  constexpr int KT = 128 / sizeof(E);
+  constexpr bool PERM = !BMN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  Loader<E, AMN, S::HM, S::LA, S::THREADS, S::MF, false> la[2];
+  Loader<E, BMN, S::HN, S::LB, S::THREADS, S::NF, PERM> lb[2];
+  Reader<E, AMN, S::HM, S::MF> ra;
+  Reader<E, BMN, S::HN, S::NF> rb;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    la[h].init(tid, o.lda, o.a_inside[h]);
+    lb[h].init(tid, o.ldb, o.b_inside[h]);
+  }
+  ra.init(lane, wm * 16 * S::MF);
+  rb.init(lane, wn * 16 * S::NF);
+  const int steps = (o.k + KT - 1) / KT, total = SEGMENTS * steps;
+  const unsigned lds_wave = lds_offset(lds) + wave * 1024;
+  // pieces of a stage: B0, A0, B1, A1, the order of their loads
+  constexpr int at_b[2] = {0, S::B_BYTES + S::A_BYTES}, at_a[2] = {S::B_BYTES, 2 * S::B_BYTES + S::A_BYTES};
+  const char *pa[2] = {o.a[0], o.a[1]}, *pb[2] = {o.b[0], o.b[1]};
+  auto left = [&](int t) { return o.k - (SEGMENTS == 2 && t >= steps ? t - steps : t) * KT; };
+  auto issue_a = [&](int h, int t) {
+    if (SEGMENTS == 2 && t == steps) pa[h] = o.a2[h];
+    la[h].issue(pa[h], t < total ? left(t) : 0, lds_wave + (t & 1) * S::STAGE + at_a[h]);
+    pa[h] += o.a_step;
+  };
+  auto issue_b = [&](int h, int t) {
+    if (SEGMENTS == 2 && t == steps) pb[h] = o.b2[h];
+    lb[h].issue(pb[h], t < total ? left(t) : 0, lds_wave + (t & 1) * S::STAGE + at_b[h]);
+    pb[h] += o.b_step;
+  };
+#pragma unroll
+  for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+    for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+      for (int m = 0; m < S::MF; ++m)
+#pragma unroll
+        for (int n = 0; n < S::NF; ++n) acc.v[hm][hn][m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frag a[S::MF], b0[S::NF], b1[S::NF];
+  auto multiply = [&](f32x4 (&c)[S::MF][S::NF], const Frag (&b)[S::NF]) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int m = 0; m < S::MF; ++m)
+#pragma unroll
+      for (int n = 0; n < S::NF; ++n) c[m][n] = mma<E>(b[n], a[m], c[m][n]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    issue_b(0, t);
+    issue_a(0, t);
+    issue_b(1, t);
+    issue_a(1, t);
+  }
+  wait_loads_and_lds<S::FLIGHT>();
+  barrier();
+  rb.read(lds + at_b[0], b0);
+  wait_loads_and_lds<S::FLIGHT>();
+  barrier();
+  if (S::STAGGER && wave >= S::WM * S::WN / 2) barrier();
+  for (int t = 0; t < total; ++t) {
+    const char* st = lds + (t & 1) * S::STAGE;
+    ra.read(st + at_a[0], a);
+    issue_b(0, t + 2);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[0][0], b0);
+    barrier();
+    rb.read(st + at_b[1], b1);
+    issue_a(0, t + 2);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[0][1], b1);
+    barrier();
+    ra.read(st + at_a[1], a);
+    issue_b(1, t + 2);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[1][0], b0);
+    barrier();
+    rb.read(lds + ((t + 1) & 1) * S::STAGE + at_b[0], b0);
+    issue_a(1, t + 2);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[1][1], b1);
+    barrier();
+  }
+  if (S::STAGGER && wave < S::WM * S::WN / 2) barrier();
+  wait_loads_and_lds<0>();  // no load may write LDS after the workgroup's end
+}
+
+// The first of the 4 (PERM: 4 * NF over all of a wave's fragments) consecutive columns of a lane's accumulator n.
+template <typename S, bool PERM> __device__ __forceinline__ int column_of(int wn, int lane, int n) {
+  const int g = lane >> 4;
+  return wn * 16 * S::NF + (PERM ? g * 4 * S::NF + n * 4 : n * 16 + g * 4);
+}
+
+// A workgroup's tile: eight XCDs take workgroups in turn, so each gets a run of neighbouring tiles (its own L2 then holds
+// their operands), in columns of up to `GROUP` rows of tiles.
+__device__ __forceinline__ void tile_of(int block, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
+  const int n = tiles_m * tiles_n, xcd = block & 7, i = block >> 3, each = n >> 3, rest = n & 7;
+  const int t = xcd * each + (xcd < rest ? xcd : rest) + i;
+  const int per = group * tiles_n, first = t / per * group, rows = tiles_m - first < group ? tiles_m - first : group;
+  tm = first + (t % per) % rows;
+  tn = (t % per) / rows;
+}
+
+}  // namespace prod
+}  // namespace vmi

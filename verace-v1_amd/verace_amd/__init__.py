@@ -34,11 +34,16 @@ Drop-in replacements for the reference's SSSD hot path:
 * ``short_conv`` / ``short_conv_step_``
                                -- the short causal convolution before it, and its single-token step
 * ``gated_norm_add``           -- the norms either side of a block with its gate and residual scale
+* ``gated_linear``             -- both gated projections with their activation and product in one kernel
+* ``linear_add``               -- a projection with bias, activation and residual in its epilogue
+* ``norm_add_quant`` / ``quantize_rows``
+                               -- the residual's addition and the norm with an 8-bit result; rows in 8 bits
 * ``HAS_HIP``                  <- ``verace_v1.serving.triton_kernels.HAS_TRITON``
 
 ``torch.ops.verace.{sssd_scan, sssd_scan_bwd, sssd_step_, sssd_scan_fused, cham_scan, cham_step_,
 ns_retraction, selective_scan, selective_scan_bwd, selective_step_, short_conv, short_conv_bwd,
-short_conv_step_, gated_norm, gated_norm_bwd}`` are the same launchers registered as torch operators with fake kernels and
+short_conv_step_, gated_norm, gated_norm_bwd, gated_linear, gated_linear_bwd, linear_add, linear_add_bwd, norm_add_quant,
+quantize_rows}`` are the same launchers registered as torch operators with fake kernels and
 autograd (``ops.py``), for FakeTensor / meta tracing and ``torch.compile``.
 
 All compute runs in ``libverace_sssd.so`` (C ABI: ``include/verace_sssd.h``).
@@ -56,6 +61,7 @@ from .mcmoe import ManifoldContinuousMoE, SiTUGLU
 from .backbone import (AdaptiveCognitiveDepthEngine, DecodeGraph, DecodeState, LayerDecodeState,
                        VeraceV1Config, VeraceV1Layer, VeraceV1Model)
 from .block_norm import gated_norm_add
+from .feed_forward import gated_linear, linear_add, norm_add_quant, quantize_rows
 from .selective import (launch_selective_hip_scan, launch_selective_hip_scan_bwd, selective_scan,
                         selective_step_, short_conv, short_conv_step_)
 from .state_cache import SlotTable, SSSDStateCache
@@ -93,6 +99,10 @@ __all__ = [
     "short_conv",
     "short_conv_step_",
     "gated_norm_add",
+    "gated_linear",
+    "linear_add",
+    "norm_add_quant",
+    "quantize_rows",
     "newton_schulz_unitary_retraction",
     "parallel_newton_schulz_retraction",
 ]

@@ -14,7 +14,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libverace_sssd.so")
 
-VMI_F32, VMI_BF16, VMI_F16 = 0, 1, 2
+VMI_F32, VMI_BF16, VMI_F16, VMI_E4M3 = 0, 1, 2, 3
 _DTYPE_CODE = {torch.float32: VMI_F32, torch.bfloat16: VMI_BF16, torch.float16: VMI_F16}
 
 EXPORTED = (
@@ -70,6 +70,13 @@ EXPORTED = (
     "vmi_selective_step",
     "vmi_selective_scan_bwd_workspace_bytes",
     "vmi_selective_scan_bwd",
+    "vmi_linear_add",
+    "vmi_linear_add_bwd_workspace_bytes",
+    "vmi_linear_add_bwd",
+    "vmi_gated_linear",
+    "vmi_gated_linear_bwd_workspace_bytes",
+    "vmi_gated_linear_bwd",
+    "vmi_norm_add_quant",
 )
 
 ERR_WORKSPACE = 3  # VMI_ERR_WORKSPACE
@@ -191,9 +198,20 @@ def _declare(lib):
     lib.vmi_selective_scan_bwd.argtypes = [vp, i64, i64, vp, i64, i64, i32, vp, vp, i64, i64, vp, i64, i64, vp, vp,
                                            i32, i32, vp, vp, i32, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                            i64, i64, i64, i64, i64, i64, vp, sz, vp]
+    lib.vmi_linear_add.argtypes = [vp, i64, vp, vp, i64, vp, i32, vp, vp, i64, i32, vp, i64, i32, i64, i64, i64, vp]
+    lib.vmi_linear_add_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, psz]
+    lib.vmi_linear_add_bwd.argtypes = [vp, i64, vp, i64, i32, vp, i32, vp, i64, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.vmi_gated_linear.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, i32, f32, f32, vp, i64, i32, i64, i64, i64,
+                                     vp]
+    lib.vmi_gated_linear_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, psz]
+    lib.vmi_gated_linear_bwd.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, f32, f32, vp, i64, vp, vp, i64, i64, i64, vp,
+                                         sz, vp]
+    lib.vmi_norm_add_quant.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, f32, vp, vp, vp, i64, i64, vp]
     for name in ("gated_norm", "gated_norm_bwd_workspace_bytes", "gated_norm_bwd", "short_conv", "short_conv_step",
                  "short_conv_bwd_workspace_bytes", "short_conv_bwd", "selective_scan_workspace_bytes",
-                 "selective_scan_fwd", "selective_step", "selective_scan_bwd_workspace_bytes", "selective_scan_bwd"):
+                 "selective_scan_fwd", "selective_step", "selective_scan_bwd_workspace_bytes", "selective_scan_bwd",
+                 "linear_add", "linear_add_bwd_workspace_bytes", "linear_add_bwd", "gated_linear",
+                 "gated_linear_bwd_workspace_bytes", "gated_linear_bwd", "norm_add_quant"):
         getattr(lib, "vmi_" + name).restype = i32
 
 

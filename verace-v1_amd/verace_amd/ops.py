@@ -23,6 +23,11 @@ Replaces, for tracing purposes, the reference's Triton launcher ``launch_sssd_tr
   ``verace::short_conv_bwd``; ``verace::short_conv_step_(x, weight, bias?, state!, activation?, mask?) -> y``.
 * ``verace::gated_norm(y, residual, gate?, w1?, scale?, w2?, eps, next_eps, activation) -> (s, n, stats)`` -- differentiable
   through ``verace::gated_norm_bwd`` (n empty without w2).
+* ``verace::gated_linear(x, w_gate, w_up, x_scale?, gate_scale?, up_scale?, activation, beta1, beta2, out_dtype) -> h`` --
+  differentiable through ``verace::gated_linear_bwd``.
+* ``verace::linear_add(x, weight, bias?, residual?, x_scale?, weight_scale?, activation?, out_dtype) -> y`` -- differentiable
+  through ``verace::linear_add_bwd``.
+* ``verace::norm_add_quant(a, residual?, norm_weight?, eps) -> (s, q, scale)``; ``verace::quantize_rows(x) -> (q, scale)``.
 
 The eager module path calls the launchers directly (no dispatcher overhead in a decode loop);
 :class:`~verace_amd.SSSDAttention` switches to these operators while ``torch.compile`` traces.
@@ -35,6 +40,7 @@ import torch
 from torch import Tensor
 
 from . import block_norm as bn
+from . import feed_forward as ff
 from . import hip_kernels as hk
 from . import selective as sel
 
@@ -368,3 +374,104 @@ def _norm_backward(ctx, ds, dn, _):
 
 
 gated_norm.register_autograd(_norm_backward, setup_context=_norm_setup)
+
+
+# ------------------------------------------------------------------------------------ feed-forward
+
+@torch.library.custom_op("verace::gated_linear", mutates_args=())
+def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, x_scale: Optional[Tensor], gate_scale: Optional[Tensor],
+                 up_scale: Optional[Tensor], activation: str, beta1: float, beta2: float, out_dtype: torch.dtype) -> Tensor:
+    ff._gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, beta1, beta2, out_dtype)
+    return ff._launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, ff._GATED_ACT[activation], beta1, beta2, out_dtype)
+
+
+@gated_linear.register_fake
+def _gated_linear_fake(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, beta1, beta2, out_dtype):
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("verace::gated_linear_bwd", mutates_args=())
+def gated_linear_bwd(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str, beta1: float, beta2: float,
+                     dh: Tensor) -> List[Tensor]:
+    ff._gated_check(x, w_gate, w_up, None, None, None, activation, beta1, beta2, None)
+    dx, dg, du = ff._launch_gated_bwd(x, w_gate, w_up, ff._GATED_ACT[activation], beta1, beta2, dh, (True,) * 3)
+    return [dx, dg, du.clone()]  # separate storages: both are halves of one tensor
+
+
+@gated_linear_bwd.register_fake
+def _gated_linear_bwd_fake(x, w_gate, w_up, activation, beta1, beta2, dh):
+    return _new_like(x, (x, w_gate, w_up))
+
+
+def _gated_linear_setup(ctx, inputs, output):
+    x, w_gate, w_up, *_, activation, beta1, beta2, out_dtype = inputs
+    ctx.save_for_backward(x, w_gate, w_up)
+    ctx.form = (activation, beta1, beta2)
+
+
+def _gated_linear_backward(ctx, dh):
+    return (*torch.ops.verace.gated_linear_bwd(*ctx.saved_tensors, *ctx.form, dh), *(None,) * 7)
+
+
+gated_linear.register_autograd(_gated_linear_backward, setup_context=_gated_linear_setup)
+
+
+@torch.library.custom_op("verace::linear_add", mutates_args=())
+def linear_add(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], x_scale: Optional[Tensor],
+               weight_scale: Optional[Tensor], activation: Optional[str], out_dtype: torch.dtype) -> Tensor:
+    ff._linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype)
+    return ff._launch_linear(x, weight, bias, residual, x_scale, weight_scale, ff._LINEAR_ACT[activation], out_dtype)
+
+
+@linear_add.register_fake
+def _linear_add_fake(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("verace::linear_add_bwd", mutates_args=())
+def linear_add_bwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], dy: Tensor) -> List[Tensor]:
+    ff._linear_check(x, weight, bias, None, None, None, activation, None)
+    return _or_empty(x, ff._launch_linear_bwd(x, weight, bias, ff._LINEAR_ACT[activation], dy, (True,) * 3))
+
+
+@linear_add_bwd.register_fake
+def _linear_add_bwd_fake(x, weight, bias, activation, dy):
+    return _new_like(x, (x, weight, bias))
+
+
+def _linear_add_setup(ctx, inputs, output):
+    x, weight, bias, residual, _, _, ctx.activation, _ = inputs
+    ctx.save_for_backward(x, weight, bias)
+    ctx.residual = residual is not None
+
+
+def _linear_add_backward(ctx, dy):
+    x, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.verace.linear_add_bwd(x, weight, bias, ctx.activation, dy)
+    return dx, dw, None if bias is None else db, dy if ctx.residual else None, None, None, None, None
+
+
+linear_add.register_autograd(_linear_add_backward, setup_context=_linear_add_setup)
+
+
+@torch.library.custom_op("verace::norm_add_quant", mutates_args=())
+def norm_add_quant(a: Tensor, residual: Optional[Tensor], norm_weight: Optional[Tensor],
+                   eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    ff._quant_check(a, residual, norm_weight)
+    return ff._launch_quant(a, residual, norm_weight, True, eps, True)
+
+
+@norm_add_quant.register_fake
+def _norm_add_quant_fake(a, residual, norm_weight, eps):
+    return (a.new_empty(a.shape), a.new_empty(a.shape, dtype=ff.E4M3), a.new_empty(a.shape[:-1], dtype=torch.float32))
+
+
+@torch.library.custom_op("verace::quantize_rows", mutates_args=())
+def quantize_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
+    ff._quant_check(x, None, None)
+    return ff._launch_quant(x, None, None, False, 0.0, False)[1:]
+
+
+@quantize_rows.register_fake
+def _quantize_rows_fake(x):
+    return x.new_empty(x.shape, dtype=ff.E4M3), x.new_empty(x.shape[:-1], dtype=torch.float32)
