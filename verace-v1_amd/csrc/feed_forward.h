@@ -48,15 +48,6 @@ struct Args {
 template <typename E> struct memory { typedef E type; };
 template <> struct memory<__bf16> { typedef bf16_t type; };
 
-// tanh to a few 2^-24 relative; for a 16-bit result by v_exp_f32 and v_rcp_f32, and a polynomial where their difference
-// from 1 would cancel.
-template <typename T> __device__ __forceinline__ float tanh_for(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  const float x2 = x * x, e = __expf(2.f * fabsf(x));
-  const float far = copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f), x);
-  const float near = x + x * x2 * (-0.333333333f + x2 * (0.133333333f + x2 * (-0.0539682540f + x2 * 0.0218694885f)));
-  return x2 < 0.09f ? near : far;
-}
 // act(z) and its derivative of the ungated projection.
 template <typename T> __device__ __forceinline__ float activate(float z, int act) {
   if (act == ACT_SILU) return z * sigmoid_for<T>(z);
@@ -78,21 +69,49 @@ struct Gate {
   int act;
   float b1, b2, i1, i2;
 };
+// The parts of tanh(x) = sign(x) num / den: (1 - e) / (1 + e) with e = exp(-2|x|), and near 0, where 1 - e cancels, a polynomial
+// (the next term is below 2^-24 of it) over 1.
+template <typename T> __device__ __forceinline__ void tanh_parts(float x, float& num, float& den) {
+  const float a = fabsf(x), x2 = x * x;
+  const float e = __expf(-2.f * a);
+  const float near = a + a * x2 * (-0.333333333f + x2 * (0.133333333f + x2 * -0.0539682540f));
+  num = x2 < 0.01f ? near : 1.f - e;
+  den = x2 < 0.01f ? 1.f : 1.f + e;
+}
+// a(g) b(u).  16-bit results: the quotients of the two tanh and the sigmoid over one reciprocal, their exponentials at most 1.
 template <typename T> __device__ __forceinline__ float gated(float g, float u, const Gate& c) {
-  const float s = sigmoid_for<T>(g);
-  if (c.act == ACT_SILU) return g * s * u;
-  return c.b1 * tanh_for<T>(g * c.i1) * s * (c.b2 * tanh_for<T>(u * c.i2));
+  if (c.act == ACT_SILU) return g * sigmoid_for<T>(g) * u;
+  if constexpr (sizeof(T) == 4) return c.b1 * tanhf(g * c.i1) * sigmoid_for<T>(g) * (c.b2 * tanhf(u * c.i2));
+  float n1, d1, n2, d2;
+  tanh_parts<T>(g * c.i1, n1, d1);
+  tanh_parts<T>(u * c.i2, n2, d2);
+  const float e = __expf(-fabsf(g)), s = g < 0.f ? e : 1.f;  // sigmoid(g) = s / (1 + e)
+  const float h = c.b1 * c.b2 * n1 * n2 * s * __builtin_amdgcn_rcpf(d1 * d2 * (1.f + e));
+  return (__float_as_uint(g) ^ __float_as_uint(u)) >> 31 ? -h : h;
 }
 template <typename T>
 __device__ __forceinline__ void gated_slopes(float g, float u, float dh, const Gate& c, float& dg, float& du) {
-  const float s = sigmoid_for<T>(g);
   if (c.act == ACT_SILU) {
+    const float s = sigmoid_for<T>(g);
     dg = dh * u * s * (1.f + g * (1.f - s));
     du = dh * g * s;
     return;
   }
-  const float t1 = tanh_for<T>(g * c.i1), t2 = tanh_for<T>(u * c.i2), a = c.b1 * t1 * s;
-  dg = dh * c.b2 * t2 * s * ((1.f - t1 * t1) + c.b1 * t1 * (1.f - s));
+  float s, ns, t1, t2;  // sigmoid(g) and sigmoid(-g)
+  if constexpr (sizeof(T) == 4) {
+    s = sigmoid_for<T>(g), ns = sigmoid_for<T>(-g);
+    t1 = tanhf(g * c.i1), t2 = tanhf(u * c.i2);
+  } else {
+    float n1, d1, n2, d2;
+    tanh_parts<T>(g * c.i1, n1, d1);
+    tanh_parts<T>(u * c.i2, n2, d2);
+    const float e = __expf(-fabsf(g)), d3 = 1.f + e, d12 = d1 * d2, r = __builtin_amdgcn_rcpf(d12 * d3);
+    const float big = d12 * r, small = e * big;
+    s = g < 0.f ? small : big, ns = g < 0.f ? big : small;
+    t1 = copysignf(n1 * (d2 * d3) * r, g), t2 = copysignf(n2 * (d1 * d3) * r, u);
+  }
+  const float a = c.b1 * t1 * s;
+  dg = dh * c.b2 * t2 * (s * (1.f - t1 * t1) + a * ns);
   du = dh * a * (1.f - t2 * t2);
 }
 
@@ -307,7 +326,14 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
   return launch_product<E, KIND, Small>(p, stream);
 }
 
+template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
+constexpr int kFewRows = 64;
+
 template <typename E> int product_of(Kind kind, const Args& p, hipStream_t stream) {
+  if (p.m <= kFewRows) {
+    if (kind == LINEAR) return launch_rows<E, LINEAR>(p, stream);
+    if (kind == GATED) return launch_rows<E, GATED>(p, stream);
+  }
   switch (kind) {
     case LINEAR: return product_of_kind<E, LINEAR>(p, stream);
     case GATED: return product_of_kind<E, GATED>(p, stream);

@@ -32,25 +32,40 @@ __global__ __launch_bounds__(NTH) void join_kernel(const float* partial, T* out,
   store_cols<T, 4>(out, i, n, vec, s);
 }
 
-// Column sums of [rows, n]: workgroup (b, s) those of 64 columns over the s-th share of the rows, 4 rows at a time.
+// Column sums of [rows, n]: workgroup (b, s) those of 256 columns over the s-th share of the rows.  A thread adds 8 columns of
+// every eighth row (16 or 32 bytes a load), the eight are added in LDS.
 template <typename T>
-__global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, int rows, int n, int share, float* partial) {
-  __shared__ float part[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r0 = threadIdx.x >> 6;
-  const int first = blockIdx.y * share, last = rows - first < share ? rows : first + share;
-  float s = 0.f;
-  if (c < n)
-    for (int r = first + r0; r < last; r += 4) s += io<T>::load(x + r * ld, c);
-  part[r0][threadIdx.x & 63] = s;
+__global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, int rows, int n, int share, bool vec, float* partial) {
+  __shared__ float part[8][256];
+  const int c = (threadIdx.x & 31) * 8, c0 = blockIdx.x * 256 + c, r0 = threadIdx.x >> 5;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * share, last = rows - first < share ? rows : first + share;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, t[8];
+  if (c0 < n)
+    for (int64_t r = first + r0; r < last; r += 8) {
+      load_cols<T, 8>(x + r * ld, c0, n, vec, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += t[j];
+    }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[r0][c + j] = s[j];
   __syncthreads();
-  if (r0 == 0 && c < n) partial[static_cast<int64_t>(blockIdx.y) * n + c] = part[0][c & 63] + part[1][c & 63] + part[2][c & 63] + part[3][c & 63];
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sum += part[r][threadIdx.x];
+  if (const int col = blockIdx.x * 256 + threadIdx.x; col < n) partial[static_cast<int64_t>(blockIdx.y) * n + col] = sum;
 }
+// 32 columns a workgroup, each share's eighth by 32 threads.
 template <typename T>
 __global__ __launch_bounds__(NTH) void columns_join_kernel(const float* partial, int shares, int n, T* out) {
-  const int c = blockIdx.x * NTH + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float part[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
   float s = 0.f;
-  for (int k = 0; k < shares; ++k) s += partial[static_cast<int64_t>(k) * n + c];
+  if (c < n)
+    for (int k = r; k < shares; k += 8) s += partial[static_cast<int64_t>(k) * n + c];
+  part[r][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (r != 0 || c >= n) return;
+  for (int k = 1; k < 8; ++k) s += part[k][threadIdx.x & 31];
   io<T>::store(out, c, s);
 }
 
@@ -133,7 +148,7 @@ size_t weight_bytes(int64_t rows, int64_t valid, int64_t cols, int64_t m) {
   return s.n > 1 ? align256(static_cast<size_t>(s.n) * valid * cols * 4) : 0;
 }
 int column_shares(int64_t m, int64_t n) {
-  const int64_t t = (n + 63) / 64, want = t == 0 ? 1 : (1024 + t - 1) / t, most = (m + 63) / 64;
+  const int64_t t = (n + 255) / 256, want = t == 0 ? 1 : (256 + t - 1) / t, most = (m + 31) / 32;
   const int64_t s = want < most ? want : most;
   return static_cast<int>(s < 1 ? 1 : s);
 }
@@ -234,9 +249,11 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
     float* sums = reinterpret_cast<float*>(at);
     return by_type(dtype, [&](auto tag) -> int {
       using T = decltype(tag);
-      hipLaunchKernelGGL(columns_kernel<T>, dim3(static_cast<unsigned>((N + 63) / 64), static_cast<unsigned>(shares)), dim3(NTH), 0, s,
-                         static_cast<const T*>(dz), lddz, static_cast<int>(M), static_cast<int>(N), share, sums);
-      hipLaunchKernelGGL(columns_join_kernel<T>, dim3(static_cast<unsigned>((N + NTH - 1) / NTH)), dim3(NTH), 0, s, sums, shares,
+      const bool vec = out_vectors(dz, lddz, nullptr, 0, size);
+      if (!grid_fits((N + 31) / 32, NTH)) return VMI_ERR_UNSUPPORTED;
+      hipLaunchKernelGGL(columns_kernel<T>, dim3(static_cast<unsigned>((N + 255) / 256), static_cast<unsigned>(shares)), dim3(NTH), 0,
+                         s, static_cast<const T*>(dz), lddz, static_cast<int>(M), static_cast<int>(N), share, vec, sums);
+      hipLaunchKernelGGL(columns_join_kernel<T>, dim3(static_cast<unsigned>((N + 31) / 32)), dim3(NTH), 0, s, sums, shares,
                          static_cast<int>(N), static_cast<T*>(db));
       return hip_status(hipGetLastError());
     });

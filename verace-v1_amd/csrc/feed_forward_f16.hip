@@ -1,5 +1,5 @@
 // The feed-forward products over f16 operands.
-#include "feed_forward.h"
+#include "feed_forward_rows.h"
 
 namespace vmi {
 namespace prod {

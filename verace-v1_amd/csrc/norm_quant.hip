@@ -4,14 +4,16 @@
 // and the same without the norm (rms = 1, w = 1) for rows as they are.  rms cancels in q, so q depends on one quotient alone.
 //
 // A result of 3 mantissa bits meets a tie, or comes near one, in a few values of every million, and 32-bit arithmetic would
-// round those by its own errors.  s, p and the quotient are therefore formed in 64 bits: sums and products of two 24-bit
-// values are exact there, the quotient gets one Newton step (correctly rounded, exact where it has 53 bits), and it goes to
-// 32 bits by rounding to odd, so that the last rounding, to e4m3, is the only one.  One read of each input, one write of
-// each result: HBM bounds it.
+// round those by its own errors.  In 64 bits s and p are exact (sums and products of two 24-bit values), and the quotient with
+// one Newton step is correctly rounded, exact where it has 53 bits; it goes to 32 bits by rounding to odd, so that the rounding
+// to e4m3 is the only one.  That is needed where the 32-bit quotient, four roundings of 2^-24 off, lies within 16 of its steps
+// of a tie (and below 2^-6, where e4m3's steps are of one size): one value of about 5000, so a wave takes the 64-bit form for
+// a whole piece where one of its lanes needs it.  max|p| in 64 bits is that of the pieces whose 32-bit maximum is within
+// 2^-21 of the row's.  Rows whose 32-bit terms are not all finite, or all below 2^-60, take the 64-bit form throughout.
 //
-// A row is one wave's (up to 64 pieces of 16 bytes each lane) or four waves'; its inputs stay in registers between the pass
-// that sums and the pass that writes.  Longer rows are read again.  A row with a NaN or an infinity in p has the scale NaN
-// and q NaN everywhere; its s is what it is.
+// One read of each input, one write of each result: HBM bounds it.  A row is one wave's (up to 8 pieces of 16 bytes a lane)
+// or four waves'; its inputs stay in registers, as they came, between the pass that sums and the pass that writes.  Longer rows
+// are read again.  A row with a NaN or an infinity in p has the scale NaN and q NaN everywhere; its s is what it is.
 #include "vmi_dispatch.h"
 #include "vmi_vec.h"
 
@@ -43,18 +45,6 @@ __device__ __forceinline__ float round_to_odd(double r) {
   return __uint_as_float(b);
 }
 
-template <typename T, typename W> struct Piece {
-  static constexpr int N = Vec<T>::N;
-  // p and s of the N elements from i0
-  static __device__ __forceinline__ void terms(const float (&a)[N], const float (&r)[N], const float (&w)[N], double (&s)[N], double (&p)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      s[j] = static_cast<double>(a[j]) + static_cast<double>(r[j]);
-      p[j] = s[j] * static_cast<double>(w[j]);
-    }
-  }
-};
-
 template <typename T, typename W, int N>
 __device__ __forceinline__ void load_weights(const W* w, int i0, int d, bool vec, float (&x)[N]) {
   if (w == nullptr) {
@@ -72,11 +62,57 @@ __device__ __forceinline__ void load_weights(const W* w, int i0, int d, bool vec
   }
 }
 
+// 16 bytes of a row from element i0 as they lie, zeros past its end.
+template <typename T> __device__ __forceinline__ Vec<T> load_raw(const T* row, int i0, int d, bool vec) {
+  if (vec) return ldv(row + i0);
+  Vec<T> v;
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N; ++j) {
+    if (i0 + j < d) v.e[j] = row[i0 + j];
+    else io<T>::store(v.e, j, 0.f);
+  }
+  return v;
+}
+
+// The terms of one piece in 32 bits and, where it matters, in 64.
+template <typename T> struct Terms {
+  static constexpr int N = Vec<T>::N;
+  Vec<T> a, r;
+  float w[N];
+  bool residual;
+  __device__ __forceinline__ float s(int j) const {
+    const float x = io<T>::to_f32(a.e[j]);
+    return residual ? x + io<T>::to_f32(r.e[j]) : x;
+  }
+  __device__ __forceinline__ double s64(int j) const {
+    const double x = io<T>::to_f32(a.e[j]);
+    return residual ? x + static_cast<double>(io<T>::to_f32(r.e[j])) : x;
+  }
+  __device__ __forceinline__ float p(int j) const { return s(j) * w[j]; }
+  __device__ __forceinline__ double p64(int j) const { return s64(j) * static_cast<double>(w[j]); }
+};
+
+// Keeps the compiler from carrying a piece's terms from one pass to the next in registers (64 of them at 8 pieces of 16 bits):
+// they are formed again from the 16 bytes.
+template <typename T> __device__ __forceinline__ void forget(Vec<T>& v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 x = __builtin_bit_cast(u32x4, v);
+  asm volatile("" : "+v"(x));
+  v = __builtin_bit_cast(Vec<T>, x);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+
 // G threads a row, NV pieces each; LONG: any number of pieces, read again for the second pass.
 template <typename T, typename W, int G, int NV, bool LONG, bool VEC>
 __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   constexpr int N = Vec<T>::N, WAVES = G / 64;
-  __shared__ double red[3][4];
+  __shared__ double red[2][4];
+  __shared__ float red32[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (NTH / G) + threadIdx.x / G;
   if (G < NTH && row >= k.rows) return;
@@ -84,72 +120,121 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   const T* rr = k.r == nullptr ? nullptr : static_cast<const T*>(k.r) + row * k.r_stride;
   const W* w = static_cast<const W*>(k.w);
   T* sr = k.sum == nullptr ? nullptr : static_cast<T*>(k.sum) + row * k.d;
-  float a[LONG ? 1 : NV][N], r[LONG ? 1 : NV][N];
-  auto load = [&](int i0, float (&x)[N], float (&y)[N]) {
-    load_piece<T>(ar, i0, k.d, VEC, x);
-    if (rr != nullptr) {
-      load_piece<T>(rr, i0, k.d, VEC, y);
+  Vec<T> a[LONG ? 1 : NV] = {}, r[LONG ? 1 : NV] = {};
+  auto load = [&](int v, int i0) {
+    a[v] = load_raw<T>(ar, i0, k.d, VEC);
+    if (rr != nullptr) r[v] = load_raw<T>(rr, i0, k.d, VEC);
+  };
+  auto terms = [&](int v, int i0) {
+    Terms<T> t;
+    t.a = a[v], t.residual = rr != nullptr;
+    if (t.residual) t.r = r[v];
+    load_weights<T, W, N>(w, i0, k.d, VEC, t.w);
+    return t;
+  };
+  // f(v, i0) for each of the thread's pieces, `again`: after another pass over them
+  auto pieces = [&](bool again, auto&& f) {
+    if constexpr (LONG) {
+      for (int i0 = g * N; i0 < k.d; i0 += G * N) {
+        load(0, i0);
+        f(0, i0);
+      }
     } else {
+      if (!again) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = 0.f;
+        for (int v = 0; v < NV; ++v)
+          if (const int i0 = (v * G + g) * N; i0 < k.d) load(v, i0);
+      } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          forget(a[v]);
+          forget(r[v]);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (const int i0 = (v * G + g) * N; i0 < k.d) f(v, i0);
     }
   };
-  double ss = 0.0, top = 0.0;
-  bool bad = false;
-  auto gather = [&](int i0, const float (&x)[N], const float (&y)[N]) {
-    float wt[N], st[N];
-    double s[N], p[N];
-    load_weights<T, W, N>(w, i0, k.d, VEC, wt);
-    Piece<T, W>::terms(x, y, wt, s, p);
+  double ss = 0.0;
+  float odd = 0.f, high = 0.f, of_piece[LONG ? 1 : NV];  // odd: NaN after a NaN or an infinity
+#pragma unroll
+  for (int v = 0; v < (LONG ? 1 : NV); ++v) of_piece[v] = 0.f;
+  pieces(false, [&](int v, int i0) {
+    const Terms<T> t = terms(v, i0);
+    float st[N], m = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      st[j] = static_cast<float>(s[j]);
-      ss += s[j] * s[j];
-      top = fmax(top, fabs(p[j]));
-      bad |= !(fabs(p[j]) <= 1.7976931348623157e308);
+      const double s = t.s64(j);
+      const float p = t.p(j);
+      st[j] = static_cast<float>(s);
+      ss += s * s;
+      m = fmaxf(m, fabsf(p));
+      odd = fmaf(p, 0.f, odd);
     }
+    high = fmaxf(high, m);
+    of_piece[v] = m;
     if (sr != nullptr) store_piece<T>(sr, i0, k.d, VEC, st);
-  };
-  if constexpr (LONG) {
-    for (int i0 = g * N; i0 < k.d; i0 += G * N) {
-      load(i0, a[0], r[0]);
-      gather(i0, a[0], r[0]);
-    }
-  } else {
+  });
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (const int i0 = (v * G + g) * N; i0 < k.d) load(i0, a[v], r[v]);
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (const int i0 = (v * G + g) * N; i0 < k.d) gather(i0, a[v], r[v]);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    ss += __shfl_xor(ss, o);
-    top = fmax(top, __shfl_xor(top, o));
-  }
-  bad = __any(bad);
+  for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+  high = wave_max(high);
+  bool wild = __any(!(odd == 0.f));
   if constexpr (WAVES > 1) {
-    if (lane == 0) red[0][wave] = ss, red[1][wave] = top, red[2][wave] = bad ? 1.0 : 0.0;
+    if (lane == 0) red[0][wave] = ss, red32[0][wave] = high, red32[1][wave] = wild ? 1.f : 0.f;
     __syncthreads();
     ss = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+    high = fmaxf(fmaxf(red32[0][0], red32[0][1]), fmaxf(red32[0][2], red32[0][3]));
+    wild = red32[1][0] + red32[1][1] + red32[1][2] + red32[1][3] != 0.f;
+  }
+  wild = wild || high < 0x1p-60f;
+  // the largest |p| in 64 bits
+  const float near = wild ? -1.f : high * (1.f - 0x1p-21f);
+  double top = 0.0;
+  bool bad = false;
+  pieces(true, [&](int v, int i0) {
+    if (LONG || __any(of_piece[v] >= near)) {
+      const Terms<T> t = terms(v, i0);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const double p = fabs(t.p64(j));
+        top = fmax(top, p);
+        bad |= !(p <= 1.7976931348623157e308);
+      }
+    }
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmax(top, __shfl_xor(top, o));
+  bad = __any(bad);
+  if constexpr (WAVES > 1) {
+    __syncthreads();
+    if (lane == 0) red[1][wave] = top, red32[0][wave] = bad ? 1.f : 0.f;
+    __syncthreads();
     top = fmax(fmax(red[1][0], red[1][1]), fmax(red[1][2], red[1][3]));
-    bad = red[2][0] + red[2][1] + red[2][2] + red[2][3] != 0.0;
+    bad = red32[0][0] + red32[0][1] + red32[0][2] + red32[0][3] != 0.f;
   }
   const double rms = k.norm ? sqrt(ss / k.d + static_cast<double>(k.eps)) : 1.0;
   const double D = fmax(top, kTop * kLeast * rms), inv = 1.0 / D;
+  const float F = static_cast<float>(kTop * inv);
   if (g == 0) k.scale[row] = bad ? __builtin_nanf("") : static_cast<float>(D / (kTop * rms));
   uint8_t* qr = k.q + row * k.d;
-  auto write = [&](int i0, const float (&x)[N], const float (&y)[N]) {
-    float wt[N], f[N];
-    double s[N], p[N];
-    load_weights<T, W, N>(w, i0, k.d, VEC, wt);
-    Piece<T, W>::terms(x, y, wt, s, p);
+  pieces(true, [&](int v, int i0) {
+    const Terms<T> t = terms(v, i0);
+    float f[N];
+    bool doubt = wild;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const double t = kTop * p[j], q0 = t * inv;
-      f[j] = round_to_odd(fma(fma(-q0, D, t), inv, q0));
-      if (bad) f[j] = __builtin_nanf("");
+      f[j] = t.p(j) * F;
+      const uint32_t u = __float_as_uint(f[j]);
+      // within 16 steps of the middle between two values (the low 20 bits half way), or of one size of steps, but for 0
+      doubt |= (u & 0xFFFFFu) - 0x7FFF0u <= 0x20u || ((u & 0x7FFFFFFFu) - 1u < 0x3C800000u - 1u);
+    }
+    if (__any(doubt)) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const double x = kTop * t.p64(j), q0 = x * inv;
+        f[j] = bad ? __builtin_nanf("") : round_to_odd(fma(fma(-q0, D, x), inv, q0));
+      }
     }
     uint32_t packed[N / 4];
 #pragma unroll
@@ -158,24 +243,14 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
       packed[j / 4] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[j + 2], f[j + 3], u, true));
     }
     if (VEC) {
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j) reinterpret_cast<uint32_t*>(qr + i0)[j] = packed[j];
+      if constexpr (N == 8) *reinterpret_cast<uint2*>(qr + i0) = make_uint2(packed[0], packed[1]);
+      else *reinterpret_cast<uint32_t*>(qr + i0) = packed[0];
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (i0 + j < k.d) qr[i0 + j] = static_cast<uint8_t>(packed[j / 4] >> (8 * (j % 4)));
     }
-  };
-  if constexpr (LONG) {
-    for (int i0 = g * N; i0 < k.d; i0 += G * N) {
-      load(i0, a[0], r[0]);
-      write(i0, a[0], r[0]);
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (const int i0 = (v * G + g) * N; i0 < k.d) write(i0, a[v], r[v]);
-  }
+  });
 }
 
 template <typename T, typename W, int G, int NV, bool LONG> int launch(Args k, bool vec, hipStream_t stream) {
@@ -217,7 +292,7 @@ extern "C" int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* r
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
     const bool vec = d % Vec<T>::N == 0 && k.a_stride % Vec<T>::N == 0 && k.r_stride % Vec<T>::N == 0 && aligned16({a, residual, w, sum}) &&
-                     reinterpret_cast<uintptr_t>(q) % 4 == 0;
+                     reinterpret_cast<uintptr_t>(q) % Vec<T>::N == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if constexpr (sizeof(T) == 2)
       if (w != nullptr && w_dtype == VMI_F32) return by_row<T, float>(k, vec, s);

@@ -25,10 +25,11 @@ E4M3 = torch.float8_e4m3fn
 _LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2}
 _GATED_ACT = {"silu": 1, "situ": 3}
 _MAX_ROW_BYTES = 1 << 24  # from a row to the next
+_ITEMSIZE = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, E4M3: 1}
 
 
 def _code(dtype: torch.dtype) -> int:
-    return _lib.VMI_E4M3 if dtype == E4M3 else _lib.dtype_code(dtype)
+    return _lib.VMI_E4M3 if dtype is E4M3 else _lib.dtype_code(dtype)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -47,6 +48,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return out[:, :k]
 
 
+def _operand(t: torch.Tensor, k: int) -> Tuple[torch.Tensor, int, int]:
+    """(what has to stay alive, address, elements from a row to the next) of t [..., k] as :func:`_rows`."""
+    if t.is_contiguous():
+        p = t.data_ptr()
+        if not (p | k * _ITEMSIZE[t.dtype]) & 15 and k * _ITEMSIZE[t.dtype] < _MAX_ROW_BYTES:
+            return t, p, k
+    t = _rows(t)
+    return t, t.data_ptr(), _ld(t)
+
+
 def _ld(t: Optional[torch.Tensor]) -> int:
     """Elements from a row of [M, K] to the next, also where it has but one."""
     if t is None:
@@ -55,48 +66,58 @@ def _ld(t: Optional[torch.Tensor]) -> int:
     return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // piece) * piece
 
 
-def _plain_rows(t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
-    """t [..., n] as [M, n] whose rows do not overlap, for the epilogue's reads."""
+def _plain_rows(t: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    """(what has to stay alive, address, elements from a row to the next) of t [..., n] for reads element by element: rows of
+    their own."""
     if t is None:
-        return None
+        return None, None, 0
+    if t.is_contiguous():
+        return t, t.data_ptr(), n
     t = t if t.dim() == 2 else t.reshape(-1, n)
-    return t if (n <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= n) else t.contiguous()
+    if not ((n <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= n)):
+        t = t.contiguous()
+    return t, t.data_ptr(), t.stride(0) if t.shape[0] > 1 else n
 
 
-def _weight_check(x, name, w, scale_name, scale) -> None:
-    K = x.shape[-1]
-    if w.dim() != 2 or w.shape[1] != K or w.dtype != x.dtype or w.device != x.device:
+def _weight_check(x, K, name, w, scale_name, scale) -> None:
+    s = w.shape
+    if len(s) != 2 or s[1] != K or w.dtype is not x.dtype or w.device != x.device:
         raise RuntimeError(f"verace_amd: {name} must be [N, {K}] {x.dtype} on {x.device}, "
-                           f"got {tuple(w.shape)} {w.dtype} on {w.device}")
-    _scale_check(x, scale_name, scale, (w.shape[0],))
+                           f"got {tuple(s)} {w.dtype} on {w.device}")
+    if scale is not None or x.dtype is E4M3:
+        _scale_check(x, scale_name, scale, s[:1])
 
 
 def _scale_check(x, name, scale, shape) -> None:
-    if (scale is not None) != (x.dtype == E4M3):
+    if (scale is not None) != (x.dtype is E4M3):
         raise RuntimeError(f"verace_amd: {name} belongs to float8_e4m3fn rows, and they to it (x is {x.dtype})")
-    if scale is not None and (tuple(scale.shape) != tuple(shape) or scale.dtype != torch.float32 or scale.device != x.device):
+    if scale is not None and (scale.shape != shape or scale.dtype is not torch.float32 or scale.device != x.device):
         raise RuntimeError(f"verace_amd: {name} must be {tuple(shape)} float32 on {x.device}, "
                            f"got {tuple(scale.shape)} {scale.dtype} on {scale.device}")
 
 
 def _x_check(x, x_scale, out_dtype) -> torch.dtype:
     """The result's dtype."""
-    _require_device(x, "x")
-    _code(x.dtype)
+    if not x.is_cuda:
+        _require_device(x, "x")
+    dtype = x.dtype
+    if dtype not in _ITEMSIZE:
+        _code(dtype)
     if x.dim() < 1:
         raise RuntimeError("verace_amd: x must be [..., K]")
-    _scale_check(x, "x_scale", x_scale, x.shape[:-1])
-    if x.dtype != E4M3:
-        if out_dtype not in (None, x.dtype):
-            raise RuntimeError(f"verace_amd: out_dtype is for float8_e4m3fn rows; with {x.dtype} the result is {x.dtype}")
-        return x.dtype
+    if x_scale is not None or dtype is E4M3:
+        _scale_check(x, "x_scale", x_scale, x.shape[:-1])
+    if dtype is not E4M3:
+        if out_dtype is not None and out_dtype is not dtype:
+            raise RuntimeError(f"verace_amd: out_dtype is for float8_e4m3fn rows; with {dtype} the result is {dtype}")
+        return dtype
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     _lib.dtype_code(out_dtype)
     return out_dtype
 
 
 def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.reshape(-1).contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _workspace(query, *args, device) -> Tuple[Optional[torch.Tensor], int]:
@@ -116,8 +137,9 @@ def _no_grad_rows(**tensors) -> None:
 
 def _gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, beta1, beta2, out_dtype) -> torch.dtype:
     out_dtype = _x_check(x, x_scale, out_dtype)
-    _weight_check(x, "w_gate", w_gate, "gate_scale", gate_scale)
-    _weight_check(x, "w_up", w_up, "up_scale", up_scale)
+    K = x.shape[-1]
+    _weight_check(x, K, "w_gate", w_gate, "gate_scale", gate_scale)
+    _weight_check(x, K, "w_up", w_up, "up_scale", up_scale)
     if w_up.shape != w_gate.shape:
         raise RuntimeError(f"verace_amd: w_up {tuple(w_up.shape)} != w_gate {tuple(w_gate.shape)}")
     if activation not in _GATED_ACT:
@@ -127,24 +149,30 @@ def _gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, bet
     return out_dtype
 
 
-def _pair(w_gate, w_up):
+def _pair(w_gate, w_up, K: int):
     """Both weights' rows at one distance."""
-    g, u = _rows(w_gate), _rows(w_up)
-    if _ld(g) != _ld(u):
-        g, u = _rows(w_gate.contiguous()), _rows(w_up.contiguous())
+    g, u = _operand(w_gate, K), _operand(w_up, K)
+    if g[2] != u[2]:
+        g, u = _operand(w_gate.contiguous(), K), _operand(w_up.contiguous(), K)
     return g, u
+
+
+def _rows_of(t: torch.Tensor, k: int) -> int:
+    """The product of t's leading sizes (k the last)."""
+    return t.numel() // k if k else t.shape[:-1].numel()
 
 
 def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, beta2, out_dtype):
     F, K = w_gate.shape
-    x2 = _rows(x)
-    g, u = _pair(w_gate, w_up)
-    out = torch.empty(*x.shape[:-1], F, device=x.device, dtype=out_dtype)
+    x2, xp, ldx = _operand(x, K)
+    (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
+    out = x.new_empty(x.shape[:-1] + (F,), dtype=out_dtype)
+    if x_scale is not None:
+        x_scale, gate_scale, up_scale = _vector(x_scale), _vector(gate_scale), _vector(up_scale)
     with device_guard(x):
         _lib.check(_lib.load().vmi_gated_linear(
-            address(x2), _ld(x2), address(_vector(x_scale)), address(g), _ld(g), address(_vector(gate_scale)), address(u), _ld(u),
-            address(_vector(up_scale)), _code(x.dtype), act, beta1, beta2, address(out), F, _lib.dtype_code(out_dtype),
-            x2.shape[0], F, K, _lib.raw_stream(x.device)), "vmi_gated_linear")
+            xp, ldx, address(x_scale), gp, ldg, address(gate_scale), up, ldu, address(up_scale), _code(x.dtype), act, beta1, beta2,
+            out.data_ptr(), F, _lib.dtype_code(out_dtype), _rows_of(x, K), F, K, _lib.raw_stream(x.device)), "vmi_gated_linear")
     return out
 
 
@@ -154,17 +182,17 @@ def _launch_gated_bwd(x, w_gate, w_up, act, beta1, beta2, dh, need):
     if dh.shape != x.shape[:-1] + (F,) or dh.dtype != x.dtype or dh.device != x.device:
         raise RuntimeError(f"verace_amd: dh must be {tuple(x.shape[:-1] + (F,))} {x.dtype} on {x.device}, "
                            f"got {tuple(dh.shape)} {dh.dtype} on {dh.device}")
-    x2, dh2 = _rows(x), _plain_rows(dh, F)
-    g, u = _pair(w_gate, w_up)
-    M = x2.shape[0]
+    x2, xp, ldx = _operand(x, K)
+    dh2, dhp, lddh = _plain_rows(dh, F)
+    (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
+    M = _rows_of(x, K)
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
     dw = torch.empty(2, F, K, device=x.device, dtype=x.dtype) if need[1] or need[2] else None
     code = _code(x.dtype)
     ws, ws_bytes = _workspace("vmi_gated_linear_bwd_workspace_bytes", M, F, K, code, device=x.device)
     with device_guard(x):
         _lib.check(_lib.load().vmi_gated_linear_bwd(
-            address(x2), _ld(x2), address(g), _ld(g), address(u), _ld(u), code, act, beta1, beta2, address(dh2),
-            dh2.stride(0) if M > 1 else F, address(dx), address(dw), M, F, K, address(ws), ws_bytes,
+            xp, ldx, gp, ldg, up, ldu, code, act, beta1, beta2, dhp, lddh, address(dx), address(dw), M, F, K, address(ws), ws_bytes,
             _lib.raw_stream(x.device)), "vmi_gated_linear_bwd")
     return dx, dw[0] if need[1] else None, dw[1] if need[2] else None
 
@@ -223,27 +251,31 @@ def gated_linear(
 
 def _linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype) -> torch.dtype:
     out_dtype = _x_check(x, x_scale, out_dtype)
-    _weight_check(x, "weight", weight, "weight_scale", weight_scale)
+    _weight_check(x, x.shape[-1], "weight", weight, "weight_scale", weight_scale)
     if activation not in _LINEAR_ACT:
         raise RuntimeError(f"verace_amd: activation must be one of {tuple(_LINEAR_ACT)}, got {activation!r}")
-    N = weight.shape[0]
-    for name, t, shape in (("bias", bias, (N,)), ("residual", residual, (*x.shape[:-1], N))):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != out_dtype or t.device != x.device):
-            raise RuntimeError(f"verace_amd: {name} must be {shape} {out_dtype} on {x.device}, "
-                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if bias is not None or residual is not None:
+        n = weight.shape[:1]
+        for name, t, shape in (("bias", bias, n), ("residual", residual, x.shape[:-1] + n)):
+            if t is not None and (t.shape != shape or t.dtype is not out_dtype or t.device != x.device):
+                raise RuntimeError(f"verace_amd: {name} must be {tuple(shape)} {out_dtype} on {x.device}, "
+                                   f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     return out_dtype
 
 
 def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dtype):
     N, K = weight.shape
-    x2, w, r = _rows(x), _rows(weight), _plain_rows(residual, N)
-    M = x2.shape[0]
-    out = torch.empty(*x.shape[:-1], N, device=x.device, dtype=out_dtype)
+    x2, xp, ldx = _operand(x, K)
+    w, wp, ldw = _operand(weight, K)
+    r, rp, ldr = _plain_rows(residual, N)
+    bias = _vector(bias)
+    out = x.new_empty(x.shape[:-1] + (N,), dtype=out_dtype)
+    if x_scale is not None:
+        x_scale, weight_scale = _vector(x_scale), _vector(weight_scale)
     with device_guard(x):
         _lib.check(_lib.load().vmi_linear_add(
-            address(x2), _ld(x2), address(_vector(x_scale)), address(w), _ld(w), address(_vector(weight_scale)), _code(x.dtype),
-            address(_vector(bias)), address(r), 0 if r is None else r.stride(0) if M > 1 else N, act, address(out), N,
-            _lib.dtype_code(out_dtype), M, N, K, _lib.raw_stream(x.device)), "vmi_linear_add")
+            xp, ldx, address(x_scale), wp, ldw, address(weight_scale), _code(x.dtype), address(bias), rp, ldr, act, out.data_ptr(), N,
+            _lib.dtype_code(out_dtype), _rows_of(x, K), N, K, _lib.raw_stream(x.device)), "vmi_linear_add")
     return out
 
 
@@ -253,8 +285,11 @@ def _launch_linear_bwd(x, weight, bias, act, dy, need):
     if dy.shape != x.shape[:-1] + (N,) or dy.dtype != x.dtype or dy.device != x.device:
         raise RuntimeError(f"verace_amd: dy must be {tuple(x.shape[:-1] + (N,))} {x.dtype} on {x.device}, "
                            f"got {tuple(dy.shape)} {dy.dtype} on {dy.device}")
-    x2, w, dy2 = _rows(x), _rows(weight), _rows(dy)
-    M = x2.shape[0]
+    x2, xp, ldx = _operand(x, K)
+    w, wp, ldw = _operand(weight, K)
+    dy2, dyp, lddy = _operand(dy, N)
+    bias = _vector(bias)
+    M = _rows_of(x, K)
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
     dw = torch.empty(N, K, device=x.device, dtype=x.dtype) if need[1] else None
     db = torch.empty(N, device=x.device, dtype=x.dtype) if need[2] and bias is not None else None
@@ -262,8 +297,8 @@ def _launch_linear_bwd(x, weight, bias, act, dy, need):
     ws, ws_bytes = _workspace("vmi_linear_add_bwd_workspace_bytes", M, N, K, code, act, device=x.device)
     with device_guard(x):
         _lib.check(_lib.load().vmi_linear_add_bwd(
-            address(x2), _ld(x2), address(w), _ld(w), code, address(_vector(bias)), act, address(dy2), _ld(dy2), address(dx),
-            address(dw), address(db), M, N, K, address(ws), ws_bytes, _lib.raw_stream(x.device)), "vmi_linear_add_bwd")
+            xp, ldx, wp, ldw, code, address(bias), act, dyp, lddy, address(dx), address(dw), address(db), M, N, K, address(ws),
+            ws_bytes, _lib.raw_stream(x.device)), "vmi_linear_add_bwd")
     return dx, dw, db
 
 
@@ -319,33 +354,35 @@ def linear_add(
 # ------------------------------------------------------------------------------------ rows in 8 bits
 
 def _quant_check(a, residual, norm_weight) -> None:
-    _require_device(a, "a")
-    _lib.dtype_code(a.dtype)
-    if a.dim() < 1 or a.shape[-1] < 1:
-        raise RuntimeError(f"verace_amd: rows must be [..., d], got {tuple(a.shape)}")
-    if residual is not None and (residual.shape != a.shape or residual.dtype != a.dtype or residual.device != a.device):
-        raise RuntimeError(f"verace_amd: residual must be {tuple(a.shape)} {a.dtype} on {a.device}, "
+    if not a.is_cuda:
+        _require_device(a, "a")
+    dtype, shape = a.dtype, a.shape
+    _lib.dtype_code(dtype)
+    if len(shape) < 1 or shape[-1] < 1:
+        raise RuntimeError(f"verace_amd: rows must be [..., d], got {tuple(shape)}")
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype or residual.device != a.device):
+        raise RuntimeError(f"verace_amd: residual must be {tuple(shape)} {dtype} on {a.device}, "
                            f"got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
-    d = a.shape[-1]
-    if norm_weight is not None and (tuple(norm_weight.shape) != (d,) or norm_weight.dtype not in (a.dtype, torch.float32)
+    if norm_weight is not None and (norm_weight.shape != shape[-1:] or norm_weight.dtype not in (dtype, torch.float32)
                                     or norm_weight.device != a.device):
-        raise RuntimeError(f"verace_amd: norm_weight must be [{d}] {a.dtype} or float32 on {a.device}, "
+        raise RuntimeError(f"verace_amd: norm_weight must be [{shape[-1]}] {dtype} or float32 on {a.device}, "
                            f"got {tuple(norm_weight.shape)} {norm_weight.dtype} on {norm_weight.device}")
 
 
 def _launch_quant(a, residual, weight, norm: bool, eps: float, want_sum: bool):
-    d = a.shape[-1]
-    a2, r2 = _plain_rows(a, d), _plain_rows(residual, d)
+    shape = a.shape
+    d = shape[-1]
+    a2, ap, lda = _plain_rows(a, d)
+    r2, rp, ldr = _plain_rows(residual, d)
     w = _vector(weight)
-    q = torch.empty(a.shape, device=a.device, dtype=E4M3)
-    scale = torch.empty(a.shape[:-1], device=a.device, dtype=torch.float32)
-    s = torch.empty(a.shape, device=a.device, dtype=a.dtype) if want_sum else None
+    q = torch.empty(shape, device=a.device, dtype=E4M3)
+    scale = torch.empty(shape[:-1], device=a.device, dtype=torch.float32)
+    s = torch.empty(shape, device=a.device, dtype=a.dtype) if want_sum else None
     code = _lib.dtype_code(a.dtype)
     with device_guard(a):
         _lib.check(_lib.load().vmi_norm_add_quant(
-            address(a2), a2.stride(0), address(r2), 0 if r2 is None else r2.stride(0), address(w), code,
-            code if w is None else _lib.dtype_code(w.dtype), int(norm), eps, address(s), address(q), address(scale),
-            a2.shape[0], d, _lib.raw_stream(a.device)), "vmi_norm_add_quant")
+            ap, lda, rp, ldr, address(w), code, code if w is None else _lib.dtype_code(w.dtype), norm, eps, address(s), q.data_ptr(),
+            scale.data_ptr(), scale.numel(), d, _lib.raw_stream(a.device)), "vmi_norm_add_quant")
     return s, q, scale
 
 
