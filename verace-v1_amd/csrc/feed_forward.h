@@ -43,76 +43,141 @@ struct Args {
   int act;
   float beta1, beta2;
   int vec;                 // rows of out and other are whole 16-byte pieces
+  int ws_vec, bias_vec;    // ws and ws2, bias start on 16 bytes
 };
 
 template <typename E> struct memory { typedef E type; };
 template <> struct memory<__bf16> { typedef bf16_t type; };
 
-// act(z) and its derivative of the ungated projection.
-template <typename T> __device__ __forceinline__ float activate(float z, int act) {
-  if (act == ACT_SILU) return z * sigmoid_for<T>(z);
-  if (act == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.707106781f));
-  return z;
-}
-template <typename T> __device__ __forceinline__ float slope(float z, int act) {
+// act(z) of the ungated projection, and its derivative.
+template <typename T, int W> __device__ __forceinline__ void activate_all(float (&z)[W], int act) {
   if (act == ACT_SILU) {
-    const float s = sigmoid_for<T>(z);
-    return s * (1.f + z * (1.f - s));
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] *= sigmoid_for<T>(z[j]);
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] = 0.5f * z[j] * (1.f + erff(z[j] * 0.707106781f));
   }
-  if (act == ACT_GELU) {
-    const float e = sizeof(T) == 4 ? expf(-0.5f * z * z) : __expf(-0.5f * z * z);
-    return 0.5f * (1.f + erff(z * 0.707106781f)) + z * 0.398942280f * e;
+}
+template <typename T, int W> __device__ __forceinline__ void slope_all(float (&z)[W], int act) {
+  if (act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float s = sigmoid_for<T>(z[j]);
+      z[j] = s * (1.f + z[j] * (1.f - s));
+    }
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float e = sizeof(T) == 4 ? expf(-0.5f * z[j] * z[j]) : __expf(-0.5f * z[j] * z[j]);
+      z[j] = 0.5f * (1.f + erff(z[j] * 0.707106781f)) + z[j] * 0.398942280f * e;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] = 1.f;
   }
-  return 1.f;
 }
 struct Gate {
   int act;
   float b1, b2, i1, i2;
 };
-// The parts of tanh(x) = sign(x) num / den: (1 - e) / (1 + e) with e = exp(-2|x|), and near 0, where 1 - e cancels, a polynomial
-// (the next term is below 2^-24 of it) over 1.
-template <typename T> __device__ __forceinline__ void tanh_parts(float x, float& num, float& den) {
-  const float a = fabsf(x), x2 = x * x;
-  const float e = __expf(-2.f * a);
-  const float near = a + a * x2 * (-0.333333333f + x2 * (0.133333333f + x2 * -0.0539682540f));
-  num = x2 < 0.01f ? near : 1.f - e;
-  den = x2 < 0.01f ? 1.f : 1.f + e;
+// For 16-bit results both tanh and the sigmoid come from exponentials of at most 1 and one reciprocal:
+//   tanh(|g| / b1) = (1 - a) / (1 + a), a = exp(-2 |g| / b1);  sigmoid(|g|) = 1 / (1 + b), b = exp(-|g|)
+// and where 1 - a cancels, tanh from a polynomial (relative error 2^-23 below 0.1).  The other factor's tanh is a polynomial
+// below 0.6 (2^-22), where all of a wave's values are in nearly every epilogue.
+struct Parts {
+  float a, b, num, den;  // tanh = num / (1 + a), den = (1 + a) (1 + b)
+};
+__device__ __forceinline__ Parts gate_parts(float g, const Gate& c) {
+  constexpr float kLog2e = 1.44269504f;
+  Parts r;
+  const float x = fabsf(g) * c.i1, x2 = x * x;
+  r.a = __builtin_amdgcn_exp2f(x * (-2.f * kLog2e));
+  r.b = __builtin_amdgcn_exp2f(fabsf(g) * -kLog2e);
+  const float near = x * (0.999999998f + x2 * (-0.333330316f + x2 * 0.132527533f)), t = 1.f + r.b;
+  r.num = x2 < 0.01f ? fmaf(near, r.a, near) : 1.f - r.a;
+  r.den = fmaf(r.a, t, t);
+  return r;
 }
-// a(g) b(u).  16-bit results: the quotients of the two tanh and the sigmoid over one reciprocal, their exponentials at most 1.
-template <typename T> __device__ __forceinline__ float gated(float g, float u, const Gate& c) {
-  if (c.act == ACT_SILU) return g * sigmoid_for<T>(g) * u;
-  if constexpr (sizeof(T) == 4) return c.b1 * tanhf(g * c.i1) * sigmoid_for<T>(g) * (c.b2 * tanhf(u * c.i2));
-  float n1, d1, n2, d2;
-  tanh_parts<T>(g * c.i1, n1, d1);
-  tanh_parts<T>(u * c.i2, n2, d2);
-  const float e = __expf(-fabsf(g)), s = g < 0.f ? e : 1.f;  // sigmoid(g) = s / (1 + e)
-  const float h = c.b1 * c.b2 * n1 * n2 * s * __builtin_amdgcn_rcpf(d1 * d2 * (1.f + e));
-  return (__float_as_uint(g) ^ __float_as_uint(u)) >> 31 ? -h : h;
+__device__ __forceinline__ float tanh_below(float x) {
+  const float x2 = x * x;
+  return x * (0.999999927f + x2 * (-0.333323102f + x2 * (0.133101752f + x2 * (-0.0521015118f + x2 * 0.0154754365f))));
 }
-template <typename T>
-__device__ __forceinline__ void gated_slopes(float g, float u, float dh, const Gate& c, float& dg, float& du) {
-  if (c.act == ACT_SILU) {
-    const float s = sigmoid_for<T>(g);
-    dg = dh * u * s * (1.f + g * (1.f - s));
-    du = dh * g * s;
+__device__ __forceinline__ float tanh_any(float x) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(x) * (-2.f * 1.44269504f));
+  const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+  return x * x < 0.36f ? tanh_below(x) : far;
+}
+// tanh(u / b2) of W values
+template <typename T, int W> __device__ __forceinline__ void tanh_all(const float (&u)[W], float scale, float (&t)[W]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) t[j] = tanhf(u[j] * scale);
     return;
   }
-  float s, ns, t1, t2;  // sigmoid(g) and sigmoid(-g)
-  if constexpr (sizeof(T) == 4) {
-    s = sigmoid_for<T>(g), ns = sigmoid_for<T>(-g);
-    t1 = tanhf(g * c.i1), t2 = tanhf(u * c.i2);
-  } else {
-    float n1, d1, n2, d2;
-    tanh_parts<T>(g * c.i1, n1, d1);
-    tanh_parts<T>(u * c.i2, n2, d2);
-    const float e = __expf(-fabsf(g)), d3 = 1.f + e, d12 = d1 * d2, r = __builtin_amdgcn_rcpf(d12 * d3);
-    const float big = d12 * r, small = e * big;
-    s = g < 0.f ? small : big, ns = g < 0.f ? big : small;
-    t1 = copysignf(n1 * (d2 * d3) * r, g), t2 = copysignf(n2 * (d1 * d3) * r, u);
+  bool below = true;
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    t[j] = u[j] * scale;
+    below = below && fabsf(t[j]) < 0.6f;
   }
-  const float a = c.b1 * t1 * s;
-  dg = dh * c.b2 * t2 * (s * (1.f - t1 * t1) + a * ns);
-  du = dh * a * (1.f - t2 * t2);
+  if (__all(below)) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) t[j] = tanh_below(t[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) t[j] = tanh_any(t[j]);
+  }
+}
+// g = a(g) b(u)
+template <typename T, int W> __device__ __forceinline__ void gated(float (&g)[W], const float (&u)[W], const Gate& c) {
+  if (c.act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) g[j] = g[j] * sigmoid_for<T>(g[j]) * u[j];
+    return;
+  }
+  float t[W];
+  tanh_all<T, W>(u, c.i2, t);
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      g[j] = c.b1 * tanhf(g[j] * c.i1) * sigmoid_for<T>(g[j]) * (c.b2 * t[j]);
+    } else {
+      const Parts r = gate_parts(g[j], c);
+      const float s = g[j] < 0.f ? -r.b : 1.f;  // the sign, and sigmoid(g) = b / (1 + b) below 0
+      g[j] = r.num * s * __builtin_amdgcn_rcpf(r.den) * (c.b1 * c.b2 * t[j]);
+    }
+  }
+}
+// g, u = dh a'(g) b(u), dh a(g) b'(u)
+template <typename T, int W>
+__device__ __forceinline__ void gated_slopes(float (&g)[W], float (&u)[W], const float (&dh)[W], const Gate& c) {
+  if (c.act == ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float s = sigmoid_for<T>(g[j]), a = g[j] * s;
+      g[j] = dh[j] * u[j] * (s + a * (1.f - s));
+      u[j] = dh[j] * a;
+    }
+    return;
+  }
+  float t2[W];
+  tanh_all<T, W>(u, c.i2, t2);
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    float s, ns, t1;  // sigmoid(g), sigmoid(-g), tanh
+    if constexpr (sizeof(T) == 4) {
+      s = sigmoid_for<T>(g[j]), ns = sigmoid_for<T>(-g[j]), t1 = tanhf(g[j] * c.i1);
+    } else {
+      const Parts r = gate_parts(g[j], c);
+      const float q = __builtin_amdgcn_rcpf(r.den), big = fmaf(r.a, q, q), small = r.b * big;
+      t1 = copysignf(r.num * fmaf(r.b, q, q), g[j]);
+      s = g[j] < 0.f ? small : big, ns = g[j] < 0.f ? big : small;
+    }
+    const float a = c.b1 * t1 * s;
+    g[j] = dh[j] * (c.b2 * t2[j]) * (s * (1.f - t1 * t1) + a * ns);
+    u[j] = dh[j] * a * (1.f - t2[j] * t2[j]);
+  }
 }
 
 // W consecutive elements of a row from column n, zeros from `n_end` on.
@@ -143,24 +208,40 @@ template <typename T, int W> __device__ __forceinline__ void store_cols(T* row, 
   }
 }
 
+// What the epilogue needs of W consecutive columns from n, for all of a lane's rows.
+template <int W> struct Columns {
+  float ws[W], ws2[W], bias[W];
+};
+template <typename E, typename T, int KIND, int W> __device__ __forceinline__ Columns<W> columns_at(const Args& p, int n) {
+  Columns<W> c = {};
+  if constexpr (sizeof(E) == 1) {
+    load_cols<float, W>(p.ws, n, p.n, p.ws_vec, c.ws);
+    if constexpr (KIND == GATED) load_cols<float, W>(p.ws2, n, p.n, p.ws_vec, c.ws2);
+  }
+  if constexpr (KIND == LINEAR || KIND == LINEAR_DZ)
+    if (p.bias != nullptr) load_cols<T, W>(static_cast<const T*>(p.bias), n, p.n, p.bias_vec, c.bias);
+  return c;
+}
+
 // The lane's columns of one row of one product (two for the gated kinds), W consecutive ones from n.
 template <typename E, typename T, int KIND, int W>
-__device__ __forceinline__ void finish(const Args& p, int m, int n, float (&z)[W], float (&z2)[W], float xs, int split) {
+__device__ __forceinline__ void finish(const Args& p, int m, int n, const Columns<W>& c, float (&z)[W], float (&z2)[W], float xs, int split) {
   const bool vec = p.vec;
+  if constexpr (sizeof(E) == 1) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      z[j] *= xs * c.ws[j];
+      if constexpr (KIND == GATED) z2[j] *= xs * c.ws2[j];
+    }
+  }
   if constexpr (KIND == LINEAR || KIND == LINEAR_DZ) {
     float t[W];
-    if constexpr (sizeof(E) == 1) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) z[j] *= xs * (n + j < p.n ? p.ws[n + j] : 0.f);
-    }
     if (p.bias != nullptr) {
-      load_cols<T, W>(static_cast<const T*>(p.bias), n, p.n, false, t);
 #pragma unroll
-      for (int j = 0; j < W; ++j) z[j] += t[j];
+      for (int j = 0; j < W; ++j) z[j] += c.bias[j];
     }
     if constexpr (KIND == LINEAR) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) z[j] = activate<T>(z[j], p.act);
+      activate_all<T, W>(z, p.act);
       if (p.other != nullptr) {
         load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, t);
 #pragma unroll
@@ -169,33 +250,25 @@ __device__ __forceinline__ void finish(const Args& p, int m, int n, float (&z)[W
       store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, vec, z);
     } else {
       load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, t);
+      slope_all<T, W>(z, p.act);
       // up to the row's end: the columns past the last are read as the contraction's of a later product
 #pragma unroll
-      for (int j = 0; j < W; ++j) z[j] = n + j < p.n ? t[j] * slope<T>(z[j], p.act) : 0.f;
+      for (int j = 0; j < W; ++j) z[j] = n + j < p.n ? t[j] * z[j] : 0.f;
       store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, static_cast<int>(p.ldo), vec, z);
     }
   } else if constexpr (KIND == GATED || KIND == GATED_DZ) {
-    const Gate c{p.act, p.beta1, p.beta2, 1.f / p.beta1, 1.f / p.beta2};
-    if constexpr (sizeof(E) == 1) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        z[j] *= xs * (n + j < p.n ? p.ws[n + j] : 0.f);
-        z2[j] *= xs * (n + j < p.n ? p.ws2[n + j] : 0.f);
-      }
-    }
+    const Gate gate{p.act, p.beta1, p.beta2, 1.f / p.beta1, 1.f / p.beta2};
     if constexpr (KIND == GATED) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) z[j] = gated<T>(z[j], z2[j], c);
+      gated<T, W>(z, z2, gate);
       store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, vec, z);
     } else {
       float dh[W];
       load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, dh);
+      gated_slopes<T, W>(z, z2, dh, gate);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        float dg = 0.f, du = 0.f;
-        if (n + j < p.n) gated_slopes<T>(z[j], z2[j], dh[j], c, dg, du);
-        z[j] = dg;
-        z2[j] = du;
+        z[j] = n + j < p.n ? z[j] : 0.f;
+        z2[j] = n + j < p.n ? z2[j] : 0.f;
       }
       T* row = static_cast<T*>(p.out) + m * p.ldo;
       store_cols<T, W>(row, n, static_cast<int>(p.second), vec, z);
@@ -260,25 +333,24 @@ void product_kernel(Args p) {
   auto write = [&](auto tag) {
     using T = decltype(tag);
 #pragma unroll
-    for (int hm = 0; hm < 2; ++hm)
+    for (int hn = 0; hn < (PAIR ? 1 : 2); ++hn)
 #pragma unroll
-      for (int f = 0; f < S::MF; ++f) {
-        const int m = m0 + hm * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
-        if (m >= p.m) continue;
-        float xs = 1.f;
-        if constexpr (SIZE == 1) xs = p.xs[m];
+      for (int q = 0; q < PARTS; ++q) {
+        const int n = n0 + hn * S::HN + column_of<S, PERM>(wn, lane, q);
+        const Columns<W> cols = columns_at<E, T, KIND, W>(p, n);
 #pragma unroll
-        for (int hn = 0; hn < (PAIR ? 1 : 2); ++hn)
+        for (int hm = 0; hm < 2; ++hm)
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
-            const int n = n0 + hn * S::HN + column_of<S, PERM>(wn, lane, q);
+          for (int f = 0; f < S::MF; ++f) {
+            const int m = m0 + hm * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
+            if (m >= p.m) continue;
             float z[W], z2[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
               z[j] = acc.v[hm][hn][f][PERM ? j / 4 : q][j % 4];
               z2[j] = PAIR ? acc.v[hm][1][f][PERM ? j / 4 : q][j % 4] : 0.f;
             }
-            finish<E, T, KIND, W>(p, m, n, z, z2, xs, split);
+            finish<E, T, KIND, W>(p, m, n, cols, z, z2, SIZE == 1 ? p.xs[m] : 1.f, split);
           }
       }
   };
@@ -292,8 +364,8 @@ void product_kernel(Args p) {
 }
 
 typedef Shape<128, 128, 2, 4> Large;
-typedef Shape<128, 64, 2, 4> Tall;
-typedef Shape<64, 64, 2, 4> Middle;
+typedef Shape<128, 64, 4, 2> Tall;
+typedef Shape<64, 64, 4, 2> Middle;
 typedef Shape<32, 32, 2, 2> Small;
 
 // kind over operands of one type (feed_forward_*.hip).

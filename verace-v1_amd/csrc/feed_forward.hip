@@ -172,6 +172,7 @@ extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, 
   p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
   p.bias = bias, p.other = residual, p.ldother = ldr, p.act = act, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
   p.vec = out_vectors(out, ldo, residual, ldr, size_of(out_dtype));
+  p.ws_vec = aligned16({w_scale}), p.bias_vec = aligned16({bias});
   return product(dtype, LINEAR, p, static_cast<hipStream_t>(stream));
 }
 
@@ -194,7 +195,7 @@ extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale
   p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.xs = x_scale, p.ws = gate_scale, p.ws2 = up_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(F), p.k = static_cast<int>(K);
   p.act = act, p.beta1 = beta1, p.beta2 = beta2, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
-  p.vec = out_vectors(out, ldo, nullptr, 0, size_of(out_dtype));
+  p.vec = out_vectors(out, ldo, nullptr, 0, size_of(out_dtype)), p.ws_vec = aligned16({gate_scale, up_scale});
   return product(dtype, GATED, p, static_cast<hipStream_t>(stream));
 }
 
@@ -229,7 +230,7 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
       Args p{};
       p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
       p.bias = bias, p.other = dy, p.ldother = lddy, p.act = act, p.out = const_cast<void*>(dz), p.ldo = lddz;
-      p.vec = out_vectors(dz, lddz, dy, lddy, size);
+      p.vec = out_vectors(dz, lddz, dy, lddy, size), p.bias_vec = aligned16({bias});
       if (const int st = product(dtype, LINEAR_DZ, p, s); st != VMI_OK) return st;
     }
   }

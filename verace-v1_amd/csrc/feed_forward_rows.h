@@ -73,7 +73,7 @@ template <typename E, int KIND, int MT> __global__ __launch_bounds__(512, 2) voi
         z[0] += part[v][0][m][c];
         if constexpr (PAIR) z2[0] += part[v][1][m][c];
       }
-      finish<E, T, KIND, 1>(p, m, n0 + c, z, z2, sizeof(E) == 1 ? p.xs[m] : 1.f, 0);
+      finish<E, T, KIND, 1>(p, m, n0 + c, columns_at<E, T, KIND, 1>(p, n0 + c), z, z2, sizeof(E) == 1 ? p.xs[m] : 1.f, 0);
     }
   };
   if constexpr (sizeof(E) == 1) {

@@ -3,19 +3,17 @@
 // (the same tensors in a backward pass).  The epilogue gets the accumulators.
 //
 // A tile has two pieces of HM rows of A and two of HN rows of B; 128 bytes of k are a step.  A step's four pieces lie in one
-// of two LDS stages, filled by direct loads two steps ahead, a piece a phase.  A phase reads one piece into registers, issues the
-// loads of the piece that went free a phase ago, and multiplies A's piece with B's:
+// of two LDS stages, filled by direct loads.  A step has two phases; a phase reads two pieces into registers, issues the loads
+// of two that went free a phase ago, and multiplies A's piece with both of B's:
 //
-//     phase   reads             loads of step t + 2   product
-//       0     A0                B0                    A0 B0
-//       1     B1                A0                    A0 B1
-//       2     A1                B1                    A1 B0
-//       3     B0 of step t + 1  A1                    A1 B1
+//     phase   reads                   loads                              products
+//       P     A0, B1                  B0 of step t + 2, A1 of t + 1      A0 B0, A0 B1
+//       Q     A1, B0 of step t + 1    A0 of step t + 2, B1 of t + 2      A1 B0, A1 B1
 //
 // A barrier ends the reading and the multiplying half of each phase.  With two waves a SIMD the halves of the workgroup go
 // one half-phase apart, so one wave of a SIMD multiplies while the other reads (STAGGER).  A wave waits for its own loads
-// of a piece at the end of the reading half before the one that reads it, one barrier ahead of every reader, with the six
-// pieces issued later still in flight: about 3000 clocks to cover the latency of HBM.
+// of a piece at the end of the reading half before the one that reads it, one barrier ahead of every reader, with the four
+// pieces issued later still in flight.
 //
 // LDS is read at 16 bytes a lane (k contiguous), by transposing reads of 8 (m contiguous, 16 bits) or 4 bytes a lane (fp32),
 // and its 16-byte slots are permuted so that the lanes of an access fall in distinct banks.  The direct loads write LDS in
@@ -92,7 +90,7 @@ template <int HM_, int HN_, int WM_, int WN_> struct Shape {
   static constexpr int MF = HM / (16 * WM), NF = HN / (16 * WN);
   static constexpr int LA = HM * 8 / THREADS, LB = HN * 8 / THREADS;  // loads of a thread for a piece
   static constexpr int A_BYTES = HM * 128, B_BYTES = HN * 128, STAGE = 2 * (A_BYTES + B_BYTES);
-  static constexpr int FLIGHT = 3 * (LA + LB);  // the loads of six pieces
+  static constexpr int FLIGHT = 2 * (LA + LB);  // the loads of four pieces
   static constexpr bool STAGGER = WM * WN == 8;
   static_assert(LA >= 1 && LB >= 1 && MF >= 1 && NF >= 1);
 };
@@ -255,55 +253,57 @@ __device__ __forceinline__ void tile_product(Operands& o, char* lds, Acc<S>& acc
       for (int m = 0; m < S::MF; ++m)
 #pragma unroll
         for (int n = 0; n < S::NF; ++n) acc.v[hm][hn][m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Frag a[S::MF], b0[S::NF], b1[S::NF];
-  auto multiply = [&](f32x4 (&c)[S::MF][S::NF], const Frag (&b)[S::NF]) {
+  Frag a[S::MF], b0[S::NF], b0_next[S::NF], b1[S::NF];
+  auto multiply = [&](f32x4 (&c0)[S::MF][S::NF], f32x4 (&c1)[S::MF][S::NF], const Frag (&x0)[S::NF]) {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int m = 0; m < S::MF; ++m)
 #pragma unroll
-      for (int n = 0; n < S::NF; ++n) c[m][n] = mma<E>(b[n], a[m], c[m][n]);
+      for (int n = 0; n < S::NF; ++n) c0[m][n] = mma<E>(x0[n], a[m], c0[m][n]);
+#pragma unroll
+    for (int m = 0; m < S::MF; ++m)
+#pragma unroll
+      for (int n = 0; n < S::NF; ++n) c1[m][n] = mma<E>(b1[n], a[m], c1[m][n]);
     __builtin_amdgcn_s_setprio(0);
   };
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    issue_b(0, t);
-    issue_a(0, t);
-    issue_b(1, t);
-    issue_a(1, t);
-  }
+  auto step = [&](int t, Frag (&x0)[S::NF], Frag (&x0_next)[S::NF]) {
+    const char* st = lds + (t & 1) * S::STAGE;
+    ra.read(st + at_a[0], a);
+    rb.read(st + at_b[1], b1);
+    issue_b(0, t + 2);
+    issue_a(1, t + 1);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[0][0], acc.v[0][1], x0);
+    barrier();
+    ra.read(st + at_a[1], a);
+    rb.read(lds + ((t + 1) & 1) * S::STAGE + at_b[0], x0_next);
+    issue_a(0, t + 2);
+    issue_b(1, t + 2);
+    wait_loads_and_lds<S::FLIGHT>();
+    barrier();
+    multiply(acc.v[1][0], acc.v[1][1], x0);
+    barrier();
+  };
+  issue_b(0, 0);
+  issue_a(0, 0);
+  issue_b(1, 0);
+  issue_b(0, 1);
+  issue_a(1, 0);
+  issue_a(0, 1);
+  issue_b(1, 1);
   wait_loads_and_lds<S::FLIGHT>();
   barrier();
   rb.read(lds + at_b[0], b0);
   wait_loads_and_lds<S::FLIGHT>();
   barrier();
   if (S::STAGGER && wave >= S::WM * S::WN / 2) barrier();
-  for (int t = 0; t < total; ++t) {
-    const char* st = lds + (t & 1) * S::STAGE;
-    ra.read(st + at_a[0], a);
-    issue_b(0, t + 2);
-    wait_loads_and_lds<S::FLIGHT>();
-    barrier();
-    multiply(acc.v[0][0], b0);
-    barrier();
-    rb.read(st + at_b[1], b1);
-    issue_a(0, t + 2);
-    wait_loads_and_lds<S::FLIGHT>();
-    barrier();
-    multiply(acc.v[0][1], b1);
-    barrier();
-    ra.read(st + at_a[1], a);
-    issue_b(1, t + 2);
-    wait_loads_and_lds<S::FLIGHT>();
-    barrier();
-    multiply(acc.v[1][0], b0);
-    barrier();
-    rb.read(lds + ((t + 1) & 1) * S::STAGE + at_b[0], b0);
-    issue_a(1, t + 2);
-    wait_loads_and_lds<S::FLIGHT>();
-    barrier();
-    multiply(acc.v[1][1], b1);
-    barrier();
+  int t = 0;
+  for (; t + 1 < total; t += 2) {
+    step(t, b0, b0_next);
+    step(t + 1, b0_next, b0);
   }
+  if (t < total) step(t, b0, b0_next);
   if (S::STAGGER && wave < S::WM * S::WN / 2) barrier();
   wait_loads_and_lds<0>();  // no load may write LDS after the workgroup's end
 }
