@@ -543,7 +543,7 @@ int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t
 
 /* Root-mean-square norm with the residual's addition and a result in 8 bits:
  *   s = a + residual,  n = s w / sqrt(mean s^2 + eps) (norm = 0: n = s w),
- *   scale = max(max|n| / 448, 2^-126),  q = e4m3(n / scale), each rounded once from 64 bits
+ *   scale = max(max|n| / 448, 2^-126),  q = e4m3(n / scale), q rounded once from 64 bits
  * over rows of d elements, a_stride and r_stride apart; residual, w [d] (dtype or float32) and sum (s, dtype) may be NULL;
  * sum, q [rows, d] and scale [rows] are contiguous.  A row with a NaN or an infinity in s w has NaN for scale and q. */
 int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* residual, int64_t r_stride, const void* w,

@@ -42,8 +42,6 @@ struct Args {
   int seg, seg_valid;      // DW: rows of the result come in segments of seg, of which seg_valid are stored
   int act;
   float beta1, beta2;
-  int vec;                 // rows of out and other are whole 16-byte pieces
-  int ws_vec, bias_vec;    // ws and ws2, bias start on 16 bytes
 };
 
 template <typename E> struct memory { typedef E type; };
@@ -180,31 +178,30 @@ __device__ __forceinline__ void gated_slopes(float (&g)[W], float (&u)[W], const
   }
 }
 
-// W consecutive elements of a row from column n, zeros from `n_end` on.
-template <typename T, int W> __device__ __forceinline__ void load_cols(const T* row, int n, int n_end, bool vec, float (&x)[W]) {
-  if (vec && n + W <= n_end) {
-    typedef typename native<T>::type N;
-    typedef N Piece __attribute__((ext_vector_type(W)));
-    const Piece v = *reinterpret_cast<const Piece*>(row + n);
+// W consecutive elements of a row from column n, zeros from `n_end` on.  Rows start anywhere: the hardware takes vectors at any
+// address.  FULL: none is beyond.
+template <typename T, int W, bool FULL = false> __device__ __forceinline__ void load_cols(const T* row, int n, int n_end, float (&x)[W]) {
+  if (FULL || n + W <= n_end) {
+    T v[W];
+    __builtin_memcpy(v, row + n, sizeof(v));
 #pragma unroll
-    for (int j = 0; j < W; ++j) x[j] = static_cast<float>(v[j]);
+    for (int j = 0; j < W; ++j) x[j] = io<T>::to_f32(v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j) x[j] = n + j < n_end ? io<T>::load(row, n + j) : 0.f;
   }
 }
-template <typename T, int W> __device__ __forceinline__ void store_cols(T* row, int n, int n_end, bool vec, const float (&x)[W]) {
-  if (vec && n + W <= n_end) {
-    typedef typename native<T>::type N;
-    typedef N Piece __attribute__((ext_vector_type(W)));
-    Piece v;
+template <typename T, int W, bool FULL = false> __device__ __forceinline__ void store_cols(T* row, int n, int n_end, const float (&x)[W]) {
+  typedef typename native<T>::type N;
+  N v[W];
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = static_cast<N>(x[j]);
-    *reinterpret_cast<Piece*>(row + n) = v;
+  for (int j = 0; j < W; ++j) v[j] = static_cast<N>(x[j]);
+  if (FULL || n + W <= n_end) {
+    __builtin_memcpy(row + n, v, sizeof(v));
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j)
-      if (n + j < n_end) io<T>::store(row, n + j, x[j]);
+      if (n + j < n_end) __builtin_memcpy(row + n + j, v + j, sizeof(T));
   }
 }
 
@@ -212,21 +209,22 @@ template <typename T, int W> __device__ __forceinline__ void store_cols(T* row, 
 template <int W> struct Columns {
   float ws[W], ws2[W], bias[W];
 };
-template <typename E, typename T, int KIND, int W> __device__ __forceinline__ Columns<W> columns_at(const Args& p, int n) {
+template <typename E, typename T, int KIND, int W, bool FULL = false> __device__ __forceinline__ Columns<W> columns_at(const Args& p, int n) {
   Columns<W> c = {};
   if constexpr (sizeof(E) == 1) {
-    load_cols<float, W>(p.ws, n, p.n, p.ws_vec, c.ws);
-    if constexpr (KIND == GATED) load_cols<float, W>(p.ws2, n, p.n, p.ws_vec, c.ws2);
+    load_cols<float, W, FULL>(p.ws, n, p.n, c.ws);
+    if constexpr (KIND == GATED) load_cols<float, W, FULL>(p.ws2, n, p.n, c.ws2);
   }
   if constexpr (KIND == LINEAR || KIND == LINEAR_DZ)
-    if (p.bias != nullptr) load_cols<T, W>(static_cast<const T*>(p.bias), n, p.n, p.bias_vec, c.bias);
+    if (p.bias != nullptr) load_cols<T, W, FULL>(static_cast<const T*>(p.bias), n, p.n, c.bias);
   return c;
 }
 
 // The lane's columns of one row of one product (two for the gated kinds), W consecutive ones from n.
-template <typename E, typename T, int KIND, int W>
-__device__ __forceinline__ void finish(const Args& p, int m, int n, const Columns<W>& c, float (&z)[W], float (&z2)[W], float xs, int split) {
-  const bool vec = p.vec;
+// other: the row's residual (dy, dh) where the caller has read it.
+template <typename E, typename T, int KIND, int W, bool FULL = false>
+__device__ __forceinline__ void finish(const Args& p, int m, int n, const Columns<W>& c, float (&z)[W], float (&z2)[W], float xs, int split,
+                                       const float* other = nullptr) {
   if constexpr (sizeof(E) == 1) {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
@@ -243,48 +241,58 @@ __device__ __forceinline__ void finish(const Args& p, int m, int n, const Column
     if constexpr (KIND == LINEAR) {
       activate_all<T, W>(z, p.act);
       if (p.other != nullptr) {
-        load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, t);
+        if (other == nullptr) load_cols<T, W, FULL>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, t);
 #pragma unroll
-        for (int j = 0; j < W; ++j) z[j] += t[j];
+        for (int j = 0; j < W; ++j) z[j] += other != nullptr ? other[j] : t[j];
       }
-      store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, vec, z);
+      store_cols<T, W, FULL>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, z);
     } else {
-      load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, t);
+      load_cols<T, W, FULL>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, t);
       slope_all<T, W>(z, p.act);
       // up to the row's end: the columns past the last are read as the contraction's of a later product
 #pragma unroll
-      for (int j = 0; j < W; ++j) z[j] = n + j < p.n ? t[j] * z[j] : 0.f;
-      store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, static_cast<int>(p.ldo), vec, z);
+      for (int j = 0; j < W; ++j) z[j] = FULL || n + j < p.n ? t[j] * z[j] : 0.f;
+      store_cols<T, W, FULL>(static_cast<T*>(p.out) + m * p.ldo, n, static_cast<int>(p.ldo), z);
     }
   } else if constexpr (KIND == GATED || KIND == GATED_DZ) {
     const Gate gate{p.act, p.beta1, p.beta2, 1.f / p.beta1, 1.f / p.beta2};
     if constexpr (KIND == GATED) {
       gated<T, W>(z, z2, gate);
-      store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, vec, z);
+      store_cols<T, W, FULL>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, z);
     } else {
       float dh[W];
-      load_cols<T, W>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, vec, dh);
+      load_cols<T, W, FULL>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, dh);
       gated_slopes<T, W>(z, z2, dh, gate);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        z[j] = n + j < p.n ? z[j] : 0.f;
-        z2[j] = n + j < p.n ? z2[j] : 0.f;
+        z[j] = FULL || n + j < p.n ? z[j] : 0.f;
+        z2[j] = FULL || n + j < p.n ? z2[j] : 0.f;
       }
       T* row = static_cast<T*>(p.out) + m * p.ldo;
-      store_cols<T, W>(row, n, static_cast<int>(p.second), vec, z);
-      store_cols<T, W>(row + p.second, n, static_cast<int>(p.second), vec, z2);
+      store_cols<T, W, FULL>(row, n, static_cast<int>(p.second), z);
+      store_cols<T, W, FULL>(row + p.second, n, static_cast<int>(p.second), z2);
     }
   } else if constexpr (KIND == DX) {
-    store_cols<T, W>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, vec, z);
+    store_cols<T, W, FULL>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, z);
   } else {
     const int s = m / p.seg, r = m - s * p.seg;
     if (r >= p.seg_valid) return;
     const int64_t row = static_cast<int64_t>(s) * p.seg_valid + r;
     if (p.partial != nullptr)
-      store_cols<float, W>(p.partial + (static_cast<int64_t>(split) * (p.m / p.seg) * p.seg_valid + row) * p.n, n, p.n,
-                           p.n % W == 0, z);
+      store_cols<float, W, FULL>(p.partial + (static_cast<int64_t>(split) * (p.m / p.seg) * p.seg_valid + row) * p.n, n, p.n, z);
     else
-      store_cols<T, W>(static_cast<T*>(p.out) + row * p.ldo, n, p.n, vec, z);
+      store_cols<T, W, FULL>(static_cast<T*>(p.out) + row * p.ldo, n, p.n, z);
+  }
+}
+
+// f of the result's type: the operands', or for 8-bit ones that of the call.
+template <typename E, typename F> __device__ __forceinline__ void by_result(const Args& p, F&& f) {
+  if constexpr (sizeof(E) == 1) {
+    if (p.out_dtype == VMI_F32) f(float{});
+    else if (p.out_dtype == VMI_BF16) f(bf16_t{});
+    else f(f16_t{});
+  } else {
+    f(typename memory<E>::type{});
   }
 }
 
@@ -329,38 +337,55 @@ void product_kernel(Args p) {
   else
     tile_product<E, AMN, BMN, S, 1>(o, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  constexpr int W = PERM ? 4 * S::NF : 4, PARTS = PERM ? 1 : S::NF;
-  auto write = [&](auto tag) {
+  constexpr bool SWAP = !PERM && S::NF == 2;
+  constexpr int W = PERM ? 4 * S::NF : SWAP ? 8 : 4, PARTS = PERM || SWAP ? 1 : S::NF;
+  // (C's columns 16 j + 4 g .. of lane group g) to 8 consecutive ones: groups 2 i and 2 i + 1 exchange one of their two fours,
+  // after which group g holds 8 columns of fragment g % 2.
+  if constexpr (SWAP) {
+#pragma unroll
+    for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+      for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+        for (int f = 0; f < S::MF; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f32x4 &lo = acc.v[hm][hn][f][0], &hi = acc.v[hm][hn][f][1];
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo[r]), __float_as_uint(hi[r]), false, false);
+            lo[r] = __uint_as_float(x[0]), hi[r] = __uint_as_float(x[1]);
+          }
+  }
+  auto write = [&](auto tag, auto full) {
     using T = decltype(tag);
+    constexpr bool FULL = decltype(full)::value;
 #pragma unroll
     for (int hn = 0; hn < (PAIR ? 1 : 2); ++hn)
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) {
-        const int n = n0 + hn * S::HN + column_of<S, PERM>(wn, lane, q);
-        const Columns<W> cols = columns_at<E, T, KIND, W>(p, n);
+        const int g = lane >> 4;
+        const int n = n0 + hn * S::HN + (SWAP ? wn * 32 + (g & 1) * 16 + (g >> 1) * 8 : column_of<S, PERM>(wn, lane, q));
+        const Columns<W> cols = columns_at<E, T, KIND, W, FULL>(p, n);
 #pragma unroll
         for (int hm = 0; hm < 2; ++hm)
 #pragma unroll
           for (int f = 0; f < S::MF; ++f) {
             const int m = m0 + hm * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
-            if (m >= p.m) continue;
+            if (!FULL && m >= p.m) continue;
             float z[W], z2[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-              z[j] = acc.v[hm][hn][f][PERM ? j / 4 : q][j % 4];
+              z[j] = acc.v[hm][hn][f][PERM || SWAP ? j / 4 : q][j % 4];
               z2[j] = PAIR ? acc.v[hm][1][f][PERM ? j / 4 : q][j % 4] : 0.f;
             }
-            finish<E, T, KIND, W>(p, m, n, cols, z, z2, SIZE == 1 ? p.xs[m] : 1.f, split);
+            finish<E, T, KIND, W, FULL>(p, m, n, cols, z, z2, SIZE == 1 ? p.xs[m] : 1.f, split);
           }
       }
   };
-  if constexpr (SIZE == 1) {
-    if (p.out_dtype == VMI_F32) write(float{});
-    else if (p.out_dtype == VMI_BF16) write(bf16_t{});
-    else write(f16_t{});
-  } else {
-    write(typename memory<E>::type{});
-  }
+  // most tiles lie inside the result: their accesses need no conditions, which would keep them from being in flight together
+  if (m0 + 2 * S::HM <= p.m && n0 + TN <= p.n)
+    by_result<E>(p, [&](auto tag) { write(tag, std::true_type{}); });
+  else
+    by_result<E>(p, [&](auto tag) { write(tag, std::false_type{}); });
 }
 
 typedef Shape<128, 128, 2, 4> Large;

@@ -22,27 +22,28 @@ __global__ __launch_bounds__(NTH) void join_kernel(const float* partial, T* out,
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x) * 4;
   if (i >= n) return;
   float s[4], t[4];
-  const bool vec = n % 4 == 0;
-  load_cols<float, 4>(partial, i, n, vec, s);
+  const int rest = n - i < 4 ? static_cast<int>(n - i) : 4;
+  partial += i;
+  load_cols<float, 4>(partial, 0, rest, s);
   for (int k = 1; k < splits; ++k) {
-    load_cols<float, 4>(partial + k * n, i, n, vec, t);
+    load_cols<float, 4>(partial + k * n, 0, rest, t);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[j] += t[j];
   }
-  store_cols<T, 4>(out, i, n, vec, s);
+  store_cols<T, 4>(out + i, 0, rest, s);
 }
 
 // Column sums of [rows, n]: workgroup (b, s) those of 256 columns over the s-th share of the rows.  A thread adds 8 columns of
 // every eighth row (16 or 32 bytes a load), the eight are added in LDS.
 template <typename T>
-__global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, int rows, int n, int share, bool vec, float* partial) {
+__global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, int rows, int n, int share, float* partial) {
   __shared__ float part[8][256];
   const int c = (threadIdx.x & 31) * 8, c0 = blockIdx.x * 256 + c, r0 = threadIdx.x >> 5;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * share, last = rows - first < share ? rows : first + share;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, t[8];
   if (c0 < n)
     for (int64_t r = first + r0; r < last; r += 8) {
-      load_cols<T, 8>(x + r * ld, c0, n, vec, t);
+      load_cols<T, 8>(x + r * ld, c0, n, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += t[j];
     }
@@ -98,9 +99,6 @@ bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   const int64_t most = INT64_C(1) << 30;
   return m >= 0 && n >= 0 && k >= 0 && m <= most && n <= most && k <= most;
 }
-bool out_vectors(const void* out, int64_t ldo, const void* other, int64_t ldother, int64_t size) {
-  return aligned16({out, other}) && ldo * size % 16 == 0 && (other == nullptr || ldother * size % 16 == 0);
-}
 int first_error(std::initializer_list<int> status) {
   for (int s : status)
     if (s != VMI_OK) return s;
@@ -132,7 +130,6 @@ int weight_gradient(const void* dz, int64_t lddz, int segments, int64_t seg, int
   p.m = static_cast<int>(segments * seg), p.n = static_cast<int>(cols), p.k = static_cast<int>(m);
   p.splits = s.n, p.split_k = s.length, p.seg = static_cast<int>(seg), p.seg_valid = static_cast<int>(valid);
   p.out = dw, p.ldo = cols, p.partial = s.n > 1 ? partial : nullptr;
-  p.vec = out_vectors(dw, cols, nullptr, 0, size_of(dtype));
   if (const int st = product(dtype, DW, p, stream); st != VMI_OK || s.n == 1) return st;
   const int64_t n = segments * valid * cols, blocks = (n + 4 * NTH - 1) / (4 * NTH);
   if (!grid_fits(blocks, NTH)) return VMI_ERR_UNSUPPORTED;
@@ -171,8 +168,6 @@ extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, 
   p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.xs = x_scale, p.ws = w_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
   p.bias = bias, p.other = residual, p.ldother = ldr, p.act = act, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
-  p.vec = out_vectors(out, ldo, residual, ldr, size_of(out_dtype));
-  p.ws_vec = aligned16({w_scale}), p.bias_vec = aligned16({bias});
   return product(dtype, LINEAR, p, static_cast<hipStream_t>(stream));
 }
 
@@ -195,7 +190,6 @@ extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale
   p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.xs = x_scale, p.ws = gate_scale, p.ws2 = up_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(F), p.k = static_cast<int>(K);
   p.act = act, p.beta1 = beta1, p.beta2 = beta2, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
-  p.vec = out_vectors(out, ldo, nullptr, 0, size_of(out_dtype)), p.ws_vec = aligned16({gate_scale, up_scale});
   return product(dtype, GATED, p, static_cast<hipStream_t>(stream));
 }
 
@@ -230,7 +224,6 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
       Args p{};
       p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
       p.bias = bias, p.other = dy, p.ldother = lddy, p.act = act, p.out = const_cast<void*>(dz), p.ldo = lddz;
-      p.vec = out_vectors(dz, lddz, dy, lddy, size), p.bias_vec = aligned16({bias});
       if (const int st = product(dtype, LINEAR_DZ, p, s); st != VMI_OK) return st;
     }
   }
@@ -239,7 +232,7 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
   if (dx != nullptr && M > 0 && K > 0) {
     Args p{};
     p.a = dz, p.lda = lddz, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(K), p.k = static_cast<int>(N);
-    p.out = dx, p.ldo = K, p.vec = out_vectors(dx, K, nullptr, 0, size);
+    p.out = dx, p.ldo = K;
     if (const int st = product(dtype, DX, p, s); st != VMI_OK) return st;
   }
   if (dw != nullptr)
@@ -250,10 +243,9 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
     float* sums = reinterpret_cast<float*>(at);
     return by_type(dtype, [&](auto tag) -> int {
       using T = decltype(tag);
-      const bool vec = out_vectors(dz, lddz, nullptr, 0, size);
       if (!grid_fits((N + 31) / 32, NTH)) return VMI_ERR_UNSUPPORTED;
       hipLaunchKernelGGL(columns_kernel<T>, dim3(static_cast<unsigned>((N + 255) / 256), static_cast<unsigned>(shares)), dim3(NTH), 0,
-                         s, static_cast<const T*>(dz), lddz, static_cast<int>(M), static_cast<int>(N), share, vec, sums);
+                         s, static_cast<const T*>(dz), lddz, static_cast<int>(M), static_cast<int>(N), share, sums);
       hipLaunchKernelGGL(columns_join_kernel<T>, dim3(static_cast<unsigned>((N + 31) / 32)), dim3(NTH), 0, s, sums, shares,
                          static_cast<int>(N), static_cast<T*>(db));
       return hip_status(hipGetLastError());
@@ -292,14 +284,14 @@ extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_ga
     Args p{};
     p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.m = static_cast<int>(M), p.n = static_cast<int>(F);
     p.k = static_cast<int>(K), p.other = dh, p.ldother = lddh, p.act = act, p.beta1 = beta1, p.beta2 = beta2;
-    p.out = dz, p.ldo = lddz, p.second = f, p.vec = out_vectors(dz, lddz, dh, lddh, size);
+    p.out = dz, p.ldo = lddz, p.second = f;
     if (const int st = product(dtype, GATED_DZ, p, s); st != VMI_OK) return st;
   }
   if (dx != nullptr && M > 0 && K > 0) {
     Args p{};
     p.a = dz, p.lda = lddz, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.second = f;
     p.m = static_cast<int>(M), p.n = static_cast<int>(K), p.k = static_cast<int>(F);
-    p.out = dx, p.ldo = K, p.vec = out_vectors(dx, K, nullptr, 0, size);
+    p.out = dx, p.ldo = K;
     if (const int st = product(dtype, DX, p, s); st != VMI_OK) return st;
   }
   if (dw != nullptr) return weight_gradient(dz, lddz, 2, f, F, x, ldx, dtype, M, K, dw, partial, s);

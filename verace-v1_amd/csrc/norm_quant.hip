@@ -10,10 +10,13 @@
 // of a tie (and below 2^-6, where e4m3's steps are of one size): one value of about 5000, so a wave takes the 64-bit form for
 // a whole piece where one of its lanes needs it.  max|p| in 64 bits is that of the pieces whose 32-bit maximum is within
 // 2^-21 of the row's.  Rows whose 32-bit terms are not all finite, or all below 2^-60, take the 64-bit form throughout.
+// The sum of squares is of 64 bits, over s of 32 for 16-bit inputs: the scale is within 2^-23.
 //
 // One read of each input, one write of each result: HBM bounds it.  A row is one wave's (up to 8 pieces of 16 bytes a lane)
 // or four waves'; its inputs stay in registers, as they came, between the pass that sums and the pass that writes.  Longer rows
 // are read again.  A row with a NaN or an infinity in p has the scale NaN and q NaN everywhere; its s is what it is.
+#include <type_traits>
+
 #include "vmi_dispatch.h"
 #include "vmi_vec.h"
 
@@ -45,17 +48,16 @@ __device__ __forceinline__ float round_to_odd(double r) {
   return __uint_as_float(b);
 }
 
-template <typename T, typename W, int N>
-__device__ __forceinline__ void load_weights(const W* w, int i0, int d, bool vec, float (&x)[N]) {
+// Pieces of a row start where the row does; the hardware takes 16 bytes at any address.
+template <typename W, int N, bool WHOLE> __device__ __forceinline__ void load_weights(const W* w, int i0, int d, float (&x)[N]) {
   if (w == nullptr) {
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = 1.f;
-  } else if (vec) {
-    typedef typename native<W>::type E;
-    typedef E P __attribute__((ext_vector_type(N)));
-    const P v = *reinterpret_cast<const P*>(w + i0);
+  } else if (WHOLE || i0 + N <= d) {
+    W v[N];
+    __builtin_memcpy(v, w + i0, sizeof(v));
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = static_cast<float>(v[j]);
+    for (int j = 0; j < N; ++j) x[j] = io<W>::to_f32(v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = i0 + j < d ? io<W>::load(w, i0 + j) : 0.f;
@@ -63,9 +65,12 @@ __device__ __forceinline__ void load_weights(const W* w, int i0, int d, bool vec
 }
 
 // 16 bytes of a row from element i0 as they lie, zeros past its end.
-template <typename T> __device__ __forceinline__ Vec<T> load_raw(const T* row, int i0, int d, bool vec) {
-  if (vec) return ldv(row + i0);
+template <typename T, bool WHOLE> __device__ __forceinline__ Vec<T> load_raw(const T* row, int i0, int d) {
   Vec<T> v;
+  if (WHOLE || i0 + Vec<T>::N <= d) {
+    __builtin_memcpy(&v, row + i0, 16);
+    return v;
+  }
 #pragma unroll
   for (int j = 0; j < Vec<T>::N; ++j) {
     if (i0 + j < d) v.e[j] = row[i0 + j];
@@ -73,20 +78,32 @@ template <typename T> __device__ __forceinline__ Vec<T> load_raw(const T* row, i
   }
   return v;
 }
+template <typename T, bool WHOLE> __device__ __forceinline__ void store_sum(T* row, int i0, int d, const float (&x)[Vec<T>::N]) {
+  typename native<T>::type e[Vec<T>::N];
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N; ++j) e[j] = static_cast<typename native<T>::type>(x[j]);
+  if (WHOLE || i0 + Vec<T>::N <= d) {
+    __builtin_memcpy(row + i0, e, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < Vec<T>::N; ++j)
+      if (i0 + j < d) __builtin_memcpy(row + i0 + j, e + j, sizeof(T));
+  }
+}
 
-// The terms of one piece in 32 bits and, where it matters, in 64.
-template <typename T> struct Terms {
+// The terms of one piece in 32 bits and, where it matters, in 64.  Sums of two 16-bit values are exact in 32 bits, but where
+// one is 2^16 times the other and more.
+template <typename T, bool RES> struct Terms {
   static constexpr int N = Vec<T>::N;
   Vec<T> a, r;
   float w[N];
-  bool residual;
   __device__ __forceinline__ float s(int j) const {
     const float x = io<T>::to_f32(a.e[j]);
-    return residual ? x + io<T>::to_f32(r.e[j]) : x;
+    return RES ? x + io<T>::to_f32(r.e[j]) : x;
   }
   __device__ __forceinline__ double s64(int j) const {
     const double x = io<T>::to_f32(a.e[j]);
-    return residual ? x + static_cast<double>(io<T>::to_f32(r.e[j])) : x;
+    return RES ? x + static_cast<double>(io<T>::to_f32(r.e[j])) : x;
   }
   __device__ __forceinline__ float p(int j) const { return s(j) * w[j]; }
   __device__ __forceinline__ double p64(int j) const { return s64(j) * static_cast<double>(w[j]); }
@@ -107,8 +124,9 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
-// G threads a row, NV pieces each; LONG: any number of pieces, read again for the second pass.
-template <typename T, typename W, int G, int NV, bool LONG, bool VEC>
+// G threads a row, NV pieces each; LONG: any number of pieces, read again for the second pass; RES: with a residual; WHOLE: rows
+// are whole pieces (a row's last piece otherwise goes element by element).
+template <typename T, typename W, int G, int NV, bool LONG, bool RES, bool WHOLE>
 __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   constexpr int N = Vec<T>::N, WAVES = G / 64;
   __shared__ double red[2][4];
@@ -117,19 +135,18 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (NTH / G) + threadIdx.x / G;
   if (G < NTH && row >= k.rows) return;
   const T* ar = static_cast<const T*>(k.a) + row * k.a_stride;
-  const T* rr = k.r == nullptr ? nullptr : static_cast<const T*>(k.r) + row * k.r_stride;
+  const T* rr = static_cast<const T*>(k.r) + (RES ? row * k.r_stride : 0);
   const W* w = static_cast<const W*>(k.w);
   T* sr = k.sum == nullptr ? nullptr : static_cast<T*>(k.sum) + row * k.d;
   Vec<T> a[LONG ? 1 : NV] = {}, r[LONG ? 1 : NV] = {};
   auto load = [&](int v, int i0) {
-    a[v] = load_raw<T>(ar, i0, k.d, VEC);
-    if (rr != nullptr) r[v] = load_raw<T>(rr, i0, k.d, VEC);
+    a[v] = load_raw<T, WHOLE>(ar, i0, k.d);
+    if constexpr (RES) r[v] = load_raw<T, WHOLE>(rr, i0, k.d);
   };
   auto terms = [&](int v, int i0) {
-    Terms<T> t;
-    t.a = a[v], t.residual = rr != nullptr;
-    if (t.residual) t.r = r[v];
-    load_weights<T, W, N>(w, i0, k.d, VEC, t.w);
+    Terms<T, RES> t;
+    t.a = a[v], t.r = r[v];
+    load_weights<W, N, WHOLE>(w, i0, k.d, t.w);
     return t;
   };
   // f(v, i0) for each of the thread's pieces, `again`: after another pass over them
@@ -148,7 +165,7 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           forget(a[v]);
-          forget(r[v]);
+          if constexpr (RES) forget(r[v]);
         }
       }
 #pragma unroll
@@ -161,11 +178,11 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
 #pragma unroll
   for (int v = 0; v < (LONG ? 1 : NV); ++v) of_piece[v] = 0.f;
   pieces(false, [&](int v, int i0) {
-    const Terms<T> t = terms(v, i0);
+    const Terms<T, RES> t = terms(v, i0);
     float st[N], m = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const double s = t.s64(j);
+      const double s = sizeof(T) == 2 ? static_cast<double>(t.s(j)) : t.s64(j);
       const float p = t.p(j);
       st[j] = static_cast<float>(s);
       ss += s * s;
@@ -174,7 +191,7 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
     }
     high = fmaxf(high, m);
     of_piece[v] = m;
-    if (sr != nullptr) store_piece<T>(sr, i0, k.d, VEC, st);
+    if (sr != nullptr) store_sum<T, WHOLE>(sr, i0, k.d, st);
   });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
@@ -194,7 +211,7 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   bool bad = false;
   pieces(true, [&](int v, int i0) {
     if (LONG || __any(of_piece[v] >= near)) {
-      const Terms<T> t = terms(v, i0);
+      const Terms<T, RES> t = terms(v, i0);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const double p = fabs(t.p64(j));
@@ -219,16 +236,18 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   if (g == 0) k.scale[row] = bad ? __builtin_nanf("") : static_cast<float>(D / (kTop * rms));
   uint8_t* qr = k.q + row * k.d;
   pieces(true, [&](int v, int i0) {
-    const Terms<T> t = terms(v, i0);
+    const Terms<T, RES> t = terms(v, i0);
     float f[N];
-    bool doubt = wild;
+    // how far above 16 steps before the middle between two values (the low 20 bits half way), and above the least 32-bit value
+    uint32_t middle = ~0u, least = ~0u;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       f[j] = t.p(j) * F;
       const uint32_t u = __float_as_uint(f[j]);
-      // within 16 steps of the middle between two values (the low 20 bits half way), or of one size of steps, but for 0
-      doubt |= (u & 0xFFFFFu) - 0x7FFF0u <= 0x20u || ((u & 0x7FFFFFFFu) - 1u < 0x3C800000u - 1u);
+      middle = min(middle, (u << 12) - 0x7FFF0000u);
+      least = min(least, (u << 1) - 2u);
     }
+    const bool doubt = wild || middle <= 0x20000u || least < 0x79000000u - 2u;  // 0x3C800000 is 2^-6
     if (__any(doubt)) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -242,9 +261,8 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
       int u = __builtin_amdgcn_cvt_pk_fp8_f32(f[j], f[j + 1], 0, false);
       packed[j / 4] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[j + 2], f[j + 3], u, true));
     }
-    if (VEC) {
-      if constexpr (N == 8) *reinterpret_cast<uint2*>(qr + i0) = make_uint2(packed[0], packed[1]);
-      else *reinterpret_cast<uint32_t*>(qr + i0) = packed[0];
+    if (WHOLE || i0 + N <= k.d) {
+      __builtin_memcpy(qr + i0, packed, N);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -253,29 +271,34 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   });
 }
 
-template <typename T, typename W, int G, int NV, bool LONG> int launch(Args k, bool vec, hipStream_t stream) {
+template <typename T, typename W, int G, int NV, bool LONG> int launch(const Args& k, hipStream_t stream) {
   return in_launches(k.rows, NTH, NTH / G, [&](int64_t row, int64_t n) -> int {
     Args c = k;
     c.a = advance<const T>(k.a, row * k.a_stride), c.r = advance<const T>(k.r, row * k.r_stride);
     c.sum = advance<T>(k.sum, row * k.d), c.q = k.q + row * k.d, c.scale = k.scale + row, c.rows = n;
     const dim3 grid(static_cast<unsigned>((n + NTH / G - 1) / (NTH / G)));
-    if (vec)
-      hipLaunchKernelGGL((norm_quant_kernel<T, W, G, NV, LONG, true>), grid, dim3(NTH), 0, stream, c);
-    else
-      hipLaunchKernelGGL((norm_quant_kernel<T, W, G, NV, LONG, false>), grid, dim3(NTH), 0, stream, c);
+    auto go = [&](auto res, auto whole) {
+      hipLaunchKernelGGL((norm_quant_kernel<T, W, G, NV, LONG, decltype(res)::value, decltype(whole)::value>), grid, dim3(NTH), 0,
+                         stream, c);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    const bool whole = k.d % Vec<T>::N == 0;
+    if (k.r != nullptr) whole ? go(yes, yes) : go(yes, no);
+    else whole ? go(no, yes) : go(no, no);
     return hip_status(hipGetLastError());
   });
 }
 
-template <typename T, typename W> int by_row(const Args& k, bool vec, hipStream_t stream) {
+template <typename T, typename W> int by_row(const Args& k, hipStream_t stream) {
   const int pieces = (k.d + Vec<T>::N - 1) / Vec<T>::N;
-  if (pieces <= 64) return launch<T, W, 64, 1, false>(k, vec, stream);
-  if (pieces <= 128) return launch<T, W, 64, 2, false>(k, vec, stream);
-  if (pieces <= 256) return launch<T, W, 64, 4, false>(k, vec, stream);
-  if (pieces <= 512) return launch<T, W, 64, 8, false>(k, vec, stream);
-  if (pieces <= 1024) return launch<T, W, 256, 4, false>(k, vec, stream);
-  if (pieces <= 2048) return launch<T, W, 256, 8, false>(k, vec, stream);
-  return launch<T, W, 256, 1, true>(k, vec, stream);
+  if (pieces <= 64) return launch<T, W, 64, 1, false>(k, stream);
+  if (pieces <= 128) return launch<T, W, 64, 2, false>(k, stream);
+  if (pieces <= 256) return launch<T, W, 64, 4, false>(k, stream);
+  if (pieces <= 512) return launch<T, W, 64, 8, false>(k, stream);
+  if (pieces <= 1024) return launch<T, W, 256, 4, false>(k, stream);
+  if (pieces <= 2048) return launch<T, W, 256, 8, false>(k, stream);
+  return launch<T, W, 256, 1, true>(k, stream);
 }
 
 }  // namespace
@@ -291,11 +314,9 @@ extern "C" int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* r
          static_cast<int>(d)};
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    const bool vec = d % Vec<T>::N == 0 && k.a_stride % Vec<T>::N == 0 && k.r_stride % Vec<T>::N == 0 && aligned16({a, residual, w, sum}) &&
-                     reinterpret_cast<uintptr_t>(q) % Vec<T>::N == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if constexpr (sizeof(T) == 2)
-      if (w != nullptr && w_dtype == VMI_F32) return by_row<T, float>(k, vec, s);
-    return by_row<T, T>(k, vec, s);
+      if (w != nullptr && w_dtype == VMI_F32) return by_row<T, float>(k, s);
+    return by_row<T, T>(k, s);
   });
 }

@@ -162,11 +162,16 @@ def _rows_of(t: torch.Tensor, k: int) -> int:
     return t.numel() // k if k else t.shape[:-1].numel()
 
 
+def _result(x: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    shape = x.shape[:-1] + (n,)
+    return x.new_empty(shape) if dtype is x.dtype else torch.empty(shape, device=x.device, dtype=dtype)
+
+
 def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, beta2, out_dtype):
     F, K = w_gate.shape
     x2, xp, ldx = _operand(x, K)
     (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
-    out = x.new_empty(x.shape[:-1] + (F,), dtype=out_dtype)
+    out = _result(x, F, out_dtype)
     if x_scale is not None:
         x_scale, gate_scale, up_scale = _vector(x_scale), _vector(gate_scale), _vector(up_scale)
     with device_guard(x):
@@ -269,7 +274,7 @@ def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dt
     w, wp, ldw = _operand(weight, K)
     r, rp, ldr = _plain_rows(residual, N)
     bias = _vector(bias)
-    out = x.new_empty(x.shape[:-1] + (N,), dtype=out_dtype)
+    out = _result(x, N, out_dtype)
     if x_scale is not None:
         x_scale, weight_scale = _vector(x_scale), _vector(weight_scale)
     with device_guard(x):
