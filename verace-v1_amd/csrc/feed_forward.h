@@ -424,10 +424,16 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
 }
 
 template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
-constexpr int kFewRows = 64;
+// The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536), and any of up to 16 rows.  Both sides in
+// us, rows / tiles: bf16 K 2048 N 1024 M 128 7.6 / 9.5, M 256 11.3 / 9.8; bf16 K 1024 N 4096 M 32 5.5 / 6.4, M 64 8.1 / 6.4; fp32
+// K 2048 N 1024 M 384 38 / 40, M 512 38 / 40; fp32 K 4096 N 4096 M 96 63 / 76, M 192 108 / 77.
+template <typename E> inline bool few_rows(Kind kind, const Args& p) {
+  const int64_t cols = kind == GATED ? 2 * static_cast<int64_t>(p.n) : p.n;
+  return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (sizeof(E) == 4 ? 1536 : 512);
+}
 
 template <typename E> int product_of(Kind kind, const Args& p, hipStream_t stream) {
-  if (p.m <= kFewRows) {
+  if (few_rows<E>(kind, p)) {
     if (kind == LINEAR) return launch_rows<E, LINEAR>(p, stream);
     if (kind == GATED) return launch_rows<E, GATED>(p, stream);
   }

@@ -41,12 +41,16 @@ __global__ __launch_bounds__(NTH) void columns_kernel(const T* x, int64_t ld, in
   const int c = (threadIdx.x & 31) * 8, c0 = blockIdx.x * 256 + c, r0 = threadIdx.x >> 5;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * share, last = rows - first < share ? rows : first + share;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, t[8];
-  if (c0 < n)
+  auto add = [&](auto full) {
+#pragma unroll 4
     for (int64_t r = first + r0; r < last; r += 8) {
-      load_cols<T, 8>(x + r * ld, c0, n, t);
+      load_cols<T, 8, decltype(full)::value>(x + r * ld, c0, n, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += t[j];
     }
+  };
+  if (c0 + 8 <= n) add(std::true_type{});
+  else if (c0 < n) add(std::false_type{});
 #pragma unroll
   for (int j = 0; j < 8; ++j) part[r0][c + j] = s[j];
   __syncthreads();
