@@ -523,6 +523,9 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  *                     3: a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2).  ldg = ldu.
  * Gradients from the inputs alone, for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
  * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */
+/* Rows of any address and length (row_bytes, ld_bytes apart) as these products take them: contiguous rows of whole 16-byte
+ * pieces at dst, zeros behind the last byte. */
+int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_t rows, int64_t row_bytes, void* stream);
 int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
                    const float* w_scale, int dtype, const void* bias, const void* residual, int64_t ldr,
                    int act, void* out, int64_t ldo, int out_dtype, int64_t M, int64_t N, int64_t K,

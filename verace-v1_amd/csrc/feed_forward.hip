@@ -74,6 +74,24 @@ __global__ __launch_bounds__(NTH) void columns_join_kernel(const float* partial,
   io<T>::store(out, c, s);
 }
 
+// Rows of `bytes` to rows of whole 16-byte pieces, zeros behind them: a piece a thread.
+__global__ __launch_bounds__(NTH) void pad_kernel(const char* src, int64_t ld, char* dst, int64_t bytes, int64_t pieces, int64_t n) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x;
+  if (e >= n) return;
+  const int64_t row = e / pieces, at = (e - row * pieces) * 16;
+  const char* from = src + row * ld + at;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (at + 16 <= bytes) {
+    __builtin_memcpy(&v, from, 16);
+  } else {
+    unsigned char* b = reinterpret_cast<unsigned char*>(&v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (at + j < bytes) b[j] = from[j];
+  }
+  *reinterpret_cast<uint4*>(dst + e * 16) = v;
+}
+
 int product(int dtype, Kind kind, const Args& p, hipStream_t stream) {
   switch (dtype) {
     case VMI_BF16: return product_bf16(kind, p, stream);
@@ -157,6 +175,24 @@ bool gate_act(int act) { return act == ACT_SILU || act == ACT_SITU; }
 bool linear_act(int act) { return act == ACT_NONE || act == ACT_SILU || act == ACT_GELU; }
 
 }  // namespace
+
+extern "C" int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_t rows, int64_t row_bytes, void* stream) {
+  if (rows < 0 || row_bytes < 0 || ld_bytes < 0) return VMI_ERR_INVALID_ARG;
+  if (rows == 0 || row_bytes == 0) return VMI_OK;
+  if (src == nullptr || dst == nullptr || reinterpret_cast<uintptr_t>(dst) % 16 != 0) return VMI_ERR_INVALID_ARG;
+  const int64_t pieces = (row_bytes + 15) / 16;
+  if (rows > INT64_MAX / 16 / pieces) return VMI_ERR_INVALID_ARG;
+  const int64_t per = UINT32_MAX / NTH / pieces * NTH;  // rows of a launch
+  if (per == 0) return VMI_ERR_UNSUPPORTED;
+  for (int64_t row = 0; row < rows; row += per) {
+    const int64_t n = (rows - row < per ? rows - row : per) * pieces;
+    hipLaunchKernelGGL(pad_kernel, dim3(static_cast<unsigned>((n + NTH - 1) / NTH)), dim3(NTH), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const char*>(src) + row * ld_bytes, ld_bytes, static_cast<char*>(dst) + row * pieces * 16, row_bytes,
+                       pieces, n);
+    if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+  }
+  return VMI_OK;
+}
 
 extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
                               int dtype, const void* bias, const void* residual, int64_t ldr, int act, void* out, int64_t ldo,

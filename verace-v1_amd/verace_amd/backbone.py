@@ -284,6 +284,13 @@ class VeraceV1Model(nn.Module):
         self.acd_engine = AdaptiveCognitiveDepthEngine(config.hidden_dim, config.energy_halting_threshold)
         self.final_norm = nn.RMSNorm(config.hidden_dim, eps=config.rms_norm_eps)
 
+    def quantize_feed_forward_(self, on: bool = True) -> "VeraceV1Model":
+        """Every layer's feed-forward base path in 8 bits, for inference
+        (:meth:`~verace_amd.ManifoldContinuousMoE.quantize_base_`)."""
+        for layer in self.layers:
+            layer.mcmoe.quantize_base_(on)
+        return self
+
     def load_reference_state_dict(self, sd: dict, strict: bool = True):
         """A reference ``VeraceV1Model.state_dict()``; the vision encoder's and the energy
         critic's entries (not built here) are skipped."""

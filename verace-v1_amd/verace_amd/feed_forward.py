@@ -32,20 +32,24 @@ def _code(dtype: torch.dtype) -> int:
     return _lib.VMI_E4M3 if dtype is E4M3 else _lib.dtype_code(dtype)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [..., K] as [M, K] with rows as the kernels load them: contiguous, starting on 16 bytes, filled with zeros to whole
-    16-byte pieces.  A view of t where it lies so, otherwise a copy."""
-    k = t.shape[-1]
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(tensor, elements from a row to the next) of t [..., K] as [M, K] with rows as the kernels load them: contiguous,
+    starting on 16 bytes, filled with zeros to whole 16-byte pieces.  A view of t where it lies so, otherwise a copy."""
+    k, size = t.shape[-1], _ITEMSIZE[t.dtype]
     t = t if t.dim() == 2 else t.reshape(-1, k)
-    m, piece = t.shape[0], 16 // t.dtype.itemsize
-    if k % piece == 0 and t.data_ptr() % 16 == 0 and (k <= 1 or t.stride(1) == 1):
-        if m <= 1 or (t.stride(0) % piece == 0 and t.stride(0) >= k and t.stride(0) * t.dtype.itemsize < _MAX_ROW_BYTES):
-            return t
-    out = torch.empty(m, -(-k // piece) * piece, device=t.device, dtype=t.dtype)
-    if out.shape[1] > k:
-        out[:, k:].view(torch.uint8).zero_() if t.dtype == E4M3 else out[:, k:].zero_()
-    out[:, :k].copy_(t)
-    return out[:, :k]
+    m, piece = t.shape[0], 16 // size
+    whole = -(-k // piece) * piece
+    if k == whole and t.data_ptr() % 16 == 0 and (k <= 1 or t.stride(1) == 1):
+        ld = t.stride(0) if m > 1 else k
+        if ld % piece == 0 and ld >= k and ld * size < _MAX_ROW_BYTES:
+            return t, ld
+    if k > 1 and t.stride(1) != 1 or m > 1 and t.stride(0) < 0:
+        t = t.contiguous()
+    out = torch.empty((m, whole), device=t.device, dtype=t.dtype)
+    with device_guard(t):
+        _lib.check(_lib.load().vmi_pad_rows(t.data_ptr(), t.stride(0) * size, out.data_ptr(), m, k * size,
+                                            _lib.raw_stream(t.device)), "vmi_pad_rows")
+    return out, whole
 
 
 def _operand(t: torch.Tensor, k: int) -> Tuple[torch.Tensor, int, int]:
@@ -54,16 +58,8 @@ def _operand(t: torch.Tensor, k: int) -> Tuple[torch.Tensor, int, int]:
         p = t.data_ptr()
         if not (p | k * _ITEMSIZE[t.dtype]) & 15 and k * _ITEMSIZE[t.dtype] < _MAX_ROW_BYTES:
             return t, p, k
-    t = _rows(t)
-    return t, t.data_ptr(), _ld(t)
-
-
-def _ld(t: Optional[torch.Tensor]) -> int:
-    """Elements from a row of [M, K] to the next, also where it has but one."""
-    if t is None:
-        return 0
-    piece = 16 // t.dtype.itemsize
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // piece) * piece
+    t, ld = _rows(t)
+    return t, t.data_ptr(), ld
 
 
 def _plain_rows(t: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:

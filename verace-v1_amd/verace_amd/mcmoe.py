@@ -16,11 +16,16 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .feed_forward import gated_linear, linear_add, quantize_rows
 from .layer_ops import mcmoe_coef, norm_add, situ_glu
 
 
 class SiTUGLU(nn.Module):
-    """``[b1 tanh(W_g x / b1) sigmoid(W_g x)] * [b2 tanh(W_u x / b2)]`` (activations.py:8-31)."""
+    """``[b1 tanh(W_g x / b1) sigmoid(W_g x)] * [b2 tanh(W_u x / b2)]`` (activations.py:8-31).
+
+    ``fuse_products = True`` takes both projections, the activations and their product as one kernel, in training too
+    (:func:`~verace_amd.gated_linear`); the projections are then not rounded in between, so results differ from the separate
+    ops' by their rounding."""
 
     def __init__(self, in_features: int, hidden_features: int, beta1: float = 4.0,
                  beta2: float = 25.0):
@@ -31,8 +36,11 @@ class SiTUGLU(nn.Module):
         self.beta2 = beta2
         self.w_gate = nn.Linear(in_features, hidden_features, bias=False)
         self.w_up = nn.Linear(in_features, hidden_features, bias=False)
+        self.fuse_products = False
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.fuse_products:
+            return gated_linear(x, self.w_gate.weight, self.w_up.weight, beta1=self.beta1, beta2=self.beta2)
         g = self.w_gate(x)
         u = self.w_up(x)
         return situ_glu(g, u, self.beta1, self.beta2)
@@ -53,13 +61,33 @@ class ManifoldContinuousMoE(nn.Module):
         self.router = nn.Linear(hidden_dim, num_components, bias=False)
         self.hyper_sigma = nn.Linear(hidden_dim, num_components * rank, bias=False)
         self.norm = nn.RMSNorm(hidden_dim)
+        self._base8 = None
+
+    def quantize_base_(self, on: bool = True) -> "ManifoldContinuousMoE":
+        """Holds the base path's three weights in 8 bits with a scale for each output channel (``on=False``: no longer) and
+        runs the path on rows in 8 bits, for inference.  The weights themselves stay; after a change of theirs, or a move to
+        another device, this is called again.  Not part of the ``state_dict``."""
+        glu = self.base_situ_glu
+        with torch.no_grad():
+            self._base8 = tuple(quantize_rows(m.weight.detach()) for m in (glu.w_gate, glu.w_up, self.base_w_down)) if on else None
+        return self
+
+    def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled():
+            raise RuntimeError("verace_amd.ManifoldContinuousMoE: the base path in 8 bits has no gradients; run under "
+                               "torch.no_grad(), or call quantize_base_(False)")
+        (wg, sg), (wu, su), (wd, sd) = self._base8
+        glu = self.base_situ_glu
+        x, xs = quantize_rows(xf)
+        h, hs = quantize_rows(gated_linear(x, wg, wu, xs, sg, su, beta1=glu.beta1, beta2=glu.beta2, out_dtype=xf.dtype))
+        return linear_add(h, wd, x_scale=hs, weight_scale=sd, out_dtype=xf.dtype)
 
     def parts(self, x: torch.Tensor):
         """The base path and the manifold path before its norm, both [tokens, hidden]."""
         b, s, d = x.shape
         C, r = self.num_components, self.rank
         xf = x.reshape(b * s, d)
-        base_out = self.base_w_down(self.base_situ_glu(xf))
+        base_out = self.base_w_down(self.base_situ_glu(xf)) if self._base8 is None else self._base_in_8_bits(xf)
         # v_proj[n, j, :] = V_j x_n for every component, then the selected ones' coefficients
         vproj = xf @ self.v_basis.reshape(C * r, d).t()
         coef = mcmoe_coef(self.router(xf), self.hyper_sigma(xf), vproj, min(self.top_k_components, C), C)
