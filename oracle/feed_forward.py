@@ -5,6 +5,9 @@ most a whole step where the matrix cores cut instead of rounding); an activation
 terms' magnitude (an exponential and a reciprocal of a few 2^-23 each, their differences from 1 no closer than 2^-3); a result
 rounded to its type by half a step, ``eps / 2`` relative, or half the smallest subnormal.  A gradient of a projection is rounded to
 x's type between the backward's products, half a step of each term.
+
+An fp32 number below 2^-126, the least normal one, may be taken as 0: an exponential (the sigmoid of -90 is 8e-40; what it
+multiplies, at most the larger of |g| and b1 and the other factor, scales that), an operand of a product, a result.
 """
 import math
 
@@ -12,6 +15,7 @@ import torch
 
 E4M3 = torch.float8_e4m3fn
 ACT_ERROR = 2.0 ** -18
+TINY = 2.0 ** -126
 
 
 def values(t, scale=None):
@@ -26,7 +30,7 @@ def half_step(dtype):
 
 def rounding(x, dtype):
     """How far rounding x to dtype may take it."""
-    return x.abs() * half_step(dtype) * (1 + 1e-6) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    return x.abs() * half_step(dtype) * (1 + 1e-6) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 + TINY
 
 
 def product(x, w):
@@ -44,12 +48,17 @@ def gate_terms(g, u, activation, b1=4.0, b2=25.0):
     return b1 * t1 * s, (1 - t1 * t1) * s + b1 * t1 * s * (1 - s), b2 * t2, 1 - t2 * t2
 
 
+def flushed(g, b1):
+    """What a sigmoid taken as 0 may take from a(g) or a'(g)."""
+    return TINY * (1 + g.abs().clamp_min(b1))
+
+
 def gated(x, wg, wu, activation, dtype, b1=4.0, b2=25.0):
     """(h, bound) of gated_linear for values in 64 bits."""
     (g, eg), (u, eu) = product(x, wg), product(x, wu)
     a, da, b, db = gate_terms(g, u, activation, b1, b2)
     h = a * b
-    e = (da * b).abs() * eg + (a * db).abs() * eu + 2 * eg * eu + ACT_ERROR * h.abs()
+    e = (da * b).abs() * eg + (a * db).abs() * eu + 2 * eg * eu + ACT_ERROR * h.abs() + flushed(g, b1) * b.abs()
     return h, e + rounding(h, dtype)
 
 
@@ -59,8 +68,8 @@ def gated_bwd(x, wg, wu, activation, dh, dtype, b1=4.0, b2=25.0):
     a, da, b, db = gate_terms(g, u, activation, b1, b2)
     dg, du = dh * da * b, dh * a * db
     # slopes change by at most twice their argument's error and the other factor's
-    edg = dh.abs() * (2 * b.abs() * eg + da.abs() * eu + 2 * eg * eu) + ACT_ERROR * dh.abs() * b.abs() + rounding(dg, dtype)
-    edu = dh.abs() * (2 * a.abs() * eu + da.abs() * eg + 2 * eg * eu) + ACT_ERROR * dh.abs() * a.abs() + rounding(du, dtype)
+    edg = dh.abs() * (2 * b.abs() * eg + da.abs() * eu + 2 * eg * eu) + (ACT_ERROR + flushed(g, b1)) * dh.abs() * b.abs() + rounding(dg, dtype)
+    edu = dh.abs() * (2 * a.abs() * eu + da.abs() * eg + 2 * eg * eu) + (ACT_ERROR * a.abs() + flushed(g, b1)) * dh.abs() + rounding(du, dtype)
     out = []
     n = 2 * dg.shape[1] + 8
     dx = dg @ wg + du @ wu
