@@ -521,27 +521,28 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  *                     act 0: none, 1: z sigmoid(z), 2: z Phi(z).  out may be residual.
  *   vmi_gated_linear: out = a(x w_gate^T) b(x w_up^T); act 1: a(z) = z sigmoid(z), b(z) = z;
  *                     3: a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2).  ldg = ldu.
- * Gradients from the inputs alone, for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
+ * keep (or NULL) receives the sums before the activation, contiguous [M, N] (with the bias; gated [M, 2F], a row's gates first).
+ * Gradients from the inputs, and from those sums where they were kept (kept; NULL: formed again), for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
  * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */
 /* Rows of any address and length (row_bytes, ld_bytes apart) as these products take them: contiguous rows of whole 16-byte
  * pieces at dst, zeros behind the last byte. */
 int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_t rows, int64_t row_bytes, void* stream);
 int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
                    const float* w_scale, int dtype, const void* bias, const void* residual, int64_t ldr,
-                   int act, void* out, int64_t ldo, int out_dtype, int64_t M, int64_t N, int64_t K,
-                   void* stream);
+                   int act, void* out, int64_t ldo, int out_dtype, float* keep, int64_t M, int64_t N,
+                   int64_t K, void* stream);
 int vmi_linear_add_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, size_t* bytes);
 int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const void* bias,
-                       int act, const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M,
+                       int act, const float* kept, const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M,
                        int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale, const void* w_gate, int64_t ldg,
                      const float* gate_scale, const void* w_up, int64_t ldu, const float* up_scale, int dtype,
-                     int act, float beta1, float beta2, void* out, int64_t ldo, int out_dtype, int64_t M,
-                     int64_t F, int64_t K, void* stream);
+                     int act, float beta1, float beta2, void* out, int64_t ldo, int out_dtype, float* keep,
+                     int64_t M, int64_t F, int64_t K, void* stream);
 int vmi_gated_linear_bwd_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype, size_t* bytes);
 int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up,
-                         int64_t ldu, int dtype, int act, float beta1, float beta2, const void* dh,
-                         int64_t lddh, void* dx, void* dw, int64_t M, int64_t F, int64_t K, void* workspace,
+                         int64_t ldu, int dtype, int act, float beta1, float beta2, const float* kept,
+                         const void* dh, int64_t lddh, void* dx, void* dw, int64_t M, int64_t F, int64_t K, void* workspace,
                          size_t workspace_bytes, void* stream);
 
 /* Root-mean-square norm with the residual's addition and a result in 8 bits:

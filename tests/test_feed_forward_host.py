@@ -125,7 +125,7 @@ def test_c_refusals(lib):
 
     def linear(x=one, ldx=16, xs=null, w=one, ldw=16, ws=null, dtype=1, bias=null, res=null, ldr=0, act=0, out=one, ldo=8, od=1, M=2, N=8,
                K=16):
-        return lib.vmi_linear_add(x, ldx, xs, w, ldw, ws, dtype, bias, res, ldr, act, out, ldo, od, M, N, K, null)
+        return lib.vmi_linear_add(x, ldx, xs, w, ldw, ws, dtype, bias, res, ldr, act, out, ldo, od, null, M, N, K, null)
 
     for kw in (dict(x=null), dict(w=null), dict(out=null), dict(ldx=8), dict(ldw=8), dict(ldo=7), dict(res=one, ldr=7), dict(act=3), dict(act=-1),
                dict(dtype=4), dict(dtype=-1), dict(od=0), dict(od=3, dtype=3), dict(dtype=3, ldx=16, ldw=16), dict(M=-1), dict(N=-1), dict(K=-1),
@@ -137,7 +137,7 @@ def test_c_refusals(lib):
 
     def gated(x=one, ldx=16, xs=null, wg=one, ldg=16, gs=null, wu=one, ldu=16, us=null, dtype=1, act=3, b1=4.0, b2=25.0, out=one, ldo=8, od=1,
               M=2, F=8, K=16):
-        return lib.vmi_gated_linear(x, ldx, xs, wg, ldg, gs, wu, ldu, us, dtype, act, b1, b2, out, ldo, od, M, F, K, null)
+        return lib.vmi_gated_linear(x, ldx, xs, wg, ldg, gs, wu, ldu, us, dtype, act, b1, b2, out, ldo, od, null, M, F, K, null)
 
     for kw in (dict(wu=null), dict(act=0), dict(act=2), dict(ldo=7), dict(dtype=3, xs=one, gs=one), dict(F=-1), dict(od=2)):
         assert gated(**kw) == INVALID, kw
@@ -152,16 +152,16 @@ def test_c_refusals(lib):
     assert lib.vmi_gated_linear_bwd_workspace_bytes(100, 20, 16, 1, ctypes.byref(n)) == 0 and n.value >= 100 * 48 * 2
     assert lib.vmi_gated_linear_bwd_workspace_bytes(100, 20, -16, 1, ctypes.byref(n)) == INVALID
     bwd = lib.vmi_linear_add_bwd
-    assert bwd(one, 16, one, 16, 1, null, 1, one, 8, one, one, one, 2, 8, 16, null, 0, null) == WORKSPACE
-    assert bwd(one, 16, one, 16, 1, null, 1, one, 8, one, one, one, 2, 8, 16, ctypes.c_void_p(8), 1 << 30, null) == WORKSPACE
-    assert bwd(one, 16, one, 16, 1, null, 5, one, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
-    assert bwd(one, 16, one, 16, 1, null, 1, odd, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
-    assert bwd(one, 16, one, 16, 1, null, 1, null, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
+    assert bwd(one, 16, one, 16, 1, null, 1, null, one, 8, one, one, one, 2, 8, 16, null, 0, null) == WORKSPACE
+    assert bwd(one, 16, one, 16, 1, null, 1, null, one, 8, one, one, one, 2, 8, 16, ctypes.c_void_p(8), 1 << 30, null) == WORKSPACE
+    assert bwd(one, 16, one, 16, 1, null, 5, null, one, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
+    assert bwd(one, 16, one, 16, 1, null, 1, null, odd, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
+    assert bwd(one, 16, one, 16, 1, null, 1, null, null, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
     gb = lib.vmi_gated_linear_bwd
-    assert gb(one, 16, one, 16, one, 16, 1, 0, 4.0, 25.0, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
-    assert gb(one, 16, one, 16, one, 24, 1, 3, 4.0, 25.0, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
-    assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, one, 7, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
-    assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, one, 8, one, one, 2, 8, 16, one, 16, null) == WORKSPACE
+    assert gb(one, 16, one, 16, one, 16, 1, 0, 4.0, 25.0, null, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
+    assert gb(one, 16, one, 16, one, 24, 1, 3, 4.0, 25.0, null, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
+    assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, null, one, 7, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
+    assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, null, one, 8, one, one, 2, 8, 16, one, 16, null) == WORKSPACE
 
     def quant(a=one, st=16, r=null, rs=0, w=null, dtype=1, wd=1, norm=1, s=one, q=one, scale=one, rows=2, d=16):
         return lib.vmi_norm_add_quant(a, st, r, rs, w, dtype, wd, norm, 1e-6, s, q, scale, rows, d, null)

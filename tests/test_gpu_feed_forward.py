@@ -79,10 +79,12 @@ def test_8_bit_result_types(out):
     within(y, *oracle.linear(X, G, oracle.values(b), oracle.values(r), "silu", out))
 
 
+@pytest.mark.parametrize("kept", [True, False])
 @pytest.mark.parametrize("activation", ["situ", "silu"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,f", SIZES + [(1500, 136, 72)])
-def test_gated_backward(m, k, f, dtype, activation):
+def test_gated_backward(m, k, f, dtype, activation, kept, monkeypatch):
+    monkeypatch.setattr("verace_amd.feed_forward._keeps", lambda *_: kept)
     g = torch.Generator().manual_seed(m + k + f)
     x, wg, wu = (t.requires_grad_() for t, _ in make(g, m, k, f, dtype, 2))
     dh = randn(g, m, f).to(dtype)
@@ -93,10 +95,12 @@ def test_gated_backward(m, k, f, dtype, activation):
         within(got, *w)
 
 
-@pytest.mark.parametrize("activation,bias", [(None, False), (None, True), ("silu", True), ("gelu", False)])
+@pytest.mark.parametrize("activation,bias,kept", [(None, False, True), (None, True, True), ("silu", True, True), ("silu", True, False),
+                                                  ("gelu", False, True), ("gelu", False, False)])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,n", SIZES + [(1500, 136, 72)])
-def test_linear_backward(m, k, n, dtype, activation, bias):
+def test_linear_backward(m, k, n, dtype, activation, bias, kept, monkeypatch):
+    monkeypatch.setattr("verace_amd.feed_forward._keeps", lambda *_: kept)
     g = torch.Generator().manual_seed(m + k + n)
     x, w = (t.requires_grad_() for t, _ in make(g, m, k, n, dtype, 1))
     b = randn(g, n).to(dtype).requires_grad_() if bias else None
@@ -112,3 +116,12 @@ def test_linear_backward(m, k, n, dtype, activation, bias):
         assert got.dtype == dtype
         within(got, *v)
     assert torch.equal(grads[-1], dy)
+
+
+def test_what_is_kept():
+    """Below a length of 1536 a 16-bit forward keeps its inputs alone; from there, and in float32, its sums too."""
+    for dtype, k, more in ((torch.bfloat16, 1528, 0), (torch.bfloat16, 1536, 1), (torch.float32, 64, 1)):
+        x, w = (torch.zeros(s, k, device="cuda", dtype=dtype, requires_grad=True) for s in (4, 8))
+        for y, n, m in ((va().gated_linear(x, w, w), 16, more), (va().linear_add(x, w, activation="silu"), 8, more), (va().linear_add(x, w), 8, 0)):
+            saved = [t for t in y.grad_fn.saved_tensors if t is not None and t.shape[1] != k]
+            assert [tuple(t.shape) for t in saved] == [(4, n)] * m and all(t.dtype == torch.float32 for t in saved)

@@ -39,6 +39,7 @@ struct Args {
   int64_t second;          // GATED_DZ: the first column of du; DX: where the second segment starts in a row of a
   int out_dtype;           // e4m3 operands: the result's
   float* partial;          // DW with several shares
+  float* keep;             // LINEAR, GATED: the sums before the activation, [m, n] (GATED [m, 2 n], a row's gates first), or null
   int seg, seg_valid;      // DW: rows of the result come in segments of seg, of which seg_valid are stored
   int act;
   float beta1, beta2;
@@ -239,6 +240,7 @@ __device__ __forceinline__ void finish(const Args& p, int m, int n, const Column
       for (int j = 0; j < W; ++j) z[j] += c.bias[j];
     }
     if constexpr (KIND == LINEAR) {
+      if (p.keep != nullptr) store_cols<float, W, FULL>(p.keep + static_cast<int64_t>(m) * p.n, n, p.n, z);
       activate_all<T, W>(z, p.act);
       if (p.other != nullptr) {
         if (other == nullptr) load_cols<T, W, FULL>(static_cast<const T*>(p.other) + m * p.ldother, n, p.n, t);
@@ -257,6 +259,11 @@ __device__ __forceinline__ void finish(const Args& p, int m, int n, const Column
   } else if constexpr (KIND == GATED || KIND == GATED_DZ) {
     const Gate gate{p.act, p.beta1, p.beta2, 1.f / p.beta1, 1.f / p.beta2};
     if constexpr (KIND == GATED) {
+      if (p.keep != nullptr) {
+        float* row = p.keep + static_cast<int64_t>(m) * 2 * p.n;
+        store_cols<float, W, FULL>(row, n, p.n, z);
+        store_cols<float, W, FULL>(row + p.n, n, p.n, z2);
+      }
       gated<T, W>(z, z2, gate);
       store_cols<T, W, FULL>(static_cast<T*>(p.out) + m * p.ldo, n, p.n, z);
     } else {

@@ -3,7 +3,7 @@
 //
 //   y = residual + act(x W^T + b)                              2 M N K operations
 //   h = act(x Wg^T) lin(x Wu^T)                                4 M F K
-// backward, from the inputs alone (nothing is kept by the forward):
+// backward, from the inputs alone or from the sums before the activation that the forward kept:
 //   dz = dy act'(x W^T + b), dx = dz W, dW = dz^T x, db = sum dz
 //   [dg du] likewise, dx = dg Wg + du Wu, [dWg; dWu] = [dg du]^T x
 // dz is rounded once to x's type, as the matrix cores take it; products are summed in fp32.
@@ -31,6 +31,41 @@ __global__ __launch_bounds__(NTH) void join_kernel(const float* partial, T* out,
     for (int j = 0; j < 4; ++j) s[j] += t[j];
   }
   store_cols<T, 4>(out + i, 0, rest, s);
+}
+
+// dz from the kept sums (PAIR: [dg du] from [g u]), a 16-byte piece of the result a thread, zeros from column n to the row's end.
+template <typename T, bool PAIR>
+__global__ __launch_bounds__(NTH) void dz_kernel(const float* z, const T* dy, int64_t lddy, T* dz, int n, int whole, int64_t count, Gate gate) {
+  constexpr int W = 16 / sizeof(T);
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * NTH + threadIdx.x;
+  if (e >= count) return;
+  const int pieces = whole / W, c = static_cast<int>(e % pieces) * W;
+  const int64_t m = e / pieces;
+  float d[W], a[W], b[W];
+  T* out = dz + m * (PAIR ? 2 : 1) * whole;
+  auto run = [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    load_cols<T, W, FULL>(dy + m * lddy, c, n, d);
+    const float* row = z + m * (PAIR ? 2 : 1) * n;
+    load_cols<float, W, FULL>(row, c, n, a);
+    if constexpr (PAIR) load_cols<float, W, FULL>(row + n, c, n, b);
+  };
+  if (c + W <= n) run(std::true_type{});
+  else run(std::false_type{});
+  if constexpr (PAIR) {
+    gated_slopes<T, W>(a, b, d, gate);
+  } else {
+    slope_all<T, W>(a, gate.act);
+#pragma unroll
+    for (int j = 0; j < W; ++j) a[j] *= d[j];
+  }
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    a[j] = c + j < n ? a[j] : 0.f;
+    if constexpr (PAIR) b[j] = c + j < n ? b[j] : 0.f;
+  }
+  store_cols<T, W, true>(out, c, whole, a);
+  if constexpr (PAIR) store_cols<T, W, true>(out + whole, c, whole, b);
 }
 
 // Column sums of [rows, n]: workgroup (b, s) those of 256 columns over the s-th share of the rows.  A thread adds 8 columns of
@@ -166,6 +201,30 @@ size_t weight_bytes(int64_t rows, int64_t valid, int64_t cols, int64_t m) {
   const Shares s = weight_shares(rows, cols, m);
   return s.n > 1 ? align256(static_cast<size_t>(s.n) * valid * cols * 4) : 0;
 }
+// dz [m, whole] (pair: [m, 2 whole]) from the sums that the forward kept.
+int dz_from_kept(int dtype, bool pair, const float* kept, const void* dy, int64_t lddy, void* dz, int64_t m, int64_t n, const Gate& gate,
+                 hipStream_t stream) {
+  const int64_t w = whole(n, dtype), per_row = w / (16 / size_of(dtype));
+  const int64_t rows_most = UINT32_MAX / NTH / per_row * NTH;
+  if (rows_most == 0) return VMI_ERR_UNSUPPORTED;
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    const int parts = pair ? 2 : 1;
+    for (int64_t row = 0; row < m; row += rows_most) {
+      const int64_t count = (m - row < rows_most ? m - row : rows_most) * per_row;
+      const dim3 grid(static_cast<unsigned>((count + NTH - 1) / NTH));
+      const float* z = kept + row * parts * n;
+      const T* d = static_cast<const T*>(dy) + row * lddy;
+      T* out = static_cast<T*>(dz) + row * parts * w;
+      if (pair)
+        hipLaunchKernelGGL((dz_kernel<T, true>), grid, dim3(NTH), 0, stream, z, d, lddy, out, static_cast<int>(n), static_cast<int>(w), count, gate);
+      else
+        hipLaunchKernelGGL((dz_kernel<T, false>), grid, dim3(NTH), 0, stream, z, d, lddy, out, static_cast<int>(n), static_cast<int>(w), count, gate);
+      if (const int st = hip_status(hipGetLastError()); st != VMI_OK) return st;
+    }
+    return VMI_OK;
+  });
+}
 int column_shares(int64_t m, int64_t n) {
   const int64_t t = (n + 255) / 256, want = t == 0 ? 1 : (256 + t - 1) / t, most = (m + 31) / 32;
   const int64_t s = want < most ? want : most;
@@ -196,7 +255,7 @@ extern "C" int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_
 
 extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
                               int dtype, const void* bias, const void* residual, int64_t ldr, int act, void* out, int64_t ldo,
-                              int out_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+                              int out_dtype, float* keep, int64_t M, int64_t N, int64_t K, void* stream) {
   if (!sizes_ok(M, N, K) || !linear_act(act) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
     return VMI_ERR_INVALID_ARG;
   if (dtype != VMI_E4M3 && out_dtype != dtype) return VMI_ERR_INVALID_ARG;
@@ -208,13 +267,14 @@ extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, 
   p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.xs = x_scale, p.ws = w_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
   p.bias = bias, p.other = residual, p.ldother = ldr, p.act = act, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
+  p.keep = keep;
   return product(dtype, LINEAR, p, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale, const void* w_gate, int64_t ldg,
                                 const float* gate_scale, const void* w_up, int64_t ldu, const float* up_scale, int dtype, int act,
-                                float beta1, float beta2, void* out, int64_t ldo, int out_dtype, int64_t M, int64_t F, int64_t K,
-                                void* stream) {
+                                float beta1, float beta2, void* out, int64_t ldo, int out_dtype, float* keep, int64_t M, int64_t F,
+                                int64_t K, void* stream) {
   if (!sizes_ok(M, F, K) || !gate_act(act) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
     return VMI_ERR_INVALID_ARG;
   if (dtype != VMI_E4M3 && out_dtype != dtype) return VMI_ERR_INVALID_ARG;
@@ -230,6 +290,7 @@ extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale
   p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.xs = x_scale, p.ws = gate_scale, p.ws2 = up_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(F), p.k = static_cast<int>(K);
   p.act = act, p.beta1 = beta1, p.beta2 = beta2, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
+  p.keep = keep;
   return product(dtype, GATED, p, static_cast<hipStream_t>(stream));
 }
 
@@ -243,7 +304,7 @@ extern "C" int vmi_linear_add_bwd_workspace_bytes(int64_t M, int64_t N, int64_t 
 }
 
 extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const void* bias, int act,
-                                  const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M, int64_t N, int64_t K,
+                                  const float* kept, const void* dy, int64_t lddy, void* dx, void* dw, void* db, int64_t M, int64_t N, int64_t K,
                                   void* workspace, size_t workspace_bytes, void* stream) {
   size_t need = 0;
   if (const int st = vmi_linear_add_bwd_workspace_bytes(M, N, K, dtype, act, &need); st != VMI_OK) return st;
@@ -260,7 +321,11 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
   if (act != ACT_NONE) {
     dz = at, lddz = n;
     at += align256(static_cast<size_t>(M) * n * size);
-    if (M > 0 && N > 0) {
+    if (M > 0 && N > 0 && kept != nullptr) {
+      Gate gate{};
+      gate.act = act;
+      if (const int st = dz_from_kept(dtype, false, kept, dy, lddy, const_cast<void*>(dz), M, N, gate, s); st != VMI_OK) return st;
+    } else if (M > 0 && N > 0) {
       Args p{};
       p.a = x, p.lda = ldx, p.b = w, p.ldb = ldw, p.m = static_cast<int>(M), p.n = static_cast<int>(N), p.k = static_cast<int>(K);
       p.bias = bias, p.other = dy, p.ldother = lddy, p.act = act, p.out = const_cast<void*>(dz), p.ldo = lddz;
@@ -302,8 +367,8 @@ extern "C" int vmi_gated_linear_bwd_workspace_bytes(int64_t M, int64_t F, int64_
 }
 
 extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
-                                    int dtype, int act, float beta1, float beta2, const void* dh, int64_t lddh, void* dx,
-                                    void* dw, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes,
+                                    int dtype, int act, float beta1, float beta2, const float* kept, const void* dh, int64_t lddh,
+                                    void* dx, void* dw, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes,
                                     void* stream) {
   size_t need = 0;
   if (const int st = vmi_gated_linear_bwd_workspace_bytes(M, F, K, dtype, &need); st != VMI_OK) return st;
@@ -320,7 +385,10 @@ extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_ga
   const int64_t size = size_of(dtype), f = whole(F, dtype), lddz = 2 * f;
   char* dz = static_cast<char*>(workspace);
   float* partial = reinterpret_cast<float*>(dz + align256(static_cast<size_t>(M) * lddz * size));
-  if (M > 0 && F > 0) {
+  if (M > 0 && F > 0 && kept != nullptr) {
+    const Gate gate{act, beta1, beta2, 1.f / beta1, 1.f / beta2};
+    if (const int st = dz_from_kept(dtype, true, kept, dh, lddh, dz, M, F, gate, s); st != VMI_OK) return st;
+  } else if (M > 0 && F > 0) {
     Args p{};
     p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.m = static_cast<int>(M), p.n = static_cast<int>(F);
     p.k = static_cast<int>(K), p.other = dh, p.ldother = lddh, p.act = act, p.beta1 = beta1, p.beta2 = beta2;

@@ -200,13 +200,13 @@ def _declare(lib):
                                            i32, i32, vp, vp, i32, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                            i64, i64, i64, i64, i64, i64, vp, sz, vp]
     lib.vmi_pad_rows.argtypes = [vp, i64, vp, i64, i64, vp]
-    lib.vmi_linear_add.argtypes = [vp, i64, vp, vp, i64, vp, i32, vp, vp, i64, i32, vp, i64, i32, i64, i64, i64, vp]
+    lib.vmi_linear_add.argtypes = [vp, i64, vp, vp, i64, vp, i32, vp, vp, i64, i32, vp, i64, i32, vp, i64, i64, i64, vp]
     lib.vmi_linear_add_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, psz]
-    lib.vmi_linear_add_bwd.argtypes = [vp, i64, vp, i64, i32, vp, i32, vp, i64, vp, vp, vp, i64, i64, i64, vp, sz, vp]
-    lib.vmi_gated_linear.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, i32, f32, f32, vp, i64, i32, i64, i64, i64,
+    lib.vmi_linear_add_bwd.argtypes = [vp, i64, vp, i64, i32, vp, i32, vp, vp, i64, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.vmi_gated_linear.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, i32, f32, f32, vp, i64, i32, vp, i64, i64, i64,
                                      vp]
     lib.vmi_gated_linear_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, psz]
-    lib.vmi_gated_linear_bwd.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, f32, f32, vp, i64, vp, vp, i64, i64, i64, vp,
+    lib.vmi_gated_linear_bwd.argtypes = [vp, i64, vp, i64, vp, i64, i32, i32, f32, f32, vp, vp, i64, vp, vp, i64, i64, i64, vp,
                                          sz, vp]
     lib.vmi_norm_add_quant.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, f32, vp, vp, vp, i64, i64, vp]
     for name in ("gated_norm", "gated_norm_bwd_workspace_bytes", "gated_norm_bwd", "short_conv", "short_conv_step",

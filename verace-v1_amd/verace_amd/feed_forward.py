@@ -163,7 +163,18 @@ def _result(x: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
     return x.new_empty(shape) if dtype is x.dtype else torch.empty(shape, device=x.device, dtype=dtype)
 
 
-def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, beta2, out_dtype):
+def _keeps(dtype: torch.dtype, k: int) -> bool:
+    """Whether a forward keeps its fp32 sums for the backward: writing and reading 8 bytes of each takes less time than a product
+    of length k.  Forward and backward in us, kept / formed again: gated, bf16, M 8192, F 2048: K 1024 261 / 268, K 1536 340 / 372,
+    K 4096 630 / 760; F 8192: K 1024 977 / 952, K 4096 2531 / 3010; linear, fp16, M 8192, N 1024: K 1024 129 / 127, K 2048 137 / 163."""
+    return dtype is torch.float32 or k >= 1536
+
+
+def _kept(x: torch.Tensor, m: int, n: int, k: int) -> Optional[torch.Tensor]:
+    return torch.empty((m, n), device=x.device, dtype=torch.float32) if _keeps(x.dtype, k) else None
+
+
+def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, beta2, out_dtype, keep=None):
     F, K = w_gate.shape
     x2, xp, ldx = _operand(x, K)
     (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
@@ -173,11 +184,11 @@ def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, be
     with device_guard(x):
         _lib.check(_lib.load().vmi_gated_linear(
             xp, ldx, address(x_scale), gp, ldg, address(gate_scale), up, ldu, address(up_scale), _code(x.dtype), act, beta1, beta2,
-            out.data_ptr(), F, _lib.dtype_code(out_dtype), _rows_of(x, K), F, K, _lib.raw_stream(x.device)), "vmi_gated_linear")
+            out.data_ptr(), F, _lib.dtype_code(out_dtype), address(keep), _rows_of(x, K), F, K, _lib.raw_stream(x.device)), "vmi_gated_linear")
     return out
 
 
-def _launch_gated_bwd(x, w_gate, w_up, act, beta1, beta2, dh, need):
+def _launch_gated_bwd(x, w_gate, w_up, act, beta1, beta2, dh, need, kept=None):
     """(dx, dw_gate, dw_up) for dL/dh, None where not needed."""
     F, K = w_gate.shape
     if dh.shape != x.shape[:-1] + (F,) or dh.dtype != x.dtype or dh.device != x.device:
@@ -193,25 +204,28 @@ def _launch_gated_bwd(x, w_gate, w_up, act, beta1, beta2, dh, need):
     ws, ws_bytes = _workspace("vmi_gated_linear_bwd_workspace_bytes", M, F, K, code, device=x.device)
     with device_guard(x):
         _lib.check(_lib.load().vmi_gated_linear_bwd(
-            xp, ldx, gp, ldg, up, ldu, code, act, beta1, beta2, dhp, lddh, address(dx), address(dw), M, F, K, address(ws), ws_bytes,
+            xp, ldx, gp, ldg, up, ldu, code, act, beta1, beta2, address(kept), dhp, lddh, address(dx), address(dw), M, F, K, address(ws), ws_bytes,
             _lib.raw_stream(x.device)), "vmi_gated_linear_bwd")
     return dx, dw[0] if need[1] else None, dw[1] if need[2] else None
 
 
 class GatedLinearFunction(torch.autograd.Function):
-    """:func:`gated_linear` as an autograd node (only the inputs are kept)."""
+    """:func:`gated_linear` as an autograd node."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act, beta1, beta2):
-        ctx.save_for_backward(x, w_gate, w_up)
+        F, K = w_gate.shape
+        keep = _kept(x, _rows_of(x, K), 2 * F, K)
+        h = _launch_gated(x, w_gate, w_up, None, None, None, act, beta1, beta2, x.dtype, keep)
+        ctx.save_for_backward(x, w_gate, w_up, keep)
         ctx.form = (act, beta1, beta2)
-        return _launch_gated(x, w_gate, w_up, None, None, None, act, beta1, beta2, x.dtype)
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up = ctx.saved_tensors
-        return (*_launch_gated_bwd(x, w_gate, w_up, *ctx.form, dh, ctx.needs_input_grad[:3]), None, None, None)
+        x, w_gate, w_up, kept = ctx.saved_tensors
+        return (*_launch_gated_bwd(x, w_gate, w_up, *ctx.form, dh, ctx.needs_input_grad[:3], kept), None, None, None)
 
 
 def gated_linear(
@@ -230,8 +244,9 @@ def gated_linear(
 
     x: [..., K]; w_gate, w_up: [F, K], all bfloat16, float16 or float32.  ``activation`` "situ" (the layer's):
     a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2); "silu": a(z) = z sigmoid(z), b(z) = z.
-    Sums and activations are fp32 and h is rounded once.  Differentiable once in x and both weights: the backward keeps the
-    inputs alone, forms both projections again and rounds their gradients to x's dtype once, as operands of its products.
+    Sums and activations are fp32 and h is rounded once.  Differentiable once in x and both weights.  For K below 1536
+    (16 bits) the backward keeps the inputs alone and forms both projections again; otherwise, and in float32, the forward keeps
+    them too, in float32 (8 bytes for each element of h).  Their gradients are rounded to x's dtype once, as operands of products.
 
     8 bits: x and the weights float8_e4m3fn with ``x_scale`` [...], ``gate_scale``, ``up_scale`` [F] float32; h is
     ``out_dtype`` (bfloat16), without gradients.
@@ -264,7 +279,7 @@ def _linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, 
     return out_dtype
 
 
-def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dtype):
+def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dtype, keep=None):
     N, K = weight.shape
     x2, xp, ldx = _operand(x, K)
     w, wp, ldw = _operand(weight, K)
@@ -276,11 +291,11 @@ def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dt
     with device_guard(x):
         _lib.check(_lib.load().vmi_linear_add(
             xp, ldx, address(x_scale), wp, ldw, address(weight_scale), _code(x.dtype), address(bias), rp, ldr, act, out.data_ptr(), N,
-            _lib.dtype_code(out_dtype), _rows_of(x, K), N, K, _lib.raw_stream(x.device)), "vmi_linear_add")
+            _lib.dtype_code(out_dtype), address(keep), _rows_of(x, K), N, K, _lib.raw_stream(x.device)), "vmi_linear_add")
     return out
 
 
-def _launch_linear_bwd(x, weight, bias, act, dy, need):
+def _launch_linear_bwd(x, weight, bias, act, dy, need, kept=None):
     """(dx, dweight, dbias) for dL/dy, None where not needed."""
     N, K = weight.shape
     if dy.shape != x.shape[:-1] + (N,) or dy.dtype != x.dtype or dy.device != x.device:
@@ -298,26 +313,29 @@ def _launch_linear_bwd(x, weight, bias, act, dy, need):
     ws, ws_bytes = _workspace("vmi_linear_add_bwd_workspace_bytes", M, N, K, code, act, device=x.device)
     with device_guard(x):
         _lib.check(_lib.load().vmi_linear_add_bwd(
-            xp, ldx, wp, ldw, code, address(bias), act, dyp, lddy, address(dx), address(dw), address(db), M, N, K, address(ws),
+            xp, ldx, wp, ldw, code, address(bias), act, address(kept), dyp, lddy, address(dx), address(dw), address(db), M, N, K, address(ws),
             ws_bytes, _lib.raw_stream(x.device)), "vmi_linear_add_bwd")
     return dx, dw, db
 
 
 class LinearAddFunction(torch.autograd.Function):
-    """:func:`linear_add` as an autograd node (only the inputs are kept; the residual's gradient is dy)."""
+    """:func:`linear_add` as an autograd node (the residual's gradient is dy)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        ctx.save_for_backward(x, weight, bias)
+        N, K = weight.shape
+        keep = _kept(x, _rows_of(x, K), N, K) if act else None
+        y = _launch_linear(x, weight, bias, residual, None, None, act, x.dtype, keep)
+        ctx.save_for_backward(x, weight, bias, keep)
         ctx.act = act
-        return _launch_linear(x, weight, bias, residual, None, None, act, x.dtype)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
+        x, weight, bias, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
-        grads = _launch_linear_bwd(x, weight, bias, ctx.act, dy, need) if any(need[:3]) else (None, None, None)
+        grads = _launch_linear_bwd(x, weight, bias, ctx.act, dy, need, kept) if any(need[:3]) else (None, None, None)
         return (*grads, dy if need[3] else None, None)
 
 
@@ -335,7 +353,8 @@ def linear_add(
 
     x: [..., K]; weight: [N, K]; bias: [N]; residual: [..., N], all of one dtype (bfloat16, float16, float32); ``activation``
     None, "silu" or "gelu" (z Phi(z)).  Sums and the epilogue are fp32 and y is rounded once.  Differentiable once in every
-    tensor; the backward keeps x, weight and bias alone.
+    tensor; the backward keeps x, weight and bias, and with an activation, for K of 1536 and more or in float32, the sum before
+    it in float32.
 
     8 bits: x and weight float8_e4m3fn with ``x_scale`` [...] and ``weight_scale`` [N] float32; bias, residual and y are
     ``out_dtype`` (bfloat16), without gradients.
