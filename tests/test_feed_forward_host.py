@@ -82,6 +82,9 @@ def test_no_gradients_through_8_bits():
             call()
         with torch.no_grad():
             call()
+    from verace_amd import feed_forward as ff
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ff._rows_fit(_e(1, 8), 1 << 23)
 
 
 @fake
@@ -157,7 +160,9 @@ def test_c_refusals(lib):
     assert bwd(one, 16, one, 16, 1, null, 5, null, one, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
     assert bwd(one, 16, one, 16, 1, null, 1, null, odd, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
     assert bwd(one, 16, one, 16, 1, null, 1, null, null, 8, one, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
+    assert bwd(one, 16, one, 16, 1, null, 1, null, one, 1 << 23, one, one, one, 0, 1 << 23, 16, one, 1 << 40, null) == UNSUPPORTED
     gb = lib.vmi_gated_linear_bwd
+    assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, null, one, 1 << 22, one, one, 0, 1 << 22, 16, one, 1 << 40, null) == UNSUPPORTED
     assert gb(one, 16, one, 16, one, 16, 1, 0, 4.0, 25.0, null, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID
     assert gb(one, 16, one, 16, one, 24, 1, 3, 4.0, 25.0, null, one, 8, one, one, 2, 8, 16, one, 1 << 30, null) == UNSUPPORTED
     assert gb(one, 16, one, 16, one, 16, 1, 3, 4.0, 25.0, null, one, 7, one, one, 2, 8, 16, one, 1 << 30, null) == INVALID

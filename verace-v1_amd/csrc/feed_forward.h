@@ -206,6 +206,22 @@ template <typename T, int W, bool FULL = false> __device__ __forceinline__ void 
   }
 }
 
+// The fp32 sums that a forward kept, read once.  (Written with ordinary stores: nontemporal ones of a lane's 16 bytes, a part of
+// a line each, took the forward and backward of 8192 x 4096 x 8192 from 2531 to 2709 us.)
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+template <int W, bool FULL> __device__ __forceinline__ void kept_cols(const float* row, int n, int n_end, float (&x)[W]) {
+  if (FULL || n + W <= n_end) {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(row + n + j));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j + i] = v[i];
+    }
+  } else {
+    load_cols<float, W, FULL>(row, n, n_end, x);
+  }
+}
+
 // What the epilogue needs of W consecutive columns from n, for all of a lane's rows.
 template <int W> struct Columns {
   float ws[W], ws2[W], bias[W];

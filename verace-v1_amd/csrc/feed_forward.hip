@@ -15,6 +15,7 @@ using namespace vmi::prod;
 namespace {
 
 constexpr int NTH = 256;
+constexpr int64_t kMaxRow = INT64_C(1) << 24;  // bytes between rows: 128 of them lie within the 31 bits of a load's offset
 
 // out = the sum of `splits` partial results of n elements.
 template <typename T>
@@ -47,8 +48,8 @@ __global__ __launch_bounds__(NTH) void dz_kernel(const float* z, const T* dy, in
     constexpr bool FULL = decltype(full)::value;
     load_cols<T, W, FULL>(dy + m * lddy, c, n, d);
     const float* row = z + m * (PAIR ? 2 : 1) * n;
-    load_cols<float, W, FULL>(row, c, n, a);
-    if constexpr (PAIR) load_cols<float, W, FULL>(row + n, c, n, b);
+    kept_cols<W, FULL>(row, c, n, a);
+    if constexpr (PAIR) kept_cols<W, FULL>(row + n, c, n, b);
   };
   if (c + W <= n) run(std::true_type{});
   else run(std::false_type{});
@@ -150,7 +151,7 @@ int rows_status(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype
   if (p == nullptr || ld < cols) return VMI_ERR_INVALID_ARG;
   const int64_t size = size_of(dtype);
   if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || ld * size % 16 != 0 || ld < whole(cols, dtype)) return VMI_ERR_UNSUPPORTED;
-  return ld * size >= (INT64_C(1) << 24) ? VMI_ERR_UNSUPPORTED : VMI_OK;
+  return ld * size >= kMaxRow ? VMI_ERR_UNSUPPORTED : VMI_OK;
 }
 bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   const int64_t most = INT64_C(1) << 30;
@@ -315,6 +316,7 @@ extern "C" int vmi_linear_add_bwd(const void* x, int64_t ldx, const void* w, int
     return st;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t size = size_of(dtype), n = whole(N, dtype);
+  if (n * size >= kMaxRow) return VMI_ERR_UNSUPPORTED;  // dz
   char* at = static_cast<char*>(workspace);
   const void* dz = dy;
   int64_t lddz = lddy;
@@ -383,6 +385,7 @@ extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_ga
   if (M > 0 && F > 0 && (dh == nullptr || lddh < F)) return VMI_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t size = size_of(dtype), f = whole(F, dtype), lddz = 2 * f;
+  if (lddz * size >= kMaxRow) return VMI_ERR_UNSUPPORTED;
   char* dz = static_cast<char*>(workspace);
   float* partial = reinterpret_cast<float*>(dz + align256(static_cast<size_t>(M) * lddz * size));
   if (M > 0 && F > 0 && kept != nullptr) {

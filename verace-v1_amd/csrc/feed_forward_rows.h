@@ -117,7 +117,7 @@ template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t strea
   if (!grid_fits(cols, 512)) return VMI_ERR_UNSUPPORTED;
   int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
   while (mt > 1 && cols * ((p.m + 16 * mt - 1) / (16 * mt)) <= 128) mt /= 2;
-  const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>((p.m + 16 * mt - 1) / (16 * mt)));  // at most 96 of the latter
+  const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>((p.m + 16 * mt - 1) / (16 * mt)));
   if (mt == 1) hipLaunchKernelGGL((rows_kernel<E, KIND, 1>), grid, dim3(512), 0, stream, p);
   else if (mt == 2) hipLaunchKernelGGL((rows_kernel<E, KIND, 2>), grid, dim3(512), 0, stream, p);
   else hipLaunchKernelGGL((rows_kernel<E, KIND, 4>), grid, dim3(512), 0, stream, p);

@@ -12,7 +12,7 @@
 // 2^-21 of the row's.  Rows whose 32-bit terms are not all finite, or all below 2^-60, take the 64-bit form throughout.
 // The sum of squares is of 64 bits, over s of 32 for 16-bit inputs: the scale is within 2^-23.
 //
-// One read of each input, one write of each result: HBM bounds it.  A row is one wave's (up to 8 pieces of 16 bytes a lane)
+// One read of each input, one write of each result: HBM bounds it.  A row is one wave's (up to 4 pieces of 16 bytes a lane)
 // or four waves'; its inputs stay in registers, as they came, between the pass that sums and the pass that writes.  Longer rows
 // are read again.  A row with a NaN or an infinity in p has the scale NaN and q NaN everywhere; its s is what it is.
 #include <type_traits>
@@ -64,12 +64,16 @@ template <typename W, int N, bool WHOLE> __device__ __forceinline__ void load_we
   }
 }
 
-// 16 bytes of a row from element i0 as they lie, zeros past its end.
-template <typename T, bool WHOLE> __device__ __forceinline__ Vec<T> load_raw(const T* row, int i0, int d) {
+// 16 bytes of a row from element i0 as they lie, zeros past its end.  ONCE: nothing reads them again (32768 x 4096 bf16 with
+// these loads 189 us, with ordinary ones 241: the results then keep more of the caches).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+template <typename T, bool WHOLE, bool ONCE> __device__ __forceinline__ Vec<T> load_raw(const T* row, int i0, int d) {
   Vec<T> v;
   if (WHOLE || i0 + Vec<T>::N <= d) {
-    __builtin_memcpy(&v, row + i0, 16);
-    return v;
+    const u32x4_any* from = reinterpret_cast<const u32x4_any*>(row + i0);
+    const u32x4 x = ONCE ? __builtin_nontemporal_load(from) : *from;
+    return __builtin_bit_cast(Vec<T>, x);
   }
 #pragma unroll
   for (int j = 0; j < Vec<T>::N; ++j) {
@@ -109,10 +113,9 @@ template <typename T, bool RES> struct Terms {
   __device__ __forceinline__ double p64(int j) const { return s64(j) * static_cast<double>(w[j]); }
 };
 
-// Keeps the compiler from carrying a piece's terms from one pass to the next in registers (64 of them at 8 pieces of 16 bits):
+// Keeps the compiler from carrying a piece's terms from one pass to the next in registers (8 a piece of 16 bits):
 // they are formed again from the 16 bytes.
 template <typename T> __device__ __forceinline__ void forget(Vec<T>& v) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   u32x4 x = __builtin_bit_cast(u32x4, v);
   asm volatile("" : "+v"(x));
   v = __builtin_bit_cast(Vec<T>, x);
@@ -140,8 +143,8 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   T* sr = k.sum == nullptr ? nullptr : static_cast<T*>(k.sum) + row * k.d;
   Vec<T> a[LONG ? 1 : NV] = {}, r[LONG ? 1 : NV] = {};
   auto load = [&](int v, int i0) {
-    a[v] = load_raw<T, WHOLE>(ar, i0, k.d);
-    if constexpr (RES) r[v] = load_raw<T, WHOLE>(rr, i0, k.d);
+    a[v] = load_raw<T, WHOLE, !LONG>(ar, i0, k.d);
+    if constexpr (RES) r[v] = load_raw<T, WHOLE, !LONG>(rr, i0, k.d);
   };
   auto terms = [&](int v, int i0) {
     Terms<T, RES> t;
@@ -295,7 +298,7 @@ template <typename T, typename W> int by_row(const Args& k, hipStream_t stream) 
   if (pieces <= 64) return launch<T, W, 64, 1, false>(k, stream);
   if (pieces <= 128) return launch<T, W, 64, 2, false>(k, stream);
   if (pieces <= 256) return launch<T, W, 64, 4, false>(k, stream);
-  if (pieces <= 512) return launch<T, W, 64, 8, false>(k, stream);
+  if (pieces <= 512) return launch<T, W, 256, 2, false>(k, stream);  // 189 us for 193 by one wave a row of 8 pieces a lane
   if (pieces <= 1024) return launch<T, W, 256, 4, false>(k, stream);
   if (pieces <= 2048) return launch<T, W, 256, 8, false>(k, stream);
   return launch<T, W, 256, 1, true>(k, stream);

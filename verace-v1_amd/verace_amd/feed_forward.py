@@ -77,7 +77,7 @@ def _plain_rows(t: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tenso
 
 def _weight_check(x, K, name, w, scale_name, scale) -> None:
     s = w.shape
-    if len(s) != 2 or s[1] != K or w.dtype is not x.dtype or w.device != x.device:
+    if len(s) != 2 or s[1] != K or w.dtype is not x.dtype or w.get_device() != x.get_device():
         raise RuntimeError(f"verace_amd: {name} must be [N, {K}] {x.dtype} on {x.device}, "
                            f"got {tuple(s)} {w.dtype} on {w.device}")
     if scale is not None or x.dtype is E4M3:
@@ -120,6 +120,12 @@ def _workspace(query, *args, device) -> Tuple[Optional[torch.Tensor], int]:
     need = ctypes.c_size_t(0)
     _lib.check(getattr(_lib.load(), query)(*args, ctypes.byref(need)), query)
     return (torch.empty(need.value, device=device, dtype=torch.uint8) if need.value else None), need.value
+
+
+def _rows_fit(x: torch.Tensor, n: int) -> None:
+    """Refuses, before its forward, a call whose backward's rows of n gradients would lie too far apart."""
+    if (n + 8) * _ITEMSIZE[x.dtype] >= _MAX_ROW_BYTES:
+        raise RuntimeError(f"verace_amd: no gradients of projections to {n} {x.dtype} columns")
 
 
 def _no_grad_rows(**tensors) -> None:
@@ -215,6 +221,7 @@ class GatedLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act, beta1, beta2):
         F, K = w_gate.shape
+        _rows_fit(x, 2 * F)
         keep = _kept(x, _rows_of(x, K), 2 * F, K)
         h = _launch_gated(x, w_gate, w_up, None, None, None, act, beta1, beta2, x.dtype, keep)
         ctx.save_for_backward(x, w_gate, w_up, keep)
@@ -254,7 +261,7 @@ def gated_linear(
     out_dtype = _gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, beta1, beta2, out_dtype)
     refuse_tangents(x, w_gate, w_up)
     if x.dtype == E4M3:
-        _no_grad_rows(x_scale=x_scale, gate_scale=gate_scale, up_scale=up_scale)
+        _no_grad_rows(x=x, w_gate=w_gate, w_up=w_up, x_scale=x_scale, gate_scale=gate_scale, up_scale=up_scale)
     if traced(x):
         return torch.ops.verace.gated_linear(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, beta1, beta2, out_dtype)
     act = _GATED_ACT[activation]
@@ -273,7 +280,7 @@ def _linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, 
     if bias is not None or residual is not None:
         n = weight.shape[:1]
         for name, t, shape in (("bias", bias, n), ("residual", residual, x.shape[:-1] + n)):
-            if t is not None and (t.shape != shape or t.dtype is not out_dtype or t.device != x.device):
+            if t is not None and (t.shape != shape or t.dtype is not out_dtype or t.get_device() != x.get_device()):
                 raise RuntimeError(f"verace_amd: {name} must be {tuple(shape)} {out_dtype} on {x.device}, "
                                    f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     return out_dtype
@@ -324,6 +331,7 @@ class LinearAddFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         N, K = weight.shape
+        _rows_fit(x, N)
         keep = _kept(x, _rows_of(x, K), N, K) if act else None
         y = _launch_linear(x, weight, bias, residual, None, None, act, x.dtype, keep)
         ctx.save_for_backward(x, weight, bias, keep)
@@ -362,7 +370,7 @@ def linear_add(
     out_dtype = _linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype)
     refuse_tangents(x, weight, bias, residual)
     if x.dtype == E4M3:
-        _no_grad_rows(x_scale=x_scale, weight_scale=weight_scale, bias=bias, residual=residual)
+        _no_grad_rows(x=x, weight=weight, x_scale=x_scale, weight_scale=weight_scale, bias=bias, residual=residual)
     if traced(x):
         return torch.ops.verace.linear_add(x, weight, bias, residual, x_scale, weight_scale, activation, out_dtype)
     act = _LINEAR_ACT[activation]
@@ -380,7 +388,7 @@ def _quant_check(a, residual, norm_weight) -> None:
     _lib.dtype_code(dtype)
     if len(shape) < 1 or shape[-1] < 1:
         raise RuntimeError(f"verace_amd: rows must be [..., d], got {tuple(shape)}")
-    if residual is not None and (residual.shape != shape or residual.dtype is not dtype or residual.device != a.device):
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype or residual.get_device() != a.get_device()):
         raise RuntimeError(f"verace_amd: residual must be {tuple(shape)} {dtype} on {a.device}, "
                            f"got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
     if norm_weight is not None and (norm_weight.shape != shape[-1:] or norm_weight.dtype not in (dtype, torch.float32)
