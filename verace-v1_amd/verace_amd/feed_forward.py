@@ -165,8 +165,7 @@ def _rows_of(t: torch.Tensor, k: int) -> int:
 
 
 def _result(x: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
-    shape = x.shape[:-1] + (n,)
-    return x.new_empty(shape) if dtype is x.dtype else torch.empty(shape, device=x.device, dtype=dtype)
+    return torch.empty(*x.shape[:-1], n, device=x.device, dtype=dtype)
 
 
 def _keeps(dtype: torch.dtype, k: int) -> bool:
@@ -403,9 +402,9 @@ def _launch_quant(a, residual, weight, norm: bool, eps: float, want_sum: bool):
     a2, ap, lda = _plain_rows(a, d)
     r2, rp, ldr = _plain_rows(residual, d)
     w = _vector(weight)
-    q = torch.empty(shape, device=a.device, dtype=E4M3)
-    scale = torch.empty(shape[:-1], device=a.device, dtype=torch.float32)
-    s = torch.empty(shape, device=a.device, dtype=a.dtype) if want_sum else None
+    q = torch.empty_like(a, dtype=E4M3, memory_format=torch.contiguous_format)
+    scale = torch.empty(tuple(shape[:-1]), device=a.device, dtype=torch.float32)
+    s = torch.empty_like(a, memory_format=torch.contiguous_format) if want_sum else None
     code = _lib.dtype_code(a.dtype)
     with device_guard(a):
         _lib.check(_lib.load().vmi_norm_add_quant(
