@@ -231,6 +231,7 @@ int column_shares(int64_t m, int64_t n) {
   const int64_t s = want < most ? want : most;
   return static_cast<int>(s < 1 ? 1 : s);
 }
+Gate gate_of(int act, float beta1, float beta2) { return {act, beta1, beta2, 1.f / beta1, 1.f / beta2}; }
 bool gate_act(int act) { return act == ACT_SILU || act == ACT_SITU; }
 bool linear_act(int act) { return act == ACT_NONE || act == ACT_SILU || act == ACT_GELU; }
 
@@ -290,7 +291,7 @@ extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale
   Args p{};
   p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.xs = x_scale, p.ws = gate_scale, p.ws2 = up_scale;
   p.m = static_cast<int>(M), p.n = static_cast<int>(F), p.k = static_cast<int>(K);
-  p.act = act, p.beta1 = beta1, p.beta2 = beta2, p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
+  p.gate = gate_of(act, beta1, beta2), p.out = out, p.ldo = ldo, p.out_dtype = out_dtype;
   p.keep = keep;
   return product(dtype, GATED, p, static_cast<hipStream_t>(stream));
 }
@@ -389,12 +390,11 @@ extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_ga
   char* dz = static_cast<char*>(workspace);
   float* partial = reinterpret_cast<float*>(dz + align256(static_cast<size_t>(M) * lddz * size));
   if (M > 0 && F > 0 && kept != nullptr) {
-    const Gate gate{act, beta1, beta2, 1.f / beta1, 1.f / beta2};
-    if (const int st = dz_from_kept(dtype, true, kept, dh, lddh, dz, M, F, gate, s); st != VMI_OK) return st;
+    if (const int st = dz_from_kept(dtype, true, kept, dh, lddh, dz, M, F, gate_of(act, beta1, beta2), s); st != VMI_OK) return st;
   } else if (M > 0 && F > 0) {
     Args p{};
     p.a = x, p.lda = ldx, p.b = w_gate, p.b2 = w_up, p.ldb = ldg, p.m = static_cast<int>(M), p.n = static_cast<int>(F);
-    p.k = static_cast<int>(K), p.other = dh, p.ldother = lddh, p.act = act, p.beta1 = beta1, p.beta2 = beta2;
+    p.k = static_cast<int>(K), p.other = dh, p.ldother = lddh, p.gate = gate_of(act, beta1, beta2);
     p.out = dz, p.ldo = lddz, p.second = f;
     if (const int st = product(dtype, GATED_DZ, p, s); st != VMI_OK) return st;
   }
