@@ -35,7 +35,7 @@ def test_gated_refusals():
                       (ok, dict(w_gate=_e(8, 15))), (ok, dict(w_up=_e(9, 16))), (ok, dict(w_up=_e(8, 16, dtype=F32))),
                       (ok, dict(w_gate=_e(16))), (ok, dict(w_gate=_e(8, 16, device="cpu"))), (ok, dict(activation="gelu")),
                       (ok, dict(activation=None)), (ok, dict(beta1=0.0)), (ok, dict(beta2=-1.0)), (ok, dict(beta2=float("inf"))),
-                      (ok, dict(beta1=float("nan"))), (ok, dict(x_scale=_e(3, dtype=F32))), (ok, dict(gate_scale=_e(8, dtype=F32))),
+                      (ok, dict(beta1=float("nan"))), (ok, dict(beta1=1e-40)), (ok, dict(beta2=1e39)), (ok, dict(x_scale=_e(3, dtype=F32))), (ok, dict(gate_scale=_e(8, dtype=F32))),
                       (ok, dict(out_dtype=F32)), (ok, dict(x=_e())), (eight, dict(x_scale=None)), (eight, dict(x_scale=_e(3))),
                       (eight, dict(x_scale=_e(3, 1, dtype=F32))), (eight, dict(up_scale=None)), (eight, dict(up_scale=_e(1, dtype=F32))),
                       (eight, dict(gate_scale=_e(8, dtype=F32, device="cpu"))), (eight, dict(out_dtype=E4M3)),

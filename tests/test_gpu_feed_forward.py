@@ -125,3 +125,6 @@ def test_what_is_kept():
         for y, n, m in ((va().gated_linear(x, w, w), 16, more), (va().linear_add(x, w, activation="silu"), 8, more), (va().linear_add(x, w), 8, 0)):
             saved = [t for t in y.grad_fn.saved_tensors if t is not None and t.shape[1] != k]
             assert [tuple(t.shape) for t in saved] == [(4, n)] * m and all(t.dtype == torch.float32 for t in saved)
+    r = torch.zeros(4, 8, device="cuda", requires_grad=True)
+    y = va().linear_add(torch.zeros(4, 64, device="cuda"), torch.zeros(8, 64, device="cuda"), None, r, activation="silu")
+    assert [t for t in y.grad_fn.saved_tensors if t is not None and t.shape == (4, 8)] == []

@@ -25,6 +25,7 @@ E4M3 = torch.float8_e4m3fn
 _LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2}
 _GATED_ACT = {"silu": 1, "situ": 3}
 _MAX_ROW_BYTES = 1 << 24  # from a row to the next
+_LEAST_BETA = 2.0 ** -64
 _ITEMSIZE = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, E4M3: 1}
 
 
@@ -146,8 +147,8 @@ def _gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, bet
         raise RuntimeError(f"verace_amd: w_up {tuple(w_up.shape)} != w_gate {tuple(w_gate.shape)}")
     if activation not in _GATED_ACT:
         raise RuntimeError(f"verace_amd: activation must be one of {tuple(_GATED_ACT)}, got {activation!r}")
-    if activation == "situ" and not (0 < beta1 < float("inf") and 0 < beta2 < float("inf")):
-        raise RuntimeError(f"verace_amd: beta1 and beta2 must be positive and finite, got {beta1}, {beta2}")
+    if activation == "situ" and not (_LEAST_BETA <= beta1 <= 1 / _LEAST_BETA and _LEAST_BETA <= beta2 <= 1 / _LEAST_BETA):
+        raise RuntimeError(f"verace_amd: beta1 and beta2 must be 2^-64 to 2^64, got {beta1}, {beta2}")
     return out_dtype
 
 
@@ -331,7 +332,7 @@ class LinearAddFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         N, K = weight.shape
         _rows_fit(x, N)
-        keep = _kept(x, _rows_of(x, K), N, K) if act else None
+        keep = _kept(x, _rows_of(x, K), N, K) if act and any(ctx.needs_input_grad[:3]) else None
         y = _launch_linear(x, weight, bias, residual, None, None, act, x.dtype, keep)
         ctx.save_for_backward(x, weight, bias, keep)
         ctx.act = act
