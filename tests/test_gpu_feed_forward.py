@@ -128,3 +128,46 @@ def test_what_is_kept():
     r = torch.zeros(4, 8, device="cuda", requires_grad=True)
     y = va().linear_add(torch.zeros(4, 64, device="cuda"), torch.zeros(8, 64, device="cuda"), None, r, activation="silu")
     assert [t for t in y.grad_fn.saved_tensors if t is not None and t.shape == (4, 8)] == []
+
+
+# contractions of 32 steps of 128 bytes and more over few tiles, which a tile's waves share: even shares, a last share that ends
+# inside a step (33 steps: 9, 9, 9 and 6; 37: 10, 10, 10 and 7), and a last step of one element
+LONG = [(130, 32, 0, 1000), (400, 33, -3, 1000), (430, 37, 0, 1040), (450, 34, -31, 1100)]
+
+
+def long_k(steps, more, dtype):
+    each = 128 // torch.empty(0, dtype=dtype).element_size()
+    return steps * each + max(more, 1 - each)
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [oracle.E4M3])
+@pytest.mark.parametrize("m,steps,more,n", LONG)
+def test_long_contraction(m, steps, more, n, dtype):
+    k = long_k(steps, more, dtype)
+    g = torch.Generator().manual_seed(m + k + n)
+    (x, xs), (w, ws) = make(g, m, k, n, dtype, 1)
+    out = torch.bfloat16 if dtype == oracle.E4M3 else dtype
+    b, r = randn(g, n).to(out), randn(g, m, n).to(out)
+    within(va().linear_add(x, w, b, r, xs, ws, activation="silu"),
+           *oracle.linear(oracle.values(x, xs), oracle.values(w, ws), oracle.values(b), oracle.values(r), "silu", out))
+    f = n // 2 + 1
+    (wg, gs), (wu, us) = make(g, 1, k, f, dtype, 2)[1:]
+    within(va().gated_linear(x, wg, wu, xs, gs, us),
+           *oracle.gated(oracle.values(x, xs), oracle.values(wg, gs), oracle.values(wu, us), "situ", out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,steps,more,n", LONG)
+def test_long_contraction_backward(m, steps, more, n, dtype):
+    """dx contracts over the columns, in one part and (gated) in two."""
+    k, n = n, long_k(steps, more, dtype)
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w = (t.requires_grad_() for t, _ in make(g, m, k, n, dtype, 1))
+    dy = randn(g, m, n).to(dtype)
+    grads = torch.autograd.grad(va().linear_add(x, w), (x, w), dy)
+    for got, v in zip(grads, oracle.linear_bwd(oracle.values(x), oracle.values(w), None, None, oracle.values(dy), dtype)):
+        within(got, *v)
+    wu = make(g, 1, k, n, dtype, 1)[1][0].requires_grad_()
+    grads = torch.autograd.grad(va().gated_linear(x, w, wu), (x, w, wu), dy)
+    for got, v in zip(grads, oracle.gated_bwd(*(oracle.values(t) for t in (x, w, wu)), "situ", oracle.values(dy), dtype)):
+        within(got, *v)

@@ -325,12 +325,12 @@ template <typename E, typename F> __device__ __forceinline__ void by_result(cons
   }
 }
 
-template <typename E, int KIND, typename S> __global__ __launch_bounds__(S::THREADS, S::THREADS == 512 && S::STAGE > 40960 ? 2 : 4)
-void product_kernel(Args p) {
+template <typename E, int KIND, typename S, int GROUPS>
+__global__ __launch_bounds__(S::THREADS * GROUPS, S::THREADS == 512 && S::STAGE > 40960 ? 2 : 4) void product_kernel(Args p) {
   constexpr bool AMN = KIND == DW, BMN = KIND == DX || KIND == DW, PERM = !BMN;
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   constexpr int SIZE = sizeof(E), KT = 128 / SIZE, TN = PAIR ? S::HN : 2 * S::HN;
-  __shared__ __align__(1024) char lds[2 * S::STAGE];
+  __shared__ __align__(1024) char lds[GROUPS * 2 * S::STAGE];
   int block = blockIdx.x, split = 0;
   if constexpr (KIND == DW) {
     split = block / (p.tiles_m * p.tiles_n);
@@ -362,19 +362,28 @@ void product_kernel(Args p) {
   }
   Acc<S> acc;
   if (KIND == DX && p.b2 != nullptr)
-    tile_product<E, AMN, BMN, S, KIND == DX ? 2 : 1>(o, lds, acc);
+    tile_product<E, AMN, BMN, S, KIND == DX ? 2 : 1, GROUPS>(o, lds, acc);
   else
-    tile_product<E, AMN, BMN, S, 1>(o, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+    tile_product<E, AMN, BMN, S, 1, GROUPS>(o, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x % S::THREADS >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  // the parts of the tile that a thread finishes
+  constexpr int HMS = GROUPS > 1 ? 1 : 2, HNS = PAIR || GROUPS < 4 ? 2 : 1;
+  int hm0 = 0, hn0 = 0;
+  if constexpr (GROUPS > 1) {
+    join_groups<S, GROUPS, HNS>(lds, acc);
+    const int group = threadIdx.x / S::THREADS;
+    if (PAIR && group >= 2) return;
+    hm0 = group & 1, hn0 = HNS == 1 ? group >> 1 : 0;
+  }
   constexpr bool SWAP = !PERM && S::NF == 2;
   constexpr int W = PERM ? 4 * S::NF : SWAP ? 8 : 4, PARTS = PERM || SWAP ? 1 : S::NF;
   // (C's columns 16 j + 4 g .. of lane group g) to 8 consecutive ones: groups 2 i and 2 i + 1 exchange one of their two fours,
   // after which group g holds 8 columns of fragment g % 2.
   if constexpr (SWAP) {
 #pragma unroll
-    for (int hm = 0; hm < 2; ++hm)
+    for (int hm = 0; hm < HMS; ++hm)
 #pragma unroll
-      for (int hn = 0; hn < 2; ++hn)
+      for (int hn = 0; hn < HNS; ++hn)
 #pragma unroll
         for (int f = 0; f < S::MF; ++f)
 #pragma unroll
@@ -388,17 +397,17 @@ void product_kernel(Args p) {
     using T = decltype(tag);
     constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-    for (int hn = 0; hn < (PAIR ? 1 : 2); ++hn)
+    for (int hn = 0; hn < (PAIR ? 1 : HNS); ++hn)
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) {
         const int g = lane >> 4;
-        const int n = n0 + hn * S::HN + (SWAP ? wn * 32 + (g & 1) * 16 + (g >> 1) * 8 : column_of<S, PERM>(wn, lane, q));
+        const int n = n0 + (hn0 + hn) * S::HN + (SWAP ? wn * 32 + (g & 1) * 16 + (g >> 1) * 8 : column_of<S, PERM>(wn, lane, q));
         const Columns<W> cols = columns_at<E, T, KIND, W, FULL>(p, n);
 #pragma unroll
-        for (int hm = 0; hm < 2; ++hm)
+        for (int hm = 0; hm < HMS; ++hm)
 #pragma unroll
           for (int f = 0; f < S::MF; ++f) {
-            const int m = m0 + hm * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
+            const int m = m0 + (hm0 + hm) * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
             if (!FULL && m >= p.m) continue;
             float z[W], z2[W];
 #pragma unroll
@@ -428,15 +437,15 @@ int product_f16(Kind kind, Args p, hipStream_t stream);
 int product_f32(Kind kind, Args p, hipStream_t stream);
 int product_e4m3(Kind kind, Args p, hipStream_t stream);
 
-template <typename E, int KIND, typename S> int launch_product(Args p, hipStream_t stream) {
+template <typename E, int KIND, typename S, int GROUPS = 1> int launch_product(Args p, hipStream_t stream) {
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   const int tn = PAIR ? S::HN : 2 * S::HN;
   const int64_t tiles_m = (static_cast<int64_t>(p.m) + 2 * S::HM - 1) / (2 * S::HM), tiles_n = (static_cast<int64_t>(p.n) + tn - 1) / tn;
   const int64_t blocks = tiles_m * tiles_n * (KIND == DW ? p.splits : 1);
   if (blocks == 0) return VMI_OK;
-  if (!grid_fits(blocks, S::THREADS)) return VMI_ERR_UNSUPPORTED;
+  if (!grid_fits(blocks, S::THREADS * GROUPS)) return VMI_ERR_UNSUPPORTED;
   p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group = 8;
-  hipLaunchKernelGGL((product_kernel<E, KIND, S>), dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS), 0, stream, p);
+  hipLaunchKernelGGL((product_kernel<E, KIND, S, GROUPS>), dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * GROUPS), 0, stream, p);
   return hip_status(hipGetLastError());
 }
 
@@ -449,16 +458,24 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
   if (tiles(p.m, cols, 256, 256) * shares >= 192) return launch_product<E, KIND, Large>(p, stream);
   if (tiles(p.m, cols, 256, 128) * shares >= 160) return launch_product<E, KIND, Tall>(p, stream);
   if (tiles(p.m, cols, 128, 128) * shares >= 160) return launch_product<E, KIND, Middle>(p, stream);
+  // Four groups of a tile's waves share a long contraction where the tiles leave compute units idle or at one workgroup: a step's
+  // latency, not its data, bounds them.  us with four / one (rows x k x columns): bf16 512 x 4096 x 512 15.5 / 21.7, 256 x 4096 x
+  // 4096 16.6 / 22.8, 1024 x 1024 x 1024 (16 steps) 7.8 / 6.9, 384 x 4096 x 4096 (384 tiles) 29.7 / 25.2; fp32 777 x 1000 x 1037
+  // 22.7 / 24.2, 256 x 4096 x 4096 70 / 86; e4m3 256 x 4096 x 4096 10.0 / 10.4.  The other kinds have short contractions: DW's
+  // shares, and dz where the forward kept no sums.
+  if constexpr (KIND == LINEAR || KIND == GATED || KIND == DX)
+    if (tiles(p.m, cols, 64, 64) <= 256 && p.k > 31 * (128 / static_cast<int>(sizeof(E)))) return launch_product<E, KIND, Small, 4>(p, stream);
   return launch_product<E, KIND, Small>(p, stream);
 }
 
 template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
-// The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536), and any of up to 16 rows.  Both sides in
-// us, rows / tiles: bf16 K 2048 N 1024 M 128 7.6 / 9.5, M 256 11.3 / 9.8; bf16 K 1024 N 4096 M 32 5.5 / 6.4, M 64 8.1 / 6.4; fp32
-// K 2048 N 1024 M 384 38 / 40, M 512 38 / 40; fp32 K 4096 N 4096 M 96 63 / 76, M 192 108 / 77.
+// The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536, and 2048 of the gated form), and any of up
+// to 16 rows.  Both sides in us, rows / tiles: bf16 K 2048 N 1024 M 128 7.7 / 9.1, M 256 11.5 / 9.2; bf16 K 1024 N 4096 M 32 5.7 /
+// 6.2, M 64 8.4 / 6.4; e4m3 K 4096 N 4096 M 32 8.1 / 9.0, M 64 12.1 / 9.0; fp32 K 2048 N 1024 M 256 22 / 37, M 384 39 / 38; fp32 K
+// 4096 N 4096 M 96 64 / 69, M 128 74 / 72, gated (F 2048) M 128 53 / 71.
 template <typename E> inline bool few_rows(Kind kind, const Args& p) {
   const int64_t cols = kind == GATED ? 2 * static_cast<int64_t>(p.n) : p.n;
-  return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (sizeof(E) == 4 ? 1536 : 512);
+  return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (sizeof(E) < 4 ? 512 : kind == GATED ? 2048 : 1536);
 }
 
 template <typename E> int product_of(Kind kind, const Args& p, hipStream_t stream) {

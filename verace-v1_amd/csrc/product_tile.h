@@ -15,6 +15,9 @@
 // of a piece at the end of the reading half before the one that reads it, one barrier ahead of every reader, with the four
 // pieces issued later still in flight.
 //
+// For few tiles of a long contraction several groups of a tile's waves take a share of the steps each, with two LDS stages of
+// their own, and add their sums through LDS in a fixed order (join_groups).
+//
 // LDS is read at 16 bytes a lane (k contiguous), by transposing reads of 8 (m contiguous, 16 bits) or 4 bytes a lane (fp32),
 // and its 16-byte slots are permuted so that the lanes of an access fall in distinct banks.  The direct loads write LDS in
 // lane order, so the permutation is made by the addresses that they read.  Loads outside the operands return zeros: their
@@ -212,11 +215,15 @@ template <typename S> struct Acc {
   f32x4 v[2][2][S::MF][S::NF];
 };
 
-template <typename E, bool AMN, bool BMN, typename S, int SEGMENTS>
+// GROUPS: that many groups of S::THREADS threads have a share of k and two LDS stages each.
+template <typename E, bool AMN, bool BMN, typename S, int SEGMENTS, int GROUPS>
 __device__ __forceinline__ void tile_product(Operands& o, char* lds, Acc<S>& acc) {
   constexpr int KT = 128 / sizeof(E);
-  constexpr bool PERM = !BMN;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr bool PERM = !BMN, STAGGER = S::STAGGER || GROUPS > 1;
+  const int tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS);
+  const bool late = STAGGER && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= S::THREADS * GROUPS / 128;
+  lds += group * 2 * S::STAGE;
   const int wm = wave / S::WN, wn = wave % S::WN;
   Loader<E, AMN, S::HM, S::LA, S::THREADS, S::MF, false> la[2];
   Loader<E, BMN, S::HN, S::LB, S::THREADS, S::NF, PERM> lb[2];
@@ -229,19 +236,21 @@ __device__ __forceinline__ void tile_product(Operands& o, char* lds, Acc<S>& acc
   }
   ra.init(lane, wm * 16 * S::MF);
   rb.init(lane, wn * 16 * S::NF);
-  const int steps = (o.k + KT - 1) / KT, total = SEGMENTS * steps;
+  const int steps = (o.k + KT * GROUPS - 1) / (KT * GROUPS), total = SEGMENTS * steps, before = group * steps;
+  const int k_left = o.k - before * KT;  // may be none
   const unsigned lds_wave = lds_offset(lds) + wave * 1024;
   // pieces of a stage: B0, A0, B1, A1, the order of their loads
   constexpr int at_b[2] = {0, S::B_BYTES + S::A_BYTES}, at_a[2] = {S::B_BYTES, 2 * S::B_BYTES + S::A_BYTES};
-  const char *pa[2] = {o.a[0], o.a[1]}, *pb[2] = {o.b[0], o.b[1]};
-  auto left = [&](int t) { return o.k - (SEGMENTS == 2 && t >= steps ? t - steps : t) * KT; };
+  const char* pa[2] = {o.a[0] + before * o.a_step, o.a[1] + before * o.a_step};
+  const char* pb[2] = {o.b[0] + before * o.b_step, o.b[1] + before * o.b_step};
+  auto left = [&](int t) { return k_left - (SEGMENTS == 2 && t >= steps ? t - steps : t) * KT; };
   auto issue_a = [&](int h, int t) {
-    if (SEGMENTS == 2 && t == steps) pa[h] = o.a2[h];
+    if (SEGMENTS == 2 && t == steps) pa[h] = o.a2[h] + before * o.a_step;
     la[h].issue(pa[h], t < total ? left(t) : 0, lds_wave + (t & 1) * S::STAGE + at_a[h]);
     pa[h] += o.a_step;
   };
   auto issue_b = [&](int h, int t) {
-    if (SEGMENTS == 2 && t == steps) pb[h] = o.b2[h];
+    if (SEGMENTS == 2 && t == steps) pb[h] = o.b2[h] + before * o.b_step;
     lb[h].issue(pb[h], t < total ? left(t) : 0, lds_wave + (t & 1) * S::STAGE + at_b[h]);
     pb[h] += o.b_step;
   };
@@ -297,15 +306,43 @@ __device__ __forceinline__ void tile_product(Operands& o, char* lds, Acc<S>& acc
   rb.read(lds + at_b[0], b0);
   wait_loads_and_lds<S::FLIGHT>();
   barrier();
-  if (S::STAGGER && wave >= S::WM * S::WN / 2) barrier();
+  if (STAGGER && late) barrier();
   int t = 0;
   for (; t + 1 < total; t += 2) {
     step(t, b0, b0_next);
     step(t + 1, b0_next, b0);
   }
   if (t < total) step(t, b0, b0_next);
-  if (S::STAGGER && wave < S::WM * S::WN / 2) barrier();
+  if (STAGGER && !late) barrier();
   wait_loads_and_lds<0>();  // no load may write LDS after the workgroup's end
+}
+
+// The groups' sums of a tile added, in order: group g gets the part (hm, hn) = (g % 2, HNS == 1 ? g / 2 : 0 and 1) in v[0].
+template <typename S, int GROUPS, int HNS> __device__ __forceinline__ void join_groups(char* lds, Acc<S>& acc) {
+  constexpr int EACH = S::MF * S::NF * S::THREADS, PART = 4 * EACH;
+  static_assert(PART * 16 <= 2 * S::STAGE);
+  const int tid = threadIdx.x % S::THREADS, group = threadIdx.x / S::THREADS;
+  __syncthreads();  // the last loads of every wave are in
+#pragma unroll
+  for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+    for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+      for (int f = 0; f < S::MF * S::NF; ++f)
+        *reinterpret_cast<f32x4*>(lds + group * 2 * S::STAGE + ((2 * hm + hn) * EACH + f * S::THREADS + tid) * 16) =
+            acc.v[hm][hn][f / S::NF][f % S::NF];
+  __syncthreads();
+  const int hm = group & 1, hn0 = HNS == 1 ? group >> 1 & 1 : 0;
+#pragma unroll
+  for (int hn = 0; hn < HNS; ++hn)
+#pragma unroll
+    for (int f = 0; f < S::MF * S::NF; ++f) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+        sum += *reinterpret_cast<const f32x4*>(lds + g * 2 * S::STAGE + ((2 * hm + hn0 + hn) * EACH + f * S::THREADS + tid) * 16);
+      acc.v[0][hn][f / S::NF][f % S::NF] = sum;
+    }
 }
 
 // The first of the 4 (PERM: 4 * NF over all of a wave's fragments) consecutive columns of a lane's accumulator n.
