@@ -437,6 +437,17 @@ int product_f16(Kind kind, Args p, hipStream_t stream);
 int product_f32(Kind kind, Args p, hipStream_t stream);
 int product_e4m3(Kind kind, Args p, hipStream_t stream);
 
+// Rows of tiles in a column of tile_of: the tiles that an XCD's 32 compute units have at a time then cover about as many rows of
+// the result as columns, and read the fewest of the operands' rows into its L2.  dW of 2048 x 1024 over 8192 rows, 64 tiles of 256
+// x 128 in four shares, in us: columns of 1 44.7, of 2 45.6, of 4 46.0, of 8 54.8 (all of one operand in every L2).
+template <typename S> int rows_of_tiles(int64_t tiles, int concurrent) {
+  int64_t run = (tiles + 7) / 8;
+  if (run > 32 * concurrent) run = 32 * concurrent;
+  int g = 1;
+  while (2 * g * g * S::HM <= run * S::HN) g *= 2;
+  return g;
+}
+
 template <typename E, int KIND, typename S, int GROUPS = 1> int launch_product(Args p, hipStream_t stream) {
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   const int tn = PAIR ? S::HN : 2 * S::HN;
@@ -444,7 +455,7 @@ template <typename E, int KIND, typename S, int GROUPS = 1> int launch_product(A
   const int64_t blocks = tiles_m * tiles_n * (KIND == DW ? p.splits : 1);
   if (blocks == 0) return VMI_OK;
   if (!grid_fits(blocks, S::THREADS * GROUPS)) return VMI_ERR_UNSUPPORTED;
-  p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group = 8;
+  p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group = rows_of_tiles<S>(tiles_m * tiles_n, S::STAGE > 40960 || GROUPS > 1 ? 1 : 65536 / S::STAGE);
   hipLaunchKernelGGL((product_kernel<E, KIND, S, GROUPS>), dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * GROUPS), 0, stream, p);
   return hip_status(hipGetLastError());
 }
@@ -455,6 +466,11 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   const int64_t cols = PAIR ? 2 * static_cast<int64_t>(p.n) : p.n;
   const int64_t shares = KIND == DW ? p.splits : 1;
+  // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
+  // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
+  if constexpr (PAIR)
+    if (p.gate.act == ACT_SITU && p.k <= 8 * (128 / static_cast<int>(sizeof(E))) && tiles(p.m, cols, 128, 128) >= 160)
+      return launch_product<E, KIND, Middle>(p, stream);
   if (tiles(p.m, cols, 256, 256) * shares >= 192) return launch_product<E, KIND, Large>(p, stream);
   if (tiles(p.m, cols, 256, 128) * shares >= 160) return launch_product<E, KIND, Tall>(p, stream);
   if (tiles(p.m, cols, 128, 128) * shares >= 160) return launch_product<E, KIND, Middle>(p, stream);
