@@ -393,3 +393,47 @@ def test_model_in_8_bits():
     model.quantize_feed_forward_()
     with pytest.raises(RuntimeError, match="no gradients"):
         model.layers[0].mcmoe(torch.randn(1, 4, 256, device="cuda", dtype=torch.bfloat16))
+
+
+def test_under_autocast():
+    """The fused products give way to the separate ops, and the path in 8 bits gives what they would: autocast's dtype."""
+    torch.manual_seed(1)
+    m = va().ManifoldContinuousMoE(128, rank=8, num_components=8).cuda()
+    x = torch.randn(2, 20, 128, device="cuda")
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        want = m.base_situ_glu(x)
+        base = m.parts(x)[0]
+        m.base_situ_glu.fuse_products = True
+        assert torch.equal(m.base_situ_glu(x), want)
+        m.quantize_base_()
+        got = m.parts(x)[0]
+    assert got.dtype == base.dtype == torch.bfloat16
+    # as for the model: relative errors of up to 2^-4 in each of rows and weights, twice
+    assert 0 < rel(got, base) < 0.1
+
+
+def test_decode_graph_in_8_bits():
+    """A decode step captured with the base path in 8 bits: its replays keep to 8 bits after the model has gone back, and take
+    weights that are quantized anew."""
+    config = va().VeraceV1Config(vocab_size=128, hidden_dim=256, num_layers=2, num_heads=2, head_dim=128, chams_holographic_dim=64,
+                                 mcmoe_rank=8, mcmoe_num_components=8)
+    torch.manual_seed(2)
+    model = va().VeraceV1Model(config).cuda().to(torch.bfloat16).eval()
+    ids = torch.randint(0, 128, (4, 12), device="cuda")
+    nxt = torch.randint(0, 128, (4, 1), device="cuda")
+
+    with torch.no_grad():
+        for renew in (False, True):
+            model.quantize_feed_forward_()
+            held, state = (model.prefill(ids, static_depth=True)[1] for _ in range(2))  # the graph's states are its caller's to keep
+            graph = va().DecodeGraph(model, held, 4, static_depth=True)
+            if renew:
+                for layer in model.layers:
+                    layer.mcmoe.base_w_down.weight.mul_(0.5)
+                model.quantize_feed_forward_()
+            want = model.decode_step(nxt, state, static_depth=True, static_control=True)
+            model.quantize_feed_forward_(renew)
+            junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+            assert torch.equal(graph.step(nxt), want)
+            del junk
+            model.quantize_feed_forward_(False)

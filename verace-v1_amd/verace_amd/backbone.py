@@ -399,6 +399,7 @@ class DecodeGraph:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         del scratch
+        self._base8 = [layer.mcmoe._base8 for layer in model.layers]  # the graph reads them, also after the model lets go of them
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = model.decode_step(self.ids, state, static_depth, static_control=True)

@@ -25,7 +25,9 @@ class SiTUGLU(nn.Module):
 
     ``fuse_products = True`` takes both projections, the activations and their product as one kernel, in training too
     (:func:`~verace_amd.gated_linear`); the projections are then not rounded in between, so results differ from the separate
-    ops' by their rounding."""
+    ops' by their rounding.  Under autocast the separate ops run all the same."""
+
+    fuse_products = False
 
     def __init__(self, in_features: int, hidden_features: int, beta1: float = 4.0,
                  beta2: float = 25.0):
@@ -36,10 +38,9 @@ class SiTUGLU(nn.Module):
         self.beta2 = beta2
         self.w_gate = nn.Linear(in_features, hidden_features, bias=False)
         self.w_up = nn.Linear(in_features, hidden_features, bias=False)
-        self.fuse_products = False
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.fuse_products:
+        if self.fuse_products and not torch.is_autocast_enabled("cuda"):
             return gated_linear(x, self.w_gate.weight, self.w_up.weight, beta1=self.beta1, beta2=self.beta2)
         g = self.w_gate(x)
         u = self.w_up(x)
@@ -47,6 +48,8 @@ class SiTUGLU(nn.Module):
 
 
 class ManifoldContinuousMoE(nn.Module):
+    _base8 = None
+
     def __init__(self, hidden_dim: int = 16384, rank: int = 32, num_components: int = 64,
                  top_k_components: int = 8, beta1: float = 4.0, beta2: float = 25.0):
         super().__init__()
@@ -61,15 +64,21 @@ class ManifoldContinuousMoE(nn.Module):
         self.router = nn.Linear(hidden_dim, num_components, bias=False)
         self.hyper_sigma = nn.Linear(hidden_dim, num_components * rank, bias=False)
         self.norm = nn.RMSNorm(hidden_dim)
-        self._base8 = None
 
     def quantize_base_(self, on: bool = True) -> "ManifoldContinuousMoE":
         """Holds the base path's three weights in 8 bits with a scale for each output channel (``on=False``: no longer) and
         runs the path on rows in 8 bits, for inference.  The weights themselves stay; after a change of theirs, or a move to
-        another device, this is called again.  Not part of the ``state_dict``."""
-        glu = self.base_situ_glu
+        another device, this is called again, and a graph captured on the 8-bit weights then replays with the new ones.  Not part
+        of the ``state_dict``."""
+        glu, old = self.base_situ_glu, self._base8
         with torch.no_grad():
-            self._base8 = tuple(quantize_rows(m.weight.detach()) for m in (glu.w_gate, glu.w_up, self.base_w_down)) if on else None
+            new = tuple(quantize_rows(m.weight.detach()) for m in (glu.w_gate, glu.w_up, self.base_w_down)) if on else None
+            if new and old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
+                for pair, fresh in zip(old, new):
+                    for t, n in zip(pair, fresh):
+                        t.copy_(n)
+                new = old
+        self._base8 = new
         return self
 
     def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
@@ -78,9 +87,10 @@ class ManifoldContinuousMoE(nn.Module):
                                "torch.no_grad(), or call quantize_base_(False)")
         (wg, sg), (wu, su), (wd, sd) = self._base8
         glu = self.base_situ_glu
+        out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else xf.dtype
         x, xs = quantize_rows(xf)
-        h, hs = quantize_rows(gated_linear(x, wg, wu, xs, sg, su, beta1=glu.beta1, beta2=glu.beta2, out_dtype=xf.dtype))
-        return linear_add(h, wd, x_scale=hs, weight_scale=sd, out_dtype=xf.dtype)
+        h, hs = quantize_rows(gated_linear(x, wg, wu, xs, sg, su, beta1=glu.beta1, beta2=glu.beta2, out_dtype=out))
+        return linear_add(h, wd, x_scale=hs, weight_scale=sd, out_dtype=out)
 
     def parts(self, x: torch.Tensor):
         """The base path and the manifold path before its norm, both [tokens, hidden]."""
