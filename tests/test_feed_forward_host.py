@@ -183,3 +183,10 @@ def test_oracle_e4m3():
     g = torch.Generator().manual_seed(0)
     x = torch.cat([torch.randn(4000, generator=g) * s for s in (1e-3, 0.1, 1.0, 50.0)] + [torch.linspace(-448, 448, 4097)]).clamp(-448, 448)
     assert torch.equal(oracle.to_e4m3(x.double()), x.to(E4M3).double())
+
+
+@fake
+def test_eps_below_zero():
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(RuntimeError, match="eps"):
+            va.norm_add_quant(_e(3, 16), eps=eps)

@@ -427,6 +427,8 @@ def norm_add_quant(
     the unrounded sum in 64 bits.  A row with a NaN or an infinity in s * norm_weight has NaN for scale and q.  No gradients.
     """
     _quant_check(a, residual, norm_weight)
+    if not eps >= 0:
+        raise RuntimeError(f"verace_amd: eps must be 0 or more, got {eps}")
     refuse_tangents(a, residual, norm_weight)
     _no_grad_rows(a=a, residual=residual, norm_weight=norm_weight)
     if traced(a):
