@@ -525,8 +525,11 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  * Gradients from the inputs, and from those sums where they were kept (kept; NULL: formed again), for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
  * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */
 /* Rows of any address and length (row_bytes, ld_bytes apart) as these products take them: contiguous rows of whole 16-byte
- * pieces at dst, zeros behind the last byte. */
+ * pieces at dst, zeros behind the last byte; of one matrix, or of up to three in one launch (those without rows are passed over). */
 int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_t rows, int64_t row_bytes, void* stream);
+int vmi_pad_rows_3(const void* src0, int64_t ld_bytes0, void* dst0, int64_t rows0, int64_t row_bytes0,
+                   const void* src1, int64_t ld_bytes1, void* dst1, int64_t rows1, int64_t row_bytes1,
+                   const void* src2, int64_t ld_bytes2, void* dst2, int64_t rows2, int64_t row_bytes2, void* stream);
 int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
                    const float* w_scale, int dtype, const void* bias, const void* residual, int64_t ldr,
                    int act, void* out, int64_t ldo, int out_dtype, float* keep, int64_t M, int64_t N,

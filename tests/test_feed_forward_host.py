@@ -178,6 +178,20 @@ def test_c_refusals(lib):
     assert lib.vmi_pad_rows(one, -1, one, 2, 10, null) == INVALID and lib.vmi_pad_rows(null, 16, null, 0, 10, null) == 0
 
 
+def test_pad_refusals(lib):
+    """Several matrices at once: each is checked before any is copied; none with rows is no launch."""
+    from ctypes import c_void_p
+    null, one, odd = c_void_p(None), c_void_p(256), c_void_p(260)
+    INVALID = 1
+    none = (null, 0, null, 0, 0)
+    assert lib.vmi_pad_rows_3(*none, *none, *none, null) == 0
+    assert lib.vmi_pad_rows_3(null, 16, null, 0, 10, null, 16, null, 0, 10, null, 16, null, 0, 10, null) == 0
+    for bad in ((null, 16, one, 2, 10), (one, 16, odd, 2, 10), (one, -1, one, 2, 10), (one, 16, one, -2, 10), (one, 16, one, 2, -10),
+                (one, 16, one, 2 ** 62, 2 ** 62)):
+        for at in range(3):
+            assert lib.vmi_pad_rows_3(*[v for i in range(3) for v in (bad if i == at else none)], null) == INVALID
+
+
 def test_oracle_e4m3():
     """The oracle's rounding is torch's where torch's input type does not round first."""
     g = torch.Generator().manual_seed(0)

@@ -33,34 +33,51 @@ def _code(dtype: torch.dtype) -> int:
     return _lib.VMI_E4M3 if dtype is E4M3 else _lib.dtype_code(dtype)
 
 
-def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(tensor, elements from a row to the next) of t [..., K] as [M, K] with rows as the kernels load them: contiguous,
-    starting on 16 bytes, filled with zeros to whole 16-byte pieces.  A view of t where it lies so, otherwise a copy."""
-    k, size = t.shape[-1], _ITEMSIZE[t.dtype]
-    t = t if t.dim() == 2 else t.reshape(-1, k)
-    m, piece = t.shape[0], 16 // size
-    whole = -(-k // piece) * piece
-    if k == whole and t.data_ptr() % 16 == 0 and (k <= 1 or t.stride(1) == 1):
-        ld = t.stride(0) if m > 1 else k
-        if ld % piece == 0 and ld >= k and ld * size < _MAX_ROW_BYTES:
-            return t, ld
-    if k > 1 and t.stride(1) != 1 or m > 1 and t.stride(0) < 0:
-        t = t.contiguous()
-    out = torch.empty((m, whole), device=t.device, dtype=t.dtype)
-    with device_guard(t):
-        _lib.check(_lib.load().vmi_pad_rows(t.data_ptr(), t.stride(0) * size, out.data_ptr(), m, k * size,
-                                            _lib.raw_stream(t.device)), "vmi_pad_rows")
-    return out, whole
-
-
-def _operand(t: torch.Tensor, k: int) -> Tuple[torch.Tensor, int, int]:
-    """(what has to stay alive, address, elements from a row to the next) of t [..., k] as :func:`_rows`."""
+def _as_it_lies(t: torch.Tensor, k: int) -> Optional[Tuple[torch.Tensor, int, int]]:
+    """(what has to stay alive, address, elements from a row to the next) of t [..., k] where its rows lie as the kernels load
+    them: contiguous, starting on 16 bytes, of whole 16-byte pieces; None otherwise."""
+    size = _ITEMSIZE[t.dtype]
+    if k * size & 15 or k * size >= _MAX_ROW_BYTES:
+        return None
     if t.is_contiguous():
         p = t.data_ptr()
-        if not (p | k * _ITEMSIZE[t.dtype]) & 15 and k * _ITEMSIZE[t.dtype] < _MAX_ROW_BYTES:
-            return t, p, k
-    t, ld = _rows(t)
-    return t, t.data_ptr(), ld
+        return None if p & 15 else (t, p, k)
+    t = t if t.dim() == 2 else t.reshape(-1, k)
+    p, m = t.data_ptr(), t.shape[0]
+    ld = t.stride(0) if m > 1 else k
+    if p & 15 or k > 1 and t.stride(1) != 1 or ld * size & 15 or not k <= ld < _MAX_ROW_BYTES // size:
+        return None
+    return t, p, ld
+
+
+def _operands(*operands) -> list:
+    """:func:`_as_it_lies` of each (t [..., k], k), those that lie otherwise copied by one launch, with zeros up to whole
+    pieces."""
+    found = [_as_it_lies(t, k) for t, k in operands]
+    todo = [i for i, f in enumerate(found) if f is None]
+    if not todo:
+        return found
+    args, size, at = [], _ITEMSIZE[operands[0][0].dtype], 0
+    for i in todo:
+        t, k = operands[i]
+        t = t if t.dim() == 2 else t.reshape(-1, k)
+        m = t.shape[0]
+        if k > 1 and t.stride(1) != 1 or m > 1 and t.stride(0) < 0:
+            t = t.contiguous()
+        whole = -(-k * size // 16) * 16
+        args.append((t, at, m, k * size))
+        found[i] = whole // size
+        at += -(-m * whole // 256) * 256
+    x = operands[0][0]
+    out = torch.empty(at, device=x.device, dtype=torch.uint8)
+    p, call = out.data_ptr(), []
+    for i, (t, first, m, row) in zip(todo, args):
+        found[i] = (out, p + first, found[i])
+        call += (t.data_ptr(), t.stride(0) * size, p + first, m, row)
+    call += (None, 0, None, 0, 0) * (3 - len(todo))
+    with device_guard(x):
+        _lib.check(_lib.load().vmi_pad_rows_3(*call, _lib.raw_stream(x.device)), "vmi_pad_rows_3")
+    return found
 
 
 def _plain_rows(t: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
@@ -152,12 +169,12 @@ def _gated_check(x, w_gate, w_up, x_scale, gate_scale, up_scale, activation, bet
     return out_dtype
 
 
-def _pair(w_gate, w_up, K: int):
-    """Both weights' rows at one distance."""
-    g, u = _operand(w_gate, K), _operand(w_up, K)
-    if g[2] != u[2]:
-        g, u = _operand(w_gate.contiguous(), K), _operand(w_up.contiguous(), K)
-    return g, u
+def _gated_operands(x, w_gate, w_up, K: int) -> list:
+    """The operands, both weights' rows at one distance."""
+    found = _operands((x, K), (w_gate, K), (w_up, K))
+    if found[1][2] != found[2][2]:  # contiguous ones' are K, rounded up
+        found = _operands((x, K), (w_gate.contiguous(), K), (w_up.contiguous(), K))
+    return found
 
 
 def _rows_of(t: torch.Tensor, k: int) -> int:
@@ -182,8 +199,7 @@ def _kept(x: torch.Tensor, m: int, n: int, k: int) -> Optional[torch.Tensor]:
 
 def _launch_gated(x, w_gate, w_up, x_scale, gate_scale, up_scale, act, beta1, beta2, out_dtype, keep=None):
     F, K = w_gate.shape
-    x2, xp, ldx = _operand(x, K)
-    (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
+    (x2, xp, ldx), (g, gp, ldg), (u, up, ldu) = _gated_operands(x, w_gate, w_up, K)
     out = _result(x, F, out_dtype)
     if x_scale is not None:
         x_scale, gate_scale, up_scale = _vector(x_scale), _vector(gate_scale), _vector(up_scale)
@@ -200,9 +216,8 @@ def _launch_gated_bwd(x, w_gate, w_up, act, beta1, beta2, dh, need, kept=None):
     if dh.shape != x.shape[:-1] + (F,) or dh.dtype != x.dtype or dh.device != x.device:
         raise RuntimeError(f"verace_amd: dh must be {tuple(x.shape[:-1] + (F,))} {x.dtype} on {x.device}, "
                            f"got {tuple(dh.shape)} {dh.dtype} on {dh.device}")
-    x2, xp, ldx = _operand(x, K)
+    (x2, xp, ldx), (g, gp, ldg), (u, up, ldu) = _gated_operands(x, w_gate, w_up, K)
     dh2, dhp, lddh = _plain_rows(dh, F)
-    (g, gp, ldg), (u, up, ldu) = _pair(w_gate, w_up, K)
     M = _rows_of(x, K)
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
     dw = torch.empty(2, F, K, device=x.device, dtype=x.dtype) if need[1] or need[2] else None
@@ -288,8 +303,7 @@ def _linear_check(x, weight, bias, residual, x_scale, weight_scale, activation, 
 
 def _launch_linear(x, weight, bias, residual, x_scale, weight_scale, act, out_dtype, keep=None):
     N, K = weight.shape
-    x2, xp, ldx = _operand(x, K)
-    w, wp, ldw = _operand(weight, K)
+    (x2, xp, ldx), (w, wp, ldw) = _operands((x, K), (weight, K))
     r, rp, ldr = _plain_rows(residual, N)
     bias = _vector(bias)
     out = _result(x, N, out_dtype)
@@ -308,9 +322,7 @@ def _launch_linear_bwd(x, weight, bias, act, dy, need, kept=None):
     if dy.shape != x.shape[:-1] + (N,) or dy.dtype != x.dtype or dy.device != x.device:
         raise RuntimeError(f"verace_amd: dy must be {tuple(x.shape[:-1] + (N,))} {x.dtype} on {x.device}, "
                            f"got {tuple(dy.shape)} {dy.dtype} on {dy.device}")
-    x2, xp, ldx = _operand(x, K)
-    w, wp, ldw = _operand(weight, K)
-    dy2, dyp, lddy = _operand(dy, N)
+    (x2, xp, ldx), (w, wp, ldw), (dy2, dyp, lddy) = _operands((x, K), (weight, K), (dy, N))
     bias = _vector(bias)
     M = _rows_of(x, K)
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
