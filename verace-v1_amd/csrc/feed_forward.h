@@ -455,7 +455,8 @@ template <typename E, int KIND, typename S, int GROUPS = 1> int launch_product(A
   const int64_t blocks = tiles_m * tiles_n * (KIND == DW ? p.splits : 1);
   if (blocks == 0) return VMI_OK;
   if (!grid_fits(blocks, S::THREADS * GROUPS)) return VMI_ERR_UNSUPPORTED;
-  p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n), p.group = rows_of_tiles<S>(tiles_m * tiles_n, S::STAGE > 40960 || GROUPS > 1 ? 1 : 65536 / S::STAGE);
+  p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n);
+  p.group = rows_of_tiles<S>(tiles_m * tiles_n, S::STAGE > 40960 || GROUPS > 1 ? 1 : 65536 / S::STAGE);
   hipLaunchKernelGGL((product_kernel<E, KIND, S, GROUPS>), dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * GROUPS), 0, stream, p);
   return hip_status(hipGetLastError());
 }
@@ -466,6 +467,9 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   const int64_t cols = PAIR ? 2 * static_cast<int64_t>(p.n) : p.n;
   const int64_t shares = KIND == DW ? p.splits : 1;
+  // The largest tile that gives three quarters (five eighths) of the compute units one.  us of 256 x 256, 256 x 128, 128 x 128, 64 x
+  // 64, bf16, rows x k x columns: 8192 x 1024 x 2048 (256 of the largest) 30.5 33.9 34.9 51.8; 4096 x 1024 x 2048 (128) 23.9 17.5 18.6
+  // 27.1; 2048 x 1024 x 2048 (64) 22.8 15.1 12.0 14.7; 1024 x 1024 x 2048 (32) 22.0 13.7 10.9 9.1.
   // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
   // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
   if constexpr (PAIR)

@@ -22,6 +22,9 @@
 // and its 16-byte slots are permuted so that the lanes of an access fall in distinct banks.  The direct loads write LDS in
 // lane order, so the permutation is made by the addresses that they read.  Loads outside the operands return zeros: their
 // offset lies beyond the buffer's size.
+// The matrix cores bound long contractions (bf16, 8192 x 16384 x 4096, k contiguous in one operand: 740 us, 1.49 PFLOP/s, the
+// cores busy 83 % of the time at the 1.7 GHz that the power limit leaves; e4m3 8192 x 8192 x 4096 211 us, 2.6 PFLOP/s); with
+// tiles of 256 x 128 LDS does, 1408 clocks of it for 1024 of products a step (fp16, 8192 x 2048 x 1024: 45 us, 760 TFLOP/s).
 #pragma once
 
 #include "vmi_common.h"

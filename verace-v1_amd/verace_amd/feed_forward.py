@@ -14,6 +14,7 @@ workspace from torch's caching allocator.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -134,10 +135,16 @@ def _vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _workspace(query, *args, device) -> Tuple[Optional[torch.Tensor], int]:
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, *sizes: int) -> int:
     need = ctypes.c_size_t(0)
-    _lib.check(getattr(_lib.load(), query)(*args, ctypes.byref(need)), query)
-    return (torch.empty(need.value, device=device, dtype=torch.uint8) if need.value else None), need.value
+    _lib.check(getattr(_lib.load(), query)(*sizes, ctypes.byref(need)), query)
+    return need.value
+
+
+def _workspace(query, *sizes, device) -> Tuple[Optional[torch.Tensor], int]:
+    need = _workspace_bytes(query, *sizes)
+    return (torch.empty(need, device=device, dtype=torch.uint8) if need else None), need
 
 
 def _rows_fit(x: torch.Tensor, n: int) -> None:
