@@ -463,21 +463,42 @@ template <typename E, int KIND, typename S, int GROUPS = 1> int launch_product(A
 
 inline int64_t tiles(int64_t m, int64_t n, int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 
+// What the tiles of a shape take, in units of their own: rounds of one tile for each of the 256 compute units (two tiles of 128 x 128
+// or four of 64 x 64 in one at a time count alike), by what a round took in relation to one of 256 x 256 tiles.  A last round that
+// leaves compute units idle is shorter: under the power limit (16 bits) the others' clocks rise.  In fp32 the matrix cores bound every
+// tile, and a round is its tile's elements.
+//
+// us of 256 x 256, 256 x 128, 128 x 128, 64 x 64, rows x k x columns; bf16: 8192 x 1024 x 2048 (256 of the largest tiles) 30.5 33.9
+// 34.9 51.8, 4352 x 1024 x 2048 (136) 27.4 30.3 27.1 31.6, 4352 x 2048 x 1024 (68) 37.0 24.5 28.1 33.3, 2048 x 1024 x 2048 (64) 22.8
+// 15.1 12.0 14.7, 1024 x 1024 x 2048 (32) 22.0 13.7 10.9 9.1; e4m3: 4352 x 1024 x 2048 20.4 22.2 18.9 21.8, 9000 x 1024 x 2304 36.2
+// 36.2 30.2 46.2; fp32: 8192 x 4096 x 4096 1874 1910 1901 2017, 2048 x 2048 x 2048 470 244 133 134, 1787 x 3840 x 3228 874 450 445
+// 356, 2500 x 700 x 900 171 89 50 39.
+struct Rounds {
+  int size;  // an operand's element
+  int64_t time(int64_t tiles, int shape) const {
+    constexpr int weight[3][4] = {{1000, 565, 300, 130}, {1000, 565, 310, 130}, {1000, 510, 255, 67}};
+    const int least = size == 4 ? 256 : size == 2 ? 192 : 230;  // of 256, what a round with one tile takes
+    const int64_t rest = tiles % 256;
+    return (tiles / 256 * 256 + (rest == 0 ? 0 : least + (256 - least) * rest / 256)) * weight[size / 2][shape];
+  }
+};
+
 template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t stream) {
   constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
   const int64_t cols = PAIR ? 2 * static_cast<int64_t>(p.n) : p.n;
   const int64_t shares = KIND == DW ? p.splits : 1;
-  // The largest tile that gives three quarters (five eighths) of the compute units one.  us of 256 x 256, 256 x 128, 128 x 128, 64 x
-  // 64, bf16, rows x k x columns: 8192 x 1024 x 2048 (256 of the largest) 30.5 33.9 34.9 51.8; 4096 x 1024 x 2048 (128) 23.9 17.5 18.6
-  // 27.1; 2048 x 1024 x 2048 (64) 22.8 15.1 12.0 14.7; 1024 x 1024 x 2048 (32) 22.0 13.7 10.9 9.1.
   // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
   // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
   if constexpr (PAIR)
     if (p.gate.act == ACT_SITU && p.k <= 8 * (128 / static_cast<int>(sizeof(E))) && tiles(p.m, cols, 128, 128) >= 160)
       return launch_product<E, KIND, Middle>(p, stream);
-  if (tiles(p.m, cols, 256, 256) * shares >= 192) return launch_product<E, KIND, Large>(p, stream);
-  if (tiles(p.m, cols, 256, 128) * shares >= 160) return launch_product<E, KIND, Tall>(p, stream);
-  if (tiles(p.m, cols, 128, 128) * shares >= 160) return launch_product<E, KIND, Middle>(p, stream);
+  const Rounds r = {sizeof(E)};
+  const int64_t l = r.time(tiles(p.m, cols, 256, 256) * shares, 0), t = r.time(tiles(p.m, cols, 256, 128) * shares, 1);
+  const int64_t m = r.time(tiles(p.m, cols, 128, 128) * shares, 2), s = r.time(tiles(p.m, cols, 64, 64) * shares, 3);
+  const bool large = l <= t && l <= m && l <= s, tall = t <= m && t <= s, middle = m <= s;
+  if (large) return launch_product<E, KIND, Large>(p, stream);
+  if (tall) return launch_product<E, KIND, Tall>(p, stream);
+  if (middle) return launch_product<E, KIND, Middle>(p, stream);
   // Four groups of a tile's waves share a long contraction where the tiles leave compute units idle or at one workgroup: a step's
   // latency, not its data, bounds them.  us with four / one (rows x k x columns): bf16 512 x 4096 x 512 15.5 / 21.7, 256 x 4096 x
   // 4096 16.6 / 22.8, 1024 x 1024 x 1024 (16 steps) 7.8 / 6.9, 384 x 4096 x 4096 (384 tiles) 29.7 / 25.2; fp32 777 x 1000 x 1037
