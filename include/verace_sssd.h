@@ -516,7 +516,8 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  * bytes, and where K (N for dy) is no whole number of 16-byte pieces the rest of a row's last piece holds zeros.  A row is
  * less than 2^24 bytes from the next; M, N, K <= 2^30.  dtype: of x and the weights; VMI_E4M3 takes a float32 scale for each
  * row of both (the values are scale * e4m3), and bias, residual and out are then of out_dtype; otherwise out_dtype is dtype.
- * Sums are fp32; each result is rounded once.  K = 0 is a sum of nothing.
+ * Sums are fp32; each result is rounded once.  K = 0 is a sum of nothing.  VMI_E4M3: eight consecutive products of a sum are cut to
+ * multiples of 2^-13 of the largest one's power of two before they are added.
  *   vmi_linear_add:   out = residual + act(x w^T + bias); bias [N], residual (rows ldr apart) may be NULL;
  *                     act 0: none, 1: z sigmoid(z), 2: z Phi(z).  out may be residual.
  *   vmi_gated_linear: out = a(x w_gate^T) b(x w_up^T); act 1: a(z) = z sigmoid(z), b(z) = z;

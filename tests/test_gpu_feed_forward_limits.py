@@ -1,0 +1,34 @@
+"""The feed-forward operators where their arithmetic loses bits, runs out of fp32's range or cancels; each result near its own
+value, however small."""
+
+import pytest
+import torch
+
+from oracle import feed_forward as oracle
+from test_gpu_feed_forward import randn, va, within
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+E4M3 = oracle.E4M3
+
+
+@pytest.mark.parametrize("m,n", [(3, 24), (300, 640)])
+def test_sums_of_8_bit_rows(m, n):
+    """By the kernel for a few rows and by tiles, with a 32-bit result: where one value stands out of a row, its seven neighbours'
+    products keep 2^-13 of its power of two; products elsewhere, and rows without one, lose nothing to it."""
+    g = torch.Generator().manual_seed(m)
+    k = 144
+    x, w = (torch.randn(r, k, generator=g).to(E4M3) for r in (m, n))
+    x[::2, 21] = 448.0
+    one = [torch.ones(r, device="cuda") for r in (m, n)]
+    X, W = oracle.values(x), oracle.values(w)
+    y = va().linear_add(x.cuda(), w.cuda(), None, None, *one, out_dtype=torch.float32)
+    within(y, *oracle.linear(X, W, None, None, None, torch.float32, one))
+    h = va().gated_linear(x.cuda(), w.cuda(), w.cuda(), one[0], one[1], one[1], activation="silu", out_dtype=torch.float32)
+    within(h, *oracle.gated(X, W, W, "silu", torch.float32, scales=(one[0], one[1], one[1])))
+    # the outstanding value's own eight apart: the rest of its row is as exact as a row without it
+    rest = X.clone()
+    rest[:, 16:24] = 0
+    only = va().linear_add(rest.to(E4M3).cuda(), w.cuda(), None, None, *one, out_dtype=torch.float32)
+    within(only, *oracle.linear(rest, W, None, None, None, torch.float32, one))
