@@ -32,3 +32,29 @@ def test_sums_of_8_bit_rows(m, n):
     rest[:, 16:24] = 0
     only = va().linear_add(rest.to(E4M3).cuda(), w.cuda(), None, None, *one, out_dtype=torch.float32)
     within(only, *oracle.linear(rest, W, None, None, None, torch.float32, one))
+
+
+LEAST, MOST = 2.0 ** -64, 2.0 ** 64
+
+
+@pytest.mark.parametrize("dtype", DTYPES + [E4M3])
+@pytest.mark.parametrize("m", [5, 300])
+def test_betas_at_their_limits(m, dtype):
+    """By the kernel for a few rows and by tiles; u = 0 in one column."""
+    g = torch.Generator().manual_seed(m)
+    k, f = 64, 600
+    x, wg, wu = randn(g, m, k), randn(g, f, k, scale=0.1), randn(g, f, k, scale=0.1)
+    wu[7] = 0
+    out = torch.bfloat16 if dtype == E4M3 else dtype
+    (x, xs), (wg, gs), (wu, us) = ((t.to(dtype), None) if dtype != E4M3 else va().quantize_rows(t) for t in (x, wg, wu))
+    X, G, U = oracle.values(x, xs), oracle.values(wg, gs), oracle.values(wu, us)
+    for b1 in (LEAST, 4.0, MOST):
+        for b2 in (LEAST, 25.0, MOST):
+            h = va().gated_linear(x, wg, wu, xs, gs, us, beta1=b1, beta2=b2)
+            scales = None if xs is None else (xs, gs, us)
+            want, bound = oracle.gated(X, G, U, "situ", out, b1, b2, scales)
+            # the least beta makes a step of its factor, on whose other side a projection may come out that is nearer 0 than its error
+            (z, ez), (v, ev) = (oracle.product(X, W, None if s is None else (xs, s)) for W, s in ((G, gs), (U, us)))
+            bound = bound + 2 * b1 * b2 * ((z.abs() <= ez) & (b1 == LEAST) | (v.abs() <= ev) & (b2 == LEAST)).double()
+            within(h, want, bound)
+            assert bool((h[:, 7] == 0).all())

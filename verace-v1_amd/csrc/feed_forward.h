@@ -150,7 +150,8 @@ template <typename T, int W> __device__ __forceinline__ void gated(float (&g)[W]
     } else {
       const Parts r = gate_parts(g[j], c);
       const float s = g[j] < 0.f ? -r.b : 1.f;  // the sign, and sigmoid(g) = b / (1 + b) below 0
-      g[j] = r.num * s * __builtin_amdgcn_rcpf(r.den) * (c.b1 * c.b2 * t[j]);
+      // each tanh beside its own beta: b1 b2 may be 2^128
+      g[j] = r.num * s * __builtin_amdgcn_rcpf(r.den) * c.b1 * (c.b2 * t[j]);
     }
   }
 }
