@@ -521,7 +521,8 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  *   vmi_linear_add:   out = residual + act(x w^T + bias); bias [N], residual (rows ldr apart) may be NULL;
  *                     act 0: none, 1: z sigmoid(z), 2: z Phi(z).  out may be residual.
  *   vmi_gated_linear: out = a(x w_gate^T) b(x w_up^T); act 1: a(z) = z sigmoid(z), b(z) = z;
- *                     3: a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2).  ldg = ldu.
+ *                     3: a(z) = beta1 tanh(z / beta1) sigmoid(z), b(z) = beta2 tanh(z / beta2), betas of 2^-64 to 2^64.
+ *                     ldg = ldu.
  * keep (or NULL) receives the sums before the activation, contiguous [M, N] (with the bias; gated [M, 2F], a row's gates first).
  * Gradients from the inputs, and from those sums where they were kept (kept; NULL: formed again), for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
  * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */

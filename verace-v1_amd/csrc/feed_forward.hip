@@ -280,7 +280,9 @@ int column_shares(int64_t m, int64_t n) {
   return static_cast<int>(s < 1 ? 1 : s);
 }
 Gate gate_of(int act, float beta1, float beta2) { return {act, beta1, beta2, 1.f / beta1, 1.f / beta2}; }
-bool gate_act(int act) { return act == ACT_SILU || act == ACT_SITU; }
+// 2^-64 to 2^64: a beta and its inverse times any value of a projection of ordinary size stay in fp32's range.
+bool beta_ok(float b) { return b >= 0x1p-64f && b <= 0x1p64f; }
+bool gate_ok(int act, float beta1, float beta2) { return act == ACT_SILU || (act == ACT_SITU && beta_ok(beta1) && beta_ok(beta2)); }
 bool linear_act(int act) { return act == ACT_NONE || act == ACT_SILU || act == ACT_GELU; }
 
 }  // namespace
@@ -321,7 +323,7 @@ extern "C" int vmi_gated_linear(const void* x, int64_t ldx, const float* x_scale
                                 const float* gate_scale, const void* w_up, int64_t ldu, const float* up_scale, int dtype, int act,
                                 float beta1, float beta2, void* out, int64_t ldo, int out_dtype, float* keep, int64_t M, int64_t F,
                                 int64_t K, void* stream) {
-  if (!sizes_ok(M, F, K) || !gate_act(act) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
+  if (!sizes_ok(M, F, K) || !gate_ok(act, beta1, beta2) || dtype < 0 || dtype > VMI_E4M3 || out_dtype < 0 || out_dtype > VMI_F16)
     return VMI_ERR_INVALID_ARG;
   if (dtype != VMI_E4M3 && out_dtype != dtype) return VMI_ERR_INVALID_ARG;
   if (M == 0 || F == 0) return VMI_OK;
@@ -421,7 +423,7 @@ extern "C" int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_ga
                                     void* stream) {
   size_t need = 0;
   if (const int st = vmi_gated_linear_bwd_workspace_bytes(M, F, K, dtype, &need); st != VMI_OK) return st;
-  if (!gate_act(act)) return VMI_ERR_INVALID_ARG;
+  if (!gate_ok(act, beta1, beta2)) return VMI_ERR_INVALID_ARG;
   if (workspace_bytes < need || (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
     return VMI_ERR_WORKSPACE;
   if (ldg != ldu) return VMI_ERR_UNSUPPORTED;
