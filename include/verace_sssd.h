@@ -554,7 +554,7 @@ int vmi_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t
  *   s = a + residual,  n = s w / sqrt(mean s^2 + eps) (norm = 0: n = s w),
  *   scale = max(max|n| / 448, 2^-126),  q = e4m3(n / scale), q rounded once from 64 bits
  * over rows of d elements, a_stride and r_stride apart; residual, w [d] (dtype or float32) and sum (s, dtype) may be NULL;
- * sum, q [rows, d] and scale [rows] are contiguous.  A row with a NaN or an infinity in s w has NaN for scale and q. */
+ * sum, q [rows, d] and scale [rows] are contiguous; eps (with the norm) is finite, 0 or more.  A row with a NaN or an infinity in s w has NaN for scale and q. */
 int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* residual, int64_t r_stride, const void* w,
                        int dtype, int w_dtype, int norm, float eps, void* sum, void* q, float* scale,
                        int64_t rows, int64_t d, void* stream);

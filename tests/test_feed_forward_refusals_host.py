@@ -29,3 +29,24 @@ def test_betas_out_of_range(lib):
             assert call(1, bad, bad) == 0
         for b1, b2 in ((2.0 ** -64, 2.0 ** 64), (2.0 ** 64, 2.0 ** -64), (4.0, 25.0)):
             assert call(3, b1, b2) == 0
+
+
+def test_eps_out_of_range(lib):
+    """eps of the 8-bit norm is a finite fp32 number, 0 or more, at the C entry (which the registered operator calls) and in Python; rows
+    as they are do not read it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import torch
+    import verace_amd as va
+
+    def quant(norm, eps):
+        return lib.vmi_norm_add_quant(one, 16, null, 0, null, 1, 1, norm, eps, null, one, one, 0, 16, null)
+
+    for bad in (-1e-6, math.inf, -math.inf, math.nan):
+        assert quant(1, bad) == INVALID and quant(0, bad) == 0
+    assert quant(1, 0.0) == 0 and quant(1, 1e38) == 0
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        a = torch.empty(3, 16, dtype=torch.bfloat16, device="cuda")
+        for bad in (-1e-6, math.inf, math.nan, 1e39):
+            with pytest.raises(RuntimeError, match="eps"):
+                va.norm_add_quant(a, eps=bad)
+        va.norm_add_quant(a, eps=3e38)

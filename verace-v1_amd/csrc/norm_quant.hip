@@ -311,6 +311,7 @@ extern "C" int vmi_norm_add_quant(const void* a, int64_t a_stride, const void* r
                                   void* stream) {
   if (rows < 0 || d < 1 || d > INT32_MAX - 65536 || dtype < 0 || dtype > VMI_F16 || (w_dtype != dtype && w_dtype != VMI_F32))
     return VMI_ERR_INVALID_ARG;
+  if (norm && !(eps >= 0.f && eps <= 3.40282347e38f)) return VMI_ERR_INVALID_ARG;
   if (rows == 0) return VMI_OK;
   if (a == nullptr || q == nullptr || scale == nullptr) return VMI_ERR_INVALID_ARG;
   Args k{a, residual, w, a_stride, residual == nullptr ? 0 : r_stride, eps, norm, sum, static_cast<uint8_t*>(q), scale, rows,

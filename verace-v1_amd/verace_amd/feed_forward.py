@@ -28,6 +28,7 @@ _LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2}
 _GATED_ACT = {"silu": 1, "situ": 3}
 _MAX_ROW_BYTES = 1 << 24  # from a row to the next
 _LEAST_BETA = 2.0 ** -64
+_MAX_EPS = torch.finfo(torch.float32).max
 _ITEMSIZE = {torch.bfloat16: 2, torch.float16: 2, torch.float32: 4, E4M3: 1}
 
 
@@ -444,11 +445,12 @@ def norm_add_quant(
 
     a, residual: [..., d] of one dtype (bfloat16, float16, float32); norm_weight: [d] of it or float32.  s has a's dtype, q is
     float8_e4m3fn, scale [...] float32: ``scale = max(max |n| / 448, 2^-126)``, ``q = n / scale`` to nearest, ties to even, from
-    the unrounded sum in 64 bits.  A row with a NaN or an infinity in s * norm_weight has NaN for scale and q.  No gradients.
+    the unrounded sum in 64 bits.  A row with a NaN or an infinity in s * norm_weight has NaN for scale and q, as has a row of zeros
+    with eps 0.  No gradients.
     """
     _quant_check(a, residual, norm_weight)
-    if not eps >= 0:
-        raise RuntimeError(f"verace_amd: eps must be 0 or more, got {eps}")
+    if not 0 <= eps <= _MAX_EPS:
+        raise RuntimeError(f"verace_amd: eps must be 0 or more, and finite in float32, got {eps}")
     refuse_tangents(a, residual, norm_weight)
     _no_grad_rows(a=a, residual=residual, norm_weight=norm_weight)
     if traced(a):
