@@ -10,7 +10,7 @@
 // of a tie (and below 2^-6, where e4m3's steps are of one size): one value of about 5000, so a wave takes the 64-bit form for
 // a whole piece where one of its lanes needs it.  max|p| in 64 bits is that of the pieces whose 32-bit maximum is within
 // 2^-21 of the row's.  Rows whose 32-bit terms are not all finite, or all below 2^-60, take the 64-bit form throughout.
-// The sum of squares is of 64 bits, over s of 32 for 16-bit inputs: the scale is within 2^-23.
+// The sum of squares is of 64 bits, over s of 32 for 16-bit inputs (of 64 in the rows above): the scale is within 2^-23.
 //
 // One read of each input, one write of each result: HBM bounds it.  A row is one wave's (up to 4 pieces of 16 bytes a lane)
 // or four waves'; its inputs stay in registers, as they came, between the pass that sums and the pass that writes.  Longer rows
@@ -210,8 +210,10 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
   wild = wild || high < 0x1p-60f;
   // the largest |p| in 64 bits
   const float near = wild ? -1.f : high * (1.f - 0x1p-21f);
-  double top = 0.0;
+  double top = 0.0, again = 0.0;
   bool bad = false;
+  // a bf16 row's sums may lie beyond fp32: their squares are then summed again, in 64 bits throughout
+  constexpr bool AGAIN = RES && std::is_same<T, bf16_t>::value;
   pieces(true, [&](int v, int i0) {
     if (LONG || __any(of_piece[v] >= near)) {
       const Terms<T, RES> t = terms(v, i0);
@@ -221,15 +223,25 @@ __global__ __launch_bounds__(NTH) void norm_quant_kernel(Args k) {
         top = fmax(top, p);
         bad |= !(p <= 1.7976931348623157e308);
       }
+      if (AGAIN && wild) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) again += t.s64(j) * t.s64(j);
+      }
     }
   });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmax(top, __shfl_xor(top, o));
   bad = __any(bad);
+  if (AGAIN && wild) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) again += __shfl_xor(again, o);
+    ss = again;
+  }
   if constexpr (WAVES > 1) {
     __syncthreads();
-    if (lane == 0) red[1][wave] = top, red32[0][wave] = bad ? 1.f : 0.f;
+    if (lane == 0) red[0][wave] = again, red[1][wave] = top, red32[0][wave] = bad ? 1.f : 0.f;
     __syncthreads();
+    if (AGAIN && wild) ss = red[0][0] + red[0][1] + red[0][2] + red[0][3];
     top = fmax(fmax(red[1][0], red[1][1]), fmax(red[1][2], red[1][3]));
     bad = red32[0][0] + red32[0][1] + red32[0][2] + red32[0][3] != 0.f;
   }
