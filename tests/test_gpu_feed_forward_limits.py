@@ -1,6 +1,8 @@
 """The feed-forward operators where their arithmetic loses bits, runs out of fp32's range or cancels; each result near its own
 value, however small."""
 
+import math
+
 import pytest
 import torch
 
@@ -58,3 +60,46 @@ def test_betas_at_their_limits(m, dtype):
             bound = bound + 2 * b1 * b2 * ((z.abs() <= ez) & (b1 == LEAST) | (v.abs() <= ev) & (b2 == LEAST)).double()
             within(h, want, bound)
             assert bool((h[:, 7] == 0).all())
+
+
+def columns(v, dtype):
+    """A projection to each value itself: (x, w), and the values in 64 bits."""
+    x = torch.zeros(v.numel(), 16, dtype=dtype)
+    x[:, 0] = v.to(dtype)
+    w = torch.zeros(3, 16, dtype=dtype)
+    w[:, 0] = 1
+    return x.cuda(), w.cuda(), x[:, :1].double()
+
+
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gelu_far_out(dtype, kept, monkeypatch):
+    """z Phi(z) and its slope relative to their own values, where 1 + erf would cancel.
+
+    In 16 bits: within 2^-18 (a polynomial of 2^-20, an exponential and a reciprocal of a few 2^-24), and z^2 / 2 itself is off by
+    2^-23 of it (two roundings), which goes into the exponential.  fp32: 16 roundings of 2^-23 (the library's own few among them).
+    Near the slope's zero (z = -0.75) its two terms cancel: their magnitudes count."""
+    monkeypatch.setattr("verace_amd.feed_forward._keeps", lambda *_: kept)
+    v = torch.cat([torch.linspace(-13, 13, 1041), torch.tensor([0.0, 1e-6, -1e-6, -1e-3, 40.0, -40.0, 1e4, -1e4])])
+    x, w, z = columns(v, dtype)
+    x.requires_grad_()
+    y = va().linear_add(x, w, activation="gelu")
+    phi = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    density = torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    own = 2.0 ** -18 + z * z * 2.0 ** -23 if dtype != torch.float32 else torch.full_like(z, 2.0 ** -19)
+    want = z * phi
+    within(y, want.expand(-1, 3), (own * want.abs() + z.abs() * oracle.TINY + oracle.rounding(want, dtype)).expand(-1, 3))
+    slope = phi + z * density
+    dx, = torch.autograd.grad(y, x, torch.cat([torch.ones_like(y[:, :1]), torch.zeros_like(y[:, 1:])], 1))
+    # rounded as an operand, and again as the result
+    bound = own * (phi + (z * density).abs()) + (1 + z.abs()) * oracle.TINY + 2 * oracle.rounding(slope, dtype)
+    within(dx[:, :1], slope, bound)
+    if dtype == torch.float32:  # the same through 16-bit rows of a 32-bit result: the values have four bits
+        e = torch.tensor([-8.0, -6.5, -6.0, -5.5, -5.0, -4.5, -4.0, -3.0, 2.0, 448.0]).to(E4M3).float()
+        x8, w8 = torch.zeros(e.numel(), 16), torch.zeros(3, 16)
+        x8[:, 0], w8[:, 0] = e, 1
+        one, three = torch.ones(e.numel(), device="cuda"), torch.ones(3, device="cuda")
+        y = va().linear_add(x8.to(E4M3).cuda(), w8.to(E4M3).cuda(), None, None, one, three, activation="gelu", out_dtype=torch.float32)
+        z = e.double()[:, None]
+        want = z * 0.5 * torch.special.erfc(-z / math.sqrt(2))
+        within(y, want.expand(-1, 3), (2.0 ** -19 * want.abs() + oracle.rounding(want, torch.float32)).expand(-1, 3))
