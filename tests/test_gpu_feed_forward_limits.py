@@ -103,3 +103,38 @@ def test_gelu_far_out(dtype, kept, monkeypatch):
         z = e.double()[:, None]
         want = z * 0.5 * torch.special.erfc(-z / math.sqrt(2))
         within(y, want.expand(-1, 3), (2.0 ** -19 * want.abs() + oracle.rounding(want, torch.float32)).expand(-1, 3))
+
+
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_situ_slopes_where_tanh_saturates(dtype, kept, monkeypatch):
+    """1 - tanh^2 relative to its own value, where the difference would cancel.
+
+    sech^2 is formed from exp(-2 |x|), x = g / b1 or u / b2: x carries two roundings of 2^-24 (the inverse and the product) and its
+    exponent's scale two more, so sech^2 is off by 4 x 2^-23 relative beside 2^-18 for its own operations; each gradient is rounded
+    as an operand and as the result.  The gate's slope has a second term, a(g) sigmoid(-g)."""
+    monkeypatch.setattr("verace_amd.feed_forward._keeps", lambda *_: kept)
+    v = torch.tensor([0.0, 0.3, 0.59, 0.61, 1.0, 2.0, 3.0, 4.0, 5.0, 6.0, 7.0, 8.0, 9.0, 12.0, 30.0])
+    v = torch.cat([v, -v])
+    n = v.numel()
+    x = torch.zeros(n * n, 16, dtype=dtype)
+    x[:, 0], x[:, 1] = (4 * v).to(dtype).repeat_interleave(n), (25 * v).to(dtype).repeat(n)
+    wg, wu = torch.zeros(1, 16, dtype=dtype), torch.zeros(1, 16, dtype=dtype)
+    wg[:, 0], wu[:, 1] = 1, 1
+    g, u = x[:, 0].double(), x[:, 1].double()
+    x, wg, wu = (t.cuda().requires_grad_() for t in (x, wg, wu))
+    h = va().gated_linear(x, wg, wu)
+    dx, = torch.autograd.grad(h, x, torch.ones_like(h))
+
+    def sech2(t):
+        e = torch.exp(-2 * t.abs())
+        return 4 * e / (1 + e) ** 2
+
+    s, ns = torch.sigmoid(g), torch.sigmoid(-g)
+    a, b = 4 * torch.tanh(g / 4) * s, 25 * torch.tanh(u / 25)
+    one, two = sech2(g / 4) * s * b, a * ns * b
+    du = a * sech2(u / 25)
+    off_g, off_u = 2.0 ** -18 + (g / 4).abs() * 2.0 ** -21 + g.abs() * 2.0 ** -22, 2.0 ** -18 + (u / 25).abs() * 2.0 ** -21 + g.abs() * 2.0 ** -22
+    least = oracle.TINY * 100 * (1 + g.abs())
+    within(dx[:, 0], one + two, off_g * (one.abs() + two.abs()) + least + 2 * oracle.rounding(one + two, dtype))
+    within(dx[:, 1], du, off_u * du.abs() + least + 2 * oracle.rounding(du, dtype))
