@@ -138,3 +138,35 @@ def test_situ_slopes_where_tanh_saturates(dtype, kept, monkeypatch):
     least = oracle.TINY * 100 * (1 + g.abs())
     within(dx[:, 0], one + two, off_g * (one.abs() + two.abs()) + least + 2 * oracle.rounding(one + two, dtype))
     within(dx[:, 1], du, off_u * du.abs() + least + 2 * oracle.rounding(du, dtype))
+
+
+@pytest.mark.parametrize("m", [8, 304])
+def test_scales_beyond_each_other(m):
+    """8-bit rows whose two scales multiply to no normal fp32 number, where their values do not: a sum of 0 stays 0, the others keep
+    their precision, down to fp32's own least number and up to its largest."""
+    g = torch.Generator().manual_seed(m)
+    k, n = 64, 640
+    xs = torch.tensor([2.0 ** -126, 2.0 ** -100, 2.0 ** -70, 1e-3, 1.0, 2.0 ** 40, 2.0 ** 90, 2.0 ** 119]).repeat(m // 8)
+    ws = torch.tensor([2.0 ** -126, 2.0 ** -75, 2.0 ** -60, 2.0 ** -9, 3.0, 2.0 ** 20, 2.0 ** 60, 2.0 ** 118]).repeat(n // 8)
+    x, w = torch.randn(m, k, generator=g) * 30, torch.randn(n, k, generator=g) * 30
+    x[:, k // 2:] = 0                                 # the columns below meet only zeros in these rows' values
+    w[: n // 2, : k // 2] = 0
+    w[n // 2::3, 5:] = 0
+    x[::2, 5:] = 0
+    x, w = x.to(E4M3), w.to(E4M3)
+    X, W = x.double() * xs.double()[:, None], w.double() * ws.double()[:, None]
+    args = x.cuda(), w.cuda(), None, None, xs.cuda(), ws.cuda()
+    for out in DTYPES:
+        y = va().linear_add(*args, out_dtype=out)
+        want, bound = oracle.linear(X, W, None, None, None, out, (xs, ws))
+        top = torch.finfo(out).max
+        fine = want.abs() + bound < top
+        assert bool(torch.isfinite(y.cpu())[fine].all()) and bool((y.cpu()[want == 0] == 0).all())
+        within(torch.where(fine.cuda(), y, 0), torch.where(fine, want, 0), bound)
+        assert bool((y.cpu().double().abs() >= top)[want.abs() - bound > 1.01 * top].all())
+    h = va().gated_linear(args[0], args[1], args[1], args[4], args[5], args[5], activation="silu", out_dtype=torch.float32)
+    want, bound = oracle.gated(X, W, W, "silu", torch.float32, scales=(xs, ws, ws))
+    top = torch.finfo(torch.float32).max
+    fine = (want.abs() + bound < top) & ((X @ W.T).abs() < top)  # the projections themselves are fp32
+    assert bool((h.cpu()[fine & (want == 0)] == 0).all())
+    within(torch.where(fine.cuda(), h, 0), torch.where(fine, want, 0), bound)

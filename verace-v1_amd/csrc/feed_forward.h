@@ -307,17 +307,34 @@ template <typename E, typename T, int KIND, int W, bool FULL = false> __device__
   return c;
 }
 
+// z ws xs.  A sum z of products of e4m3 values is 0 or 2^-18 to 2^48, so z times an ordinary weight's scale, from 2^-100 to 2^70, is a
+// normal number, and the result is rounded as itself for any xs.  (z times xs ws, which may be infinite, would lose a z of 0.)  FAR: of
+// other columns (a row of zeros has the scale 2^-126) the powers of two are added and come last.
+template <int W> __device__ __forceinline__ bool far_scale(const float (&ws)[W]) {
+  float low = __builtin_inff(), high = 0.f;
+#pragma unroll
+  for (int j = 0; j < W; ++j) low = fminf(low, fabsf(ws[j])), high = fmaxf(high, fabsf(ws[j]));
+  return !(low >= 0x1p-100f && high <= 0x1p70f);
+}
+template <bool FAR, int W> __device__ __forceinline__ void scale_all(float (&z)[W], float xs, const float (&ws)[W]) {
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    if constexpr (FAR)
+      z[j] = ldexpf(z[j] * __builtin_amdgcn_frexp_mantf(ws[j]) * __builtin_amdgcn_frexp_mantf(xs),
+                    __builtin_amdgcn_frexp_expf(ws[j]) + __builtin_amdgcn_frexp_expf(xs));
+    else
+      z[j] = z[j] * ws[j] * xs;
+  }
+}
+
 // The lane's columns of one row of one product (two for the gated kinds), W consecutive ones from n.
 // other: the row's residual (dy, dh) where the caller has read it.
-template <typename E, typename T, int KIND, int W, bool FULL = false>
+template <typename E, typename T, int KIND, int W, bool FULL = false, bool FAR = sizeof(E) == 1>
 __device__ __forceinline__ void finish(const Args& p, int m, int n, const Columns<W>& c, float (&z)[W], float (&z2)[W], float xs, int split,
                                        const float* other = nullptr) {
   if constexpr (sizeof(E) == 1) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      z[j] *= xs * c.ws[j];
-      if constexpr (KIND == GATED) z2[j] *= xs * c.ws2[j];
-    }
+    scale_all<FAR, W>(z, xs, c.ws);
+    if constexpr (KIND == GATED) scale_all<FAR, W>(z2, xs, c.ws2);
   }
   if constexpr (KIND == LINEAR || KIND == LINEAR_DZ) {
     float t[W];
@@ -467,20 +484,25 @@ __global__ __launch_bounds__(S::THREADS * GROUPS, S::THREADS == 512 && S::STAGE 
         const int g = lane >> 4;
         const int n = n0 + (hn0 + hn) * S::HN + (SWAP ? wn * 32 + (g & 1) * 16 + (g >> 1) * 8 : column_of<S, PERM>(wn, lane, q));
         const Columns<W> cols = columns_at<E, T, KIND, W, FULL>(p, n);
+        auto rows = [&](auto far) {
 #pragma unroll
-        for (int hm = 0; hm < HMS; ++hm)
+          for (int hm = 0; hm < HMS; ++hm)
 #pragma unroll
-          for (int f = 0; f < S::MF; ++f) {
-            const int m = m0 + (hm0 + hm) * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
-            if (!FULL && m >= p.m) continue;
-            float z[W], z2[W];
+            for (int f = 0; f < S::MF; ++f) {
+              const int m = m0 + (hm0 + hm) * S::HM + wm * 16 * S::MF + f * 16 + (lane & 15);
+              if (!FULL && m >= p.m) continue;
+              float z[W], z2[W];
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-              z[j] = acc.v[hm][hn][f][PERM || SWAP ? j / 4 : q][j % 4];
-              z2[j] = PAIR ? acc.v[hm][1][f][PERM ? j / 4 : q][j % 4] : 0.f;
+              for (int j = 0; j < W; ++j) {
+                z[j] = acc.v[hm][hn][f][PERM || SWAP ? j / 4 : q][j % 4];
+                z2[j] = PAIR ? acc.v[hm][1][f][PERM ? j / 4 : q][j % 4] : 0.f;
+              }
+              finish<E, T, KIND, W, FULL, decltype(far)::value>(p, m, n, cols, z, z2, SIZE == 1 ? p.xs[m] : 1.f, split);
             }
-            finish<E, T, KIND, W, FULL>(p, m, n, cols, z, z2, SIZE == 1 ? p.xs[m] : 1.f, split);
-          }
+        };
+        if constexpr (SIZE == 1 && !FULL) rows(std::true_type{});
+        else if (SIZE == 1 && __any(far_scale<W>(cols.ws) || (PAIR && far_scale<W>(cols.ws2)))) rows(std::true_type{});
+        else rows(std::false_type{});
       }
   };
   // most tiles lie inside the result: their accesses need no conditions, which would keep them from being in flight together
