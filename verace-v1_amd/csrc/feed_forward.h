@@ -563,6 +563,7 @@ struct Rounds {
   int size;  // an operand's element
   int64_t time(int64_t tiles, int shape) const {
     constexpr int weight[3][4] = {{1000, 565, 300, 130}, {1000, 565, 310, 130}, {1000, 510, 255, 67}};
+    if (!grid_fits(tiles, shape == 3 ? Small::THREADS : Large::THREADS)) return INT64_MAX;
     const int least = size == 4 ? 256 : size == 2 ? 192 : 230;  // of 256, what a round with one tile takes
     const int64_t rest = tiles % 256;
     return (tiles / 256 * 256 + (rest == 0 ? 0 : least + (256 - least) * rest / 256)) * weight[size / 2][shape];
@@ -576,7 +577,8 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
   // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
   // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
   if constexpr (PAIR)
-    if (p.gate.act == ACT_SITU && p.k <= 8 * (128 / static_cast<int>(sizeof(E))) && tiles(p.m, cols, 128, 128) >= 160)
+    if (const int64_t t = tiles(p.m, cols, 128, 128);
+        p.gate.act == ACT_SITU && p.k <= 8 * (128 / static_cast<int>(sizeof(E))) && t >= 160 && grid_fits(t, Middle::THREADS))
       return launch_product<E, KIND, Middle>(p, stream);
   const Rounds r = {sizeof(E)};
   const int64_t l = r.time(tiles(p.m, cols, 256, 256) * shares, 0), t = r.time(tiles(p.m, cols, 256, 128) * shares, 1);
@@ -597,11 +599,12 @@ template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t s
 
 template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
 // The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536, and 2048 of the gated form), and any of up
-// to 16 rows.  Both sides in us, rows / tiles: bf16 K 2048 N 1024 M 128 7.7 / 9.1, M 256 11.5 / 9.2; bf16 K 1024 N 4096 M 32 5.7 /
+// to 16 rows that a grid's threads hold.  Both sides in us, rows / tiles: bf16 K 2048 N 1024 M 128 7.7 / 9.1, M 256 11.5 / 9.2; bf16 K 1024 N 4096 M 32 5.7 /
 // 6.2, M 64 8.4 / 6.4; e4m3 K 4096 N 4096 M 32 8.1 / 9.0, M 64 12.1 / 9.0; fp32 K 2048 N 1024 M 256 22 / 37, M 384 39 / 38; fp32 K
 // 4096 N 4096 M 96 64 / 69, M 128 74 / 72, gated (F 2048) M 128 53 / 71.
 template <typename E> inline bool few_rows(Kind kind, const Args& p) {
   const int64_t cols = kind == GATED ? 2 * static_cast<int64_t>(p.n) : p.n;
+  if (!grid_fits((static_cast<int64_t>(p.n) + 15) / 16, 512)) return false;
   return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (sizeof(E) < 4 ? 512 : kind == GATED ? 2048 : 1536);
 }
 
