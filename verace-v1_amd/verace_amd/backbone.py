@@ -399,7 +399,8 @@ class DecodeGraph:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         del scratch
-        self._base8 = [layer.mcmoe._base8 for layer in model.layers]  # the graph reads them, also after the model lets go of them
+        # the graph reads them, also after the model lets go of them
+        self._base8 = [getattr(layer.mcmoe, "_base8", None) for layer in model.layers]
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = model.decode_step(self.ids, state, static_depth, static_control=True)
