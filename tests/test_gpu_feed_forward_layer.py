@@ -33,3 +33,85 @@ def test_decode_graph_with_another_feed_forward():
         graph = va().DecodeGraph(m, held, 4, static_depth=True)
         for _ in range(3):
             assert torch.equal(graph.step(nxt), m.decode_step(nxt, state, static_depth=True, static_control=True))
+
+
+class Wider(nn.Linear):
+    """A projection with more than its weight (as an adapter adds)."""
+
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+def test_fused_products_leave_other_modules_to_themselves():
+    """A hook, a bias, a replaced module or method on a projection has its effect with fuse_products as without."""
+    torch.manual_seed(0)
+    x = torch.randn(3, 7, 96, device="cuda").to(BF)
+    wide = Wider(96, 160, bias=False).cuda().to(BF)
+
+    def hook(m):
+        m.w_gate.register_forward_hook(lambda mod, a, y: y + 1)
+
+    def bias(m):
+        m.w_up = nn.Linear(96, 160).cuda().to(BF)
+
+    def replaced(m):
+        m.w_gate = wide
+
+    def method(m):
+        m.w_up.forward = lambda t: nn.functional.linear(t, m.w_up.weight) * 2
+
+    for change in (hook, bias, replaced, method):
+        m = va().SiTUGLU(96, 160).cuda().to(BF)
+        plain = m(x)
+        change(m)
+        want = m(x)
+        assert not torch.equal(want, plain)
+        m.fuse_products = True
+        assert torch.equal(m(x), want), change.__name__
+
+
+@torch.no_grad()
+def test_8_bits_refuse_other_modules():
+    """What the 8-bit path would pass by is refused: before a weight is held where it is known then, else by the call."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+
+    def hook(m):
+        return m.base_w_down.register_forward_hook(lambda mod, a, y: y + 1)
+
+    def gate_hook(m):
+        return m.base_situ_glu.register_forward_pre_hook(lambda mod, a: None)
+
+    def bias(m):
+        m.base_w_down = nn.Linear(*m.base_w_down.weight.shape[::-1]).cuda().to(BF)
+
+    def replaced(m):
+        m.base_situ_glu.w_up = Wider(*m.base_situ_glu.w_up.weight.shape[::-1], bias=False).cuda().to(BF)
+
+    for change in (hook, gate_hook, bias, replaced):
+        m = moe()
+        change(m)
+        with pytest.raises(RuntimeError, match="plain"):
+            m.quantize_base_()
+        m(x)  # as it was
+        m = moe().quantize_base_()
+        want = m(x)
+        handle = change(m)
+        with pytest.raises(RuntimeError, match="plain"):
+            m(x)
+        if handle is not None:
+            handle.remove()
+            assert torch.equal(m(x), want)
+
+
+@torch.no_grad()
+def test_a_model_is_quantized_whole_or_not():
+    ids = torch.randint(0, 128, (2, 9), device="cuda")
+    for change in (lambda m: m.layers[1].mcmoe.base_w_down.register_forward_hook(lambda mod, a, y: y),
+                   lambda m: setattr(m.layers[1], "mcmoe", nn.Linear(256, 256).cuda().to(BF))):
+        m = model()
+        change(m)
+        want = m.prefill(ids, static_depth=True)[0]
+        with pytest.raises(RuntimeError, match="plain"):
+            m.quantize_feed_forward_()
+        assert torch.equal(m.prefill(ids, static_depth=True)[0], want)
+        m.quantize_feed_forward_(False)

@@ -286,9 +286,14 @@ class VeraceV1Model(nn.Module):
 
     def quantize_feed_forward_(self, on: bool = True) -> "VeraceV1Model":
         """Every layer's feed-forward base path in 8 bits, for inference
-        (:meth:`~verace_amd.ManifoldContinuousMoE.quantize_base_`)."""
-        for layer in self.layers:
-            layer.mcmoe.quantize_base_(on)
+        (:meth:`~verace_amd.ManifoldContinuousMoE.quantize_base_`); all of them, or with an error none."""
+        own = [m for m in (layer.mcmoe for layer in self.layers) if isinstance(m, ManifoldContinuousMoE)]
+        if on and len(own) < len(self.layers):
+            raise RuntimeError("verace_amd.VeraceV1Model: 8 bits take the plain ManifoldContinuousMoE in every layer")
+        for m in own if on else ():
+            m._base_linears()
+        for m in own:
+            m.quantize_base_(on)
         return self
 
     def load_reference_state_dict(self, sd: dict, strict: bool = True):

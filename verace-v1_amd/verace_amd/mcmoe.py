@@ -17,7 +17,12 @@ import torch
 import torch.nn as nn
 
 from .feed_forward import gated_linear, linear_add, quantize_rows
-from .layer_ops import mcmoe_coef, norm_add, situ_glu
+from .layer_ops import mcmoe_coef, norm_add, plain, situ_glu
+
+
+def _weight_alone(linear) -> bool:
+    """A projection that is no more than its weight."""
+    return plain(linear, nn.Linear) and linear.bias is None
 
 
 class SiTUGLU(nn.Module):
@@ -25,7 +30,8 @@ class SiTUGLU(nn.Module):
 
     ``fuse_products = True`` takes both projections, the activations and their product as one kernel, in training too
     (:func:`~verace_amd.gated_linear`); the projections are then not rounded in between, so results differ from the separate
-    ops' by their rounding.  Under autocast the separate ops run all the same."""
+    ops' by their rounding.  Under autocast, and where a projection is more than its weight (another class, a bias, hooks), the
+    separate ops run all the same."""
 
     fuse_products = False
 
@@ -40,7 +46,8 @@ class SiTUGLU(nn.Module):
         self.w_up = nn.Linear(in_features, hidden_features, bias=False)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.fuse_products and not torch.is_autocast_enabled("cuda"):
+        if (self.fuse_products and not torch.is_autocast_enabled("cuda") and _weight_alone(self.w_gate)
+                and _weight_alone(self.w_up)):
             return gated_linear(x, self.w_gate.weight, self.w_up.weight, beta1=self.beta1, beta2=self.beta2)
         g = self.w_gate(x)
         u = self.w_up(x)
@@ -65,14 +72,26 @@ class ManifoldContinuousMoE(nn.Module):
         self.hyper_sigma = nn.Linear(hidden_dim, num_components * rank, bias=False)
         self.norm = nn.RMSNorm(hidden_dim)
 
+    def _base_linears(self):
+        """The base path's three projections, for the path in 8 bits."""
+        glu = self.base_situ_glu
+        if plain(glu, SiTUGLU):
+            linears = glu.w_gate, glu.w_up, self.base_w_down
+            if all(_weight_alone(m) for m in linears):
+                return linears
+        raise RuntimeError("verace_amd.ManifoldContinuousMoE: the base path in 8 bits takes plain modules (SiTUGLU and nn.Linear, no "
+                           "bias, no hooks); call quantize_base_(False) to run others")
+
     def quantize_base_(self, on: bool = True) -> "ManifoldContinuousMoE":
         """Holds the base path's three weights in 8 bits with a scale for each output channel (``on=False``: no longer) and
         runs the path on rows in 8 bits, for inference.  The weights themselves stay; after a change of theirs, or a move to
         another device, this is called again, and a graph captured on the 8-bit weights then replays with the new ones.  Not part
-        of the ``state_dict``."""
-        glu, old = self.base_situ_glu, self._base8
+        of the ``state_dict``.  The path takes the weights alone: modules of another class, with a bias or with hooks are refused,
+        here and where it runs."""
+        old = self._base8
+        linears = self._base_linears() if on else ()
         with torch.no_grad():
-            new = tuple(quantize_rows(m.weight.detach()) for m in (glu.w_gate, glu.w_up, self.base_w_down)) if on else None
+            new = tuple(quantize_rows(m.weight.detach()) for m in linears) if on else None
             if new and old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
                 for pair, fresh in zip(old, new):
                     for t, n in zip(pair, fresh):
@@ -85,6 +104,7 @@ class ManifoldContinuousMoE(nn.Module):
         if torch.is_grad_enabled():
             raise RuntimeError("verace_amd.ManifoldContinuousMoE: the base path in 8 bits has no gradients; run under "
                                "torch.no_grad(), or call quantize_base_(False)")
+        self._base_linears()
         (wg, sg), (wu, su), (wd, sd) = self._base8
         glu = self.base_situ_glu
         out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else xf.dtype
