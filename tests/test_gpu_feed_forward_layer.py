@@ -115,3 +115,18 @@ def test_a_model_is_quantized_whole_or_not():
             m.quantize_feed_forward_()
         assert torch.equal(m.prefill(ids, static_depth=True)[0], want)
         m.quantize_feed_forward_(False)
+
+
+def test_weights_held_in_inference_mode_are_renewed():
+    """Held first under torch.inference_mode(), then anew outside it and inside it again."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+    m = moe()
+    for i, mode in enumerate((torch.inference_mode, torch.no_grad, torch.inference_mode)):
+        with torch.no_grad():
+            m.base_w_down.weight.mul_(0.5)
+        with mode():
+            m.quantize_base_()
+        fresh = moe()
+        fresh.load_state_dict(m.state_dict())
+        with torch.no_grad():
+            assert torch.equal(m(x), fresh.quantize_base_()(x)), i

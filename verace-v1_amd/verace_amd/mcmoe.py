@@ -90,7 +90,7 @@ class ManifoldContinuousMoE(nn.Module):
         here and where it runs."""
         old = self._base8
         linears = self._base_linears() if on else ()
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():  # tensors made in inference mode cannot be renewed outside it
             new = tuple(quantize_rows(m.weight.detach()) for m in linears) if on else None
             if new and old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
                 for pair, fresh in zip(old, new):
