@@ -130,3 +130,19 @@ def test_weights_held_in_inference_mode_are_renewed():
         fresh.load_state_dict(m.state_dict())
         with torch.no_grad():
             assert torch.equal(m(x), fresh.quantize_base_()(x)), i
+
+
+@torch.no_grad()
+def test_a_graph_sees_weights_held_again():
+    """Off and on again: a graph captured before replays with the weights that are held now, a call of the model too."""
+    m = model()
+    ids, nxt = (torch.randint(0, 128, s, device="cuda") for s in ((4, 12), (4, 1)))
+    m.quantize_feed_forward_()
+    held, state = (m.prefill(ids, static_depth=True)[1] for _ in range(2))
+    graph = va().DecodeGraph(m, held, 4, static_depth=True)
+    m.quantize_feed_forward_(False)
+    for layer in m.layers:
+        layer.mcmoe.base_w_down.weight.mul_(0.5)
+        layer.mcmoe.base_situ_glu.w_up.weight.neg_()
+    m.quantize_feed_forward_()
+    assert torch.equal(graph.step(nxt), m.decode_step(nxt, state, static_depth=True, static_control=True))

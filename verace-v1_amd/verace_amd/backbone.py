@@ -404,7 +404,7 @@ class DecodeGraph:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         del scratch
-        # the graph reads them, also after the model lets go of them
+        # the graph reads them, also after the model has moved to others
         self._base8 = [getattr(layer.mcmoe, "_base8", None) for layer in model.layers]
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):

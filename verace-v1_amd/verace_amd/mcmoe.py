@@ -55,7 +55,8 @@ class SiTUGLU(nn.Module):
 
 
 class ManifoldContinuousMoE(nn.Module):
-    _base8 = None
+    _base8 = None        # the held weights: (q, scale) of the gate's, the up and the down projection
+    _in_8_bits = False   # whether the base path takes them
 
     def __init__(self, hidden_dim: int = 16384, rank: int = 32, num_components: int = 64,
                  top_k_components: int = 8, beta1: float = 4.0, beta2: float = 25.0):
@@ -83,22 +84,26 @@ class ManifoldContinuousMoE(nn.Module):
                            "bias, no hooks); call quantize_base_(False) to run others")
 
     def quantize_base_(self, on: bool = True) -> "ManifoldContinuousMoE":
-        """Holds the base path's three weights in 8 bits with a scale for each output channel (``on=False``: no longer) and
-        runs the path on rows in 8 bits, for inference.  The weights themselves stay; after a change of theirs, or a move to
-        another device, this is called again, and a graph captured on the 8-bit weights then replays with the new ones.  Not part
-        of the ``state_dict``.  The path takes the weights alone: modules of another class, with a bias or with hooks are refused,
-        here and where it runs."""
+        """Holds the base path's three weights in 8 bits with a scale for each output channel and runs the path on rows in 8 bits, for
+        inference (``on=False``: no longer).  The weights themselves stay; after a change of theirs, or a move to another device, this is
+        called again.  What is held keeps its place, while the path is off too, so that a graph captured on the 8-bit weights replays with
+        the ones held last (until a move or a change of shape).  Not part of the ``state_dict``.  The path takes the weights alone: modules
+        of another class, with a bias or with hooks are refused, here and where it runs."""
+        if on:
+            self._hold_base()
+        self._in_8_bits = on
+        return self
+
+    def _hold_base(self) -> None:
         old = self._base8
-        linears = self._base_linears() if on else ()
         with torch.inference_mode(False), torch.no_grad():  # tensors made in inference mode cannot be renewed outside it
-            new = tuple(quantize_rows(m.weight.detach()) for m in linears) if on else None
-            if new and old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
+            new = tuple(quantize_rows(m.weight.detach()) for m in self._base_linears())
+            if old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
                 for pair, fresh in zip(old, new):
                     for t, n in zip(pair, fresh):
                         t.copy_(n)
                 new = old
         self._base8 = new
-        return self
 
     def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
         if torch.is_grad_enabled():
@@ -117,7 +122,7 @@ class ManifoldContinuousMoE(nn.Module):
         b, s, d = x.shape
         C, r = self.num_components, self.rank
         xf = x.reshape(b * s, d)
-        base_out = self.base_w_down(self.base_situ_glu(xf)) if self._base8 is None else self._base_in_8_bits(xf)
+        base_out = self.base_w_down(self.base_situ_glu(xf)) if not self._in_8_bits else self._base_in_8_bits(xf)
         # v_proj[n, j, :] = V_j x_n for every component, then the selected ones' coefficients
         vproj = xf @ self.v_basis.reshape(C * r, d).t()
         coef = mcmoe_coef(self.router(xf), self.hyper_sigma(xf), vproj, min(self.top_k_components, C), C)
