@@ -1,5 +1,6 @@
 """The layer's feed-forward on the fused products and in 8 bits, where a program has changed the modules, the weights or the mode
 around it."""
+import copy
 
 import pytest
 import torch
@@ -146,3 +147,61 @@ def test_a_graph_sees_weights_held_again():
         layer.mcmoe.base_situ_glu.w_up.weight.neg_()
     m.quantize_feed_forward_()
     assert torch.equal(graph.step(nxt), m.decode_step(nxt, state, static_depth=True, static_control=True))
+
+
+@torch.no_grad()
+def test_changed_weights_are_held_anew():
+    """An in-place change, a state_dict, other data, another type, a copy of the module: the next call quantizes what it finds."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+
+    def check(m, x):
+        fresh = va().ManifoldContinuousMoE(128, rank=8, num_components=8).cuda().to(x.dtype)
+        fresh.load_state_dict(m.state_dict())
+        got = m(x)
+        assert torch.equal(got, fresh.quantize_base_()(x))
+        return got
+
+    m = moe().quantize_base_()
+    seen = [check(m, x)]
+    m.base_w_down.weight.mul_(0.5)
+    seen.append(check(m, x))
+    m.load_state_dict({k: -v for k, v in m.state_dict().items()})
+    seen.append(check(m, x))
+    m.base_situ_glu.w_gate.weight.data = m.base_situ_glu.w_gate.weight.data * 1.5
+    seen.append(check(m, x))
+    m.base_situ_glu.w_up.weight = nn.Parameter(m.base_situ_glu.w_up.weight * 2)
+    seen.append(check(m, x))
+    for a, b in zip(seen, seen[1:]):
+        assert not torch.equal(a, b)
+    twin = copy.deepcopy(m)
+    twin.base_w_down.weight.zero_()
+    check(twin, x)
+    assert torch.equal(m(x), seen[-1])
+    m.half()
+    check(m, x.half())
+
+
+@torch.no_grad()
+def test_changed_weights_are_not_held_by_a_capture():
+    """A capture runs nothing: weights that changed since they were held are refused there, and nothing is captured half."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+    m = moe().quantize_base_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m(x)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    m.base_w_down.weight.mul_(0.5)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="quantize_base_"):
+        with torch.cuda.graph(graph):
+            m(x)
+    want = m(x)  # holds them
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m(x)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(m(x), want)

@@ -17,12 +17,18 @@ import torch
 import torch.nn as nn
 
 from .feed_forward import gated_linear, linear_add, quantize_rows
+from .hip_kernels import traced
 from .layer_ops import mcmoe_coef, norm_add, plain, situ_glu
 
 
 def _weight_alone(linear) -> bool:
     """A projection that is no more than its weight."""
     return plain(linear, nn.Linear) and linear.bias is None
+
+
+def _marks(linears) -> tuple:
+    """Of each weight what tells a change: where its data lies, its version and its type."""
+    return tuple((w.data_ptr(), -1 if w.is_inference() else w._version, w.dtype) for w in (m.weight for m in linears))
 
 
 class SiTUGLU(nn.Module):
@@ -56,6 +62,7 @@ class SiTUGLU(nn.Module):
 
 class ManifoldContinuousMoE(nn.Module):
     _base8 = None        # the held weights: (q, scale) of the gate's, the up and the down projection
+    _base8_of = None     # what the weights were then (_marks)
     _in_8_bits = False   # whether the base path takes them
 
     def __init__(self, hidden_dim: int = 16384, rank: int = 32, num_components: int = 64,
@@ -85,31 +92,37 @@ class ManifoldContinuousMoE(nn.Module):
 
     def quantize_base_(self, on: bool = True) -> "ManifoldContinuousMoE":
         """Holds the base path's three weights in 8 bits with a scale for each output channel and runs the path on rows in 8 bits, for
-        inference (``on=False``: no longer).  The weights themselves stay; after a change of theirs, or a move to another device, this is
-        called again.  What is held keeps its place, while the path is off too, so that a graph captured on the 8-bit weights replays with
-        the ones held last (until a move or a change of shape).  Not part of the ``state_dict``.  The path takes the weights alone: modules
-        of another class, with a bias or with hooks are refused, here and where it runs."""
+        inference (``on=False``: no longer).  The weights themselves stay, and a call that finds them changed in place, replaced or
+        moved holds them anew.  A change through ``.data`` or in inference mode leaves no trace, and a captured graph or a traced call
+        runs no check: after one, this is called again.  What is held keeps its place, while the path is off too, so that a graph captured on the 8-bit weights
+        replays with the ones held last (until a move or a change of shape).  Not part of the ``state_dict``.  The path takes the weights
+        alone: modules of another class, with a bias or with hooks are refused, here and where it runs."""
         if on:
             self._hold_base()
         self._in_8_bits = on
         return self
 
     def _hold_base(self) -> None:
-        old = self._base8
+        old, linears = self._base8, self._base_linears()
         with torch.inference_mode(False), torch.no_grad():  # tensors made in inference mode cannot be renewed outside it
-            new = tuple(quantize_rows(m.weight.detach()) for m in self._base_linears())
+            new = tuple(quantize_rows(m.weight.detach()) for m in linears)
             if old and all(o.shape == n.shape and o.device == n.device for (o, _), (n, _) in zip(old, new)):
                 for pair, fresh in zip(old, new):
                     for t, n in zip(pair, fresh):
                         t.copy_(n)
                 new = old
-        self._base8 = new
+        self._base8, self._base8_of = new, _marks(linears)
 
     def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
         if torch.is_grad_enabled():
             raise RuntimeError("verace_amd.ManifoldContinuousMoE: the base path in 8 bits has no gradients; run under "
                                "torch.no_grad(), or call quantize_base_(False)")
-        self._base_linears()
+        linears = self._base_linears()
+        if not traced(xf) and _marks(linears) != self._base8_of:
+            if torch.cuda.is_current_stream_capturing():  # which would run nothing
+                raise RuntimeError("verace_amd.ManifoldContinuousMoE: the weights have changed since they were held in 8 bits; call "
+                                   "quantize_base_() before the capture")
+            self._hold_base()
         (wg, sg), (wu, su), (wd, sd) = self._base8
         glu = self.base_situ_glu
         out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else xf.dtype
