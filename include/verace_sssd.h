@@ -526,6 +526,10 @@ int vmi_selective_step(const void* x, int64_t x_b, const void* delta, int64_t d_
  * keep (or NULL) receives the sums before the activation, contiguous [M, N] (with the bias; gated [M, 2F], a row's gates first).
  * Gradients from the inputs, and from those sums where they were kept (kept; NULL: formed again), for dy (dh): dx [M, K], dw [N, K] (gated: [2F, K], the gate's rows first), db [N],
  * contiguous, of dtype; each may be NULL.  dz is rounded to dtype between the products.  Sums run in a fixed order. */
+/* What a product of a call with these sizes (N: F of the gated ones) runs as.  product: 0 linear, 1 gated, 2 linear's dz, 3 gated dz, 4
+ * linear's dx, 5 gated dx, 6 linear's dw, 7 gated dw.  form: 0 tiles of 256 x 256, 1 of 256 x 128, 2 of 128 x 128, 3 of 64 x 64, 4 of
+ * 64 x 64 by four groups of waves, 5 the kernel for a few rows, 16 a workgroup, 6 the same 32, 7 the same 64. */
+int vmi_feed_forward_form(int product, int dtype, int act, int64_t M, int64_t N, int64_t K, int* form);
 /* Rows of any address and length (row_bytes, ld_bytes apart) as these products take them: contiguous rows of whole 16-byte
  * pieces at dst, zeros behind the last byte; of one matrix, or of up to three in one launch (those without rows are passed over). */
 int vmi_pad_rows(const void* src, int64_t ld_bytes, void* dst, int64_t rows, int64_t row_bytes, void* stream);

@@ -76,14 +76,20 @@ def gated(x, wg, wu, activation, dtype, b1=4.0, b2=25.0, scales=None):
     return h, e + rounding(h, dtype)
 
 
-def gated_bwd(x, wg, wu, activation, dh, dtype, b1=4.0, b2=25.0):
-    """[(gradient, bound)] of x, wg, wu."""
+def gated_dz(x, wg, wu, activation, dh, dtype, b1=4.0, b2=25.0):
+    """[(dg, bound), (du, bound)], rounded to dtype as operands of products."""
     (g, eg), (u, eu) = product(x, wg), product(x, wu)
     a, da, b, db = gate_terms(g, u, activation, b1, b2)
     dg, du = dh * da * b, dh * a * db
     # slopes change by at most twice their argument's error and the other factor's
     edg = dh.abs() * (2 * b.abs() * eg + da.abs() * eu + 2 * eg * eu) + (ACT_ERROR + flushed(g, b1)) * dh.abs() * b.abs() + rounding(dg, dtype)
     edu = dh.abs() * (2 * a.abs() * eu + da.abs() * eg + 2 * eg * eu) + (ACT_ERROR * a.abs() + flushed(g, b1)) * dh.abs() + rounding(du, dtype)
+    return [(dg, edg), (du, edu)]
+
+
+def gated_bwd(x, wg, wu, activation, dh, dtype, b1=4.0, b2=25.0):
+    """[(gradient, bound)] of x, wg, wu."""
+    (dg, edg), (du, edu) = gated_dz(x, wg, wu, activation, dh, dtype, b1, b2)
     out = []
     n = 2 * dg.shape[1] + 8
     dx = dg @ wg + du @ wu
@@ -117,16 +123,22 @@ def linear(x, w, bias, residual, activation, dtype, scales=None):
     return y, 1.2 * e + ACT_ERROR * (a.abs() if activation else 0) + 2.0 ** -23 * y.abs() + rounding(y, dtype)
 
 
-def linear_bwd(x, w, bias, activation, dy, dtype):
-    """[(gradient, bound)] of x, weight, bias."""
+def linear_dz(x, w, bias, activation, dy, dtype):
+    """(dz, bound), rounded to dtype as an operand of products where there is an activation."""
     z, e = product(x, w)
     if bias is not None:
         z = z + bias
     _, da = act(z, activation)
     dz = dy * da
-    edz = torch.zeros_like(dz)
-    if activation is not None:  # the slopes' own slopes are at most 1
-        edz = dy.abs() * (e + 2.0 ** -23 * z.abs() + ACT_ERROR) + rounding(dz, dtype)
+    if activation is None:
+        return dz, torch.zeros_like(dz)
+    # the slopes' own slopes are at most 1
+    return dz, dy.abs() * (e + 2.0 ** -23 * z.abs() + ACT_ERROR) + rounding(dz, dtype)
+
+
+def linear_bwd(x, w, bias, activation, dy, dtype):
+    """[(gradient, bound)] of x, weight, bias."""
+    dz, edz = linear_dz(x, w, bias, activation, dy, dtype)
     dx, dw, db = dz @ w, dz.T @ x, dz.sum(0)
     M, N = dz.shape
     return [(dx, edz @ w.abs() + (N + 8) * 2.0 ** -23 * (dz.abs() @ w.abs()) + rounding(dx, dtype)),

@@ -570,49 +570,75 @@ struct Rounds {
   }
 };
 
-template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t stream) {
-  constexpr bool PAIR = KIND == GATED || KIND == GATED_DZ;
-  const int64_t cols = PAIR ? 2 * static_cast<int64_t>(p.n) : p.n;
-  const int64_t shares = KIND == DW ? p.splits : 1;
+// What a product runs as: a tile (the last: four groups of its waves share the contraction), or the kernel for a few rows, 16, 32 or 64
+// of them a workgroup.
+enum Form { LARGE, TALL, MIDDLE, SMALL, SMALL_BY_FOUR, ROWS_16, ROWS_32, ROWS_64 };
+
+// The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536, and 2048 of the gated form), and any of up
+// to 16 rows that a grid's threads hold.  Both sides in us, rows / tiles: bf16 K 2048 N 1024 M 128 7.7 / 9.1, M 256 11.5 / 9.2; bf16
+// K 1024 N 4096 M 32 5.7 / 6.2, M 64 8.4 / 6.4; e4m3 K 4096 N 4096 M 32 8.1 / 9.0, M 64 12.1 / 9.0; fp32 K 2048 N 1024 M 256 22 / 37,
+// M 384 39 / 38; fp32 K 4096 N 4096 M 96 64 / 69, M 128 74 / 72, gated (F 2048) M 128 53 / 71.
+inline bool few_rows(Kind kind, int size, const Args& p) {
+  const int64_t cols = kind == GATED ? 2 * static_cast<int64_t>(p.n) : p.n;
+  if ((kind != LINEAR && kind != GATED) || !grid_fits((static_cast<int64_t>(p.n) + 15) / 16, 512)) return false;
+  return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (size < 4 ? 512 : kind == GATED ? 2048 : 1536);
+}
+// Rows are split over workgroups too while there are fewer of those than compute units: a workgroup's x and weights both go
+// through its compute unit (64 rows, K 2048, N 1024 in fp16: 16 rows a workgroup 6.6 us, 64 12.3).  A gated result of 512 fragments
+// has at most 85 columns of them with more than 32 rows, which never need workgroups of 64.
+inline Form rows_form(Kind kind, int size, const Args& p) {
+  const int64_t cols = (static_cast<int64_t>(p.n) + 15) / 16;
+  int mt = p.m <= 16 ? 1 : p.m <= 32 || (kind == GATED && size < 4) ? 2 : 4;
+  while (mt > 1 && cols * ((p.m + 16 * mt - 1) / (16 * mt)) <= 128) mt /= 2;
+  return mt == 1 ? ROWS_16 : mt == 2 ? ROWS_32 : ROWS_64;
+}
+
+inline Form form_of(Kind kind, int size, const Args& p) {
+  if (few_rows(kind, size, p)) return rows_form(kind, size, p);
+  const bool pair = kind == GATED || kind == GATED_DZ;
+  const int64_t cols = pair ? 2 * static_cast<int64_t>(p.n) : p.n;
+  const int64_t shares = kind == DW ? p.splits : 1;
   // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
   // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
-  if constexpr (PAIR)
-    if (const int64_t t = tiles(p.m, cols, 128, 128);
-        p.gate.act == ACT_SITU && p.k <= 8 * (128 / static_cast<int>(sizeof(E))) && t >= 160 && grid_fits(t, Middle::THREADS))
-      return launch_product<E, KIND, Middle>(p, stream);
-  const Rounds r = {sizeof(E)};
+  if (const int64_t t = tiles(p.m, cols, 128, 128);
+      pair && p.gate.act == ACT_SITU && p.k <= 8 * (128 / size) && t >= 160 && grid_fits(t, Middle::THREADS))
+    return MIDDLE;
+  const Rounds r = {size};
   const int64_t l = r.time(tiles(p.m, cols, 256, 256) * shares, 0), t = r.time(tiles(p.m, cols, 256, 128) * shares, 1);
   const int64_t m = r.time(tiles(p.m, cols, 128, 128) * shares, 2), s = r.time(tiles(p.m, cols, 64, 64) * shares, 3);
-  const bool large = l <= t && l <= m && l <= s, tall = t <= m && t <= s, middle = m <= s;
-  if (large) return launch_product<E, KIND, Large>(p, stream);
-  if (tall) return launch_product<E, KIND, Tall>(p, stream);
-  if (middle) return launch_product<E, KIND, Middle>(p, stream);
+  if (l <= t && l <= m && l <= s) return LARGE;
+  if (t <= m && t <= s) return TALL;
+  if (m <= s) return MIDDLE;
   // Four groups of a tile's waves share a long contraction where the tiles leave compute units idle or at one workgroup: a step's
   // latency, not its data, bounds them.  us with four / one (rows x k x columns): bf16 512 x 4096 x 512 15.5 / 21.7, 256 x 4096 x
   // 4096 16.6 / 22.8, 1024 x 1024 x 1024 (16 steps) 7.8 / 6.9, 384 x 4096 x 4096 (384 tiles) 29.7 / 25.2; fp32 777 x 1000 x 1037
   // 22.7 / 24.2, 256 x 4096 x 4096 70 / 86; e4m3 256 x 4096 x 4096 10.0 / 10.4.  The other kinds have short contractions: DW's
   // shares, and dz where the forward kept no sums.
-  if constexpr (KIND == LINEAR || KIND == GATED || KIND == DX)
-    if (tiles(p.m, cols, 64, 64) <= 256 && p.k > 31 * (128 / static_cast<int>(sizeof(E)))) return launch_product<E, KIND, Small, 4>(p, stream);
-  return launch_product<E, KIND, Small>(p, stream);
+  const bool groups = (kind == LINEAR || kind == GATED || kind == DX) && tiles(p.m, cols, 64, 64) <= 256 && p.k > 31 * (128 / size);
+  return groups ? SMALL_BY_FOUR : SMALL;
 }
 
-template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
-// The kernel for a few rows takes a result of up to 512 fragments of 16 x 16 (fp32: 1536, and 2048 of the gated form), and any of up
-// to 16 rows that a grid's threads hold.  Both sides in us, rows / tiles: bf16 K 2048 N 1024 M 128 7.7 / 9.1, M 256 11.5 / 9.2; bf16 K 1024 N 4096 M 32 5.7 /
-// 6.2, M 64 8.4 / 6.4; e4m3 K 4096 N 4096 M 32 8.1 / 9.0, M 64 12.1 / 9.0; fp32 K 2048 N 1024 M 256 22 / 37, M 384 39 / 38; fp32 K
-// 4096 N 4096 M 96 64 / 69, M 128 74 / 72, gated (F 2048) M 128 53 / 71.
-template <typename E> inline bool few_rows(Kind kind, const Args& p) {
-  const int64_t cols = kind == GATED ? 2 * static_cast<int64_t>(p.n) : p.n;
-  if (!grid_fits((static_cast<int64_t>(p.n) + 15) / 16, 512)) return false;
-  return p.m <= 16 || tiles(p.m, cols, 16, 16) <= (sizeof(E) < 4 ? 512 : kind == GATED ? 2048 : 1536);
+template <typename E, int KIND, int MT> int launch_rows(const Args& p, hipStream_t stream);  // feed_forward_rows.h
+
+template <typename E, int KIND> int product_of_kind(const Args& p, hipStream_t stream) {
+  const Form form = form_of(static_cast<Kind>(KIND), sizeof(E), p);
+  if constexpr (KIND == LINEAR || KIND == GATED) {
+    if (form == ROWS_16) return launch_rows<E, KIND, 1>(p, stream);
+    if (form == ROWS_32) return launch_rows<E, KIND, 2>(p, stream);
+    if constexpr (KIND == LINEAR || sizeof(E) == 4)
+      if (form == ROWS_64) return launch_rows<E, KIND, 4>(p, stream);
+  }
+  if constexpr (KIND == LINEAR || KIND == GATED || KIND == DX)
+    if (form == SMALL_BY_FOUR) return launch_product<E, KIND, Small, 4>(p, stream);
+  switch (form) {
+    case LARGE: return launch_product<E, KIND, Large>(p, stream);
+    case TALL: return launch_product<E, KIND, Tall>(p, stream);
+    case MIDDLE: return launch_product<E, KIND, Middle>(p, stream);
+    default: return launch_product<E, KIND, Small>(p, stream);
+  }
 }
 
 template <typename E> int product_of(Kind kind, const Args& p, hipStream_t stream) {
-  if (few_rows<E>(kind, p)) {
-    if (kind == LINEAR) return launch_rows<E, LINEAR>(p, stream);
-    if (kind == GATED) return launch_rows<E, GATED>(p, stream);
-  }
   switch (kind) {
     case LINEAR: return product_of_kind<E, LINEAR>(p, stream);
     case GATED: return product_of_kind<E, GATED>(p, stream);

@@ -301,6 +301,29 @@ extern "C" int vmi_pad_rows_3(const void* src0, int64_t ld_bytes0, void* dst0, i
   return pad_all(p, static_cast<hipStream_t>(stream));
 }
 
+extern "C" int vmi_feed_forward_form(int product, int dtype, int act, int64_t M, int64_t N, int64_t K, int* form) {
+  if (form == nullptr || !sizes_ok(M, N, K) || dtype < 0 || dtype > VMI_E4M3 || product < 0 || product > 7) return VMI_ERR_INVALID_ARG;
+  const bool gated = (product & 1) != 0;
+  if (gated ? act != ACT_SILU && act != ACT_SITU : !linear_act(act)) return VMI_ERR_INVALID_ARG;
+  if (dtype == VMI_E4M3 && product > 1) return VMI_ERR_INVALID_ARG;
+  Args p{};
+  p.gate.act = act, p.splits = 1;
+  int64_t m = M, n = N, k = K;
+  Kind kind;
+  switch (product / 2) {
+    case 0: kind = gated ? GATED : LINEAR; break;
+    case 1: kind = gated ? GATED_DZ : LINEAR_DZ; break;
+    case 2: kind = DX, n = K, k = N; break;
+    default:
+      kind = DW, m = (gated ? 2 : 1) * whole(N, dtype), n = K, k = M;
+      if (m > INT32_MAX) return VMI_ERR_UNSUPPORTED;
+      p.splits = weight_shares(m, n, k).n;
+  }
+  p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
+  *form = form_of(kind, static_cast<int>(size_of(dtype)), p);
+  return VMI_OK;
+}
+
 extern "C" int vmi_linear_add(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
                               int dtype, const void* bias, const void* residual, int64_t ldr, int act, void* out, int64_t ldo,
                               int out_dtype, float* keep, int64_t M, int64_t N, int64_t K, void* stream) {

@@ -110,17 +110,11 @@ template <typename E, int KIND, int MT> __global__ __launch_bounds__(512, 2) voi
   });
 }
 
-// Rows are split over workgroups too while there are fewer of those than compute units: a workgroup's x and weights both go
-// through its compute unit (64 rows, K 2048, N 1024 in fp16: MT 1 6.6 us, MT 4 12.3).
-template <typename E, int KIND> int launch_rows(const Args& p, hipStream_t stream) {
+template <typename E, int KIND, int MT> int launch_rows(const Args& p, hipStream_t stream) {
   const int64_t cols = (static_cast<int64_t>(p.n) + 15) / 16;
   if (!grid_fits(cols, 512)) return VMI_ERR_UNSUPPORTED;
-  int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-  while (mt > 1 && cols * ((p.m + 16 * mt - 1) / (16 * mt)) <= 128) mt /= 2;
-  const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>((p.m + 16 * mt - 1) / (16 * mt)));
-  if (mt == 1) hipLaunchKernelGGL((rows_kernel<E, KIND, 1>), grid, dim3(512), 0, stream, p);
-  else if (mt == 2) hipLaunchKernelGGL((rows_kernel<E, KIND, 2>), grid, dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((rows_kernel<E, KIND, 4>), grid, dim3(512), 0, stream, p);
+  const dim3 grid(static_cast<unsigned>(cols), static_cast<unsigned>((p.m + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((rows_kernel<E, KIND, MT>), grid, dim3(512), 0, stream, p);
   return hip_status(hipGetLastError());
 }
 

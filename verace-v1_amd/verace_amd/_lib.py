@@ -72,6 +72,7 @@ EXPORTED = (
     "vmi_selective_scan_bwd",
     "vmi_pad_rows",
     "vmi_pad_rows_3",
+    "vmi_feed_forward_form",
     "vmi_linear_add",
     "vmi_linear_add_bwd_workspace_bytes",
     "vmi_linear_add_bwd",
@@ -202,6 +203,7 @@ def _declare(lib):
                                            i64, i64, i64, i64, i64, i64, vp, sz, vp]
     lib.vmi_pad_rows.argtypes = [vp, i64, vp, i64, i64, vp]
     lib.vmi_pad_rows_3.argtypes = [vp, i64, vp, i64, i64] * 3 + [vp]
+    lib.vmi_feed_forward_form.argtypes = [i32, i32, i32, i64, i64, i64, ctypes.POINTER(i32)]
     lib.vmi_linear_add.argtypes = [vp, i64, vp, vp, i64, vp, i32, vp, vp, i64, i32, vp, i64, i32, vp, i64, i64, i64, vp]
     lib.vmi_linear_add_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, psz]
     lib.vmi_linear_add_bwd.argtypes = [vp, i64, vp, i64, i32, vp, i32, vp, vp, i64, vp, vp, vp, i64, i64, i64, vp, sz, vp]
@@ -214,7 +216,7 @@ def _declare(lib):
     for name in ("gated_norm", "gated_norm_bwd_workspace_bytes", "gated_norm_bwd", "short_conv", "short_conv_step",
                  "short_conv_bwd_workspace_bytes", "short_conv_bwd", "selective_scan_workspace_bytes",
                  "selective_scan_fwd", "selective_step", "selective_scan_bwd_workspace_bytes", "selective_scan_bwd",
-                 "pad_rows", "pad_rows_3", "linear_add", "linear_add_bwd_workspace_bytes", "linear_add_bwd", "gated_linear",
+                 "pad_rows", "pad_rows_3", "feed_forward_form", "linear_add", "linear_add_bwd_workspace_bytes", "linear_add_bwd", "gated_linear",
                  "gated_linear_bwd_workspace_bytes", "gated_linear_bwd", "norm_add_quant"):
         getattr(lib, "vmi_" + name).restype = i32
 
