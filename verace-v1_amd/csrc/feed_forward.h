@@ -30,7 +30,7 @@ struct Args {
   const void* a;     // x, dz
   const void* b;     // the weight, x
   const void* b2;    // the second weight
-  int64_t lda, ldb, ldb2;  // elements
+  int64_t lda, ldb;  // elements
   int m, n, k;       // of the result and the contraction
   int tiles_m, tiles_n, group;
   int splits, split_k;     // DW: shares of the contraction, and their length
@@ -94,6 +94,7 @@ template <typename T, int W> __device__ __forceinline__ void activate_all(float 
     for (int j = 0; j < W; ++j) z[j] *= normal<T>(z[j]).cdf;
   }
 }
+// (slopes: of the two activations; without one dz is dy)
 template <typename T, int W> __device__ __forceinline__ void slope_all(float (&z)[W], int act) {
   if (act == ACT_SILU) {
 #pragma unroll
@@ -101,15 +102,12 @@ template <typename T, int W> __device__ __forceinline__ void slope_all(float (&z
       const float s = sigmoid_for<T>(z[j]);
       z[j] = s * (1.f + z[j] * (1.f - s));
     }
-  } else if (act == ACT_GELU) {
+  } else {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const Normal r = normal<T>(z[j]);
       z[j] = fmaf(z[j] * 0.398942280f, r.e, r.cdf);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < W; ++j) z[j] = 1.f;
   }
 }
 // For 16-bit results both tanh and the sigmoid come from exponentials of at most 1 and one reciprocal:

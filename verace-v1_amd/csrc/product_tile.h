@@ -105,13 +105,8 @@ template <int HM_, int HN_, int WM_, int WN_> struct Shape {
   static_assert(LA >= 1 && LB >= 1 && MF >= 1 && NF >= 1);
 };
 
-// One operand: `MN` where its m (n) is contiguous in memory.
-struct Matrix {
-  const char* p;
-  int64_t ld;  // bytes
-};
-
-// A thread's loads of one piece of an operand.  H rows (columns) of the piece, of which `inside` are in the operand.
+// A thread's loads of one piece of an operand, `MN` where its m (n) is contiguous in memory.  H rows (columns) of the piece, of
+// which `inside` are in the operand.
 // PERM: the order in which B's columns go to fragments (see column_of).
 template <typename E, bool MN, int H, int L, int THREADS, int XF, bool PERM> struct Loader {
   static constexpr int SIZE = sizeof(E), KT = 128 / SIZE, RB = MN ? H * SIZE : 128, SLOTS = RB / 16;
