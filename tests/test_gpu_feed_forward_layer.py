@@ -205,3 +205,25 @@ def test_changed_weights_are_not_held_by_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(m(x), want)
+
+
+@torch.no_grad()
+def test_weights_held_anew_on_another_stream():
+    """A call on a busy side stream finds changed weights; one on the current stream right after it, which need not wait for the other,
+    reads what was held, not what was there before."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+    m, fresh = moe().quantize_base_(), moe()
+    m(x)
+    m.base_w_down.weight.mul_(0.5)
+    fresh.load_state_dict(m.state_dict())
+    want = fresh.quantize_base_()(x)
+    a = torch.randn(8192, 8192, device="cuda").to(BF)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            a = (a @ a).clamp(-1, 1)
+        there = m(x)
+    here = m(x).clone()
+    torch.cuda.synchronize()
+    assert torch.equal(here, want) and torch.equal(there, want)

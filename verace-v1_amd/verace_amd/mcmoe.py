@@ -111,6 +111,8 @@ class ManifoldContinuousMoE(nn.Module):
                     for t, n in zip(pair, fresh):
                         t.copy_(n)
                 new = old
+        if not torch.cuda.is_current_stream_capturing():  # calls on other streams wait for the weights' change at most, not for this
+            torch.cuda.current_stream(linears[0].weight.device).synchronize()
         self._base8, self._base8_of = new, _marks(linears)
 
     def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
