@@ -307,7 +307,8 @@ template <typename E, typename T, int KIND, int W, bool FULL = false> __device__
 
 // z ws xs.  A sum z of products of e4m3 values is 0 or 2^-18 to 2^48, so z times an ordinary weight's scale, from 2^-100 to 2^70, is a
 // normal number, and the result is rounded as itself for any xs.  (z times xs ws, which may be infinite, would lose a z of 0.)  FAR: of
-// other columns (a row of zeros has the scale 2^-126) the powers of two are added and come last.
+// other columns (a weight's row of zeros has the scale 2^-126) the powers of two are added and come last.  Asked once for a lane's
+// columns; for each of its rows that costs 7 us of 46 (e4m3 8192 x 1024 x 2 x 2048).
 template <int W> __device__ __forceinline__ bool far_scale(const float (&ws)[W]) {
   float low = __builtin_inff(), high = 0.f;
 #pragma unroll
@@ -597,7 +598,8 @@ inline Form form_of(Kind kind, int size, const Args& p) {
   const int64_t cols = pair ? 2 * static_cast<int64_t>(p.n) : p.n;
   const int64_t shares = kind == DW ? p.splits : 1;
   // With a short contraction SiTU's epilogue costs as much as the products: of two workgroups a compute unit one multiplies meanwhile.
-  // us with tiles of 128 x 128 / of 256 x 256, e4m3, 8192 rows, F 2048: K 512 34.0 / 38.2, K 1024 43.9 / 44.9, K 1536 55.9 / 54.1.
+  // us with tiles of 128 x 128 / of 256 x 256, 8192 rows, F 2048, on one card: e4m3 K 512 35.4 / 40.6, K 1024 49.1 / 50.7, K 1536 61.3 /
+  // 61.0; bf16 K 512 47.2 / 46.4, K 1024 71.3 / 66.6.
   if (const int64_t t = tiles(p.m, cols, 128, 128);
       pair && p.gate.act == ACT_SITU && p.k <= 8 * (128 / size) && t >= 160 && grid_fits(t, Middle::THREADS))
     return MIDDLE;

@@ -382,7 +382,7 @@ def linear_add(
 
     x: [..., K]; weight: [N, K]; bias: [N]; residual: [..., N], all of one dtype (bfloat16, float16, float32); ``activation``
     None, "silu" or "gelu" (z Phi(z)).  Sums and the epilogue are fp32 and y is rounded once.  Differentiable once in every
-    tensor; the backward keeps x, weight and bias, and with an activation, for K of 1536 and more or in float32, the sum before
+    tensor; the gradient before the activation is rounded to x's dtype once, as an operand of products.  The backward keeps x, weight and bias, and with an activation, for K of 1536 and more or in float32, the sum before
     it in float32.
 
     8 bits: x and weight float8_e4m3fn with ``x_scale`` [...] and ``weight_scale`` [N] float32; bias, residual and y are
