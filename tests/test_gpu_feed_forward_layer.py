@@ -227,3 +227,17 @@ def test_weights_held_anew_on_another_stream():
     here = m(x).clone()
     torch.cuda.synchronize()
     assert torch.equal(here, want) and torch.equal(there, want)
+
+
+@torch.no_grad()
+def test_weights_are_not_held_by_a_capture():
+    """Nor by asking for it there: what is held, and how the path runs, stay as they were."""
+    x = torch.randn(1, 5, 128, device="cuda").to(BF)
+    for m in (moe(), moe().quantize_base_()):
+        want = m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(graph):
+                m.quantize_base_()
+        assert torch.equal(m(x), want)

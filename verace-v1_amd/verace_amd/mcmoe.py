@@ -94,15 +94,19 @@ class ManifoldContinuousMoE(nn.Module):
         """Holds the base path's three weights in 8 bits with a scale for each output channel and runs the path on rows in 8 bits, for
         inference (``on=False``: no longer).  The weights themselves stay, and a call that finds them changed in place, replaced or
         moved holds them anew.  A change through ``.data`` or in inference mode leaves no trace, and a captured graph or a traced call
-        runs no check: after one, this is called again.  What is held keeps its place, while the path is off too, so that a graph captured on the 8-bit weights
-        replays with the ones held last (until a move or a change of shape).  Not part of the ``state_dict``.  The path takes the weights
-        alone: modules of another class, with a bias or with hooks are refused, here and where it runs."""
+        runs no check: after one, this is called again, outside a capture.  What is held keeps its place, while the path is off too,
+        so that a graph captured on the 8-bit weights replays with the ones held last (until a move or a change of shape).  Not part of
+        the ``state_dict``.  The path takes the weights alone: modules of another class, with a bias or with hooks are refused, here and
+        where it runs."""
         if on:
             self._hold_base()
         self._in_8_bits = on
         return self
 
     def _hold_base(self) -> None:
+        if torch.cuda.is_current_stream_capturing():  # which would run nothing now
+            raise RuntimeError("verace_amd.ManifoldContinuousMoE: the weights are new or have changed; call quantize_base_() before the "
+                               "capture")
         old, linears = self._base8, self._base_linears()
         with torch.inference_mode(False), torch.no_grad():  # tensors made in inference mode cannot be renewed outside it
             new = tuple(quantize_rows(m.weight.detach()) for m in linears)
@@ -111,8 +115,8 @@ class ManifoldContinuousMoE(nn.Module):
                     for t, n in zip(pair, fresh):
                         t.copy_(n)
                 new = old
-        if not torch.cuda.is_current_stream_capturing():  # calls on other streams wait for the weights' change at most, not for this
-            torch.cuda.current_stream(linears[0].weight.device).synchronize()
+        # calls on other streams wait for the weights' change at most, not for this
+        torch.cuda.current_stream(linears[0].weight.device).synchronize()
         self._base8, self._base8_of = new, _marks(linears)
 
     def _base_in_8_bits(self, xf: torch.Tensor) -> torch.Tensor:
@@ -121,9 +125,6 @@ class ManifoldContinuousMoE(nn.Module):
                                "torch.no_grad(), or call quantize_base_(False)")
         linears = self._base_linears()
         if not traced(xf) and _marks(linears) != self._base8_of:
-            if torch.cuda.is_current_stream_capturing():  # which would run nothing
-                raise RuntimeError("verace_amd.ManifoldContinuousMoE: the weights have changed since they were held in 8 bits; call "
-                                   "quantize_base_() before the capture")
             self._hold_base()
         (wg, sg), (wu, su), (wd, sd) = self._base8
         glu = self.base_situ_glu
